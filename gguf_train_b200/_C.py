@@ -52,6 +52,20 @@ class SdpaOpts(ctypes.Structure):
 
 POPTS = ctypes.POINTER(SdpaOpts)
 
+GTB_KV8_INT8, GTB_KV8_E4M3 = 0, 1  # gtb_kv8 formats
+GTB_ROPE_INTERLEAVED, GTB_ROPE_PER_AXIS = 1, 2  # gtb_rope_axes flags
+
+
+class KV8(ctypes.Structure):
+    """gtb_kv8: a block-scaled 8-bit cache (include/gtb_attn.h)."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("lens", c_void_p),
+                ("B", c_int64), ("Hkv", c_int64), ("Smax", c_int64), ("D", c_int64), ("block", c_int32),
+                ("format", c_int32)]
+
+
+PKV8 = ctypes.POINTER(KV8)
+
 
 def _configure(lib: ctypes.CDLL) -> ctypes.CDLL:
     # raw-pointer ABI (gtb_attn.h)
@@ -94,6 +108,17 @@ def _configure(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.gtb_attn_merge.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64,
                                    c_int64, c_void_p]
     lib.gtb_attn_merge.restype = c_int
+    lib.gtb_rope_axes.argtypes = [P4, P4, P4, P4, c_void_p, c_int64, c_int64, ctypes.POINTER(c_int32), c_int, c_int, c_int,
+                                  c_float, c_float, c_int, c_void_p]
+    lib.gtb_rope_axes.restype = c_int
+    lib.gtb_kv8_append.argtypes = [PKV8, P4, P4, c_void_p, c_int, c_void_p]
+    lib.gtb_kv8_append.restype = c_int
+    lib.gtb_kv8_read.argtypes = [PKV8, c_void_p, P4, P4, c_void_p]
+    lib.gtb_kv8_read.restype = c_int
+    lib.gtb_kv8_attention.argtypes = [P4, PKV8, c_float, c_void_p, c_void_p, c_void_p, P4, c_void_p, c_void_p]
+    lib.gtb_kv8_attention.restype = c_int
+    lib.gtb_kv8_evict.argtypes = [PKV8, c_void_p, c_int64, c_int64, PKV8, c_void_p, c_void_p, c_void_p]
+    lib.gtb_kv8_evict.restype = c_int
     lib.gtb_last_error.argtypes = []
     lib.gtb_last_error.restype = c_char_p
     lib.gtb_clear_error.argtypes = []

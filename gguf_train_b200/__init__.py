@@ -12,8 +12,9 @@ from . import _C
 from . import functional
 from . import gguf_io
 from . import handles
-from .functional import (FlashAttentionFn, RoPEFn, decode_q8_0, dequantize_q8_0, q8_0_append, quantize_q8_0, rope,
-                         scaled_dot_product_attention, sdpa_from_host)
+from .functional import (FlashAttentionFn, RoPEAxesFn, RoPEFn, decode_q8_0, dequantize_q8_0, q8_0_append, quantize_q8_0,
+                         rope, rope_axes, scaled_dot_product_attention, sdpa_from_host)
+from .kv8 import KV8Cache, kv8_append, kv8_attention, kv8_evict, kv8_read
 from .modules import MultiheadAttention
 
 __all__ = [
@@ -29,6 +30,13 @@ __all__ = [
     "q8_0_append",
     "rope",
     "RoPEFn",
+    "rope_axes",
+    "RoPEAxesFn",
     "dequantize_q8_0",
     "decode_q8_0",
+    "KV8Cache",
+    "kv8_append",
+    "kv8_attention",
+    "kv8_evict",
+    "kv8_read",
 ]

@@ -77,6 +77,31 @@ void register_status_word(int device, int* word) {
     }
 }
 
+// Every pointer handed to a kernel must be device (or managed) memory of the current device.
+bool check_device_ptr(const void* p, const char* ctx, const char* name) {
+    if (!p) {
+        set_errorf("%s: %s is NULL", ctx, name);
+        return false;
+    }
+    cudaPointerAttributes attr;
+    if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) {
+        cudaGetLastError();
+        set_errorf("%s: %s is not CUDA memory (this engine has no CPU path)", ctx, name);
+        return false;
+    }
+    if (attr.type != cudaMemoryTypeDevice && attr.type != cudaMemoryTypeManaged) {
+        set_errorf("%s: %s is not CUDA device memory (this engine has no CPU path)", ctx, name);
+        return false;
+    }
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (attr.type == cudaMemoryTypeDevice && attr.device != dev) {
+        set_errorf("%s: %s lives on cuda:%d but the current device is cuda:%d", ctx, name, attr.device, dev);
+        return false;
+    }
+    return true;
+}
+
 namespace {
 
 // Every status word of a device that exists so far (none is allocated here).
@@ -107,31 +132,6 @@ std::string shape_str(const int64_t* s, int n) {
     std::string r = "[";
     for (int i = 0; i < n; ++i) r += (i ? ", " : "") + std::to_string(s[i]);
     return r + "]";
-}
-
-// Every pointer handed to a kernel must be device (or managed) memory of the current device.
-bool check_device_ptr(const void* p, const char* ctx, const char* name) {
-    if (!p) {
-        set_errorf("%s: %s is NULL", ctx, name);
-        return false;
-    }
-    cudaPointerAttributes attr;
-    if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) {
-        cudaGetLastError();
-        set_errorf("%s: %s is not CUDA memory (this engine has no CPU path)", ctx, name);
-        return false;
-    }
-    if (attr.type != cudaMemoryTypeDevice && attr.type != cudaMemoryTypeManaged) {
-        set_errorf("%s: %s is not CUDA device memory (this engine has no CPU path)", ctx, name);
-        return false;
-    }
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (attr.type == cudaMemoryTypeDevice && attr.device != dev) {
-        set_errorf("%s: %s lives on cuda:%d but the current device is cuda:%d", ctx, name, attr.device, dev);
-        return false;
-    }
-    return true;
 }
 
 int64_t numel4(const gtb_tensor4& t) { return t.shape[0] * t.shape[1] * t.shape[2] * t.shape[3]; }

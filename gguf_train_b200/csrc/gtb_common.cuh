@@ -34,6 +34,9 @@ void set_errorf(const char* fmt, ...);
 const char* last_error();
 void clear_error();
 
+// Whether p is device (or managed) memory of the current device; sets the message if it is not.
+bool check_device_ptr(const void* p, const char* ctx, const char* name);
+
 // Map a CUDA error to the thread-local message; returns true if there was one.
 bool cuda_failed(cudaError_t e, const char* what);
 

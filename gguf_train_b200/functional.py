@@ -582,6 +582,88 @@ def rope(input: torch.Tensor, positions: torch.Tensor, n_dims: int | None = None
     return RoPEFn.apply(input, positions, nd, int(mode), int(n_ctx_orig), float(freq_base), float(freq_scale))
 
 
+def _rope_axes_run(xs, outs, pos, sections, mode, flags, freq_base, freq_scale, backward):
+    tx, ty = [_t4(x) for x in xs], [_t4(y) for y in outs]
+    two = len(xs) == 2
+    S = xs[0].shape[2]
+    batch = pos.stride(1) if pos.ndim == 3 and pos.shape[1] > 1 else 0
+    rc = _C.lib.gtb_rope_axes(ctypes.byref(tx[0]), ctypes.byref(ty[0]), ctypes.byref(tx[1]) if two else None,
+                              ctypes.byref(ty[1]) if two else None, pos.data_ptr() if pos.numel() else None,
+                              pos.stride(0) if S else 0, batch, sections, len(sections), mode, flags, freq_base, freq_scale,
+                              1 if backward else 0, _stream(xs[0].device))
+    _C.check_rc(rc, "rope_axes")
+
+
+def _rope_axes_new(x):
+    """An output for x: contiguous (B, H, S, D)."""
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+class RoPEAxesFn(torch.autograd.Function):
+    """rope_axes as an autograd Function: apply(pos, sections, mode, flags, freq_base, freq_scale, *xs) -> the
+    rotated xs (one, or q and k, in one launch). The backward rotates the gradients by -angle, again in one
+    launch; nothing but the positions is saved."""
+
+    @staticmethod
+    def forward(ctx, pos, sections, mode, flags, freq_base, freq_scale, *xs):
+        ctx.args = (sections, mode, flags, freq_base, freq_scale)
+        ctx.save_for_backward(pos)
+        xs = [x if x.stride(3) == 1 else x.contiguous() for x in xs]
+        outs = [_rope_axes_new(x) for x in xs]
+        _rope_axes_run(xs, outs, pos, *ctx.args, False)
+        return tuple(outs) if len(outs) > 1 else outs[0]
+
+    @staticmethod
+    def backward(ctx, *grads):
+        (pos,) = ctx.saved_tensors
+        gs = [None if g is None else g if g.stride(3) == 1 else g.contiguous() for g in grads]
+        live = [g for g, need in zip(gs, ctx.needs_input_grad[6:]) if g is not None and need]
+        outs = [_rope_axes_new(g) for g in live]
+        if live:
+            _rope_axes_run(live, outs, pos, *ctx.args, True)
+        it = iter(outs)
+        dx = [next(it) if g is not None and need else None for g, need in zip(gs, ctx.needs_input_grad[6:])]
+        return (None,) * 6 + tuple(dx)
+
+
+def rope_axes(input: torch.Tensor, positions: torch.Tensor, sections, k: torch.Tensor | None = None, mode: int = 2,
+              freq_base: float = 10000.0, freq_scale: float = 1.0, interleaved: bool = False, per_axis: bool = False):
+    """Rotary position embedding with several position axes, for tokens of images and video: positions (A, S) or
+    (A, B, S) int32, axis a (time, height, width, ...; A up to 4) rotating sections[a] of the pairs of dimensions.
+    input (B, H, S, D) and, in the same launch, k (B, Hkv, S, D); f32, f16 or bf16, any layout. Returns the
+    rotated input, or (input, k).
+
+    Pairs are (2i, 2i+1) with mode 0, (i, i + P) with mode 2, P = sum(sections); dims from 2 P on pass through.
+    The axes take the pairs in blocks or, with `interleaved`, in turn (pair i: axis i mod A while that axis
+    has pairs left, else axis 0). Pair i turns by freq_base^(-i / P) a position, or with `per_axis` each axis
+    runs through its own frequencies, freq_base^(-j / sections[a]). Differentiable in input and k.
+
+    Angles are formed modulo a turn in 64-bit fixed point, so positions may be any int32 without loss; rope()
+    instead repeats ggml's f32 accumulation of one axis."""
+    xs = (input,) if k is None else (input, k)
+    _require_cuda("rope_axes", positions, *xs)
+    for x in xs:
+        if x.ndim != 4:
+            raise RuntimeError(f"rope_axes: expected (batch, heads, seq_len, head_dim), got {list(x.shape)}")
+        if x.dtype not in (torch.float32, torch.float16, torch.bfloat16) or x.dtype != input.dtype:
+            raise RuntimeError("rope_axes: input and k must be f32, f16 or bf16, of one type")
+        if x.device != positions.device:
+            raise RuntimeError("rope_axes: input, k and positions must be on one device")
+        if (x.shape[0], x.shape[2], x.shape[3]) != (input.shape[0], input.shape[2], input.shape[3]):
+            raise RuntimeError(f"rope_axes: input {list(input.shape)} and k {list(x.shape)} do not fit together")
+    sections = tuple(int(n) for n in sections)
+    B, S, A = input.shape[0], input.shape[2], len(sections)
+    if positions.shape[-1] != S or tuple(positions.shape[:-1]) not in ((A,), (A, B), (A, 1)):
+        raise RuntimeError(f"rope_axes: positions must be ({A}, {S}) or ({A}, {B}, {S}) for {A} sections, got "
+                           f"{list(positions.shape)}")
+    if positions.dtype != torch.int32:
+        raise RuntimeError("rope_axes: positions must be int32")
+    positions = positions if S <= 1 or positions.stride(-1) == 1 else positions.contiguous()
+    flags = (_C.GTB_ROPE_INTERLEAVED if interleaved else 0) | (_C.GTB_ROPE_PER_AXIS if per_axis else 0)
+    return RoPEAxesFn.apply(positions, (ctypes.c_int32 * max(A, 1))(*sections), int(mode), flags, float(freq_base),
+                            float(freq_scale), *xs)
+
+
 def dequantize_q8_0(blocks: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
     """Inverse of quantize_q8_0: x = q * d, in `dtype`."""
     _require_cuda("dequantize", blocks)

@@ -238,6 +238,86 @@ GTB_API int gtb_attn_merge(float *o_acc, float *lse_acc, const void *o_part, con
                            int part_dtype, int64_t groups, int64_t rows, int64_t D, int64_t part_gstride,
                            int64_t lse_gstride, void *stream);
 
+/* Rotary position embedding with several position axes (time, height, width of images and video), of
+ * one tensor or of q and k in one launch. New export; gtb_rope takes one position per token.
+ *   x (B,H,S,D), out of x's shape and dtype; k, k_out (B,Hkv,S,D) or both NULL; f32/f16/bf16, any
+ *   strides with a unit innermost one; out may be x (in place) when both have the same strides.
+ *   pos: device int32, axis a's position of token (b, s) at pos[a * pos_axis + b * pos_batch + s]
+ *   (pos_batch 0: shared by the batch).
+ *   sections[n_axes] (1 to 4 axes): pairs of dimensions per axis, P = their sum, 2 P <= D <= 256.
+ *   Axis of pair i: blocks (the first sections[0] pairs axis 0, ...), or with GTB_ROPE_INTERLEAVED
+ *   a = i mod n_axes if i < n_axes * sections[a], else 0 (which has to give every axis its sections).
+ *   Frequency of pair i: freq_scale * freq_base^(-i / P); with GTB_ROPE_PER_AXIS the j-th pair of axis a
+ *   has freq_scale * freq_base^(-j / sections[a]).
+ *   mode 0 (pairs 2i, 2i+1) or 2 (pairs i, i + P); dims >= 2 P pass through; backward != 0 rotates by
+ *   -angle (the gradient).
+ * Angles are turns in 64-bit fixed point (position x frequency modulo one turn, exact to 2^-33 of a turn
+ * for any int32 position), so long positions lose nothing; gtb_rope instead follows ggml's f32
+ * accumulation, and the two differ by that rounding where they can express the same rotation. */
+#define GTB_ROPE_INTERLEAVED 1
+#define GTB_ROPE_PER_AXIS 2
+GTB_API int gtb_rope_axes(const gtb_tensor4 *x, gtb_tensor4 *out, const gtb_tensor4 *k, gtb_tensor4 *k_out,
+                          const int32_t *pos, int64_t pos_axis, int64_t pos_batch, const int32_t *sections, int n_axes,
+                          int mode, int flags, float freq_base, float freq_scale, int backward, void *stream);
+
+/* A KV cache held in 8 bits with one scale for each block of `block` tokens and kv head:
+ * value = code * scale. New exports; the reference's only 8-bit cache is Q8_0 (a scale per 32 values).
+ *   k, v: (B,Hkv,Smax,D) contiguous codes, 16-byte aligned: int8 (GTB_KV8_INT8, largest code 127) or OCP
+ *   e4m3 (GTB_KV8_E4M3, 448). k_scale, v_scale: (B,Hkv,ceil(Smax/block)) f32. lens: device int32 (B), rows
+ *   held of each sequence (values outside [0, Smax] are read as the nearest end). block 16, 32, 64 or
+ *   128; D a multiple of 16, at most 256; B * Hkv at most 2^31 - 1, Smax below 2^30.
+ * Rows at and past lens[b], and scales of blocks that hold none of the rows before it, may hold anything
+ * (NaN included): no call lets them into a result. */
+typedef struct gtb_kv8 {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int32_t *lens;
+    int64_t B, Hkv, Smax, D;
+    int32_t block;
+    int32_t format;
+} gtb_kv8;
+#define GTB_KV8_INT8 0
+#define GTB_KV8_E4M3 1
+
+/* Append rows: k, v (B,Hkv,n,D) f32/f16/bf16 (one dtype, any strides with a unit innermost one); the first
+ * counts[b] of them (device int32, clamped to [0, n]; NULL: n) go to rows lens[b] .. of sequence b.
+ * Per touched block: scale' = max(scale, amax * (1/M)), amax the largest finite |value| of the block's
+ * new rows, M the largest code and 1/M its f32 reciprocal, `scale` only if the block held rows; where that grew the rows held are
+ * requantised, code' = Q((code * scale) / scale'); new codes are Q(x / scale'). Every step is one
+ * correctly rounded f32 operation; Q rounds to nearest even and saturates; NaN becomes code 0 and a
+ * zero scale gives zero codes. With advance != 0 a second kernel sets lens[b] = min(lens[b] + counts[b],
+ * Smax). Rows that would land past Smax are dropped and leave status 61 (gtb_device_status). */
+GTB_API int gtb_kv8_append(const gtb_kv8 *cache, const gtb_tensor4 *k, const gtb_tensor4 *v, const int32_t *counts,
+                           int advance, void *stream);
+
+/* Rows start[b] .. start[b] + n - 1 of every head as values: k_out, v_out (B,Hkv,n,D) contiguous
+ * f32/f16/bf16, code * scale rounded once. lens is not consulted (stored rows come back as they are);
+ * rows outside [0, Smax) give 0. start: device int32 (B) or NULL (0). */
+GTB_API int gtb_kv8_read(const gtb_kv8 *cache, const int32_t *start, gtb_tensor4 *k_out, gtb_tensor4 *v_out, void *stream);
+
+/* Attention of q (B,H,Lq,D), H % Hkv == 0, over the cache: the queries are the last counts[b] (device int32,
+ * clamped to [0, Lq]; NULL: Lq) of the lens[b] tokens cached, query i < counts[b] attending rows
+ * s <= lens[b] - counts[b] + i. A query at or past counts[b], or with no row to attend, gives 0 and lse -inf.
+ *   q f32/f16/bf16, any strides with a unit innermost one; out (B,H,Lq,D) in q's dtype, contiguous;
+ *   lse NULL or (B,H,Lq) f32; scale <= 0 means 1/sqrt(D).
+ *   score_out NULL, or (B,Hkv,Smax) f32 that receives score_in (same shape, may be score_out itself) + the
+ *   attention weight each row s < lens[b] got, summed over the kv head's query heads and all queries; other
+ *   entries are not written. The sums run in a fixed order: the same bits on every run.
+ * Scratch comes from the stream-ordered allocator. */
+GTB_API int gtb_kv8_attention(const gtb_tensor4 *q, const gtb_kv8 *cache, float scale, const int32_t *counts,
+                              const float *score_in, float *score_out, gtb_tensor4 *out, float *lse, void *stream);
+
+/* Eviction by accumulated attention weight, from src into dst (same B, Hkv, D, format; dst.Smax >= budget; the two
+ * share no memory): of each (sequence, kv head) with more than `budget` rows the last `recent` and, of the
+ * rows before those, the budget - recent of largest score (score (B,Hkv,src.Smax) f32; NaN counts as
+ * -inf, ties go to the lowest row) are kept, in their order; a sequence of at most `budget` rows is kept whole. dst's
+ * blocks get scale' = amax * (1/M) over their kept rows' values and codes Q((code * scale) / scale'), as an
+ * append to an empty cache would; dst.lens = min(lens, budget). kept: (B,Hkv,budget) int32, the source row of
+ * each kept row, -1 past the length. score_out: NULL or (B,Hkv,dst.Smax) f32, the kept rows' scores, 0 for
+ * rows from there up to dst.Smax. 0 <= recent <= budget, 1 <= budget. */
+GTB_API int gtb_kv8_evict(const gtb_kv8 *src, const float *score, int64_t budget, int64_t recent, const gtb_kv8 *dst,
+                          float *score_out, int32_t *kept, void *stream);
+
 /* Kernel family of the calling thread's last gtb_sdpa_fwd / gtb_sdpa_fwd_rope / gtb_sdpa_bwd call:
  * "tcgen05" (tensor cores, TMA), "tcgen05+rope" (the same with q rotated inside the kernel),
  * "f32_tiled" (fp32 with head size 64, register-blocked on the CUDA cores) or "simt" (one warp per
