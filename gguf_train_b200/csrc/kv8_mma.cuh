@@ -1,0 +1,688 @@
+// Attention over the block-scaled 8-bit cache for few query rows, on warp-level matrix instructions.
+//
+// One work item is 8 * NT query rows of one (sequence, kv head): the G = H / Hkv query heads times the Lq
+// queries, row = i * G + g. The keys are cut into units of 32; all units of all items form one line, of which
+// every warp takes an equal stretch (so the split adapts to the lengths and no warp waits for another). A
+// warp that finishes an item alone writes the result; otherwise it leaves (out, max, sum) for
+// kv8_combine_kernel.
+//
+// A warp streams its units through its own ring in shared memory with 16-byte asynchronous copies (rows
+// past the length arrive as zeros: nothing stored there can reach a result). Codes become f16 in registers,
+// exactly (int8 and e4m3 both fit), and feed mma.m16n8k16 as the A operand:
+//   S^T (16 keys x 8 rows) = K (keys x D) Q^T;   O^T (16 dims x 8 rows) += V^T (dims x keys) P^T.
+// The dimensions (first product) and keys (second) of an operand may be taken in any order as long as both
+// operands agree, so a thread reads 16 consecutive bytes of a row and calls them the elements its lane owns;
+// only P^T has to change layout (movmatrix, two per 16 keys and 8 rows).
+// * Scales: K's block scale multiplies the scores. V's is folded into the exponent, P' = 2^(s + log2 sv - M), so
+//   the second product accumulates across blocks without rescaling; the row sum takes P' / sv. sv below
+//   2^-100 counts as 2^-100.
+// * q becomes f16 after a power of two per row brings its largest value to [1, 2): bf16's 8 bits fit, and what
+//   falls below f16's smallest step is 2^-24 of that value. f32 q is split into two f16 numbers (NS = 2), and
+//   so is P', which is otherwise rounded to f16 once.
+// * M is raised only when a score exceeds it by 2^7 (P' carries a factor 2^8 and f16 ends at 2^16), so most
+//   units need neither shuffles nor a rescaling of O.
+#pragma once
+
+#include "gtb_common.cuh"
+#include "kv8.cuh"
+
+namespace gtb {
+namespace kv8 {
+
+constexpr int UNIT = 32;        // keys per unit
+constexpr float SV_MIN = 7.888609052210118e-31f;  // 2^-100
+constexpr float RAISE = 7.0f, SHIFT = 8.0f;
+
+struct MmaP {
+    gtb_kv8 c;
+    Rows3 q, o;
+    int dtype;
+    int G, R, row_tiles;      // R = G * Lq rows per (b, hk), in tiles of 8 * NT
+    int64_t H, Lq;
+    float scale_log2;         // scale * log2(e)
+    const int32_t* counts;
+    float* lse;               // nullable
+    int2* meta;               // per item: first and last warp that holds a part of it
+    float* part_o;            // [slot][8 NT][DP]
+    float2* part_ml;          // [slot][8 NT]
+    float* s_out;             // nullable: scores (log2 units) [b, hk][key][R]
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
+    const int n = live ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool live) {
+    const int n = live ? 4 : 0;
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2f(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<__half2*>(&x)); }
+
+// The four codes of a word as two f16 pairs: bytes (0, 1) and (2, 3). int8: with the sign bit flipped a code is
+// an unsigned byte u = q + 128, the bits 0x6400 | u are the f16 number 1024 + u, and 1152 comes off exactly.
+template <int FMT>
+__device__ __forceinline__ uint32_t prep_word(uint32_t w) {
+    return FMT == GTB_KV8_INT8 ? w ^ 0x80808080u : w;
+}
+template <int FMT, int HALF>
+__device__ __forceinline__ uint32_t expand(uint32_t w) {
+    if constexpr (FMT == GTB_KV8_INT8) {
+        const uint32_t t = __byte_perm(w, 0x64646464u, HALF ? 0x4342 : 0x4140);
+        const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&t), __half2half2(__ushort_as_half(0xE480)));  // -1152
+        return *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        uint32_t r;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)(HALF ? w >> 16 : w)));
+        return r;
+    }
+}
+
+// Which bytes a lane (g = lane / 4, t = lane % 4) owns. K: for load q, 16 bytes of row g: chunk k_chunk(t, q).
+// V: of its four keys (2t, 2t+1, 8+2t, 9+2t in the 16), V_BYTES bytes from v_byte(g, u). Rows of 16-byte chunks
+// are stored with chunk c of row r at c ^ swz(r), keys at row krow(key), chosen so that the eight lanes of a
+// 16-byte access (sixteen of an 8-byte one) fall into different banks for both reads.
+template <int DP>
+struct Lay;
+template <>
+struct Lay<64> {
+    static constexpr int KL = 1, VL = 1, V_BYTES = 8;
+    __device__ static int k_chunk(int t, int) { return t; }
+    __device__ static int v_byte(int g, int) { return 8 * g; }
+    __device__ static int krow(int k) { return k ^ ((k >> 1) & 1); }
+    __device__ static int swz(int r) { return ((r >> 2) & 1) << 1; }
+};
+template <>
+struct Lay<128> {
+    static constexpr int KL = 2, VL = 1, V_BYTES = 16;
+    __device__ static int k_chunk(int t, int q) { return 2 * t + q; }
+    __device__ static int v_byte(int g, int) { return 16 * g; }
+    __device__ static int krow(int k) { return k; }
+    __device__ static int swz(int r) { return r & 7; }
+};
+template <>
+struct Lay<256> {
+    static constexpr int KL = 4, VL = 2, V_BYTES = 16;
+    __device__ static int k_chunk(int t, int q) { return t + 4 * q; }
+    __device__ static int v_byte(int g, int u) { return 16 * g + 128 * u; }
+    __device__ static int krow(int k) { return k; }
+    __device__ static int swz(int r) { return (r & 6) ^ ((r & 1) << 2); }
+};
+
+template <int DP, int NT, int NS>
+struct MmaCfg {
+    static constexpr bool QREG = NT * NS == 1;
+    static constexpr int KSTEPS = DP / 16;
+    static constexpr int STAGE = 2 * UNIT * DP + 16;  // K rows, V rows, scales k0 k1 v0 v1
+    static constexpr int QBYTES = QREG ? 0 : KSTEPS * NT * NS * 32 * 8;
+    static constexpr int WARPS = DP == 256 ? 4 : NT * NS == 8 ? 6 : 8;
+    // as many stages as fit beside each other, 6 at most
+    static constexpr int FIT = (224 * 1024 / WARPS - QBYTES) / STAGE;
+    static constexpr int STAGES = FIT > 6 ? 6 : FIT;
+    static_assert(STAGES >= 2, "a stage in work and one in flight");
+    static constexpr int WARP_SMEM = STAGES * STAGE + QBYTES;
+    static constexpr int SMEM = WARPS * WARP_SMEM;
+};
+
+// One query row's value d as f32, any type
+__device__ __forceinline__ float load_q(const MmaP& p, const void* row, int d) { return load_any<float>(row, d, p.dtype); }
+
+template <int DP, int FMT, int NT, int NS>
+__global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_kernel(const MmaP p) {
+    using C = MmaCfg<DP, NT, NS>;
+    using L = Lay<DP>;
+    constexpr int ROWS = 8 * NT, OM = DP / 16;  // OM: products of 16 dims
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int64_t seg[C::WARPS * 32 + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const gtb_kv8& c = p.c;
+    const int per_seq = (int)c.Hkv * p.row_tiles;
+
+    auto len_of = [&](int64_t b) { return (int)clamp64(c.lens[b], 0, c.Smax); };
+    auto units_of = [&](int64_t b) { return (int64_t)max(1, (len_of(b) + UNIT - 1) / UNIT); };
+
+    // units before each thread's share of the sequences
+    const int64_t share = (c.B + blockDim.x - 1) / blockDim.x;
+    {
+        int64_t n = 0;
+        for (int64_t b = threadIdx.x * share; b < min(c.B, (threadIdx.x + 1) * share); ++b) n += units_of(b);
+        int64_t x = n;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __shared__ int64_t wsum[C::WARPS];
+        if (lane == 31) wsum[warp] = x;
+        __syncthreads();
+        int64_t before = 0;
+        for (int w = 0; w < warp; ++w) before += wsum[w];
+        seg[threadIdx.x + 1] = (before + x) * per_seq;
+        if (threadIdx.x == 0) seg[0] = 0;
+        __syncthreads();
+    }
+    const int64_t U = seg[blockDim.x];
+    // no more warps than units, so that every warp below NW has some; neighbours in different CTAs
+    const int64_t NW = min((int64_t)gridDim.x * C::WARPS, U);
+    const int64_t wid = (int64_t)warp * gridDim.x + blockIdx.x;
+    if (wid >= NW) return;
+    const int64_t u0 = wid * U / NW, u1 = (wid + 1) * U / NW;
+
+    // the sequence and item of unit u0
+    int lo = 0, hi = blockDim.x;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (seg[mid] <= u0) lo = mid;
+        else hi = mid;
+    }
+    int64_t b = lo * share, base = seg[lo];
+    for (;;) {
+        const int64_t n = units_of(b) * per_seq;
+        if (base + n > u0) break;
+        base += n;
+        ++b;
+    }
+    // state of the unit to load next and of the unit to work on next: sequence, item in it, unit in the item
+    struct Cursor {
+        int64_t b;
+        int len, units, item, unit;
+    };
+    Cursor ld;
+    ld.b = b;
+    ld.len = len_of(b);
+    ld.units = (int)units_of(b);
+    ld.item = (int)((u0 - base) / ld.units);
+    ld.unit = (int)((u0 - base) - (int64_t)ld.item * ld.units);
+    Cursor wk = ld;
+    auto advance = [&](Cursor& k) {
+        if (++k.unit == k.units) {
+            k.unit = 0;
+            if (++k.item == per_seq) {
+                k.item = 0;
+                if (++k.b < c.B) {
+                    k.len = len_of(k.b);
+                    k.units = max(1, (k.len + UNIT - 1) / UNIT);
+                }
+            }
+        }
+    };
+
+    unsigned char* ws = smem + warp * C::WARP_SMEM;
+    const uint32_t ring = smem_addr(ws);
+    uint2* qf = (uint2*)(ws + C::STAGES * C::STAGE);
+    const int chunks = (int)c.D / 16;
+    const int64_t nblk = (c.Smax + c.block - 1) / c.block;
+
+    auto issue = [&](int stage) {  // copies of unit `ld` into a stage
+        const int64_t bh = ld.b * c.Hkv + ld.item / p.row_tiles;
+        const int k0 = ld.unit * UNIT;
+        const unsigned char* gk = (const unsigned char*)c.k + (bh * c.Smax + k0) * c.D;
+        const unsigned char* gv = (const unsigned char*)c.v + (bh * c.Smax + k0) * c.D;
+        const uint32_t dst = ring + stage * C::STAGE;
+        constexpr int CPR = DP / 16;              // chunks per stored row
+        constexpr int RPI = 32 / (CPR > 32 ? 32 : CPR);  // rows per warp instruction
+        const int cc = lane % CPR;
+#pragma unroll
+        for (int r0 = 0; r0 < UNIT; r0 += RPI) {
+            const int key = r0 + lane / CPR;
+            const bool live = k0 + key < ld.len && cc < chunks;
+            const int row = (key & ~7) | L::krow(key & 7);
+            const uint32_t at = dst + row * DP + ((cc ^ L::swz(row & 7)) << 4);
+            const int64_t off = live ? (int64_t)key * c.D + cc * 16 : 0;
+            cp16(at, live ? gk + off : (const unsigned char*)c.k, live);
+            cp16(at + UNIT * DP, live ? gv + off : (const unsigned char*)c.v, live);
+        }
+        if (lane < 4) {
+            const int k = k0 + (lane & 1) * 16;
+            const bool live = k < ld.len;
+            const float* s = lane < 2 ? c.k_scale : c.v_scale;
+            cp4(dst + 2 * UNIT * DP + lane * 4, live ? s + bh * nblk + k / c.block : s, live);
+        }
+    };
+
+    const int n_units = (int)(u1 - u0);
+#pragma unroll
+    for (int s = 0; s < C::STAGES - 1; ++s) {
+        if (s < n_units) {
+            issue(s);
+            advance(ld);
+        }
+        cp_commit();
+    }
+
+    // state of the current item
+    float o[NT][OM][4];
+    float M[NT][2], l[NT][2], qmul[NT][2];
+    int lim[NT][2];                  // keys each row may attend
+    int lim_min = 0;                 // smallest over the tile's rows
+    uint32_t qr[C::QREG ? C::KSTEPS : 1][2];
+    bool fresh = true, head_split = wk.unit != 0;
+
+    int stage = 0;
+    for (int it = 0; it < n_units; ++it) {
+        const int hk = wk.item / p.row_tiles, tile = wk.item - hk * p.row_tiles;
+        if (fresh) {  // a new item: its query rows, normalised by a power of two, as B operands
+            fresh = false;
+            const int cnt = p.counts ? (int)clamp64(p.counts[wk.b], 0, p.Lq) : (int)p.Lq;
+            float row_mul[NT];  // of row g of each group
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int r = tile * ROWS + n * 8 + g;
+                const int i = r / p.G, h = hk * p.G + (r - i * p.G);
+                const size_t es = p.dtype == F32 ? 4 : 2;
+                const unsigned char* row = (const unsigned char*)p.q.p + (wk.b * p.q.sb + h * p.q.sh + i * p.q.ss) * (int64_t)es;
+                float x[C::KSTEPS][4], m = 0.0f;
+#pragma unroll
+                for (int q = 0; q < L::KL; ++q)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int d = L::k_chunk(t, q) * 16 + w * 4;
+                        const bool live = r < p.R && d < c.D;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float v = live ? load_q(p, row, d + e) : 0.0f;
+                            x[q * 4 + w][e] = v;
+                            m = fmaxf(m, finite_abs(v));
+                        }
+                    }
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                // 2^e <= m < 2^(e+1); a row of zeros or subnormals stays as it is
+                int e = (int)(__float_as_uint(m) >> 23) - 127;
+                e = m >= 1.17549435e-38f ? min(max(e, -126), 126) : 0;
+                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                row_mul[n] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+#pragma unroll
+                for (int k = 0; k < C::KSTEPS; ++k) {
+                    const float y0 = x[k][0] * down, y1 = x[k][1] * down, y2 = x[k][2] * down, y3 = x[k][3] * down;
+                    const uint32_t b0 = pack_f16(y0, y1), b1 = pack_f16(y2, y3);
+                    if constexpr (C::QREG) {
+                        qr[k][0] = b0;
+                        qr[k][1] = b1;
+                    } else {
+                        qf[((k * NT + n) * NS) * 32 + lane] = make_uint2(b0, b1);
+                        if constexpr (NS == 2) {
+                            const float2 f0 = unpack_f16(b0), f1 = unpack_f16(b1);
+                            qf[((k * NT + n) * NS + 1) * 32 + lane] = make_uint2(pack_f16(y0 - f0.x, y1 - f0.y), pack_f16(y2 - f1.x, y3 - f1.y));
+                        }
+                    }
+                }
+            }
+            lim_min = 1 << 30;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    qmul[n][e] = __shfl_sync(0xffffffffu, row_mul[n], (2 * t + e) * 4);
+                    const int r = tile * ROWS + n * 8 + 2 * t + e, i = r / p.G;
+                    lim[n][e] = r < p.R && i < cnt ? max(0, wk.len - cnt + i + 1) : 0;
+                    if (r < p.R) lim_min = min(lim_min, lim[n][e]);
+                    M[n][e] = -INFINITY;
+                    l[n][e] = 0.0f;
+                }
+#pragma unroll
+                for (int j = 0; j < OM; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][j][e] = 0.0f;
+            }
+            lim_min = __reduce_min_sync(0xffffffffu, lim_min);
+            __syncwarp();
+        }
+
+        if (it + C::STAGES - 1 < n_units) {
+            issue(stage + C::STAGES - 1 >= C::STAGES ? stage - 1 : stage + C::STAGES - 1);
+            advance(ld);
+        }
+        cp_commit();
+        cp_wait<C::STAGES - 1>();
+        __syncwarp();
+
+        const unsigned char* kt = ws + stage * C::STAGE;
+        const unsigned char* vt = kt + UNIT * DP;
+        const float4 sc = *(const float4*)(kt + 2 * UNIT * DP);
+        const float sk[2] = {sc.x, sc.y};
+        const float sv[2] = {fmaxf(sc.z, SV_MIN), fmaxf(sc.w, SV_MIN)};
+        const int k0 = wk.unit * UNIT;
+
+        // S^T of the unit's 32 keys
+        float s[2][NT][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[u][n][e] = 0.0f;
+            const int r = L::krow(g);
+            const unsigned char* ra = kt + (u * 16 + r) * DP;
+            const unsigned char* rb = ra + 8 * DP;
+#pragma unroll
+            for (int q = 0; q < L::KL; ++q) {
+                const int at = (L::k_chunk(t, q) ^ L::swz(r)) << 4;
+                const uint4 wa = *(const uint4*)(ra + at), wb = *(const uint4*)(rb + at);
+                const uint32_t xa[4] = {wa.x, wa.y, wa.z, wa.w}, xb[4] = {wb.x, wb.y, wb.z, wb.w};
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t ya = prep_word<FMT>(xa[w]), yb = prep_word<FMT>(xb[w]);
+                    const uint32_t a[4] = {expand<FMT, 0>(ya), expand<FMT, 0>(yb), expand<FMT, 1>(ya), expand<FMT, 1>(yb)};
+                    const int k = q * 4 + w;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        if constexpr (C::QREG) {
+                            mma16816(s[u][n], a, qr[k][0], qr[k][1]);
+                        } else {
+#pragma unroll
+                            for (int z = 0; z < NS; ++z) {
+                                const uint2 bq = qf[((k * NT + n) * NS + z) * 32 + lane];
+                                mma16816(s[u][n], a, bq.x, bq.y);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        // to log2 units, masked; scores out where the weights are wanted
+        const bool edge = k0 + UNIT > lim_min;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = s[u][n][e] * (qmul[n][e & 1] * sk[u]);
+                    if (edge && k0 + u * 16 + g + (e >> 1) * 8 >= lim[n][e & 1]) x = -INFINITY;
+                    s[u][n][e] = x;
+                }
+        if (p.s_out) {
+            const int64_t bh = wk.b * c.Hkv + hk;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = k0 + u * 16 + g + (e >> 1) * 8, r = tile * ROWS + n * 8 + 2 * t + (e & 1);
+                        if (key < wk.len && r < p.R) p.s_out[(bh * c.Smax + key) * p.R + r] = s[u][n][e];
+                    }
+        }
+        const float lsv[2] = {lg2f(sv[0]), lg2f(sv[1])};
+        bool raise = false;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[u][n][e] += lsv[u];
+                    raise |= s[u][n][e] > M[n][e & 1] + RAISE;
+                }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float corr[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float m = fmaxf(fmaxf(s[0][n][e], s[0][n][e + 2]), fmaxf(s[1][n][e], s[1][n][e + 2]));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    m = fmaxf(m, M[n][e]);
+                    corr[e] = m > M[n][e] ? ex2f(M[n][e] - m) : 1.0f;
+                    M[n][e] = m;
+                    l[n][e] *= corr[e];
+                }
+#pragma unroll
+                for (int j = 0; j < OM; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[n][j][e] *= corr[e & 1];
+            }
+        }
+        uint32_t pb[2][NT][NS][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float ref[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) ref[e] = M[n][e] == -INFINITY ? 0.0f : M[n][e] - SHIFT;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = ex2f(s[u][n][e] - ref[e & 1]);
+                const float inv = __frcp_rn(sv[u]);
+                l[n][0] = fmaf(x[0] + x[2], inv, l[n][0]);
+                l[n][1] = fmaf(x[1] + x[3], inv, l[n][1]);
+                const uint32_t h0 = pack_f16(x[0], x[1]), h1 = pack_f16(x[2], x[3]);
+                pb[u][n][0][0] = transpose8x8(h0);
+                pb[u][n][0][1] = transpose8x8(h1);
+                if constexpr (NS == 2) {
+                    const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
+                    pb[u][n][NS - 1][0] = transpose8x8(pack_f16(x[0] - f0.x, x[1] - f0.y));
+                    pb[u][n][NS - 1][1] = transpose8x8(pack_f16(x[2] - f1.x, x[3] - f1.y));
+                }
+            }
+        }
+        // O^T += V^T P^T
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int vl = 0; vl < L::VL; ++vl) {
+                constexpr int WORDS = L::V_BYTES / 4;
+                uint32_t x[4][WORDS];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int key = 2 * t + (k & 1), r = L::krow(key);  // rows r and r + 8 of the 16
+                    const int by = L::v_byte(g, vl);
+                    const unsigned char* at = vt + (u * 16 + (k >> 1) * 8 + r) * DP + (((by >> 4) ^ L::swz(r)) << 4) + (by & 15);
+                    if constexpr (WORDS == 4) {
+                        const uint4 w = *(const uint4*)at;
+                        x[k][0] = prep_word<FMT>(w.x); x[k][1] = prep_word<FMT>(w.y);
+                        x[k][2] = prep_word<FMT>(w.z); x[k][3] = prep_word<FMT>(w.w);
+                    } else {
+                        const uint2 w = *(const uint2*)at;
+                        x[k][0] = prep_word<FMT>(w.x); x[k][1] = prep_word<FMT>(w.y);
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) {
+                    const uint32_t a01 = __byte_perm(x[0][w], x[1][w], 0x5140), a23 = __byte_perm(x[0][w], x[1][w], 0x7362);
+                    const uint32_t c01 = __byte_perm(x[2][w], x[3][w], 0x5140), c23 = __byte_perm(x[2][w], x[3][w], 0x7362);
+                    const uint32_t f0[4] = {expand<FMT, 0>(a01), expand<FMT, 1>(a01), expand<FMT, 0>(c01), expand<FMT, 1>(c01)};
+                    const uint32_t f1[4] = {expand<FMT, 0>(a23), expand<FMT, 1>(a23), expand<FMT, 0>(c23), expand<FMT, 1>(c23)};
+                    const int j = (vl * WORDS + w) * 2;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int z = 0; z < NS; ++z) {
+                            mma16816(o[n][j], f0, pb[u][n][z][0], pb[u][n][z][1]);
+                            mma16816(o[n][j + 1], f1, pb[u][n][z][0], pb[u][n][z][1]);
+                        }
+                }
+            }
+        }
+        __syncwarp();  // every lane has read this stage before it is copied over
+        stage = stage + 1 == C::STAGES ? 0 : stage + 1;
+
+        const bool item_done = wk.unit + 1 == wk.units, last = it + 1 == n_units;
+        if (item_done || last) {
+            const bool whole = item_done && !head_split;
+            const int64_t item = wk.b * per_seq + wk.item;
+            if (!head_split && lane == 0) {
+                // the warp of the item's last unit: the one whose stretch holds it
+                const int64_t end = u0 + it + (wk.units - 1 - wk.unit);
+                const int64_t last_warp = ((end + 1) * NW - 1) / U;
+                p.meta[item] = make_int2((int)wid, (int)last_warp);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = l[n][e];
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    l[n][e] = x;
+                    const int r = n * 8 + 2 * t + e, gr = tile * ROWS + r;
+                    if (gr >= p.R) continue;
+                    const float m = M[n][e] == -INFINITY ? 0.0f : M[n][e] - SHIFT;
+                    if (whole) {
+                        const float inv = x > 0.0f || !(x == x) ? 1.0f / x : 0.0f;
+                        const int i = gr / p.G, h = hk * p.G + (gr - i * p.G);
+                        const size_t es = p.dtype == F32 ? 4 : 2;
+                        unsigned char* dst = (unsigned char*)p.o.p + (wk.b * p.o.sb + h * p.o.sh + (int64_t)i * p.o.ss) * (int64_t)es;
+#pragma unroll
+                        for (int vl = 0; vl < L::VL; ++vl) {
+                            const int d0 = L::v_byte(g, vl);
+                            if (d0 >= c.D) continue;
+#pragma unroll
+                            for (int k = 0; k < L::V_BYTES; k += 2) {
+                                const int j = (vl * L::V_BYTES + k) / 2;
+                                const float y0 = o[n][j][e] * inv, y1 = o[n][j][e + 2] * inv;
+                                if (p.dtype == F32) *(float2*)((float*)dst + d0 + k) = make_float2(y0, y1);
+                                else if (p.dtype == F16) *(__half2*)((__half*)dst + d0 + k) = __floats2half2_rn(y0, y1);
+                                else *(__nv_bfloat162*)((__nv_bfloat16*)dst + d0 + k) = __floats2bfloat162_rn(y0, y1);
+                            }
+                        }
+                        if (p.lse && g == 0)
+                            p.lse[(wk.b * p.H + h) * p.Lq + i] = M[n][e] == -INFINITY ? -INFINITY : (m + log2f(x)) * 0.6931471805599453f;
+                    } else {
+                        const int64_t slot = 2 * wid + (head_split ? 0 : 1);
+                        float* dst = p.part_o + (slot * ROWS + r) * DP;
+#pragma unroll
+                        for (int vl = 0; vl < L::VL; ++vl) {
+                            const int d0 = L::v_byte(g, vl);
+#pragma unroll
+                            for (int k = 0; k < L::V_BYTES; k += 2) {
+                                const int j = (vl * L::V_BYTES + k) / 2;
+                                *(float2*)(dst + d0 + k) = make_float2(o[n][j][e], o[n][j][e + 2]);
+                            }
+                        }
+                        if (g == 0) p.part_ml[slot * ROWS + r] = make_float2(M[n][e] == -INFINITY ? -INFINITY : m, x);
+                    }
+                }
+            fresh = true;
+            head_split = false;
+        }
+        advance(wk);
+    }
+    cp_wait<0>();
+}
+
+// Joins the parts of the items that more than one warp worked on: one warp per (item, row)
+template <int DP>
+__global__ void __launch_bounds__(128) kv8_combine_kernel(const MmaP p, int rows_per_tile, int64_t n_items) {
+    const int lane = threadIdx.x & 31;
+    const int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int64_t item = w / rows_per_tile;
+    const int r = (int)(w - item * rows_per_tile);
+    if (item >= n_items) return;
+    const int per_seq = (int)p.c.Hkv * p.row_tiles;
+    const int64_t b = item / per_seq;
+    const int rest = (int)(item - b * per_seq), hk = rest / p.row_tiles, tile = rest - hk * p.row_tiles;
+    const int gr = tile * rows_per_tile + r;
+    if (gr >= p.R) return;
+    const int2 range = p.meta[item];
+    if (range.x == range.y) return;
+    constexpr int PER = DP / 32;
+    float acc[PER] = {}, m = -INFINITY, l = 0.0f;
+    for (int k = range.x; k <= range.y; ++k) {
+        const int64_t slot = 2 * (int64_t)k + (k == range.x ? 1 : 0);
+        const float2 ml = p.part_ml[slot * rows_per_tile + r];
+        float x[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[i] = p.part_o[(slot * rows_per_tile + r) * DP + i * 32 + lane];
+        const float m2 = fmaxf(m, ml.x);
+        const float ca = m == -INFINITY ? 0.0f : ex2f(m - m2), cb = ml.x == -INFINITY ? 0.0f : ex2f(ml.x - m2);
+        l = l * ca + ml.y * cb;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) acc[i] = acc[i] * ca + x[i] * cb;
+        m = m2;
+    }
+    const float inv = l > 0.0f || !(l == l) ? 1.0f / l : 0.0f;
+    const int i = gr / p.G, h = hk * p.G + (gr - i * p.G);
+    const int64_t at = b * p.o.sb + h * p.o.sh + (int64_t)i * p.o.ss;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+        const int d = k * 32 + lane;
+        if (d >= p.c.D) continue;
+        const float y = acc[k] * inv;
+        if (p.dtype == F32) ((float*)p.o.p)[at + d] = y;
+        else if (p.dtype == F16) ((__half*)p.o.p)[at + d] = __float2half_rn(y);
+        else ((__nv_bfloat16*)p.o.p)[at + d] = __float2bfloat16_rn(y);
+    }
+    if (p.lse && lane == 0) p.lse[(b * p.H + h) * p.Lq + i] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <int DP, int FMT, int NT, int NS>
+int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
+    using C = MmaCfg<DP, NT, NS>;
+    auto kern = kv8_mma_kernel<DP, FMT, NT, NS>;
+    if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM), "kv8_attention: shared memory"))
+        return -1;
+    p.row_tiles = (p.R + 8 * NT - 1) / (8 * NT);
+    const int64_t items = p.c.B * p.c.Hkv * p.row_tiles;
+    const int64_t warps = (int64_t)n_sm * C::WARPS;
+    const size_t slots = 2 * (size_t)warps * 8 * NT;
+    const size_t meta_bytes = ((size_t)items * sizeof(int2) + 255) & ~(size_t)255;
+    const size_t bytes = meta_bytes + slots * (sizeof(float2) + DP * sizeof(float));
+    void* scratch = nullptr;
+    if (cuda_failed(cudaMallocAsync(&scratch, bytes, st), "kv8_attention: scratch allocation")) return -1;
+    p.meta = (int2*)scratch;
+    p.part_o = (float*)((char*)scratch + meta_bytes);
+    p.part_ml = (float2*)(p.part_o + slots * DP);
+    kern<<<n_sm, C::WARPS * 32, C::SMEM, st>>>(p);
+    bool bad = cuda_failed(cudaGetLastError(), "kv8_attention launch");
+    if (!bad) {
+        const int64_t n = items * 8 * NT;
+        kv8_combine_kernel<DP><<<(unsigned)((n + 3) / 4), 128, 0, st>>>(p, 8 * NT, items);
+        bad = cuda_failed(cudaGetLastError(), "kv8_attention: combine launch");
+    }
+    cudaFreeAsync(scratch, st);
+    return bad ? -1 : 0;
+}
+
+template <int DP, int FMT>
+int launch_mma_rows(const MmaP& p, int n_sm, cudaStream_t st) {
+    const bool wide = p.dtype == F32;
+    if (p.R <= 8) return wide ? launch_mma<DP, FMT, 1, 2>(p, n_sm, st) : launch_mma<DP, FMT, 1, 1>(p, n_sm, st);
+    if (p.R <= 16 || DP == 256) return wide ? launch_mma<DP, FMT, 2, 2>(p, n_sm, st) : launch_mma<DP, FMT, 2, 1>(p, n_sm, st);
+    if constexpr (DP < 256) return wide ? launch_mma<DP, FMT, 4, 2>(p, n_sm, st) : launch_mma<DP, FMT, 4, 1>(p, n_sm, st);
+    return -1;
+}
+
+int launch_mma_64(const MmaP& p, int n_sm, cudaStream_t st);
+int launch_mma_128(const MmaP& p, int n_sm, cudaStream_t st);
+int launch_mma_256(const MmaP& p, int n_sm, cudaStream_t st);
+
+}  // namespace kv8
+}  // namespace gtb
