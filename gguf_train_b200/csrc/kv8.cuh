@@ -48,12 +48,91 @@ __device__ __forceinline__ float scale_of(float amax) {
 
 // The code of x at scale s: round(x / s), saturating; 0 for NaN and for a zero scale
 template <int FMT>
-__device__ __forceinline__ uint8_t quantise8(float x, float s) {
+__device__ __noinline__ uint8_t quantise8(float x, float s) {
     if (!(s > 0.0f)) return 0;
     float y = __fdiv_rn(x, s);
     if (!(y == y)) return 0;
     y = fminf(fmaxf(y, -Code8<FMT>::TOP), Code8<FMT>::TOP);
     return Code8<FMT>::nearest(y);
+}
+
+// The same codes without a division each: x * (1 / s) is within a few ulp of the quotient, so it rounds to the
+// same code unless it lies that close to the middle between two; those (one in some thousands) and anything
+// not finite take quantise8. Scales near either end of f32 take it throughout.
+struct Quantiser {
+    float s, inv;
+    bool plain;
+    __device__ explicit Quantiser(float scale) : s(scale), inv(0.0f), plain(!(scale > 1e-30f && scale < 1e30f)) {
+        if (!plain) inv = __frcp_rn(scale);
+    }
+};
+
+template <int FMT>
+__device__ __forceinline__ uint32_t quantise8x4(const float* x, const Quantiser& z) {
+    if (!z.plain) {
+        const float y0 = x[0] * z.inv, y1 = x[1] * z.inv, y2 = x[2] * z.inv, y3 = x[3] * z.inv;
+        if constexpr (FMT == GTB_KV8_INT8) {
+            constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the nearest integer's
+            const float r0 = y0 + MAGIC, r1 = y1 + MAGIC, r2 = y2 + MAGIC, r3 = y3 + MAGIC;
+            const float d = fmaxf(fmaxf(fabsf(y0 - (r0 - MAGIC)), fabsf(y1 - (r1 - MAGIC))),
+                                  fmaxf(fabsf(y2 - (r2 - MAGIC)), fabsf(y3 - (r3 - MAGIC))));
+            const float top = fmaxf(fmaxf(fabsf(y0), fabsf(y1)), fmaxf(fabsf(y2), fabsf(y3)));
+            // (fmaxf drops a NaN, so the sum asks for one)
+            if (d < 0.4999f && top < 127.4f && y0 + y1 + y2 + y3 == y0 + y1 + y2 + y3) {
+                const uint32_t lo = __byte_perm(__float_as_uint(r0), __float_as_uint(r1), 0x0040);
+                const uint32_t hi = __byte_perm(__float_as_uint(r2), __float_as_uint(r3), 0x0040);
+                return __byte_perm(lo, hi, 0x5410);
+            }
+        } else {
+            constexpr float UP = 1.0f + 0x1p-21f, DOWN = 1.0f - 0x1p-21f;
+            uint16_t a0, a1, b0, b1;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a0) : "f"(y1 * DOWN), "f"(y0 * DOWN));
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a1) : "f"(y3 * DOWN), "f"(y2 * DOWN));
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b0) : "f"(y1 * UP), "f"(y0 * UP));
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b1) : "f"(y3 * UP), "f"(y2 * UP));
+            const float sum = y0 + y1 + y2 + y3;
+            if (a0 == b0 && a1 == b1 && sum - sum == 0.0f) return (uint32_t)a0 | ((uint32_t)a1 << 16);
+        }
+    }
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r |= (uint32_t)quantise8<FMT>(x[i], z.s) << (8 * i);
+    return r;
+}
+
+// The four codes of a word as f32 values
+template <int FMT>
+__device__ __forceinline__ void values8x4(uint32_t w, float* x) {
+    if constexpr (FMT == GTB_KV8_INT8) {
+        const uint32_t u = w ^ 0x80808080u;  // code + 128 as a byte; 0x4B000000 | byte is 2^23 + byte
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + i)) - 8388736.0f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t h;
+            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)(w >> (16 * i))));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+}
+
+// Launch that may start while the stream's previous kernel still runs: the kernel itself waits for that one's
+// results with cudaGridDependencySynchronize(), in every thread, before it touches anything.
+template <typename... P, typename... A>
+bool launch_behind(const char* ctx, void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return !cuda_failed(cudaLaunchKernelEx(&cfg, kern, P(args)...), ctx);
 }
 
 __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }

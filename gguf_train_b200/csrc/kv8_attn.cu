@@ -80,7 +80,7 @@ int launch_score(const Kv8AttnArgs& a, const float* lse, cudaStream_t st) {
 
 int launch_kv8_attention(const Kv8AttnArgs& a, cudaStream_t st) {
     const int64_t rows = a.c.B * a.H * a.Lq;
-    int dev = 0, n_sm = 0;
+    int dev = 0, n_sm = 0;  // (reading an attribute is a look-up in the runtime)
     if (cuda_failed(cudaGetDevice(&dev), "kv8_attention") ||
         cuda_failed(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev), "kv8_attention"))
         return -1;

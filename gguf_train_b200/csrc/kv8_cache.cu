@@ -1,4 +1,6 @@
-// The block-scaled 8-bit cache: append, read back, evict.
+// The block-scaled 8-bit cache: append, read back, evict. All of it moves bytes: HBM bound, or latency bound
+// for a token at a time. Work goes in chunks of 16 codes (a head size is a multiple of 16, so a chunk
+// lies in one row): 16 bytes of codes against 16 values.
 
 #include <algorithm>
 
@@ -10,50 +12,135 @@ namespace {
 
 __device__ __forceinline__ float block_max(float v, float* red) {
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (blockDim.x == 32) return v;
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    float m = 0.0f;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) m = fmaxf(m, red[w]);
-    __syncthreads();
-    return m;
+    v = red[threadIdx.x & 31 & ((blockDim.x >> 5) - 1)];  // blockDim a power of two
+    for (int o = (int)(blockDim.x >> 6); o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
 }
 
-// One CTA per (touched block, sequence x kv head, K or V)
-template <typename T, int FMT>
-__global__ void kv8_append_kernel(const Kv8AppendArgs a) {
-    __shared__ float red[32];
+// 16 values of a row as f32: 16-byte loads where the rows allow them
+template <typename T, bool VEC>
+struct Chunk {
+    static constexpr int W = VEC ? 16 * sizeof(T) / 16 : 16;
+    using Word = typename std::conditional<VEC, uint4, T>::type;
+    Word w[W];
+    __device__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = ((const Word*)p)[i];
+    }
+    __device__ void values(int q, float* x) const {  // values 4q .. 4q + 3
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = Elem<T>::load((const T*)w + 4 * q + i);
+    }
+    __device__ float amax() const {
+        float m = 0.0f, x[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            values(q, x);
+            m = fmaxf(fmaxf(m, fmaxf(finite_abs(x[0]), finite_abs(x[1]))), fmaxf(finite_abs(x[2]), finite_abs(x[3])));
+        }
+        return m;
+    }
+    template <int FMT>
+    __device__ uint4 codes(const Quantiser& z) const {
+        float x[4];
+        uint4 r;
+        values(0, x); r.x = quantise8x4<FMT>(x, z);
+        values(1, x); r.y = quantise8x4<FMT>(x, z);
+        values(2, x); r.z = quantise8x4<FMT>(x, z);
+        values(3, x); r.w = quantise8x4<FMT>(x, z);
+        return r;
+    }
+};
+
+// 16 codes at an old scale
+template <int FMT>
+struct Codes16 {
+    uint4 w;
+    __device__ float amax() const {  // of the codes' values, without the scale
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        float m = 0.0f, x[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            values8x4<FMT>(u[q], x);
+            m = fmaxf(fmaxf(m, fmaxf(finite_abs(x[0]), finite_abs(x[1]))), fmaxf(finite_abs(x[2]), finite_abs(x[3])));
+        }
+        return m;
+    }
+    __device__ uint4 again(float s_old, const Quantiser& z) const {
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        uint32_t r[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float x[4];
+            values8x4<FMT>(u[q], x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = __fmul_rn(x[i], s_old);
+            r[q] = quantise8x4<FMT>(x, z);
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
+    }
+};
+
+// One CTA per (touched block, sequence x kv head, K or V). The new rows stay in registers between the largest
+// value and the codes (KEEP chunks a thread; what does not fit is read again, from L2).
+template <typename T, int FMT, bool VEC, int KEEP>
+__global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a, unsigned blocks) {
+    __shared__ float red[8];
     const gtb_kv8& c = a.c;
-    const int64_t bh = blockIdx.y, b = bh / c.Hkv, hk = bh - b * c.Hkv;
-    const bool is_v = blockIdx.z != 0;
-    const Rows3 x = is_v ? a.v : a.k;
-    const int64_t T_ = c.block, D = c.D;
-    const int64_t pos = clamp64(c.lens[b], 0, c.Smax);
-    const int64_t cnt = a.counts ? clamp64(a.counts[b], 0, a.n) : a.n;
-    const int64_t end = min(pos + cnt, c.Smax);
-    if (pos + cnt > c.Smax && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(a.status, 0, 61);
-    const int64_t j = pos / T_ + blockIdx.x;
-    const int64_t r0 = max(j * T_, pos), r1 = min((j + 1) * T_, end);  // new rows of this block
+    const unsigned bhx = blockIdx.x / blocks, jx = blockIdx.x - bhx * blocks;
+    const bool is_v = blockIdx.y != 0;
+    const int64_t bh = bhx, b = bhx / (unsigned)c.Hkv, hk = bh - b * c.Hkv;
+    const Rows3& x = is_v ? a.v : a.k;
+    const int bt = c.block;
+    const int pos = (int)clamp64(c.lens[b], 0, c.Smax);
+    const int cnt = a.counts ? (int)clamp64(a.counts[b], 0, a.n) : (int)a.n;
+    const int end = (int)min((int64_t)pos + cnt, c.Smax);
+    if ((int64_t)pos + cnt > c.Smax && jx == 0 && threadIdx.x == 0) atomicCAS(a.status, 0, 61);
+    const int j = pos / bt + (int)jx;
+    const int r0 = max(j * bt, pos), r1 = (int)min((int64_t)(j + 1) * bt, (int64_t)end);  // new rows of this block
     if (r0 >= r1) return;
-    const T* src = (const T*)x.p + b * x.sb + hk * x.sh;
-    uint8_t* codes = (uint8_t*)(is_v ? c.v : c.k) + bh * c.Smax * D;
-    float* scale = (is_v ? c.v_scale : c.k_scale) + bh * ((c.Smax + T_ - 1) / T_) + j;
-    const int64_t n_new = (r1 - r0) * D;
+    const unsigned cpr = (unsigned)c.D / 16, n_new = (unsigned)(r1 - r0) * cpr;
+    const T* src = (const T*)x.p + b * x.sb + hk * x.sh + (int64_t)(r0 - pos) * x.ss;
+    uint8_t* codes = (uint8_t*)(is_v ? c.v : c.k) + (bh * c.Smax + (int64_t)j * bt) * c.D;
+    float* scale = (is_v ? c.v_scale : c.k_scale) + bh * ((c.Smax + bt - 1) / bt) + j;
+    const float s_old = j * bt < pos ? *scale : 0.0f;
+    Chunk<T, VEC> kept[KEEP];
     float m = 0.0f;
-    for (int64_t e = threadIdx.x; e < n_new; e += blockDim.x) {
-        const int64_t r = e / D, d = e - r * D;
-        m = fmaxf(m, finite_abs(Elem<T>::load(src + (r0 - pos + r) * x.ss + d)));
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        const unsigned e = threadIdx.x + i * blockDim.x, r = e / cpr;
+        if (e < n_new) kept[i].load(src + r * x.ss + (e - r * cpr) * 16);
     }
-    const float s_old = j * T_ < pos ? *scale : 0.0f;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+        if (threadIdx.x + i * blockDim.x < n_new) m = fmaxf(m, kept[i].amax());
+    for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n_new; e += blockDim.x) {
+        const unsigned r = e / cpr;
+        Chunk<T, VEC> t;
+        t.load(src + r * x.ss + (e - r * cpr) * 16);
+        m = fmaxf(m, t.amax());
+    }
     const float s = fmaxf(s_old, scale_of<FMT>(block_max(m, red)));
+    const Quantiser z(s);
     if (s > s_old) {
-        uint8_t* held = codes + j * T_ * D;
-        const int64_t n_old = (r0 - j * T_) * D;
-        for (int64_t e = threadIdx.x; e < n_old; e += blockDim.x)
-            held[e] = quantise8<FMT>(__fmul_rn(Code8<FMT>::value(held[e]), s_old), s);
+        uint4* held = (uint4*)codes;
+        const unsigned n_old = (unsigned)(r0 - j * bt) * cpr;
+        for (unsigned e = threadIdx.x; e < n_old; e += blockDim.x) held[e] = Codes16<FMT>{held[e]}.again(s_old, z);
     }
-    for (int64_t e = threadIdx.x; e < n_new; e += blockDim.x) {
-        const int64_t r = e / D, d = e - r * D;
-        codes[r0 * D + e] = quantise8<FMT>(Elem<T>::load(src + (r0 - pos + r) * x.ss + d), s);
+    uint4* dst = (uint4*)(codes + (int64_t)(r0 - j * bt) * c.D);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        const unsigned e = threadIdx.x + i * blockDim.x;
+        if (e < n_new) dst[e] = kept[i].template codes<FMT>(z);
+    }
+    for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n_new; e += blockDim.x) {
+        const unsigned r = e / cpr;
+        Chunk<T, VEC> t;
+        t.load(src + r * x.ss + (e - r * cpr) * 16);
+        dst[e] = t.template codes<FMT>(z);
     }
     if (threadIdx.x == 0) *scale = s;
 }
@@ -66,23 +153,52 @@ __global__ void kv8_advance_kernel(const Kv8AppendArgs a) {
     a.c.lens[b] = (int32_t)min(pos + cnt, a.c.Smax);
 }
 
+// A thread reads chunks of READ_ROWS rows of one (sequence, kv head, K or V) and writes their values
+constexpr int READ_ROWS = 4;
 template <typename T, int FMT>
-__global__ void kv8_read_kernel(const Kv8ReadArgs a) {
+__global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ Kv8ReadArgs a) {
     const gtb_kv8& c = a.c;
-    const int64_t per = c.B * c.Hkv * a.n * c.D;
+    const unsigned cpr = (unsigned)c.D / 16, rows = 256 / cpr;  // rows a CTA covers at a time
+    const unsigned row = threadIdx.x / cpr, chunk = threadIdx.x - row * cpr;
+    if (row >= rows) return;
     const int64_t nb = (c.Smax + c.block - 1) / c.block;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < 2 * per; i += (int64_t)gridDim.x * blockDim.x) {
-        const bool is_v = i >= per;
-        const int64_t e = is_v ? i - per : i;
-        const int64_t d = e % c.D, row = e / c.D, bh = row / a.n, t = row - bh * a.n;
-        const int64_t r = t + (a.start ? a.start[bh / c.Hkv] : 0);
-        float v = 0.0f;
-        if (r >= 0 && r < c.Smax)
-            v = __fmul_rn(Code8<FMT>::value(((const uint8_t*)(is_v ? c.v : c.k))[(bh * c.Smax + r) * c.D + d]),
-                          (is_v ? c.v_scale : c.k_scale)[bh * nb + r / c.block]);
-        Elem<T>::store((T*)(is_v ? a.v : a.k) + e, v);
+    for (int64_t p = blockIdx.y; p < 2 * c.B * c.Hkv; p += gridDim.y) {
+        const bool is_v = p >= c.B * c.Hkv;
+        const int64_t bh = is_v ? p - c.B * c.Hkv : p;
+        const int64_t start = a.start ? a.start[bh / c.Hkv] : 0;
+        const uint4* codes = (const uint4*)(is_v ? c.v : c.k) + bh * c.Smax * cpr + chunk;
+        const float* scale = (is_v ? c.v_scale : c.k_scale) + bh * nb;
+        T* out = (T*)(is_v ? a.v : a.k) + bh * a.n * c.D + chunk * 16;
+        uint4 w[READ_ROWS];
+        float s[READ_ROWS];
+        const int64_t t0 = (int64_t)blockIdx.x * (rows * READ_ROWS) + row;
+#pragma unroll
+        for (int i = 0; i < READ_ROWS; ++i) {
+            const int64_t t = t0 + i * rows, r = start + t;
+            const bool live = t < a.n && r >= 0 && r < c.Smax;
+            w[i] = live ? codes[r * cpr] : make_uint4(0, 0, 0, 0);
+            s[i] = live ? scale[(unsigned)r / (unsigned)c.block] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < READ_ROWS; ++i) {
+            const int64_t t = t0 + i * rows;
+            if (t >= a.n) break;
+            const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            __align__(16) T y[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float x[4];
+                values8x4<FMT>(u[q], x);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) Elem<T>::store(y + 4 * q + k, __fmul_rn(x[k], s[i]));
+            }
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T); ++k) ((uint4*)(out + t * c.D))[k] = ((const uint4*)y)[k];
+        }
     }
 }
+
+// ------------------------------------------------------------------ eviction
 
 // Order of scores as unsigned integers: larger score, larger key; NaN as -inf, -0 as 0
 __device__ __forceinline__ uint32_t score_key(float s) {
@@ -91,143 +207,236 @@ __device__ __forceinline__ uint32_t score_key(float s) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int SEL_THREADS = 1024;
+constexpr int SEL_THREADS = 1024, SEL_WARPS = SEL_THREADS / 32, SEL_KEEP = 16, SEL_TILE = SEL_THREADS * SEL_KEEP;
+constexpr int SEL_BINS = 2048;
 
-// Exclusive prefix sum over the CTA of one 64-bit value per thread; returns the total in `total`
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* sh, uint64_t& total) {
+// Sum over the warps before this one and over all, of one packed value per warp
+__device__ __forceinline__ uint64_t warps_before(uint64_t v, uint64_t* sh, uint64_t& total) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    uint64_t x = v;
+    if (lane == 0) sh[w] = v;
+    __syncthreads();
+    uint64_t x = sh[lane], s = x;
     for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        const uint64_t y = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += y;
     }
-    if (lane == 31) sh[w] = x;
-    __syncthreads();
-    if (w == 0) {
-        uint64_t t = lane < (int)(blockDim.x >> 5) ? sh[lane] : 0, s = t;
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t y = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += y;
-        }
-        sh[lane] = s - t;
-        if (lane == 31) sh[32] = s;
-    }
-    __syncthreads();
-    const uint64_t r = sh[w] + x - v;
-    total = sh[32];
+    total = __shfl_sync(0xffffffffu, s, 31);
+    const uint64_t r = __shfl_sync(0xffffffffu, s - x, w);
     __syncthreads();
     return r;
 }
 
-// Which rows stay: one CTA per (sequence, kv head). The k-th largest key among the candidates is found 8
-// bits at a time from a histogram; a second sweep in row order takes every larger key and the first
-// `need` rows that equal it, then the recent rows, and writes their indices in order.
-__global__ void __launch_bounds__(SEL_THREADS) kv8_select_kernel(const Kv8EvictArgs a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint64_t sh[33];
-    __shared__ uint32_t s_prefix, s_need;
+// Which rows stay: one CTA per (sequence, kv head). The k-th largest key among the candidates is found by
+// digits of 11, 11 and 10 bits: a histogram of the keys that match so far, summed from the top. The first
+// digit holds the exponent and two bits of the mantissa, which spreads the atomics. Then one sweep in row
+// order takes every larger key and the first `need` that equal it. The first SEL_TILE scores stay in
+// registers (warp w holds 512 consecutive ones); longer rows read theirs again each pass, from L2.
+__global__ void __launch_bounds__(SEL_THREADS) kv8_select_kernel(const __grid_constant__ Kv8EvictArgs a) {
+    __shared__ uint32_t hist[SEL_BINS];
+    __shared__ uint64_t sh[SEL_WARPS];
+    __shared__ uint32_t found[2];
+    cudaTriggerProgrammaticLaunchCompletion();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t bh = blockIdx.x, b = bh / a.src.Hkv;
-    const int64_t len = clamp64(a.src.lens[b], 0, a.src.Smax);
-    const int64_t newlen = min(len, a.budget);
+    const int len = (int)clamp64(a.src.lens[b], 0, a.src.Smax);
+    const int budget = (int)min(a.budget, (int64_t)1 << 30), recent = (int)min(a.recent, (int64_t)1 << 30);
+    const int newlen = min(len, budget);
     int32_t* kept = a.kept + bh * a.budget;
     const float* score = a.score + bh * a.src.Smax;
-    for (int64_t j = newlen + threadIdx.x; j < a.budget; j += blockDim.x) kept[j] = -1;
-    if (bh - b * a.src.Hkv == 0 && threadIdx.x == 0) a.dst.lens[b] = (int32_t)newlen;
-    if (len <= a.budget) {
-        for (int64_t j = threadIdx.x; j < len; j += blockDim.x) kept[j] = (int32_t)j;
+    for (int64_t j = newlen + threadIdx.x; j < a.budget; j += SEL_THREADS) kept[j] = -1;
+    if (bh - b * a.src.Hkv == 0 && threadIdx.x == 0) a.dst.lens[b] = newlen;
+    if (len <= budget) {
+        for (int j = threadIdx.x; j < len; j += SEL_THREADS) kept[j] = j;
         return;
     }
-    const int64_t n = len - a.recent, k = a.budget - a.recent;  // n > k
-    for (int64_t j = threadIdx.x; j < a.recent; j += blockDim.x) kept[k + j] = (int32_t)(n + j);
+    const int n = len - recent, k = budget - recent;  // n > k
+    for (int j = threadIdx.x; j < recent; j += SEL_THREADS) kept[k + j] = n + j;
     if (k == 0) return;
+    const int base = warp * (32 * SEL_KEEP) + lane;
+    uint32_t mine[SEL_KEEP];
+#pragma unroll
+    for (int i = 0; i < SEL_KEEP; ++i) mine[i] = base + i * 32 < n ? score_key(score[base + i * 32]) : 0u;
     uint32_t prefix = 0, need = (uint32_t)k;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += blockDim.x) hist[i] = 0;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t mask = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
+        const uint32_t digit = pass == 2 ? 1023u : 2047u;
+        for (int i = threadIdx.x; i < SEL_BINS; i += SEL_THREADS) hist[i] = 0;
         __syncthreads();
-        const uint32_t mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
-        for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+#pragma unroll
+        for (int i = 0; i < SEL_KEEP; ++i)
+            if (base + i * 32 < n && (mine[i] & mask) == prefix) atomicAdd(&hist[(mine[i] >> shift) & digit], 1u);
+        for (int i = SEL_TILE + threadIdx.x; i < n; i += SEL_THREADS) {
             const uint32_t key = score_key(score[i]);
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
+            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & digit], 1u);
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            uint32_t left = need;
-            int d = 255;
-            for (; d > 0 && hist[d] < left; --d) left -= hist[d];
-            s_prefix = prefix | ((uint32_t)d << shift);
-            s_need = left;
+        // thread t takes bins 2047 - 2t and 2046 - 2t: the counts above them, from the top
+        const uint32_t c0 = hist[SEL_BINS - 1 - 2 * threadIdx.x], c1 = hist[SEL_BINS - 2 - 2 * threadIdx.x];
+        uint32_t s = c0 + c1;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += y;
         }
-        __syncthreads();
-        prefix = s_prefix;
-        need = s_need;
-    }
-    uint64_t base = 0;  // (larger << 32 | equal) keys before this sweep's rows
-    for (int64_t i0 = 0; i0 < n; i0 += blockDim.x) {
-        const int64_t i = i0 + threadIdx.x;
-        const uint32_t key = i < n ? score_key(score[i]) : 0u;
-        const bool gt = i < n && key > prefix, eq = i < n && key == prefix;
         uint64_t total;
-        const uint64_t at = base + block_scan(((uint64_t)gt << 32) | (uint64_t)eq, sh, total);
-        const uint32_t before_gt = (uint32_t)(at >> 32), before_eq = (uint32_t)at;
-        if (gt || (eq && before_eq < need)) kept[before_gt + min(before_eq, need)] = (int32_t)i;
-        base += total;
+        const uint32_t above = (uint32_t)warps_before(__shfl_sync(0xffffffffu, s, 31), sh, total) + s - c0 - c1;
+        if (above < need && above + c0 >= need) {
+            found[0] = SEL_BINS - 1 - 2 * threadIdx.x;
+            found[1] = need - above;
+        } else if (above + c0 < need && above + c0 + c1 >= need) {
+            found[0] = SEL_BINS - 2 - 2 * threadIdx.x;
+            found[1] = need - above - c0;
+        }
+        __syncthreads();
+        prefix |= found[0] << shift;
+        need = found[1];
+        __syncthreads();
+    }
+    // keys above the k-th, and the first `need` equal to it, in row order; counts packed (above << 32 | equal)
+    uint64_t done = 0;
+    for (int t0 = 0; t0 < n; t0 += SEL_TILE) {
+        if (t0 > 0) {
+#pragma unroll
+            for (int i = 0; i < SEL_KEEP; ++i) {
+                const int e = t0 + base + i * 32;
+                mine[i] = e < n ? score_key(score[e]) : 0u;
+            }
+        }
+        uint64_t own = 0;
+        uint32_t gt[SEL_KEEP], eq[SEL_KEEP];
+#pragma unroll
+        for (int i = 0; i < SEL_KEEP; ++i) {
+            const bool in = t0 + base + i * 32 < n;
+            gt[i] = __ballot_sync(0xffffffffu, in && mine[i] > prefix);
+            eq[i] = __ballot_sync(0xffffffffu, in && mine[i] == prefix);
+            own += ((uint64_t)__popc(gt[i]) << 32) | (uint64_t)__popc(eq[i]);
+        }
+        uint64_t total;
+        uint64_t at = done + warps_before(own, sh, total);
+        const uint32_t below = (1u << lane) - 1u;
+#pragma unroll
+        for (int i = 0; i < SEL_KEEP; ++i) {
+            const uint32_t g = (uint32_t)(at >> 32) + __popc(gt[i] & below), e = (uint32_t)at + __popc(eq[i] & below);
+            if ((gt[i] >> lane & 1u) || ((eq[i] >> lane & 1u) && e < need)) kept[g + min(e, need)] = t0 + base + i * 32;
+            at += ((uint64_t)__popc(gt[i]) << 32) | (uint64_t)__popc(eq[i]);
+        }
+        done += total;
     }
 }
 
-// One CTA per (destination block, sequence x kv head, K or V): the kept rows' values, their largest, the
-// new scale, the new codes
-template <int FMT>
-__global__ void kv8_gather_kernel(const Kv8EvictArgs a) {
-    __shared__ float red[32];
-    const int64_t bh = blockIdx.y, j = blockIdx.x;
-    const bool is_v = blockIdx.z != 0;
-    const int64_t T_ = a.src.block, Td = a.dst.block, D = a.src.D;
-    const int64_t newlen = a.dst.lens[bh / a.src.Hkv];
-    const int64_t r0 = j * Td, r1 = min(r0 + Td, newlen);
-    if (!is_v && a.score_out)
-        for (int64_t r = r0 + threadIdx.x; r < min(r0 + Td, a.dst.Smax); r += blockDim.x)
-            a.score_out[bh * a.dst.Smax + r] = r < newlen ? a.score[bh * a.src.Smax + a.kept[bh * a.budget + r]] : 0.0f;
-    if (r0 >= r1) return;
-    const uint8_t* src = (const uint8_t*)(is_v ? a.src.v : a.src.k) + bh * a.src.Smax * D;
-    const float* sscale = (is_v ? a.src.v_scale : a.src.k_scale) + bh * ((a.src.Smax + T_ - 1) / T_);
-    uint8_t* dst = (uint8_t*)(is_v ? a.dst.v : a.dst.k) + (bh * a.dst.Smax + r0) * D;
+// One CTA per (destination block, sequence x kv head, K or V): the kept rows' values, their largest, the new
+// scale, the new codes. As in the append, KEEP chunks a thread stay in registers.
+template <int FMT, int KEEP>
+__global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__ Kv8EvictArgs a, unsigned blocks) {
+    __shared__ float red[8];
+    cudaGridDependencySynchronize();  // the kept rows and the new lengths are there
+    const unsigned bhx = blockIdx.x / blocks, j = blockIdx.x - bhx * blocks;
+    const int64_t bh = bhx;
+    const bool is_v = blockIdx.y != 0;
+    const unsigned bs = a.src.block, bd = a.dst.block;
+    const int newlen = a.dst.lens[bhx / (unsigned)a.src.Hkv];
+    const int r0 = (int)(j * bd), r1 = min(r0 + (int)bd, newlen);
     const int32_t* kept = a.kept + bh * a.budget + r0;
-    const int64_t n = (r1 - r0) * D;
-    float m = 0.0f;
-    for (int64_t e = threadIdx.x; e < n; e += blockDim.x) {
-        const int64_t r = e / D, s = kept[r];
-        m = fmaxf(m, finite_abs(__fmul_rn(Code8<FMT>::value(src[s * D + e - r * D]), sscale[s / T_])));
+    if (!is_v && a.score_out)
+        for (int64_t r = r0 + threadIdx.x; r < min((int64_t)r0 + bd, a.dst.Smax); r += blockDim.x)
+            a.score_out[bh * a.dst.Smax + r] = r < newlen ? a.score[bh * a.src.Smax + kept[r - r0]] : 0.0f;
+    if (r0 >= r1) return;
+    const unsigned cpr = (unsigned)a.src.D / 16, n = (unsigned)(r1 - r0) * cpr;
+    const uint4* src = (const uint4*)(is_v ? a.src.v : a.src.k) + bh * a.src.Smax * cpr;
+    const float* sscale = (is_v ? a.src.v_scale : a.src.k_scale) + bh * ((a.src.Smax + bs - 1) / bs);
+    uint4* dst = (uint4*)(is_v ? a.dst.v : a.dst.k) + (bh * a.dst.Smax + r0) * cpr;
+    Codes16<FMT> w[KEEP];
+    float s_old[KEEP], m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        const unsigned e = threadIdx.x + i * blockDim.x, r = e / cpr;
+        s_old[i] = 0.0f;
+        if (e < n) {
+            const unsigned row = kept[r];
+            w[i].w = src[(int64_t)row * cpr + (e - r * cpr)];
+            s_old[i] = sscale[row / bs];
+        }
     }
-    const float sc = scale_of<FMT>(block_max(m, red));
-    for (int64_t e = threadIdx.x; e < n; e += blockDim.x) {
-        const int64_t r = e / D, s = kept[r];
-        dst[e] = quantise8<FMT>(__fmul_rn(Code8<FMT>::value(src[s * D + e - r * D]), sscale[s / T_]), sc);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+        if (threadIdx.x + i * blockDim.x < n) m = fmaxf(m, finite_abs(__fmul_rn(w[i].amax(), s_old[i])));
+    for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n; e += blockDim.x) {
+        const unsigned r = e / cpr, row = kept[r];
+        m = fmaxf(m, finite_abs(__fmul_rn(Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.amax(), sscale[row / bs])));
     }
-    if (threadIdx.x == 0) (is_v ? a.dst.v_scale : a.dst.k_scale)[bh * ((a.dst.Smax + Td - 1) / Td) + j] = sc;
+    const float s = scale_of<FMT>(block_max(m, red));
+    const Quantiser z(s);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        const unsigned e = threadIdx.x + i * blockDim.x;
+        if (e < n) dst[e] = w[i].again(s_old[i], z);
+    }
+    for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n; e += blockDim.x) {
+        const unsigned r = e / cpr, row = kept[r];
+        dst[e] = Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.again(sscale[row / bs], z);
+    }
+    if (threadIdx.x == 0) (is_v ? a.dst.v_scale : a.dst.k_scale)[bh * ((a.dst.Smax + bd - 1) / bd) + j] = s;
 }
 
-template <int FMT>
-int append_fmt(const Kv8AppendArgs& a, cudaStream_t st) {
-    const int64_t nblk = (a.n + a.c.block - 2) / a.c.block + 1;
-    const dim3 grid((unsigned)nblk, (unsigned)(a.c.B * a.c.Hkv), 2);
-    switch (a.dtype) {
-        case F32: kv8_append_kernel<float, FMT><<<grid, 128, 0, st>>>(a); break;
-        case F16: kv8_append_kernel<__half, FMT><<<grid, 128, 0, st>>>(a); break;
-        default: kv8_append_kernel<__nv_bfloat16, FMT><<<grid, 128, 0, st>>>(a); break;
-    }
+// Threads for `chunks` of work in a CTA: a power of two, two chunks a thread where there are enough
+int threads_for(int64_t chunks) {
+    int t = 32;
+    while (t < 256 && t * 2 < chunks) t *= 2;
+    return t;
+}
+
+bool grid_fits(int64_t n, const char* ctx) {
+    if (n <= INT32_MAX) return true;
+    set_errorf("%s: batch x kv heads x blocks must fit in int32", ctx);
+    return false;
+}
+
+template <typename T, int FMT>
+int append_t(const Kv8AppendArgs& a, cudaStream_t st) {
+    // a block beyond the capacity is never touched
+    const int64_t blocks = std::min((a.n + a.c.block - 2) / a.c.block + 1, (a.c.Smax + a.c.block - 1) / a.c.block + 1);
+    const int64_t n = blocks * a.c.B * a.c.Hkv;
+    if (!grid_fits(n, "kv8_append")) return -1;
+    constexpr int N = 16 / sizeof(T);
+    bool vec = true;
+    for (const Rows3* r : {&a.k, &a.v})
+        vec = vec && ((uintptr_t)r->p & 15) == 0 && r->sb % N == 0 && r->sh % N == 0 && r->ss % N == 0;
+    const int threads = threads_for(std::min<int64_t>(a.n, a.c.block) * (a.c.D / 16));
+    const dim3 grid((unsigned)n, 2);
+    if (vec) kv8_append_kernel<T, FMT, true, sizeof(T) == 4 ? 2 : 4><<<grid, threads, 0, st>>>(a, (unsigned)blocks);
+    else kv8_append_kernel<T, FMT, false, 2><<<grid, threads, 0, st>>>(a, (unsigned)blocks);
     return cuda_failed(cudaGetLastError(), "kv8_append launch") ? -1 : 0;
 }
 
 template <int FMT>
+int append_fmt(const Kv8AppendArgs& a, cudaStream_t st) {
+    switch (a.dtype) {
+        case F32: return append_t<float, FMT>(a, st);
+        case F16: return append_t<__half, FMT>(a, st);
+        default: return append_t<__nv_bfloat16, FMT>(a, st);
+    }
+}
+
+template <int FMT>
 int read_fmt(const Kv8ReadArgs& a, cudaStream_t st) {
-    const int64_t n = 2 * a.c.B * a.c.Hkv * a.n * a.c.D;
-    const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 148 * 16);
+    const int64_t rows = 256 / (a.c.D / 16) * READ_ROWS;
+    const dim3 grid((unsigned)((a.n + rows - 1) / rows), (unsigned)std::min<int64_t>(2 * a.c.B * a.c.Hkv, 65535));
     switch (a.dtype) {
         case F32: kv8_read_kernel<float, FMT><<<grid, 256, 0, st>>>(a); break;
         case F16: kv8_read_kernel<__half, FMT><<<grid, 256, 0, st>>>(a); break;
         default: kv8_read_kernel<__nv_bfloat16, FMT><<<grid, 256, 0, st>>>(a); break;
     }
     return cuda_failed(cudaGetLastError(), "kv8_read launch") ? -1 : 0;
+}
+
+template <int FMT>
+bool gather(const Kv8EvictArgs& a, cudaStream_t st) {
+    // score_out covers dst.Smax rows, the codes only the budget
+    const int64_t rows = a.score_out ? a.dst.Smax : a.budget;
+    const int64_t blocks = (rows + a.dst.block - 1) / a.dst.block, n = blocks * a.src.B * a.src.Hkv;
+    if (!grid_fits(n, "kv8_evict")) return false;
+    const int threads = threads_for(std::min<int64_t>(a.budget, a.dst.block) * (a.src.D / 16));
+    return launch_behind("kv8_evict: gather launch", kv8_gather_kernel<FMT, 4>, dim3((unsigned)n, 2), threads, st, a, (unsigned)blocks);
 }
 
 }  // namespace
@@ -244,15 +453,9 @@ int launch_kv8_read(const Kv8ReadArgs& a, cudaStream_t st) {
 }
 
 int launch_kv8_evict(const Kv8EvictArgs& a, cudaStream_t st) {
-    const unsigned bh = (unsigned)(a.src.B * a.src.Hkv);
-    kv8_select_kernel<<<bh, SEL_THREADS, 0, st>>>(a);
+    kv8_select_kernel<<<(unsigned)(a.src.B * a.src.Hkv), SEL_THREADS, 0, st>>>(a);
     if (cuda_failed(cudaGetLastError(), "kv8_evict: select launch")) return -1;
-    // score_out covers dst.Smax rows, the codes only the budget
-    const int64_t rows = a.score_out ? a.dst.Smax : a.budget;
-    const dim3 grid((unsigned)((rows + a.dst.block - 1) / a.dst.block), bh, 2);
-    if (a.src.format == GTB_KV8_INT8) kv8_gather_kernel<GTB_KV8_INT8><<<grid, 128, 0, st>>>(a);
-    else kv8_gather_kernel<GTB_KV8_E4M3><<<grid, 128, 0, st>>>(a);
-    return cuda_failed(cudaGetLastError(), "kv8_evict: gather launch") ? -1 : 0;
+    return (a.src.format == GTB_KV8_INT8 ? gather<GTB_KV8_INT8>(a, st) : gather<GTB_KV8_E4M3>(a, st)) ? 0 : -1;
 }
 
 }  // namespace gtb

@@ -23,6 +23,8 @@
 //   units need neither shuffles nor a rescaling of O.
 #pragma once
 
+#include <atomic>
+
 #include "gtb_common.cuh"
 #include "kv8.cuh"
 
@@ -170,6 +172,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const gtb_kv8& c = p.c;
     const int per_seq = (int)c.Hkv * p.row_tiles;
+    cudaTriggerProgrammaticLaunchCompletion();
 
     auto len_of = [&](int64_t b) { return (int)clamp64(c.lens[b], 0, c.Smax); };
     auto units_of = [&](int64_t b) { return (int64_t)max(1, (len_of(b) + UNIT - 1) / UNIT); };
@@ -601,6 +604,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
 // Joins the parts of the items that more than one warp worked on: one warp per (item, row)
 template <int DP>
 __global__ void __launch_bounds__(128) kv8_combine_kernel(const MmaP p, int rows_per_tile, int64_t n_items) {
+    cudaGridDependencySynchronize();
     const int lane = threadIdx.x & 31;
     const int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     const int64_t item = w / rows_per_tile;
@@ -647,8 +651,14 @@ template <int DP, int FMT, int NT, int NS>
 int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
     using C = MmaCfg<DP, NT, NS>;
     auto kern = kv8_mma_kernel<DP, FMT, NT, NS>;
-    if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM), "kv8_attention: shared memory"))
-        return -1;
+    static std::atomic<uint64_t> ready{0};  // devices on which the attribute is set
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM), "kv8_attention: shared memory"))
+            return -1;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
     p.row_tiles = (p.R + 8 * NT - 1) / (8 * NT);
     const int64_t items = p.c.B * p.c.Hkv * p.row_tiles;
     const int64_t warps = (int64_t)n_sm * C::WARPS;
@@ -664,8 +674,7 @@ int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
     bool bad = cuda_failed(cudaGetLastError(), "kv8_attention launch");
     if (!bad) {
         const int64_t n = items * 8 * NT;
-        kv8_combine_kernel<DP><<<(unsigned)((n + 3) / 4), 128, 0, st>>>(p, 8 * NT, items);
-        bad = cuda_failed(cudaGetLastError(), "kv8_attention: combine launch");
+        bad = !launch_behind("kv8_attention: combine launch", kv8_combine_kernel<DP>, dim3((unsigned)((n + 3) / 4)), 128, st, p, 8 * NT, items);
     }
     cudaFreeAsync(scratch, st);
     return bad ? -1 : 0;
