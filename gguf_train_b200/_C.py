@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -43,6 +44,13 @@ class Tensor4(ctypes.Structure):
 
 
 P4 = ctypes.POINTER(Tensor4)
+
+# A Tensor4 as the bytes of one, for arguments declared c_void_p: 0.7 us against the structure's 1.7
+_pack4 = struct.Struct("P4q4qi4x").pack
+
+
+def tensor4(t, code: int) -> bytes:
+    return _pack4(t.data_ptr(), *t.shape, *t.stride(), code)
 
 
 class SdpaOpts(ctypes.Structure):
@@ -108,14 +116,14 @@ def _configure(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.gtb_attn_merge.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64,
                                    c_int64, c_void_p]
     lib.gtb_attn_merge.restype = c_int
-    lib.gtb_rope_axes.argtypes = [P4, P4, P4, P4, c_void_p, c_int64, c_int64, ctypes.POINTER(c_int32), c_int, c_int, c_int,
+    lib.gtb_rope_axes.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, ctypes.POINTER(c_int32), c_int, c_int, c_int,
                                   c_float, c_float, c_int, c_void_p]
     lib.gtb_rope_axes.restype = c_int
-    lib.gtb_kv8_append.argtypes = [PKV8, P4, P4, c_void_p, c_int, c_void_p]
+    lib.gtb_kv8_append.argtypes = [PKV8, c_void_p, c_void_p, c_void_p, c_int, c_void_p]
     lib.gtb_kv8_append.restype = c_int
-    lib.gtb_kv8_read.argtypes = [PKV8, c_void_p, P4, P4, c_void_p]
+    lib.gtb_kv8_read.argtypes = [PKV8, c_void_p, c_void_p, c_void_p, c_void_p]
     lib.gtb_kv8_read.restype = c_int
-    lib.gtb_kv8_attention.argtypes = [P4, PKV8, c_float, c_void_p, c_void_p, c_void_p, P4, c_void_p, c_void_p]
+    lib.gtb_kv8_attention.argtypes = [c_void_p, PKV8, c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     lib.gtb_kv8_attention.restype = c_int
     lib.gtb_kv8_evict.argtypes = [PKV8, c_void_p, c_int64, c_int64, PKV8, c_void_p, c_void_p, c_void_p]
     lib.gtb_kv8_evict.restype = c_int

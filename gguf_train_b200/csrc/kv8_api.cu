@@ -78,8 +78,8 @@ int guarded(const char* ctx, F&& f) {
     return -1;
 }
 
-// axis and frequency of each pair
-bool rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags, float freq_base, float freq_scale,
+// axis and frequency of each pair (64 powers: 3 us, so the last one made stays with the thread)
+bool make_rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags, float freq_base, float freq_scale,
                 int64_t D, RopeAxesTable& t, int& pairs) {
     if (!sections || n_axes < 1 || n_axes > 4) return fail(ctx, "there must be 1 to 4 sections");
     if (flags & ~(GTB_ROPE_INTERLEAVED | GTB_ROPE_PER_AXIS)) return fail(ctx, "unknown flags");
@@ -121,6 +121,39 @@ bool rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags,
     for (int a = 0; a < n_axes; ++a)
         if (used[a] != sections[a])
             return fail(ctx, "interleaved sections must give every axis but the first its turns (n_axes * sections[a] pairs fit)");
+    return true;
+}
+
+struct RopeKey {
+    int32_t sections[4] = {};
+    int n_axes = 0, flags = 0;
+    float base = 0.0f, scale = 0.0f;
+    int64_t D = 0;
+    bool operator==(const RopeKey& o) const {
+        return std::equal(sections, sections + 4, o.sections) && n_axes == o.n_axes && flags == o.flags && base == o.base &&
+               scale == o.scale && D == o.D;
+    }
+};
+
+bool rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags, float freq_base, float freq_scale, int64_t D,
+                RopeAxesTable& t, int& pairs) {
+    thread_local RopeKey last;
+    thread_local RopeAxesTable table;
+    thread_local int last_pairs;
+    RopeKey key;
+    if (sections && n_axes >= 1 && n_axes <= 4) std::copy(sections, sections + n_axes, key.sections);
+    key.n_axes = n_axes;
+    key.flags = flags;
+    key.base = freq_base;
+    key.scale = freq_scale;
+    key.D = D;
+    if (!(key == last)) {
+        last = RopeKey{};
+        if (!make_rope_table(ctx, sections, n_axes, flags, freq_base, freq_scale, D, table, last_pairs)) return false;
+        last = key;
+    }
+    t = table;
+    pairs = last_pairs;
     return true;
 }
 
@@ -237,6 +270,7 @@ GTB_API int gtb_kv8_attention(const gtb_tensor4* q, const gtb_kv8* cache, float 
             return fail(ctx, "too many query rows"), -1;
         if (!same_shape(*q, *out) || out->dtype != q->dtype || !contiguous(*out))
             return fail(ctx, "out must be contiguous, of q's shape and type"), -1;
+        if ((uintptr_t)out->data & 15) return fail(ctx, "out must be 16-byte aligned"), -1;
         if (!unit_inner(*q)) return fail(ctx, "the innermost stride of q must be 1"), -1;
         if (!score_in != !score_out) return fail(ctx, "score_in and score_out go together"), -1;
         if (std::isnan(scale) || std::isinf(scale)) return fail(ctx, "scale must be finite"), -1;

@@ -91,6 +91,7 @@ int launch_kv8_attention(const Kv8AttnArgs& a, cudaStream_t st) {
         lse = (float*)scratch;
     }
     int rc = 0;
+    bool kept = false;
     if (rows > 0) {
         kv8::MmaP p{};
         p.c = a.c;
@@ -104,9 +105,14 @@ int launch_kv8_attention(const Kv8AttnArgs& a, cudaStream_t st) {
         p.scale_log2 = a.scale * 1.4426950408889634f;
         p.counts = a.counts;
         p.lse = lse;
+        kept = a.score_out && a.c.Smax > 0 && kv8::keep_scores(p.R, a.c.D);
+        if (kept) {
+            p.score_in = a.score_in;
+            p.score_out = a.score_out;
+        }
         rc = a.c.D <= 64 ? kv8::launch_mma_64(p, n_sm, st) : a.c.D <= 128 ? kv8::launch_mma_128(p, n_sm, st) : kv8::launch_mma_256(p, n_sm, st);
     }
-    if (!rc && a.score_out) rc = launch_score(a, lse, st);
+    if (!rc && a.score_out && !kept) rc = launch_score(a, lse, st);
     if (scratch) cudaFreeAsync(scratch, st);
     return rc;
 }

@@ -4,7 +4,7 @@
 // queries, row = i * G + g. The keys are cut into units of 32; all units of all items form one line, of which
 // every warp takes an equal stretch (so the split adapts to the lengths and no warp waits for another). A
 // warp that finishes an item alone writes the result; otherwise it leaves (out, max, sum) for
-// kv8_combine_kernel.
+// kv8_finish_kernel.
 //
 // A warp streams its units through its own ring in shared memory with 16-byte asynchronous copies (rows
 // past the length arrive as zeros: nothing stored there can reach a result). Codes become f16 in registers,
@@ -23,6 +23,7 @@
 //   units need neither shuffles nor a rescaling of O.
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 
 #include "gtb_common.cuh"
@@ -47,7 +48,9 @@ struct MmaP {
     int2* meta;               // per item: first and last warp that holds a part of it
     float* part_o;            // [slot][8 NT][DP]
     float2* part_ml;          // [slot][8 NT]
-    float* s_out;             // nullable: scores (log2 units) [b, hk][key][R]
+    const float* score_in;    // nullable, with score_out: the rows' weights are wanted (one row tile)
+    float* score_out;
+    float* s_out;             // then: scores (log2 units) [b, hk][key][R]
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -577,7 +580,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                             }
                         }
                         if (p.lse && g == 0)
-                            p.lse[(wk.b * p.H + h) * p.Lq + i] = M[n][e] == -INFINITY ? -INFINITY : (m + log2f(x)) * 0.6931471805599453f;
+                            p.lse[(wk.b * p.H + h) * p.Lq + i] = x == 0.0f ? -INFINITY : (m + log2f(x)) * 0.6931471805599453f;
                     } else {
                         const int64_t slot = 2 * wid + (head_split ? 0 : 1);
                         float* dst = p.part_o + (slot * ROWS + r) * DP;
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                                 *(float2*)(dst + d0 + k) = make_float2(o[n][j][e], o[n][j][e + 2]);
                             }
                         }
-                        if (g == 0) p.part_ml[slot * ROWS + r] = make_float2(M[n][e] == -INFINITY ? -INFINITY : m, x);
+                        if (g == 0) p.part_ml[slot * ROWS + r] = make_float2(!(x == x) ? x : M[n][e] == -INFINITY ? -INFINITY : m, x);
                     }
                 }
             fresh = true;
@@ -601,50 +604,120 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
     cp_wait<0>();
 }
 
-// Joins the parts of the items that more than one warp worked on: one warp per (item, row)
-template <int DP>
-__global__ void __launch_bounds__(128) kv8_combine_kernel(const MmaP p, int rows_per_tile, int64_t n_items) {
-    cudaGridDependencySynchronize();
+// What is left once the units are done, in one launch of 128-thread CTAs.
+//   CTAs below `joins`: one (item, row) each whose item several warps worked on. The lanes weigh the parts by their
+//     maxima, the four warps each add up a quarter of them, and the sums meet in shared memory: always in the
+//     same order.
+//   CTAs from there on (scores kept): KEYS_PER_CTA cached rows of one (sequence, kv head): score_in + the sum over the
+//     query rows of exp(s - lse), from the scores the first kernel wrote and the rows' (max, sum) parts.
+constexpr int KEYS_PER_CTA = 1024;
+
+// A row's parts summed by one warp: (m, l) with sum of 2^score = l 2^m. Parts that saw no key have maximum -inf; those
+// of a row of NaN have sum and maximum NaN, and make l NaN.
+__device__ __forceinline__ float2 row_lse2(const MmaP& p, const int2 range, int rows, int r) {
     const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int64_t item = w / rows_per_tile;
-    const int r = (int)(w - item * rows_per_tile);
-    if (item >= n_items) return;
+    float m = -INFINITY;
+    for (int k = range.x + lane; k <= range.y; k += 32) m = fmaxf(m, p.part_ml[(2 * (int64_t)k + (k == range.x)) * rows + r].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (m == -INFINITY) m = 0.0f;
+    float l = 0.0f;
+    for (int k = range.x + lane; k <= range.y; k += 32) {
+        const float2 ml = p.part_ml[(2 * (int64_t)k + (k == range.x)) * rows + r];
+        l += ml.y * ex2f(ml.x - m);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    return make_float2(m, l);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(128) kv8_finish_kernel(const __grid_constant__ MmaP p, int rows, unsigned joins) {
+    cudaGridDependencySynchronize();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per_seq = (int)p.c.Hkv * p.row_tiles;
-    const int64_t b = item / per_seq;
-    const int rest = (int)(item - b * per_seq), hk = rest / p.row_tiles, tile = rest - hk * p.row_tiles;
-    const int gr = tile * rows_per_tile + r;
-    if (gr >= p.R) return;
+    if (blockIdx.x < joins) {
+        const unsigned per_item = min(rows, p.R);
+        const unsigned item = blockIdx.x / per_item;
+        const int r = (int)(blockIdx.x - item * per_item);
+        const int b = (int)(item / (unsigned)per_seq), rest = (int)(item - (unsigned)b * per_seq);
+        const int hk = rest / p.row_tiles, tile = rest - hk * p.row_tiles, gr = tile * rows + r;
+        if (gr >= p.R) return;
+        const int2 range = p.meta[item];
+        if (range.x == range.y) return;
+        const float2 all = row_lse2(p, range, rows, r);
+        constexpr int PER = DP / 32;
+        float acc[PER] = {};
+        // parts of this warp: k = range.x + warp, + 4, ...; 4 at a time, the loads of all before their use
+        for (int k0 = range.x + warp; k0 <= range.y; k0 += 16) {
+            float x[4][PER], w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int k = min(k0 + 4 * q, range.y);
+                const int64_t slot = (2 * (int64_t)k + (k == range.x)) * rows + r;
+                const float m = p.part_ml[slot].x;
+                w[q] = k0 + 4 * q <= range.y ? ex2f(m - all.x) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) x[q][i] = p.part_o[slot * DP + i * 32 + lane];
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (w[q] != 0.0f) acc[i] = fmaf(x[q][i], w[q], acc[i]);
+        }
+        __shared__ float sum[4][DP];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) sum[warp][i * 32 + lane] = acc[i];
+        __syncthreads();
+        const float inv = all.y > 0.0f || !(all.y == all.y) ? 1.0f / all.y : 0.0f;
+        const int i = gr / p.G, h = hk * p.G + (gr - i * p.G);
+        const int64_t at = b * p.o.sb + h * p.o.sh + (int64_t)i * p.o.ss;
+        for (int d = threadIdx.x; d < p.c.D; d += 128) {
+            const float y = ((sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d])) * inv;
+            if (p.dtype == F32) ((float*)p.o.p)[at + d] = y;
+            else if (p.dtype == F16) ((__half*)p.o.p)[at + d] = __float2half_rn(y);
+            else ((__nv_bfloat16*)p.o.p)[at + d] = __float2bfloat16_rn(y);
+        }
+        if (p.lse && threadIdx.x == 0)
+            p.lse[((int64_t)b * p.H + h) * p.Lq + i] = all.y == 0.0f ? -INFINITY : (all.x + log2f(all.y)) * 0.6931471805599453f;
+        return;
+    }
+    // one row tile, so the item is the (sequence, kv head)
+    const unsigned per_head = (unsigned)((p.c.Smax + KEYS_PER_CTA - 1) / KEYS_PER_CTA);
+    const unsigned x = blockIdx.x - joins, item = x / per_head;
+    const int k0 = (int)(x - item * per_head) * KEYS_PER_CTA;
+    const int64_t b = item / (unsigned)p.c.Hkv;
+    const int len = (int)clamp64(p.c.lens[b], 0, p.c.Smax);
+    if (k0 >= len) return;
+    __shared__ float lse2[32];
     const int2 range = p.meta[item];
-    if (range.x == range.y) return;
-    constexpr int PER = DP / 32;
-    float acc[PER] = {}, m = -INFINITY, l = 0.0f;
-    for (int k = range.x; k <= range.y; ++k) {
-        const int64_t slot = 2 * (int64_t)k + (k == range.x ? 1 : 0);
-        const float2 ml = p.part_ml[slot * rows_per_tile + r];
-        float x[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) x[i] = p.part_o[(slot * rows_per_tile + r) * DP + i * 32 + lane];
-        const float m2 = fmaxf(m, ml.x);
-        const float ca = m == -INFINITY ? 0.0f : ex2f(m - m2), cb = ml.x == -INFINITY ? 0.0f : ex2f(ml.x - m2);
-        l = l * ca + ml.y * cb;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) acc[i] = acc[i] * ca + x[i] * cb;
-        m = m2;
+    for (int r = warp; r < p.R; r += 4) {
+        float z;
+        if (range.x == range.y) {
+            const int i = r / p.G, h = (int)(item - (unsigned)b * p.c.Hkv) * p.G + (r - i * p.G);
+            z = p.lse[(b * p.H + h) * p.Lq + i] * 1.4426950408889634f;
+        } else {
+            const float2 ml = row_lse2(p, range, rows, r);
+            z = ml.y == 0.0f ? -INFINITY : ml.x + log2f(ml.y);
+        }
+        if (lane == 0) lse2[r] = z == -INFINITY ? INFINITY : z;  // a row that attends nothing gives no weight
     }
-    const float inv = l > 0.0f || !(l == l) ? 1.0f / l : 0.0f;
-    const int i = gr / p.G, h = hk * p.G + (gr - i * p.G);
-    const int64_t at = b * p.o.sb + h * p.o.sh + (int64_t)i * p.o.ss;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const int d = k * 32 + lane;
-        if (d >= p.c.D) continue;
-        const float y = acc[k] * inv;
-        if (p.dtype == F32) ((float*)p.o.p)[at + d] = y;
-        else if (p.dtype == F16) ((__half*)p.o.p)[at + d] = __float2half_rn(y);
-        else ((__nv_bfloat16*)p.o.p)[at + d] = __float2bfloat16_rn(y);
+    __syncthreads();
+    const float* s = p.s_out + (int64_t)item * p.c.Smax * p.R;
+    for (int k = k0 + threadIdx.x; k < min(k0 + KEYS_PER_CTA, len); k += 128) {
+        const float* row = s + (int64_t)k * p.R;
+        float w = 0.0f;
+        if ((p.R & 3) == 0) {
+            for (int r = 0; r < p.R; r += 4) {
+                const float4 v = *(const float4*)(row + r);
+                w += (ex2f(v.x - lse2[r]) + ex2f(v.y - lse2[r + 1])) + (ex2f(v.z - lse2[r + 2]) + ex2f(v.w - lse2[r + 3]));
+            }
+        } else {
+            for (int r = 0; r < p.R; ++r) w += ex2f(row[r] - lse2[r]);
+        }
+        p.score_out[(int64_t)item * p.c.Smax + k] = p.score_in[(int64_t)item * p.c.Smax + k] + w;
     }
-    if (p.lse && lane == 0) p.lse[(b * p.H + h) * p.Lq + i] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 template <int DP, int FMT, int NT, int NS>
@@ -664,17 +737,26 @@ int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
     const int64_t warps = (int64_t)n_sm * C::WARPS;
     const size_t slots = 2 * (size_t)warps * 8 * NT;
     const size_t meta_bytes = ((size_t)items * sizeof(int2) + 255) & ~(size_t)255;
-    const size_t bytes = meta_bytes + slots * (sizeof(float2) + DP * sizeof(float));
+    const size_t part_bytes = slots * (sizeof(float2) + DP * sizeof(float));
+    const size_t s_bytes = p.score_out ? (size_t)p.c.B * p.c.Hkv * p.c.Smax * p.R * sizeof(float) : 0;
     void* scratch = nullptr;
-    if (cuda_failed(cudaMallocAsync(&scratch, bytes, st), "kv8_attention: scratch allocation")) return -1;
+    if (cuda_failed(cudaMallocAsync(&scratch, meta_bytes + part_bytes + s_bytes, st), "kv8_attention: scratch allocation")) return -1;
     p.meta = (int2*)scratch;
     p.part_o = (float*)((char*)scratch + meta_bytes);
     p.part_ml = (float2*)(p.part_o + slots * DP);
+    p.s_out = p.score_out ? (float*)((char*)scratch + meta_bytes + part_bytes) : nullptr;
     kern<<<n_sm, C::WARPS * 32, C::SMEM, st>>>(p);
     bool bad = cuda_failed(cudaGetLastError(), "kv8_attention launch");
     if (!bad) {
-        const int64_t n = items * 8 * NT;
-        bad = !launch_behind("kv8_attention: combine launch", kv8_combine_kernel<DP>, dim3((unsigned)((n + 3) / 4)), 128, st, p, 8 * NT, items);
+        const int64_t joins = items * std::min(8 * NT, p.R);
+        const int64_t sums = p.score_out ? p.c.B * p.c.Hkv * ((p.c.Smax + KEYS_PER_CTA - 1) / KEYS_PER_CTA) : 0;
+        if (joins + sums > INT32_MAX) {
+            set_error("kv8_attention: too many query rows");
+            bad = true;
+        } else {
+            bad = !launch_behind("kv8_attention: finish launch", kv8_finish_kernel<DP>, dim3((unsigned)(joins + sums)), 128, st, p,
+                                 8 * NT, (unsigned)joins);
+        }
     }
     cudaFreeAsync(scratch, st);
     return bad ? -1 : 0;
@@ -688,6 +770,10 @@ int launch_mma_rows(const MmaP& p, int n_sm, cudaStream_t st) {
     if constexpr (DP < 256) return wide ? launch_mma<DP, FMT, 4, 2>(p, n_sm, st) : launch_mma<DP, FMT, 4, 1>(p, n_sm, st);
     return -1;
 }
+
+// Whether the first kernel should keep its scores for the weights: R f32 scores a key written and read against the
+// key's D codes read again.
+inline bool keep_scores(int R, int64_t D) { return 8 * (int64_t)R <= D && R <= (D > 128 ? 16 : 32); }
 
 int launch_mma_64(const MmaP& p, int n_sm, cudaStream_t st);
 int launch_mma_128(const MmaP& p, int n_sm, cudaStream_t st);

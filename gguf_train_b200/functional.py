@@ -582,21 +582,19 @@ def rope(input: torch.Tensor, positions: torch.Tensor, n_dims: int | None = None
     return RoPEFn.apply(input, positions, nd, int(mode), int(n_ctx_orig), float(freq_base), float(freq_scale))
 
 
-def _rope_axes_run(xs, outs, pos, sections, mode, flags, freq_base, freq_scale, backward):
-    tx, ty = [_t4(x) for x in xs], [_t4(y) for y in outs]
+def _rope_axes_all(pos, sections, mode, flags, freq_base, freq_scale, backward, xs):
+    """The rotated xs (one or two), contiguous, in one launch."""
+    xs = [x if x.stride(3) == 1 else x.contiguous() for x in xs]
+    outs = tuple(x.new_empty(x.shape) for x in xs)
+    code = _DTYPE_CODE[xs[0].dtype]
+    t = [_C.tensor4(z, code) for pair in zip(xs, outs) for z in pair]
     two = len(xs) == 2
-    S = xs[0].shape[2]
     batch = pos.stride(1) if pos.ndim == 3 and pos.shape[1] > 1 else 0
-    rc = _C.lib.gtb_rope_axes(ctypes.byref(tx[0]), ctypes.byref(ty[0]), ctypes.byref(tx[1]) if two else None,
-                              ctypes.byref(ty[1]) if two else None, pos.data_ptr() if pos.numel() else None,
-                              pos.stride(0) if S else 0, batch, sections, len(sections), mode, flags, freq_base, freq_scale,
-                              1 if backward else 0, _stream(xs[0].device))
+    rc = _C.lib.gtb_rope_axes(t[0], t[1], t[2] if two else None, t[3] if two else None, pos.data_ptr(), pos.stride(0), batch, sections,
+                              len(sections), mode, flags, freq_base, freq_scale, 1 if backward else 0,
+                              torch._C._cuda_getCurrentRawStream(xs[0].device.index))
     _C.check_rc(rc, "rope_axes")
-
-
-def _rope_axes_new(x):
-    """An output for x: contiguous (B, H, S, D)."""
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return outs
 
 
 class RoPEAxesFn(torch.autograd.Function):
@@ -608,22 +606,16 @@ class RoPEAxesFn(torch.autograd.Function):
     def forward(ctx, pos, sections, mode, flags, freq_base, freq_scale, *xs):
         ctx.args = (sections, mode, flags, freq_base, freq_scale)
         ctx.save_for_backward(pos)
-        xs = [x if x.stride(3) == 1 else x.contiguous() for x in xs]
-        outs = [_rope_axes_new(x) for x in xs]
-        _rope_axes_run(xs, outs, pos, *ctx.args, False)
-        return tuple(outs) if len(outs) > 1 else outs[0]
+        outs = _rope_axes_all(pos, *ctx.args, False, xs)
+        return outs if len(outs) > 1 else outs[0]
 
     @staticmethod
     def backward(ctx, *grads):
         (pos,) = ctx.saved_tensors
-        gs = [None if g is None else g if g.stride(3) == 1 else g.contiguous() for g in grads]
-        live = [g for g, need in zip(gs, ctx.needs_input_grad[6:]) if g is not None and need]
-        outs = [_rope_axes_new(g) for g in live]
-        if live:
-            _rope_axes_run(live, outs, pos, *ctx.args, True)
-        it = iter(outs)
-        dx = [next(it) if g is not None and need else None for g, need in zip(gs, ctx.needs_input_grad[6:])]
-        return (None,) * 6 + tuple(dx)
+        need = ctx.needs_input_grad[6:]
+        live = [g for g, n in zip(grads, need) if g is not None and n]
+        outs = iter(_rope_axes_all(pos, *ctx.args, True, live) if live else ())
+        return (None,) * 6 + tuple(next(outs) if g is not None and n else None for g, n in zip(grads, need))
 
 
 def rope_axes(input: torch.Tensor, positions: torch.Tensor, sections, k: torch.Tensor | None = None, mode: int = 2,
@@ -660,8 +652,11 @@ def rope_axes(input: torch.Tensor, positions: torch.Tensor, sections, k: torch.T
         raise RuntimeError("rope_axes: positions must be int32")
     positions = positions if S <= 1 or positions.stride(-1) == 1 else positions.contiguous()
     flags = (_C.GTB_ROPE_INTERLEAVED if interleaved else 0) | (_C.GTB_ROPE_PER_AXIS if per_axis else 0)
-    return RoPEAxesFn.apply(positions, (ctypes.c_int32 * max(A, 1))(*sections), int(mode), flags, float(freq_base),
-                            float(freq_scale), *xs)
+    args = (positions, (ctypes.c_int32 * max(A, 1))(*sections), int(mode), flags, float(freq_base), float(freq_scale))
+    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        return RoPEAxesFn.apply(*args, *xs)
+    outs = _rope_axes_all(*args, False, xs)
+    return outs[0] if k is None else outs
 
 
 def dequantize_q8_0(blocks: torch.Tensor, dtype=torch.float32) -> torch.Tensor:

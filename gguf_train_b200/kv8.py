@@ -19,15 +19,20 @@ import ctypes
 import torch
 
 from . import _C
-from .functional import _require_cuda, _stream
+from .functional import _require_cuda
 
 _FORMAT = {torch.int8: _C.GTB_KV8_INT8, torch.float8_e4m3fn: _C.GTB_KV8_E4M3}
 _CODE = {torch.float32: _C.GT_F32, torch.float16: _C.GT_F16, torch.bfloat16: _C.GT_BF16}
 BLOCKS = (16, 32, 64, 128)
 
 
-def _t4(t: torch.Tensor) -> _C.Tensor4:
-    return _C.Tensor4(t.data_ptr(), t.shape, t.stride(), _CODE[t.dtype])
+def _t4(t: torch.Tensor) -> bytes:
+    return _C.tensor4(t, _CODE[t.dtype])
+
+
+def _stream(dev: torch.device) -> int:
+    # the current stream's handle without making a torch.cuda.Stream of it (2 us of a call's 20)
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _unit_inner(t: torch.Tensor) -> torch.Tensor:
@@ -118,8 +123,7 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, counts: torch.
     if k.dtype not in _CODE or v.dtype != k.dtype:
         raise RuntimeError("kv8_append: k and v must be f32, f16 or bf16, of one type")
     k, v = _unit_inner(k), _unit_inner(v)
-    tk, tv = _t4(k), _t4(v)
-    rc = _C.lib.gtb_kv8_append(ctypes.byref(cache._native), ctypes.byref(tk), ctypes.byref(tv),
+    rc = _C.lib.gtb_kv8_append(ctypes.byref(cache._native), _t4(k), _t4(v),
                                _counts("kv8_append", counts, B), 1 if advance else 0, _stream(k.device))
     _C.check_rc(rc, "kv8_append")
     return cache
@@ -137,9 +141,8 @@ def kv8_read(cache: KV8Cache, start: torch.Tensor | None, n: int, dtype=torch.fl
         raise RuntimeError(f"kv8_read: the number of rows must not be negative, got {n}")
     k = torch.empty((B, Hkv, int(n), D), dtype=dtype, device=cache.k.device)
     v = torch.empty_like(k)
-    tk, tv = _t4(k), _t4(v)
-    rc = _C.lib.gtb_kv8_read(ctypes.byref(cache._native), _counts("kv8_read", start, B), ctypes.byref(tk),
-                             ctypes.byref(tv), _stream(k.device))
+    rc = _C.lib.gtb_kv8_read(ctypes.byref(cache._native), _counts("kv8_read", start, B), _t4(k), _t4(v),
+                             _stream(k.device))
     _C.check_rc(rc, "kv8_read")
     return k, v
 
@@ -168,13 +171,12 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, scale: float | None = None, 
         if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, Hkv, cap) or not t.is_contiguous()):
             raise RuntimeError(f"kv8_attention: score must be a contiguous float32 tensor ({B}, {Hkv}, {cap})")
     q = _unit_inner(q)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if need_lse else None
+    out = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:3], dtype=torch.float32) if need_lse else None
     s_in = None if score is None else score.data_ptr()
     s_out = s_in if score_out is None else score_out.data_ptr()
-    tq, to = _t4(q), _t4(out)
-    rc = _C.lib.gtb_kv8_attention(ctypes.byref(tq), ctypes.byref(cache._native), 0.0 if scale is None else float(scale),
-                                  _counts("kv8_attention", counts, B), s_in, s_out, ctypes.byref(to),
+    rc = _C.lib.gtb_kv8_attention(_t4(q), ctypes.byref(cache._native), 0.0 if scale is None else float(scale),
+                                  _counts("kv8_attention", counts, B), s_in, s_out, _t4(out),
                                   None if lse is None else lse.data_ptr(), _stream(q.device))
     _C.check_rc(rc, "kv8_attention")
     return (out, lse) if need_lse else out

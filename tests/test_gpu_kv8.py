@@ -540,11 +540,11 @@ def test_refusals():
     bad = _C.KV8.from_buffer_copy(cache._native)
     bad.block = 20
     t = _t4(x)
-    assert _C.lib.gtb_kv8_append(ctypes.byref(bad), ctypes.byref(t), ctypes.byref(t), None, 0, None) == -1
+    assert _C.lib.gtb_kv8_append(ctypes.byref(bad), t, t, None, 0, None) == -1
     assert b"16, 32, 64 or 128" in _C.lib.gtb_last_error()
     bad = _C.KV8.from_buffer_copy(cache._native)
     bad.k = bad.k + 1
-    assert _C.lib.gtb_kv8_append(ctypes.byref(bad), ctypes.byref(t), ctypes.byref(t), None, 0, None) == -1
+    assert _C.lib.gtb_kv8_append(ctypes.byref(bad), t, t, None, 0, None) == -1
     host = torch.zeros((2, 2, 3, 32))
-    assert _C.lib.gtb_kv8_append(ctypes.byref(cache._native), ctypes.byref(_t4(host)), ctypes.byref(t), None, 0, None) == -1
+    assert _C.lib.gtb_kv8_append(ctypes.byref(cache._native), _t4(host), t, None, 0, None) == -1
     assert b"no CPU path" in _C.lib.gtb_last_error()
