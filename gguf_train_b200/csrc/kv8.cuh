@@ -122,10 +122,11 @@ __device__ __forceinline__ void values8x4(uint32_t w, float* x) {
 // Launch that may start while the stream's previous kernel still runs: the kernel itself waits for that one's
 // results with cudaGridDependencySynchronize(), in every thread, before it touches anything.
 template <typename... P, typename... A>
-bool launch_behind(const char* ctx, void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, A... args) {
+bool launch_behind(const char* ctx, void (*kern)(P...), dim3 grid, int threads, cudaStream_t st, int smem, const A&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = st;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -6,6 +6,7 @@
 
 #include "gtb_common.cuh"
 #include "kv8.cuh"
+#include "kv8_chunk.h"
 #include "kv8_mma.cuh"
 
 namespace gtb {
@@ -92,7 +93,9 @@ int launch_kv8_attention(const Kv8AttnArgs& a, cudaStream_t st) {
     }
     int rc = 0;
     bool kept = false;
-    if (rows > 0) {
+    if (rows > 0 && kv8::chunk_supported(a)) {
+        rc = kv8::launch_chunk(a, lse, n_sm, st);
+    } else if (rows > 0) {
         kv8::MmaP p{};
         p.c = a.c;
         p.q = a.q;

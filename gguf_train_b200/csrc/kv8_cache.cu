@@ -436,7 +436,7 @@ bool gather(const Kv8EvictArgs& a, cudaStream_t st) {
     const int64_t blocks = (rows + a.dst.block - 1) / a.dst.block, n = blocks * a.src.B * a.src.Hkv;
     if (!grid_fits(n, "kv8_evict")) return false;
     const int threads = threads_for(std::min<int64_t>(a.budget, a.dst.block) * (a.src.D / 16));
-    return launch_behind("kv8_evict: gather launch", kv8_gather_kernel<FMT, 4>, dim3((unsigned)n, 2), threads, st, a, (unsigned)blocks);
+    return launch_behind("kv8_evict: gather launch", kv8_gather_kernel<FMT, 4>, dim3((unsigned)n, 2), threads, st, 0, a, (unsigned)blocks);
 }
 
 }  // namespace

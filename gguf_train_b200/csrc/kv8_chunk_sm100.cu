@@ -1,0 +1,677 @@
+// Attention over the block-scaled 8-bit cache for many query rows (a chunk of a prompt): tcgen05 tensor cores.
+//
+// With hundreds of rows per kv head every cached value is used that often, so its codes are made into f16 once, by
+// a first kernel, and the second is a flash-style forward over f16 tiles:
+//   kv8_widen_kernel  K, V codes -> f16 (exact: int8 and e4m3 both fit), rows past the length zero, head size
+//                     padded to DP; q -> f16 rows r = i * G + g of each (sequence, kv head), normalised by a power
+//                     of two per row as in kv8_mma.cuh; the scales of every 16 keys as (sk, log2 sv, 1 / sv).
+//   kv8_chunk_kernel  one CTA per SM claims items (sequence, kv head, pair of 128-row tiles, part of the keys),
+//                     heaviest first. Twelve warps: TMA producer, MMA issuer, two idle, and four softmax warps per
+//                     tile, one row a thread, which ping-pong with the tensor core:
+//                       S_t = Q_t K_j^T (M = N = 128, K = DP),  O_t += P_t V_j (A = P_t from TMEM, V read MN-major).
+//                     Scores become log2 units with their 16 keys' scale, V's scale is folded into the exponent
+//                     (P' = 2^(s + log2 sv - M + 8), M raised when a block exceeds it by 2^7) and the row sum
+//                     takes P' / sv, so scales cost three packed operations per 16 keys and no accuracy.
+//   kv8_chunk_join_kernel  joins the parts where the keys were split (few items on many SMs).
+// The tile pair reuses each K/V tile for 256 rows; the second kernel is bound by the tensor core and the
+// exponentials. Every wait is bounded: a timeout records a status code, drains the CTA's own copies and MMAs,
+// frees TMEM and returns.
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "gtb_common.cuh"
+#include "kv8_chunk.h"
+#include "kv8_mma.cuh"
+#include "sdpa_args.h"
+#include "sm100_ptx.cuh"
+
+namespace gtb {
+namespace kv8 {
+namespace {
+
+using namespace sm100;
+
+constexpr int BM = 128, BN = 128, NTHREADS = 384, REG_LO = 104, REG_HI = 200;
+constexpr uint32_t TMEM_COLS = 512;
+
+template <int D>
+struct ChunkCfg {
+    static constexpr int ATOMS = D / 64;
+    static constexpr int TILE = BM * D * 2;
+    static constexpr int ATOM_BYTES = BM * 128;
+    static constexpr int OFF_K = 2 * TILE, OFF_V = 4 * TILE, OFF_BAR = 6 * TILE;  // Q_0 Q_1, two K stages, two V stages
+    static constexpr int NBAR = 1 + 8 + 2 + 2 + 2 + 1 + 1 + 2 + 2 + 2;
+    static constexpr int SMEM = OFF_BAR + NBAR * 8 + 32 + 1024;
+};
+
+struct ChunkP {
+    gtb_kv8 c;
+    Rows3 q, o;
+    int dtype, G, R, pairs, splits;
+    int64_t b0, nb;              // sequences of this launch
+    int64_t H, Lq;
+    float scale_log2;
+    const int32_t* counts;
+    float* lse;
+    int64_t Spad, Rpad;
+    __half *k16, *v16, *q16;     // [nb * Hkv][Spad | Rpad][DP]
+    float4* scl;                 // [nb * Hkv][Spad / 16]: sk, log2 sv, 1 / sv
+    float* qmul;                 // [nb * Hkv][Rpad]
+    float* part_o;               // [item][split][256][DP], splits > 1
+    float2* part_ml;             // [item][split][256]
+    int* claim;
+    int* status;
+};
+
+// Rows of codes to f16, q to normalised f16: one warp per row of 32-row groups; blockIdx.y = (sequence, kv head)
+template <int FMT, int DP>
+__global__ void __launch_bounds__(256) kv8_widen_kernel(const __grid_constant__ ChunkP p) {
+    const gtb_kv8& c = p.c;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.claim = 0;
+    const int k_ctas = (int)(p.Spad / 64);
+    const int64_t lbh = blockIdx.y, b = p.b0 + lbh / c.Hkv, hk = lbh % c.Hkv, bh = b * c.Hkv + hk;
+    const int len = (int)clamp64(c.lens[b], 0, c.Smax);
+    if ((int)blockIdx.x < k_ctas) {
+        // 64 rows of K and V; a thread makes 16 codes into 32 bytes
+        const int r0 = blockIdx.x * 64;
+        if (r0 >= (len + BN - 1) / BN * BN) return;  // no tile reads them
+        constexpr int CPR = DP / 16;
+        for (int e = threadIdx.x; e < 2 * 64 * CPR; e += 256) {
+            const int v = e >= 64 * CPR, x = v ? e - 64 * CPR : e, row = r0 + x / CPR, ch = x % CPR;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (row < len && ch * 16 < c.D) w = *(const uint4*)((const uint8_t*)(v ? c.v : c.k) + (bh * c.Smax + row) * c.D + ch * 16);
+            const uint32_t u[4] = {prep_word<FMT>(w.x), prep_word<FMT>(w.y), prep_word<FMT>(w.z), prep_word<FMT>(w.w)};
+            uint4* dst = (uint4*)((v ? p.v16 : p.k16) + (lbh * p.Spad + row) * DP + ch * 16);
+            dst[0] = make_uint4(expand<FMT, 0>(u[0]), expand<FMT, 1>(u[0]), expand<FMT, 0>(u[1]), expand<FMT, 1>(u[1]));
+            dst[1] = make_uint4(expand<FMT, 0>(u[2]), expand<FMT, 1>(u[2]), expand<FMT, 0>(u[3]), expand<FMT, 1>(u[3]));
+        }
+        if (threadIdx.x < 4) {
+            const int k = r0 + threadIdx.x * 16;
+            float4 s = make_float4(0.0f, 0.0f, 1.0f, 0.0f);
+            if (k < len) {
+                const int64_t at = bh * ((c.Smax + c.block - 1) / c.block) + k / c.block;
+                const float sv = fmaxf(c.v_scale[at], SV_MIN);
+                s = make_float4(c.k_scale[at], lg2f(sv), __frcp_rn(sv), 0.0f);
+            }
+            p.scl[lbh * (p.Spad / 16) + k / 16] = s;
+        }
+        return;
+    }
+    // 32 rows of q, a warp each four
+    const int g0 = ((int)blockIdx.x - k_ctas) * 32;
+    for (int rr = warp; rr < 32; rr += 8) {
+        const int r = g0 + rr, i = r / p.G, h = (int)hk * p.G + (r - i * p.G);
+        const int64_t es = p.dtype == F32 ? 4 : 2;
+        const unsigned char* row = (const unsigned char*)p.q.p + (b * p.q.sb + h * p.q.sh + (int64_t)i * p.q.ss) * es;
+        float x[DP / 32], m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k) {
+            const int d = 2 * lane + (k & 1) + 64 * (k >> 1);
+            x[k] = r < p.R && d < c.D ? load_any<float>(row, d, p.dtype) : 0.0f;
+            m = fmaxf(m, finite_abs(x[k]));
+        }
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        int e = (int)(__float_as_uint(m) >> 23) - 127;
+        e = m >= 1.17549435e-38f ? min(max(e, -126), 126) : 0;
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        __half2* dst = (__half2*)(p.q16 + (lbh * p.Rpad + r) * DP);
+#pragma unroll
+        for (int k = 0; k < DP / 64; ++k) dst[lane + 32 * k] = __floats2half2_rn(x[2 * k] * down, x[2 * k + 1] * down);
+        if (lane == 0) p.qmul[lbh * p.Rpad + r] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+    }
+}
+
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+    const bool ok = mbar_wait(bar, parity, status, code);
+    return __all_sync(0xffffffffu, ok);
+}
+
+template <int D>
+__global__ void __launch_bounds__(NTHREADS, 1)
+kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ ChunkP p) {
+    using C = ChunkCfg<D>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = (uint64_t*)(smem + C::OFF_BAR);
+    uint64_t* q_full = bars;
+    uint64_t* k_full = bars + 1;         // [2]
+    uint64_t* k_empty = k_full + 2;      // [2]
+    uint64_t* v_full = k_empty + 2;      // [2]
+    uint64_t* v_empty = v_full + 2;      // [2]
+    uint64_t* s_full = v_empty + 2;      // [2] per tile: S_t(j) computed
+    uint64_t* p_full = s_full + 2;       // [2] per tile: P_t(j) written (128 arrivals)
+    uint64_t* o_final = p_full + 2;      // [2] per tile: every MMA of the tile done
+    uint64_t* drain = o_final + 2;
+    uint64_t* q_empty = drain + 1;       // every S MMA of an item done
+    uint64_t* o_empty = q_empty + 1;     // [2] per tile: the epilogue has read O_t (128 arrivals)
+    uint64_t* item_full = o_empty + 2;   // [2] ring of claimed items
+    uint64_t* item_empty = item_full + 2;
+    uint32_t* tmem_slot = (uint32_t*)(bars + C::NBAR);
+    int* abort_flag = (int*)(tmem_slot + 1);
+    int* item_slot = abort_flag + 1;     // [2]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int heads = (int)(p.nb * p.c.Hkv), n_items = heads * p.pairs * p.splits;
+
+    // Item i = (pair of tiles, last first; part of the keys; sequence x kv head fastest). nblk[t]: key blocks of tile
+    // t in this part; j0: the part's first block; n: blocks to load.
+    struct Item {
+        int bh, pair, split, row0[2], nblk[2], j0, n, len, cnt;
+    };
+    auto item_of = [&](int i) {
+        Item it;
+        const int rest = i / heads;
+        it.bh = i - rest * heads;
+        it.pair = p.pairs - 1 - rest / p.splits;
+        it.split = rest % p.splits;
+        const int64_t b = p.b0 + it.bh / p.c.Hkv;
+        it.len = (int)clamp64(p.c.lens[b], 0, p.c.Smax);
+        it.cnt = p.counts ? (int)clamp64(p.counts[b], 0, p.Lq) : (int)p.Lq;
+        int blk[2];
+        for (int t = 0; t < 2; ++t) {
+            it.row0[t] = it.pair * 2 * BM + t * BM;
+            const int last = min(it.row0[t] + BM, it.cnt * p.G) - 1;  // last row that has a query
+            const int lim = last < it.row0[t] ? -1 : it.len - it.cnt + last / p.G;
+            blk[t] = lim < 0 ? 0 : lim / BN + 1;
+        }
+        const int all = max(blk[0], blk[1]);
+        it.j0 = (int)((int64_t)all * it.split / p.splits);
+        const int j1 = (int)((int64_t)all * (it.split + 1) / p.splits);
+        it.n = 0;
+        for (int t = 0; t < 2; ++t) {
+            it.nblk[t] = max(0, min(j1, blk[t]) - it.j0);
+            it.n = max(it.n, it.nblk[t]);
+        }
+        return it;
+    };
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&o_final[i], 1); mbar_init(&o_empty[i], 128);
+            mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], 9);
+        }
+        mbar_init(q_empty, 1);
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, TMEM_COLS);
+    cudaTriggerProgrammaticLaunchCompletion();
+    cudaGridDependencySynchronize();  // the widened rows and the item counter are there
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    static_assert(128 * REG_LO + 256 * REG_HI <= NTHREADS * 168, "register split above the launch's registers");
+
+    if (warp < 4) {
+        setmaxnreg_dec<REG_LO>();
+        if (warp == 0) {
+            if (lane == 0) {
+                prefetch_tmap(&tmQ);
+                prefetch_tmap(&tmK);
+                prefetch_tmap(&tmV);
+                int J = 0, work = 0, nk = 0, nv = 0, nq = 0;  // blocks, items with work, loads so far
+                bool ok = true;
+                int next = atomicAdd(p.claim, 1);
+                for (int nitem = 0;; ++nitem) {
+                    const int i = next, slot = nitem & 1;
+                    if (nitem >= 2) ok = mbar_wait(&item_empty[slot], ((nitem >> 1) - 1) & 1, p.status, 111);
+                    if (!ok || *(volatile int*)abort_flag) { ok = false; break; }
+                    item_slot[slot] = i < n_items ? i : -1;
+                    mbar_arrive(&item_full[slot]);
+                    if (i >= n_items) break;
+                    next = atomicAdd(p.claim, 1);
+                    const Item it = item_of(i);
+                    if (it.n == 0) continue;
+                    const int nt = it.nblk[1] > 0 ? 2 : 1;
+                    auto load_q = [&]() {
+                        mbar_expect_tx(q_full, nt * C::TILE);
+                        for (int t = 0; t < nt; ++t)
+                            for (int a = 0; a < C::ATOMS; ++a)
+                                tma_load_4d(smem + t * C::TILE + a * C::ATOM_BYTES, &tmQ, a * 64, it.row0[t], it.bh, 0, q_full);
+                        ++nq;
+                    };
+                    if (work == 0) load_q();
+                    for (int j = 0; j < it.n; ++j, ++J) {
+                        const int s = J & 1;
+                        if (J >= 2) ok = mbar_wait(&k_empty[s], ((J >> 1) - 1) & 1, p.status, 112);
+                        if (!ok || *(volatile int*)abort_flag) { ok = false; break; }
+                        mbar_expect_tx(&k_full[s], C::TILE);
+                        for (int a = 0; a < C::ATOMS; ++a)
+                            tma_load_4d(smem + C::OFF_K + s * C::TILE + a * C::ATOM_BYTES, &tmK, a * 64, (it.j0 + j) * BN, it.bh, 0, &k_full[s]);
+                        ++nk;
+                        if (J >= 2) ok = mbar_wait(&v_empty[s], ((J >> 1) - 1) & 1, p.status, 113);
+                        if (!ok || *(volatile int*)abort_flag) { ok = false; break; }
+                        mbar_expect_tx(&v_full[s], C::TILE);
+                        for (int a = 0; a < C::ATOMS; ++a)
+                            tma_load_4d(smem + C::OFF_V + s * C::TILE + a * C::ATOM_BYTES, &tmV, a * 64, (it.j0 + j) * BN, it.bh, 0, &v_full[s]);
+                        ++nv;
+                        if (j == 0 && work > 0) {  // Q once the previous item's S MMAs have read theirs
+                            ok = mbar_wait(q_empty, (work - 1) & 1, p.status, 114);
+                            if (!ok || *(volatile int*)abort_flag) { ok = false; break; }
+                            load_q();
+                        }
+                    }
+                    if (!ok) break;
+                    ++work;
+                }
+                if (!ok) *(volatile int*)abort_flag = 1;
+                if (*(volatile int*)abort_flag) {  // drain our own copies (bounded)
+                    if (nq > 0) mbar_wait(q_full, (nq - 1) & 1, nullptr, 0);
+                    for (int j = max(0, nk - 2); j < nk; ++j) mbar_wait(&k_full[j & 1], (j >> 1) & 1, nullptr, 0);
+                    for (int j = max(0, nv - 2); j < nv; ++j) mbar_wait(&v_full[j & 1], (j >> 1) & 1, nullptr, 0);
+                }
+            }
+        } else if (warp == 1) {
+            if (lane == 0) {
+                constexpr uint32_t IDESC_S = idesc_f16(BM, BN, false, false), IDESC_PV = idesc_f16(BM, D, false, true);
+                const uint64_t qd[2] = {desc_sw128(smem_u32(smem), 16, 1024), desc_sw128(smem_u32(smem + C::TILE), 16, 1024)};
+                const uint64_t kd0 = desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024);
+                const uint64_t kd1 = desc_sw128(smem_u32(smem + C::OFF_K + C::TILE), 16, 1024);
+                const uint64_t vd0 = desc_sw128(smem_u32(smem + C::OFF_V), C::ATOM_BYTES, 1024);
+                const uint64_t vd1 = desc_sw128(smem_u32(smem + C::OFF_V + C::TILE), C::ATOM_BYTES, 1024);
+                int J = 0, u[2] = {0, 0}, nf[2] = {0, 0}, work = 0;
+                auto issue_s = [&](int t, int jg) -> bool {
+                    if (!mbar_wait(&k_full[jg & 1], (jg >> 1) & 1, p.status, 122)) return false;
+                    tc_fence_after();
+                    const uint64_t qb = t ? qd[1] : qd[0], kb = (jg & 1) ? kd1 : kd0;
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (uint32_t)((kk / 4) * C::ATOM_BYTES + (kk % 4) * 32);
+                        mma_ss(tmem + t * 128u, desc_advance(qb, off), desc_advance(kb, off), IDESC_S, kk > 0 ? 1u : 0u);
+                    }
+                    mma_commit(&s_full[t]);
+                    return true;
+                };
+                auto issue_pv = [&](int t, int jg, int ut, bool first) -> bool {
+                    if (!mbar_wait(&p_full[t], ut & 1, p.status, 123)) return false;
+                    if (!mbar_wait(&v_full[jg & 1], (jg >> 1) & 1, p.status, 124)) return false;
+                    tc_fence_after();
+                    const uint64_t vb = (jg & 1) ? vd1 : vd0;
+                    const uint32_t pa = tmem + t * 128u;
+#pragma unroll
+                    for (int kk = 0; kk < BN / 16; ++kk)
+                        mma_ts(tmem + 256u + t * 128u, pa + 32 * (kk >> 1) + 8 * (kk & 1), desc_advance(vb, kk * 2048), IDESC_PV,
+                               (!first || kk > 0) ? 1u : 0u);
+                    return true;
+                };
+                bool ok = true;
+                for (int nitem = 0;; ++nitem) {
+                    const int slot = nitem & 1;
+                    ok = mbar_wait(&item_full[slot], (nitem >> 1) & 1, p.status, 127);
+                    if (!ok) break;
+                    const int i = item_slot[slot];
+                    mbar_arrive(&item_empty[slot]);
+                    if (i < 0) break;
+                    const Item it = item_of(i);
+                    if (it.n == 0) continue;
+                    ok = mbar_wait(q_full, work & 1, p.status, 121);
+                    ++work;
+                    for (int t = 0; t < 2 && ok; ++t)
+                        if (it.nblk[t] > 0) ok = issue_s(t, J);
+                    if (!ok) break;
+                    mma_commit(&k_empty[J & 1]);
+                    if (it.n == 1) mma_commit(q_empty);
+                    for (int j = 0; j < it.n && ok; ++j) {
+                        for (int t = 0; t < 2 && ok; ++t) {
+                            if (j >= it.nblk[t]) continue;
+                            if (j == 0 && nf[t] > 0) ok = mbar_wait(&o_empty[t], (nf[t] - 1) & 1, p.status, 126);
+                            if (ok) ok = issue_pv(t, J + j, u[t] + j, j == 0);
+                            if (ok && j + 1 < it.nblk[t]) ok = issue_s(t, J + j + 1);
+                            if (ok && j + 1 == it.nblk[t]) mma_commit(&o_final[t]);
+                        }
+                        if (!ok || *(volatile int*)abort_flag) { ok = false; break; }
+                        mma_commit(&v_empty[(J + j) & 1]);
+                        if (j + 1 < it.n) mma_commit(&k_empty[(J + j + 1) & 1]);
+                        if (j + 2 == it.n) mma_commit(q_empty);
+                    }
+                    if (!ok) break;
+                    J += it.n;
+                    for (int t = 0; t < 2; ++t) {
+                        u[t] += it.nblk[t];
+                        nf[t] += it.nblk[t] > 0 ? 1 : 0;
+                    }
+                }
+                if (!ok) *(volatile int*)abort_flag = 1;
+                if (*(volatile int*)abort_flag) {
+                    mma_commit(drain);
+                    mbar_wait(drain, 0, nullptr, 0);
+                }
+            }
+        }
+    } else {
+        setmaxnreg_inc<REG_HI>();
+        const int t = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane;
+        const uint32_t s_tmem = tmem + ((uint32_t)(quad * 32) << 16) + t * 128u;
+        const uint32_t o_tmem = s_tmem - t * 128u + 256u + t * 128u;
+        int u = 0, nf = 0;
+        bool ok = true;
+        for (int nitem = 0; ok; ++nitem) {
+            const int slot = nitem & 1;
+            ok = warp_wait(&item_full[slot], (nitem >> 1) & 1, p.status, 134);
+            if (!ok) break;
+            const int i = item_slot[slot];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&item_empty[slot]);
+            if (i < 0) break;
+            const Item it = item_of(i);
+            const int nb = it.nblk[t], row = it.row0[t] + r, qi = row / p.G;
+            const bool valid = row < p.R && qi < it.cnt;
+            const int lim = valid ? it.len - it.cnt + qi : -1;          // last key this row may see
+            const int lim0 = it.row0[t] / p.G + it.len - it.cnt;        // ... the tile's first row
+            const float qmul = p.qmul[(int64_t)it.bh * p.Rpad + row];
+            const float4* scl = p.scl + (int64_t)it.bh * (p.Spad / 16) + it.j0 * 8;
+            float m_used = -INFINITY, lsum = 0.0f;
+            for (int j = 0; j < nb; ++j) {
+                ok = warp_wait(&s_full[t], (u + j) & 1, p.status, 131);
+                if (!ok || __any_sync(0xffffffffu, *(volatile int*)abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const int kv0 = (it.j0 + j) * BN;
+                const float4* sc = scl + j * 8;
+                uint32_t raw[128];
+                tmem_ld32(s_tmem, raw);
+                tmem_ld32(s_tmem + 32, raw + 32);
+                tmem_ld32(s_tmem + 64, raw + 64);
+                tmem_ld32(s_tmem + 96, raw + 96);
+                tmem_ld_wait();
+                float* x = (float*)raw;
+                if (kv0 + BN - 1 > lim0) {
+#pragma unroll
+                    for (int e = 0; e < 128; ++e)
+                        if (kv0 + e > lim) x[e] = -INFINITY;
+                }
+                // largest s + log2 sv of the block: per 16 keys the scale is one
+                const float m_start = m_used;
+                float cm = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    const float4 z = __ldg(sc + g);
+                    const float* y = x + 16 * g;
+                    float a = fmax3(y[0], y[1], y[2]), b = fmax3(y[3], y[4], y[5]), d = fmax3(y[6], y[7], y[8]);
+                    a = fmax3(a, y[9], y[10]);
+                    b = fmax3(b, y[11], y[12]);
+                    d = fmax3(d, y[13], y[14]);
+                    a = fmax3(fmax3(a, b, d), y[15], y[15]);
+                    cm = fmaxf(cm, fmaf(a, fmaxf(qmul * z.x, 1e-37f), z.y));
+                }
+                if (cm > m_used + RAISE) m_used = cm;  // never while the row has no finite score
+                const bool grew = m_used != m_start;
+                const float off = m_used == -INFINITY ? 0.0f : SHIFT - m_used;
+                float block_sum = 0.0f;
+#pragma unroll
+                for (int g2 = 0; g2 < 4; ++g2) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float4 z = __ldg(sc + 2 * g2 + h);
+                        const float mul = fmaxf(qmul * z.x, 1e-37f), add = z.y + off;
+                        const uint64_t mul2 = f2_pack(mul, mul), add2 = f2_pack(add, add);
+                        uint64_t sum2 = 0ull;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const int at = 32 * g2 + 16 * h + e;
+                            float a0, a1;
+                            f2_unpack(f2_fma(f2_pack(x[at], x[at + 1]), mul2, add2), a0, a1);
+                            const float p0 = ex2(a0), p1 = ex2(a1);
+                            sum2 = f2_add(sum2, f2_pack(p0, p1));
+                            pk[8 * h + e / 2] = pack_f16(p0, p1);
+                        }
+                        float s0, s1;
+                        f2_unpack(sum2, s0, s1);
+                        block_sum = fmaf(s0 + s1, z.z, block_sum);
+                    }
+                    tmem_st16(s_tmem + 32 * g2, pk);
+                }
+                if (__any_sync(0xffffffffu, grew && j > 0)) {
+                    // PV_t(j-1) is complete: it was issued before S_t(j), whose completion we have seen
+                    const float alpha = grew ? ex2(m_start - m_used) : 1.0f;
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t ov[32];
+                        tmem_ld32(o_tmem + c * 32, ov);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) ov[e] = __float_as_uint(__uint_as_float(ov[e]) * alpha);
+                        tmem_st32(o_tmem + c * 32, ov);
+                    }
+                }
+                lsum = (grew ? lsum * ex2(m_start - m_used) : lsum) + block_sum;
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(&p_full[t]);
+            }
+            if (!ok) break;
+            u += nb;
+            // results: the row's values, or its part of them; zeros for a row that attends nothing
+            const bool whole = p.splits == 1;
+            if (nb > 0) {
+                if (*(volatile int*)abort_flag) ok = false;
+                ok = __all_sync(0xffffffffu, ok) && warp_wait(&o_final[t], nf & 1, p.status, 133);
+                if (!ok) break;
+                tc_fence_after();
+            }
+            const float inv = !whole ? 1.0f : lsum > 0.0f || !(lsum == lsum) ? 1.0f / lsum : 0.0f;
+            const int64_t b = p.b0 + it.bh / p.c.Hkv;
+            const int h = (it.bh % (int)p.c.Hkv) * p.G + (row - qi * p.G);
+            const int64_t at = b * p.o.sb + (int64_t)h * p.o.sh + (int64_t)qi * p.o.ss;
+            const int64_t prow = (((int64_t)(it.bh * p.pairs + it.pair) * p.splits + it.split) * 2 + t) * BM + r;
+            const float m_out = m_used == -INFINITY ? -INFINITY : m_used - SHIFT;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t ov[32];
+                if (nb > 0) {
+                    tmem_ld32(o_tmem + c * 32, ov);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) ov[e] = 0u;
+                }
+                if (!whole) {
+                    uint4* dst = (uint4*)(p.part_o + prow * D + c * 32);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) dst[q] = make_uint4(ov[4 * q], ov[4 * q + 1], ov[4 * q + 2], ov[4 * q + 3]);
+                } else if (row < p.R) {
+                    float y[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) y[e] = valid ? __uint_as_float(ov[e]) * inv : 0.0f;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int d = c * 32 + 8 * q;
+                        if (d >= p.c.D) continue;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (p.dtype == F16) w[e] = pack_f16(y[8 * q + 2 * e], y[8 * q + 2 * e + 1]);
+                            else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e]) : "f"(y[8 * q + 2 * e + 1]), "f"(y[8 * q + 2 * e]));
+                        }
+                        *(uint4*)((uint16_t*)p.o.p + at + d) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+            if (!whole) p.part_ml[prow] = make_float2(!(lsum == lsum) ? lsum : m_out, lsum);
+            else if (p.lse && row < p.R)
+                p.lse[(b * p.H + h) * p.Lq + qi] = !valid || lsum == 0.0f ? -INFINITY : (m_out + log2f(lsum)) * 0.6931471805599453f;
+            if (nb > 0) {
+                tc_fence_before();
+                mbar_arrive(&o_empty[t]);
+                ++nf;
+            }
+        }
+        if (!ok) *(volatile int*)abort_flag = 1;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+// One warp per row joins its parts
+template <int D>
+__global__ void __launch_bounds__(256) kv8_chunk_join_kernel(const __grid_constant__ ChunkP p) {
+    cudaGridDependencySynchronize();
+    const int lane = threadIdx.x & 31;
+    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t bh = w / p.R;
+    const int row = (int)(w - bh * p.R);
+    if (bh >= p.nb * p.c.Hkv) return;
+    const int64_t b = p.b0 + bh / p.c.Hkv;
+    const int cnt = p.counts ? (int)clamp64(p.counts[b], 0, p.Lq) : (int)p.Lq;
+    const int pair = row / (2 * BM), qi = row / p.G, h = (int)(bh % p.c.Hkv) * p.G + (row - qi * p.G);
+    const int64_t first = ((bh * p.pairs + pair) * p.splits * 2) * BM + row % (2 * BM);  // + split * 2 * BM
+    float m = -INFINITY, l = 0.0f, acc[D / 32] = {};
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[first + (int64_t)s * 2 * BM].x);
+    if (m == -INFINITY) m = 0.0f;
+    for (int s = 0; s < p.splits; ++s) {
+        const int64_t at = first + (int64_t)s * 2 * BM;
+        const float2 ml = p.part_ml[at];
+        const float f = ex2f(ml.x - m);
+        l = fmaf(ml.y, f, l);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(p.part_o[at * D + i * 32 + lane], f, acc[i]);
+    }
+    const bool none = qi >= cnt || l == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / l;
+    const int64_t at = b * p.o.sb + (int64_t)h * p.o.sh + (int64_t)qi * p.o.ss;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+        const int d = i * 32 + lane;
+        if (d >= p.c.D) continue;
+        const float y = none ? 0.0f : acc[i] * inv;
+        if (p.dtype == F16) ((__half*)p.o.p)[at + d] = __float2half_rn(y);
+        else ((__nv_bfloat16*)p.o.p)[at + d] = __float2bfloat16_rn(y);
+    }
+    if (p.lse && lane == 0) p.lse[(b * p.H + h) * p.Lq + qi] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+template <int D>
+int set_up() {
+    static std::atomic<uint64_t> ready{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 64 && (ready.load(std::memory_order_relaxed) >> dev & 1)) return 0;
+    auto kern = kv8_chunk_kernel<D>;
+    if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkCfg<D>::SMEM), "kv8_attention: shared memory"))
+        return -1;
+    // setmaxnreg.inc waits until the block's registers cover the split: refuse a build with fewer
+    cudaFuncAttributes fa;
+    if (cuda_failed(cudaFuncGetAttributes(&fa, kern), "kv8_attention: attributes")) return -1;
+    if ((int64_t)fa.numRegs * NTHREADS < 128 * REG_LO + 256 * REG_HI) {
+        set_errorf("kv8_attention: the chunk kernel was built with %d registers a thread, too few for its split", fa.numRegs);
+        return -1;
+    }
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    return 0;
+}
+
+bool map_rows(CUtensorMap* tm, void* data, int64_t heads, int64_t rows, int64_t D) {
+    gtb_tensor4 t{};
+    t.data = data;
+    t.shape[0] = 1; t.shape[1] = heads; t.shape[2] = rows; t.shape[3] = D;
+    t.stride[0] = heads * rows * D; t.stride[1] = rows * D; t.stride[2] = D; t.stride[3] = 1;
+    t.dtype = F16;
+    return make_tma_map_4d(tm, t, D, false, 128);
+}
+
+template <int D>
+int run(const Kv8AttnArgs& a, float* lse, int n_sm, cudaStream_t st) {
+    if (set_up<D>()) return -1;
+    ChunkP p{};
+    p.c = a.c;
+    p.q = a.q;
+    p.o = a.o;
+    p.dtype = a.dtype;
+    p.G = (int)(a.H / a.c.Hkv);
+    p.R = p.G * (int)a.Lq;
+    p.pairs = (p.R + 2 * BM - 1) / (2 * BM);
+    p.H = a.H;
+    p.Lq = a.Lq;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.counts = a.counts;
+    p.lse = lse;
+    p.Spad = (a.c.Smax + BN - 1) / BN * BN;
+    p.Rpad = (int64_t)p.pairs * 2 * BM;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    p.status = device_status_word(dev);
+    auto up = [](int64_t n) { return (n + 1023) / 1024 * 1024; };
+    // scratch of one sequence; as many sequences a launch as stay within 2 GB (one at least)
+    const int64_t Hkv = a.c.Hkv;
+    const int64_t per_seq = Hkv * (p.Spad * D * 4 + p.Spad + p.Rpad * (D * 2 + 4));
+    const int64_t nb = std::max<int64_t>(1, std::min<int64_t>(a.c.B, (2ll << 30) / std::max<int64_t>(per_seq, 1)));
+    // split the keys where there are too few items for the SMs, down to 512 keys a part
+    const int64_t items = nb * Hkv * p.pairs;
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * n_sm + items - 1) / items, p.Spad / 512));
+    if (items >= n_sm) p.splits = 1;
+    if (items * p.splits > INT32_MAX / 2 || nb * Hkv > 65535) {
+        set_error("kv8_attention: too many work items");
+        return -1;
+    }
+    const int64_t heads = nb * Hkv;
+    const int64_t b_kv = up(heads * p.Spad * D * 2), b_q = up(heads * p.Rpad * D * 2), b_s = up(heads * p.Spad), b_m = up(heads * p.Rpad * 4);
+    const int64_t prows = p.splits > 1 ? items * p.splits * 2 * BM : 0;
+    const int64_t b_po = up(prows * D * 4), b_pm = up(prows * 8);
+    char* mem = nullptr;
+    if (cuda_failed(cudaMallocAsync((void**)&mem, 2 * b_kv + b_q + b_s + b_m + b_po + b_pm + 1024, st), "kv8_attention: scratch allocation"))
+        return -1;
+    char* at = mem;
+    auto take = [&](int64_t n) { char* r = at; at += n; return (void*)r; };
+    p.k16 = (__half*)take(b_kv);
+    p.v16 = (__half*)take(b_kv);
+    p.q16 = (__half*)take(b_q);
+    p.scl = (float4*)take(b_s);
+    p.qmul = (float*)take(b_m);
+    p.part_o = (float*)take(b_po);
+    p.part_ml = (float2*)take(b_pm);
+    p.claim = (int*)take(1024);
+    bool bad = false;
+    for (int64_t b0 = 0; b0 < a.c.B && !bad; b0 += nb) {
+        p.b0 = b0;
+        p.nb = std::min(nb, a.c.B - b0);
+        const int64_t h = p.nb * Hkv;
+        CUtensorMap mq, mk, mv;
+        if (!map_rows(&mq, p.q16, h, p.Rpad, D) || !map_rows(&mk, p.k16, h, p.Spad, D) || !map_rows(&mv, p.v16, h, p.Spad, D)) {
+            bad = true;
+            break;
+        }
+        const dim3 grid((unsigned)(p.Spad / 64 + p.Rpad / 32), (unsigned)h);
+        if (a.c.format == GTB_KV8_INT8) kv8_widen_kernel<GTB_KV8_INT8, D><<<grid, 256, 0, st>>>(p);
+        else kv8_widen_kernel<GTB_KV8_E4M3, D><<<grid, 256, 0, st>>>(p);
+        bad = cuda_failed(cudaGetLastError(), "kv8_attention: widen launch");
+        if (bad) break;
+        const int64_t n = h * p.pairs * p.splits;
+        bad = !launch_behind("kv8_attention: chunk launch", kv8_chunk_kernel<D>, dim3((unsigned)std::min<int64_t>(n, n_sm)), NTHREADS, st,
+                             ChunkCfg<D>::SMEM, mq, mk, mv, p);
+        if (!bad && p.splits > 1)
+            bad = !launch_behind("kv8_attention: join launch", kv8_chunk_join_kernel<D>, dim3((unsigned)((h * p.R + 7) / 8)), 256, st, 0, p);
+    }
+    cudaFreeAsync(mem, st);
+    return bad ? -1 : 0;
+}
+
+}  // namespace
+
+bool chunk_supported(const Kv8AttnArgs& a) {
+    const int64_t R = a.H / a.c.Hkv * a.Lq;
+    return a.dtype != F32 && a.c.D <= 128 && R > CHUNK_ROWS && a.c.Smax > 0 && a.c.Hkv <= 65535 && R < (1 << 28) && encode_fn() != nullptr;
+}
+
+int launch_chunk(const Kv8AttnArgs& a, float* lse, int n_sm, cudaStream_t st) {
+    return a.c.D <= 64 ? run<64>(a, lse, n_sm, st) : run<128>(a, lse, n_sm, st);
+}
+
+}  // namespace kv8
+}  // namespace gtb

@@ -754,7 +754,7 @@ int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
             set_error("kv8_attention: too many query rows");
             bad = true;
         } else {
-            bad = !launch_behind("kv8_attention: finish launch", kv8_finish_kernel<DP>, dim3((unsigned)(joins + sums)), 128, st, p,
+            bad = !launch_behind("kv8_attention: finish launch", kv8_finish_kernel<DP>, dim3((unsigned)(joins + sums)), 128, st, 0, p,
                                  8 * NT, (unsigned)joins);
         }
     }
