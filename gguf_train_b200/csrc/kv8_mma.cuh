@@ -1,7 +1,7 @@
 // Attention over the block-scaled 8-bit cache for few query rows, on warp-level matrix instructions.
 //
 // One work item is 8 * NT query rows of one (sequence, kv head): the G = H / Hkv query heads times the Lq
-// queries, row = i * G + g. The keys are cut into units of 32; all units of all items form one line, of which
+// queries, row = i * G + g. The keys are cut into units of 16 or 32; all units of all items form one line, of which
 // every warp takes an equal stretch (so the split adapts to the lengths and no warp waits for another). A
 // warp that finishes an item alone writes the result; otherwise it leaves (out, max, sum) for
 // kv8_finish_kernel.
@@ -32,9 +32,8 @@
 namespace gtb {
 namespace kv8 {
 
-constexpr int UNIT = 32;        // keys per unit
 constexpr float SV_MIN = 7.888609052210118e-31f;  // 2^-100
-constexpr float RAISE = 7.0f, SHIFT = 8.0f;
+constexpr float RAISE = 7.0f, SHIFT = 8.0f, NONE = -1e30f;  // NONE: no key seen yet
 
 struct MmaP {
     gtb_kv8 c;
@@ -147,29 +146,37 @@ struct Lay<256> {
     __device__ static int swz(int r) { return (r & 6) ^ ((r & 1) << 2); }
 };
 
+// Units, warps and stages. More warps hide the dependent chain of a unit (scores, exponentials, second product); their
+// number is what the registers (O alone takes NT DP / 4) and two stages of each warp's ring allow.
 template <int DP, int NT, int NS>
 struct MmaCfg {
-    static constexpr bool QREG = NT * NS == 1;
+    static constexpr bool QREG = NT * NS == 1 && DP <= 128;
     static constexpr int KSTEPS = DP / 16;
-    static constexpr int STAGE = 2 * UNIT * DP + 16;  // K rows, V rows, scales k0 k1 v0 v1
+    static constexpr int OREGS = NT * DP / 4;
+    static constexpr int SUB = OREGS > 32 ? 1 : 2;    // 16-key products per unit
+    static constexpr int UNIT = 16 * SUB;
+    static constexpr int STAGE = 2 * UNIT * DP + 16;  // K rows, V rows, scales (k, v of each 16 keys)
     static constexpr int QBYTES = QREG ? 0 : KSTEPS * NT * NS * 32 * 8;
-    static constexpr int WARPS = DP == 256 ? 4 : NT * NS == 8 ? 6 : 8;
-    // as many stages as fit beside each other, 6 at most
-    static constexpr int FIT = (224 * 1024 / WARPS - QBYTES) / STAGE;
-    static constexpr int STAGES = FIT > 6 ? 6 : FIT;
+    static constexpr int SPACE = 224 * 1024;
+    static constexpr int fit(int warps) { return (SPACE / warps - QBYTES) / STAGE; }
+    static constexpr int pick() {
+        const int most = OREGS <= 16 ? 16 : OREGS <= 64 ? 12 : 8;
+        for (int w = most; w > 4; w -= 2)
+            if (fit(w) >= 2) return w;
+        return 4;
+    }
+    static constexpr int WARPS = pick();
+    static constexpr int STAGES = fit(WARPS) > 6 ? 6 : fit(WARPS);
     static_assert(STAGES >= 2, "a stage in work and one in flight");
     static constexpr int WARP_SMEM = STAGES * STAGE + QBYTES;
     static constexpr int SMEM = WARPS * WARP_SMEM;
 };
 
-// One query row's value d as f32, any type
-__device__ __forceinline__ float load_q(const MmaP& p, const void* row, int d) { return load_any<float>(row, d, p.dtype); }
-
 template <int DP, int FMT, int NT, int NS>
-__global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_kernel(const MmaP p) {
+__global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_kernel(const __grid_constant__ MmaP p) {
     using C = MmaCfg<DP, NT, NS>;
     using L = Lay<DP>;
-    constexpr int ROWS = 8 * NT, OM = DP / 16;  // OM: products of 16 dims
+    constexpr int ROWS = 8 * NT, OM = DP / 16, SUB = C::SUB, UNIT = C::UNIT;  // OM: products of 16 dims
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int64_t seg[C::WARPS * 32 + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -178,13 +185,13 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
     cudaTriggerProgrammaticLaunchCompletion();
 
     auto len_of = [&](int64_t b) { return (int)clamp64(c.lens[b], 0, c.Smax); };
-    auto units_of = [&](int64_t b) { return (int64_t)max(1, (len_of(b) + UNIT - 1) / UNIT); };
+    auto units_in = [&](int len) { return max(1, (len + UNIT - 1) / UNIT); };
 
     // units before each thread's share of the sequences
     const int64_t share = (c.B + blockDim.x - 1) / blockDim.x;
     {
         int64_t n = 0;
-        for (int64_t b = threadIdx.x * share; b < min(c.B, (threadIdx.x + 1) * share); ++b) n += units_of(b);
+        for (int64_t b = threadIdx.x * share; b < min(c.B, (threadIdx.x + 1) * share); ++b) n += units_in(len_of(b));
         int64_t x = n;
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
@@ -204,87 +211,97 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
     const int64_t NW = min((int64_t)gridDim.x * C::WARPS, U);
     const int64_t wid = (int64_t)warp * gridDim.x + blockIdx.x;
     if (wid >= NW) return;
-    const int64_t u0 = wid * U / NW, u1 = (wid + 1) * U / NW;
+    const int64_t u0 = wid * U / NW;
+    const int n_units = (int)((wid + 1) * U / NW - u0);
 
-    // the sequence and item of unit u0
+    // where unit u0 is: its sequence, the item in it, the unit in the item
     int lo = 0, hi = blockDim.x;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (seg[mid] <= u0) lo = mid;
         else hi = mid;
     }
-    int64_t b = lo * share, base = seg[lo];
+    int b = (int)(lo * share);
+    int64_t base = seg[lo];
+    int len = len_of(b);
     for (;;) {
-        const int64_t n = units_of(b) * per_seq;
+        const int64_t n = (int64_t)units_in(len) * per_seq;
         if (base + n > u0) break;
         base += n;
-        ++b;
+        len = len_of(++b);
     }
-    // state of the unit to load next and of the unit to work on next: sequence, item in it, unit in the item
     struct Cursor {
-        int64_t b;
-        int len, units, item, unit;
+        int b, len, units, item, unit;
     };
-    Cursor ld;
-    ld.b = b;
-    ld.len = len_of(b);
-    ld.units = (int)units_of(b);
-    ld.item = (int)((u0 - base) / ld.units);
-    ld.unit = (int)((u0 - base) - (int64_t)ld.item * ld.units);
-    Cursor wk = ld;
+    Cursor wk;
+    wk.b = b;
+    wk.len = len;
+    wk.units = units_in(len);
+    wk.item = (int)((u0 - base) / wk.units);
+    wk.unit = (int)((u0 - base) - (int64_t)wk.item * wk.units);
+    Cursor ld = wk;
+    // to the next unit; whether that is in another item
     auto advance = [&](Cursor& k) {
-        if (++k.unit == k.units) {
-            k.unit = 0;
-            if (++k.item == per_seq) {
-                k.item = 0;
-                if (++k.b < c.B) {
-                    k.len = len_of(k.b);
-                    k.units = max(1, (k.len + UNIT - 1) / UNIT);
-                }
+        if (++k.unit < k.units) return false;
+        k.unit = 0;
+        if (++k.item == per_seq) {
+            k.item = 0;
+            if (++k.b < c.B) {
+                k.len = len_of(k.b);
+                k.units = units_in(k.len);
             }
         }
+        return true;
     };
 
     unsigned char* ws = smem + warp * C::WARP_SMEM;
     const uint32_t ring = smem_addr(ws);
     uint2* qf = (uint2*)(ws + C::STAGES * C::STAGE);
-    const int chunks = (int)c.D / 16;
     const int64_t nblk = (c.Smax + c.block - 1) / c.block;
+    const int block_shift = 31 - __clz(c.block);
 
-    auto issue = [&](int stage) {  // copies of unit `ld` into a stage
-        const int64_t bh = ld.b * c.Hkv + ld.item / p.row_tiles;
+    // copies of unit `ld` into a stage, a row's chunk a lane
+    constexpr int CPR = DP / 16, RPI = 32 / CPR;  // chunks of a row, rows a warp instruction copies
+    const int cc = lane % CPR, rl = lane / CPR;
+    const uint32_t lane_row = L::krow(rl & 7) * DP, lane_swz = (uint32_t)(cc ^ L::swz(L::krow(rl & 7))) << 4;
+    int64_t ld_head = 0;                          // (sequence, kv head) of the item
+    auto enter = [&]() { ld_head = (int64_t)ld.b * c.Hkv + ld.item / p.row_tiles; };
+    enter();
+    auto issue = [&](int stage) {
         const int k0 = ld.unit * UNIT;
-        const unsigned char* gk = (const unsigned char*)c.k + (bh * c.Smax + k0) * c.D;
-        const unsigned char* gv = (const unsigned char*)c.v + (bh * c.Smax + k0) * c.D;
-        const uint32_t dst = ring + stage * C::STAGE;
-        constexpr int CPR = DP / 16;              // chunks per stored row
-        constexpr int RPI = 32 / (CPR > 32 ? 32 : CPR);  // rows per warp instruction
-        const int cc = lane % CPR;
+        const int64_t off = (ld_head * c.Smax + k0 + rl) * c.D + cc * 16;
+        const uint32_t dst = ring + stage * C::STAGE + lane_row;
+        if (k0 + UNIT <= ld.len && c.D == DP) {
+            const unsigned char *gk = (const unsigned char*)c.k + off, *gv = (const unsigned char*)c.v + off;
 #pragma unroll
-        for (int r0 = 0; r0 < UNIT; r0 += RPI) {
-            const int key = r0 + lane / CPR;
-            const bool live = k0 + key < ld.len && cc < chunks;
-            const int row = (key & ~7) | L::krow(key & 7);
-            const uint32_t at = dst + row * DP + ((cc ^ L::swz(row & 7)) << 4);
-            const int64_t off = live ? (int64_t)key * c.D + cc * 16 : 0;
-            cp16(at, live ? gk + off : (const unsigned char*)c.k, live);
-            cp16(at + UNIT * DP, live ? gv + off : (const unsigned char*)c.v, live);
+            for (int r0 = 0; r0 < UNIT; r0 += RPI) {
+                // (swz of a sum of rows whose bits do not meet is the xor of theirs)
+                const uint32_t at = dst + r0 * DP + (lane_swz ^ (uint32_t)(RPI < 8 ? L::swz(r0 & 7) << 4 : 0));
+                cp16(at, gk + r0 * DP, true);
+                cp16(at + UNIT * DP, gv + r0 * DP, true);
+            }
+        } else {
+#pragma unroll 1
+            for (int r0 = 0; r0 < UNIT; r0 += RPI) {
+                const bool live = k0 + r0 + rl < ld.len && cc * 16 < c.D;
+                const int64_t o = live ? off + (int64_t)r0 * c.D : 0;
+                const uint32_t at = dst + r0 * DP + (lane_swz ^ (uint32_t)(RPI < 8 ? L::swz(r0 & 7) << 4 : 0));
+                cp16(at, (const unsigned char*)c.k + o, live);
+                cp16(at + UNIT * DP, (const unsigned char*)c.v + o, live);
+            }
         }
-        if (lane < 4) {
-            const int k = k0 + (lane & 1) * 16;
+        if (lane < 2 * SUB) {
+            const int k = k0 + (lane % SUB) * 16;
             const bool live = k < ld.len;
-            const float* s = lane < 2 ? c.k_scale : c.v_scale;
-            cp4(dst + 2 * UNIT * DP + lane * 4, live ? s + bh * nblk + k / c.block : s, live);
+            const float* s = lane < SUB ? c.k_scale : c.v_scale;
+            cp4(ring + stage * C::STAGE + 2 * UNIT * DP + lane * 4, live ? s + ld_head * nblk + (k >> block_shift) : s, live);
         }
+        if (advance(ld)) enter();
     };
 
-    const int n_units = (int)(u1 - u0);
 #pragma unroll
     for (int s = 0; s < C::STAGES - 1; ++s) {
-        if (s < n_units) {
-            issue(s);
-            advance(ld);
-        }
+        if (s < n_units) issue(s);
         cp_commit();
     }
 
@@ -298,41 +315,45 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
 
     int stage = 0;
     for (int it = 0; it < n_units; ++it) {
-        const int hk = wk.item / p.row_tiles, tile = wk.item - hk * p.row_tiles;
         if (fresh) {  // a new item: its query rows, normalised by a power of two, as B operands
             fresh = false;
+            const int hk = wk.item / p.row_tiles, tile = wk.item - hk * p.row_tiles;
             const int cnt = p.counts ? (int)clamp64(p.counts[wk.b], 0, p.Lq) : (int)p.Lq;
-            float row_mul[NT];  // of row g of each group
+            lim_min = 1 << 30;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int r = tile * ROWS + n * 8 + g;
                 const int i = r / p.G, h = hk * p.G + (r - i * p.G);
                 const size_t es = p.dtype == F32 ? 4 : 2;
                 const unsigned char* row = (const unsigned char*)p.q.p + (wk.b * p.q.sb + h * p.q.sh + i * p.q.ss) * (int64_t)es;
-                float x[C::KSTEPS][4], m = 0.0f;
+                float m = 0.0f;
+                auto load4 = [&](int k, float* x) {
+                    const int d = L::k_chunk(t, k >> 2) * 16 + (k & 3) * 4;
+                    const bool live = r < p.R && d < c.D;
 #pragma unroll
-                for (int q = 0; q < L::KL; ++q)
+                    for (int e = 0; e < 4; ++e) x[e] = live ? load_any<float>(row, d + e, p.dtype) : 0.0f;
+                };
+                // f32 values of all dims only fit beside the rest for DP <= 128; 256 loads them twice
+                float x[DP <= 128 ? C::KSTEPS : 1][4];
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int d = L::k_chunk(t, q) * 16 + w * 4;
-                        const bool live = r < p.R && d < c.D;
+                for (int k = 0; k < C::KSTEPS; ++k) {
+                    float* y = x[DP <= 128 ? k : 0];
+                    load4(k, y);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float v = live ? load_q(p, row, d + e) : 0.0f;
-                            x[q * 4 + w][e] = v;
-                            m = fmaxf(m, finite_abs(v));
-                        }
-                    }
+                    for (int e = 0; e < 4; ++e) m = fmaxf(m, finite_abs(y[e]));
+                }
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 // 2^e <= m < 2^(e+1); a row of zeros or subnormals stays as it is
-                int e = (int)(__float_as_uint(m) >> 23) - 127;
-                e = m >= 1.17549435e-38f ? min(max(e, -126), 126) : 0;
-                const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                row_mul[n] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+                int e2 = (int)(__float_as_uint(m) >> 23) - 127;
+                e2 = m >= 1.17549435e-38f ? min(max(e2, -126), 126) : 0;
+                const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
+                const float row_mul = __uint_as_float((uint32_t)(127 + e2) << 23) * p.scale_log2;
 #pragma unroll
                 for (int k = 0; k < C::KSTEPS; ++k) {
-                    const float y0 = x[k][0] * down, y1 = x[k][1] * down, y2 = x[k][2] * down, y3 = x[k][3] * down;
+                    float* y = x[DP <= 128 ? k : 0];
+                    if constexpr (DP > 128) load4(k, y);
+                    const float y0 = y[0] * down, y1 = y[1] * down, y2 = y[2] * down, y3 = y[3] * down;
                     const uint32_t b0 = pack_f16(y0, y1), b1 = pack_f16(y2, y3);
                     if constexpr (C::QREG) {
                         qr[k][0] = b0;
@@ -345,17 +366,13 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                         }
                     }
                 }
-            }
-            lim_min = 1 << 30;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    qmul[n][e] = __shfl_sync(0xffffffffu, row_mul[n], (2 * t + e) * 4);
-                    const int r = tile * ROWS + n * 8 + 2 * t + e, i = r / p.G;
-                    lim[n][e] = r < p.R && i < cnt ? max(0, wk.len - cnt + i + 1) : 0;
-                    if (r < p.R) lim_min = min(lim_min, lim[n][e]);
-                    M[n][e] = -INFINITY;
+                    qmul[n][e] = __shfl_sync(0xffffffffu, row_mul, (2 * t + e) * 4);
+                    const int r2 = tile * ROWS + n * 8 + 2 * t + e, i2 = r2 / p.G;
+                    lim[n][e] = r2 < p.R && i2 < cnt ? max(0, wk.len - cnt + i2 + 1) : 0;
+                    if (r2 < p.R) lim_min = min(lim_min, lim[n][e]);
+                    M[n][e] = NONE;
                     l[n][e] = 0.0f;
                 }
 #pragma unroll
@@ -367,25 +384,20 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
             __syncwarp();
         }
 
-        if (it + C::STAGES - 1 < n_units) {
-            issue(stage + C::STAGES - 1 >= C::STAGES ? stage - 1 : stage + C::STAGES - 1);
-            advance(ld);
-        }
+        if (it + C::STAGES - 1 < n_units) issue(stage == 0 ? C::STAGES - 1 : stage - 1);
         cp_commit();
         cp_wait<C::STAGES - 1>();
         __syncwarp();
 
         const unsigned char* kt = ws + stage * C::STAGE;
         const unsigned char* vt = kt + UNIT * DP;
-        const float4 sc = *(const float4*)(kt + 2 * UNIT * DP);
-        const float sk[2] = {sc.x, sc.y};
-        const float sv[2] = {fmaxf(sc.z, SV_MIN), fmaxf(sc.w, SV_MIN)};
+        const float* scales = (const float*)(kt + 2 * UNIT * DP);
         const int k0 = wk.unit * UNIT;
 
-        // S^T of the unit's 32 keys
-        float s[2][NT][4];
+        // S^T of the unit's keys
+        float s[SUB][NT][4];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < SUB; ++u) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -418,53 +430,63 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                 }
             }
         }
-        // to log2 units, masked; scores out where the weights are wanted
-        const bool edge = k0 + UNIT > lim_min;
+        if (p.s_out) {  // the scores themselves, where the weights are wanted (one row tile then)
+            float* so = p.s_out + ((int64_t)wk.b * c.Hkv + wk.item) * c.Smax * p.R;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = s[u][n][e] * (qmul[n][e & 1] * sk[u]);
-                    if (edge && k0 + u * 16 + g + (e >> 1) * 8 >= lim[n][e & 1]) x = -INFINITY;
-                    s[u][n][e] = x;
-                }
-        if (p.s_out) {
-            const int64_t bh = wk.b * c.Hkv + hk;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < SUB; ++u)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int key = k0 + u * 16 + g + (e >> 1) * 8, r = tile * ROWS + n * 8 + 2 * t + (e & 1);
-                        if (key < wk.len && r < p.R) p.s_out[(bh * c.Smax + key) * p.R + r] = s[u][n][e];
+                        const int key = k0 + u * 16 + g + (e >> 1) * 8, r = n * 8 + 2 * t + (e & 1);
+                        if (key < wk.len && r < p.R)
+                            so[(int64_t)key * p.R + r] = key < lim[n][e & 1] ? s[u][n][e] * (qmul[n][e & 1] * scales[u]) : -INFINITY;
                     }
         }
-        const float lsv[2] = {lg2f(sv[0]), lg2f(sv[1])};
+        // s + log2 sv in log2 units, masked, and whether any row's maximum has to rise
+        float sv[SUB];
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            sv[u] = fmaxf(scales[SUB + u], SV_MIN);
+            const float lsv = lg2f(sv[u]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float m0 = qmul[n][0] * scales[u], m1 = qmul[n][1] * scales[u];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[u][n][e] = fmaf(s[u][n][e], e & 1 ? m1 : m0, lsv);
+            }
+        }
+        if (k0 + UNIT > lim_min) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (k0 + u * 16 + g + (e >> 1) * 8 >= lim[n][e & 1]) s[u][n][e] = -INFINITY;
+        }
+        float top[NT][2];
         bool raise = false;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[u][n][e] += lsv[u];
-                    raise |= s[u][n][e] > M[n][e & 1] + RAISE;
-                }
+            for (int e = 0; e < 2; ++e) {
+                top[n][e] = fmaxf(s[0][n][e], s[0][n][e + 2]);
+                if constexpr (SUB == 2) top[n][e] = fmaxf(top[n][e], fmaxf(s[SUB - 1][n][e], s[SUB - 1][n][e + 2]));
+                raise |= top[n][e] > M[n][e] + RAISE;
+            }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float corr[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    float m = fmaxf(fmaxf(s[0][n][e], s[0][n][e + 2]), fmaxf(s[1][n][e], s[1][n][e + 2]));
+                    float m = top[n][e];
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                     m = fmaxf(m, M[n][e]);
-                    corr[e] = m > M[n][e] ? ex2f(M[n][e] - m) : 1.0f;
+                    corr[e] = ex2f(M[n][e] - m);
                     M[n][e] = m;
                     l[n][e] *= corr[e];
                 }
@@ -474,18 +496,15 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                     for (int e = 0; e < 4; ++e) o[n][j][e] *= corr[e & 1];
             }
         }
-        uint32_t pb[2][NT][NS][2];
+        uint32_t pb[SUB][NT][NS][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float ref[2];
+        for (int u = 0; u < SUB; ++u) {
+            const float inv = __frcp_rn(sv[u]);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) ref[e] = M[n][e] == -INFINITY ? 0.0f : M[n][e] - SHIFT;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int n = 0; n < NT; ++n) {
                 float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = ex2f(s[u][n][e] - ref[e & 1]);
-                const float inv = __frcp_rn(sv[u]);
+                for (int e = 0; e < 4; ++e) x[e] = ex2f(s[u][n][e] - (M[n][e & 1] - SHIFT));
                 l[n][0] = fmaf(x[0] + x[2], inv, l[n][0]);
                 l[n][1] = fmaf(x[1] + x[3], inv, l[n][1]);
                 const uint32_t h0 = pack_f16(x[0], x[1]), h1 = pack_f16(x[2], x[3]);
@@ -500,14 +519,14 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
         }
         // O^T += V^T P^T
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < SUB; ++u) {
 #pragma unroll
             for (int vl = 0; vl < L::VL; ++vl) {
                 constexpr int WORDS = L::V_BYTES / 4;
                 uint32_t x[4][WORDS];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int key = 2 * t + (k & 1), r = L::krow(key);  // rows r and r + 8 of the 16
+                    const int r = L::krow(2 * t + (k & 1));  // rows r and r + 8 of the 16
                     const int by = L::v_byte(g, vl);
                     const unsigned char* at = vt + (u * 16 + (k >> 1) * 8 + r) * DP + (((by >> 4) ^ L::swz(r)) << 4) + (by & 15);
                     if constexpr (WORDS == 4) {
@@ -539,15 +558,14 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
         __syncwarp();  // every lane has read this stage before it is copied over
         stage = stage + 1 == C::STAGES ? 0 : stage + 1;
 
-        const bool item_done = wk.unit + 1 == wk.units, last = it + 1 == n_units;
-        if (item_done || last) {
+        const bool item_done = wk.unit + 1 == wk.units;
+        if (item_done || it + 1 == n_units) {
+            const int hk = wk.item / p.row_tiles, tile = wk.item - hk * p.row_tiles;
             const bool whole = item_done && !head_split;
-            const int64_t item = wk.b * per_seq + wk.item;
             if (!head_split && lane == 0) {
                 // the warp of the item's last unit: the one whose stretch holds it
                 const int64_t end = u0 + it + (wk.units - 1 - wk.unit);
-                const int64_t last_warp = ((end + 1) * NW - 1) / U;
-                p.meta[item] = make_int2((int)wid, (int)last_warp);
+                p.meta[(int64_t)wk.b * per_seq + wk.item] = make_int2((int)wid, (int)(((end + 1) * NW - 1) / U));
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
@@ -557,10 +575,9 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                     x += __shfl_xor_sync(0xffffffffu, x, 4);
                     x += __shfl_xor_sync(0xffffffffu, x, 8);
                     x += __shfl_xor_sync(0xffffffffu, x, 16);
-                    l[n][e] = x;
                     const int r = n * 8 + 2 * t + e, gr = tile * ROWS + r;
                     if (gr >= p.R) continue;
-                    const float m = M[n][e] == -INFINITY ? 0.0f : M[n][e] - SHIFT;
+                    const float m = M[n][e] - SHIFT;
                     if (whole) {
                         const float inv = x > 0.0f || !(x == x) ? 1.0f / x : 0.0f;
                         const int i = gr / p.G, h = hk * p.G + (gr - i * p.G);
@@ -593,7 +610,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                                 *(float2*)(dst + d0 + k) = make_float2(o[n][j][e], o[n][j][e + 2]);
                             }
                         }
-                        if (g == 0) p.part_ml[slot * ROWS + r] = make_float2(!(x == x) ? x : M[n][e] == -INFINITY ? -INFINITY : m, x);
+                        if (g == 0) p.part_ml[slot * ROWS + r] = make_float2(x == 0.0f ? -INFINITY : x == x ? m : x, x);
                     }
                 }
             fresh = true;
@@ -767,7 +784,10 @@ int launch_mma_rows(const MmaP& p, int n_sm, cudaStream_t st) {
     const bool wide = p.dtype == F32;
     if (p.R <= 8) return wide ? launch_mma<DP, FMT, 1, 2>(p, n_sm, st) : launch_mma<DP, FMT, 1, 1>(p, n_sm, st);
     if (p.R <= 16 || DP == 256) return wide ? launch_mma<DP, FMT, 2, 2>(p, n_sm, st) : launch_mma<DP, FMT, 2, 1>(p, n_sm, st);
-    if constexpr (DP < 256) return wide ? launch_mma<DP, FMT, 4, 2>(p, n_sm, st) : launch_mma<DP, FMT, 4, 1>(p, n_sm, st);
+    if constexpr (DP < 256) {
+        if (p.R <= 24) return wide ? launch_mma<DP, FMT, 3, 2>(p, n_sm, st) : launch_mma<DP, FMT, 3, 1>(p, n_sm, st);
+        return wide ? launch_mma<DP, FMT, 4, 2>(p, n_sm, st) : launch_mma<DP, FMT, 4, 1>(p, n_sm, st);
+    }
     return -1;
 }
 
