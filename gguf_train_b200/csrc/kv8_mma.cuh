@@ -38,7 +38,7 @@ constexpr float RAISE = 7.0f, SHIFT = 8.0f, NONE = -1e30f;  // NONE: no key seen
 struct MmaP {
     gtb_kv8 c;
     Rows3 q, o;
-    int dtype;
+    int dtype, q_vec;
     int G, R, row_tiles;      // R = G * Lq rows per (b, hk), in tiles of 8 * NT
     int64_t H, Lq;
     float scale_log2;         // scale * log2(e)
@@ -146,6 +146,37 @@ struct Lay<256> {
     __device__ static int swz(int r) { return (r & 6) ^ ((r & 1) << 2); }
 };
 
+// Four values of a query row as f32, 0 where it has none; in one load where every row starts on 16 (f32) or 8 bytes
+__device__ __forceinline__ void load_q4(const MmaP& p, int64_t at, bool live, float* x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = 0.0f;
+    if (!live) return;
+    if (p.q_vec) {
+        if (p.dtype == F32) {
+            const float4 v = *(const float4*)((const float*)p.q.p + at);
+            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else {
+            const uint2 v = *(const uint2*)((const uint16_t*)p.q.p + at);
+            if (p.dtype == BF16) {
+                x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+                x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+            } else {
+                const float2 a = unpack_f16(v.x), b = unpack_f16(v.y);
+                x[0] = a.x; x[1] = a.y; x[2] = b.x; x[3] = b.y;
+            }
+        }
+    } else {
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+            const float v = load_any<float>(p.q.p, at + e, p.dtype);
+            if (e == 0) x[0] = v;
+            else if (e == 1) x[1] = v;
+            else if (e == 2) x[2] = v;
+            else x[3] = v;
+        }
+    }
+}
+
 // Units, warps and stages. More warps hide the dependent chain of a unit (scores, exponentials, second product); their
 // number is what the registers (O alone takes NT DP / 4) and two stages of each warp's ring allow.
 template <int DP, int NT, int NS>
@@ -156,11 +187,11 @@ struct MmaCfg {
     static constexpr int SUB = OREGS > 32 ? 1 : 2;    // 16-key products per unit
     static constexpr int UNIT = 16 * SUB;
     static constexpr int STAGE = 2 * UNIT * DP + 16;  // K rows, V rows, scales (k, v of each 16 keys)
-    static constexpr int QBYTES = QREG ? 0 : KSTEPS * NT * NS * 32 * 8;
-    static constexpr int SPACE = 224 * 1024;
+    static constexpr int QBYTES = QREG ? 0 : KSTEPS * NT * NS * 32 * 8 + NT * 32;
+    static constexpr int SPACE = 224 * 1024, MOST12 = 64;
     static constexpr int fit(int warps) { return (SPACE / warps - QBYTES) / STAGE; }
     static constexpr int pick() {
-        const int most = OREGS <= 16 ? 16 : OREGS <= 64 ? 12 : 8;
+        const int most = OREGS <= 16 ? 16 : OREGS <= MOST12 ? 12 : 8;
         for (int w = most; w > 4; w -= 2)
             if (fit(w) >= 2) return w;
         return 4;
@@ -256,7 +287,8 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
 
     unsigned char* ws = smem + warp * C::WARP_SMEM;
     const uint32_t ring = smem_addr(ws);
-    uint2* qf = (uint2*)(ws + C::STAGES * C::STAGE);
+    uint2* qf = (uint2*)(ws + C::STAGES * C::STAGE);  // B operands of the rows, then their multipliers
+    float* qm = (float*)(qf + C::KSTEPS * NT * NS * 32);
     const int64_t nblk = (c.Smax + c.block - 1) / c.block;
     const int block_shift = 31 - __clz(c.block);
 
@@ -319,41 +351,33 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
             fresh = false;
             const int hk = wk.item / p.row_tiles, tile = wk.item - hk * p.row_tiles;
             const int cnt = p.counts ? (int)clamp64(p.counts[wk.b], 0, p.Lq) : (int)p.Lq;
-            lim_min = 1 << 30;
-#pragma unroll
+            float row_mul = 0.0f;  // (QREG) of row g
+#pragma unroll 1
             for (int n = 0; n < NT; ++n) {
-                const int r = tile * ROWS + n * 8 + g;
-                const int i = r / p.G, h = hk * p.G + (r - i * p.G);
-                const size_t es = p.dtype == F32 ? 4 : 2;
-                const unsigned char* row = (const unsigned char*)p.q.p + (wk.b * p.q.sb + h * p.q.sh + i * p.q.ss) * (int64_t)es;
-                float m = 0.0f;
-                auto load4 = [&](int k, float* x) {
-                    const int d = L::k_chunk(t, k >> 2) * 16 + (k & 3) * 4;
-                    const bool live = r < p.R && d < c.D;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = live ? load_any<float>(row, d + e, p.dtype) : 0.0f;
-                };
-                // f32 values of all dims only fit beside the rest for DP <= 128; 256 loads them twice
-                float x[DP <= 128 ? C::KSTEPS : 1][4];
+                const int r = tile * ROWS + n * 8 + g, i = r / p.G, h = hk * p.G + (r - i * p.G);
+                const int64_t at = wk.b * p.q.sb + h * p.q.sh + i * p.q.ss;
+                float x[C::KSTEPS][4], m = 0.0f;
 #pragma unroll
                 for (int k = 0; k < C::KSTEPS; ++k) {
-                    float* y = x[DP <= 128 ? k : 0];
-                    load4(k, y);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) m = fmaxf(m, finite_abs(y[e]));
+                    const int d = L::k_chunk(t, k >> 2) * 16 + (k & 3) * 4;
+                    load_q4(p, at + d, r < p.R && d < c.D, x[k]);
                 }
+#pragma unroll
+                for (int k = 0; k < C::KSTEPS; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) m = fmaxf(m, finite_abs(x[k][e]));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 // 2^e <= m < 2^(e+1); a row of zeros or subnormals stays as it is
                 int e2 = (int)(__float_as_uint(m) >> 23) - 127;
                 e2 = m >= 1.17549435e-38f ? min(max(e2, -126), 126) : 0;
                 const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
-                const float row_mul = __uint_as_float((uint32_t)(127 + e2) << 23) * p.scale_log2;
+                const float mul = __uint_as_float((uint32_t)(127 + e2) << 23) * p.scale_log2;
+                if constexpr (C::QREG) row_mul = mul;
+                else if (t == 0) qm[n * 8 + g] = mul;
 #pragma unroll
                 for (int k = 0; k < C::KSTEPS; ++k) {
-                    float* y = x[DP <= 128 ? k : 0];
-                    if constexpr (DP > 128) load4(k, y);
-                    const float y0 = y[0] * down, y1 = y[1] * down, y2 = y[2] * down, y3 = y[3] * down;
+                    const float y0 = x[k][0] * down, y1 = x[k][1] * down, y2 = x[k][2] * down, y3 = x[k][3] * down;
                     const uint32_t b0 = pack_f16(y0, y1), b1 = pack_f16(y2, y3);
                     if constexpr (C::QREG) {
                         qr[k][0] = b0;
@@ -366,12 +390,17 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                         }
                     }
                 }
+            }
+            __syncwarp();
+            lim_min = 1 << 30;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    qmul[n][e] = __shfl_sync(0xffffffffu, row_mul, (2 * t + e) * 4);
-                    const int r2 = tile * ROWS + n * 8 + 2 * t + e, i2 = r2 / p.G;
-                    lim[n][e] = r2 < p.R && i2 < cnt ? max(0, wk.len - cnt + i2 + 1) : 0;
-                    if (r2 < p.R) lim_min = min(lim_min, lim[n][e]);
+                    qmul[n][e] = C::QREG ? __shfl_sync(0xffffffffu, row_mul, (2 * t + e) * 4) : qm[n * 8 + 2 * t + e];
+                    const int r = tile * ROWS + n * 8 + 2 * t + e, i = r / p.G;
+                    lim[n][e] = r < p.R && i < cnt ? max(0, wk.len - cnt + i + 1) : 0;
+                    if (r < p.R) lim_min = min(lim_min, lim[n][e]);
                     M[n][e] = NONE;
                     l[n][e] = 0.0f;
                 }
@@ -381,7 +410,6 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                     for (int e = 0; e < 4; ++e) o[n][j][e] = 0.0f;
             }
             lim_min = __reduce_min_sync(0xffffffffu, lim_min);
-            __syncwarp();
         }
 
         if (it + C::STAGES - 1 < n_units) issue(stage == 0 ? C::STAGES - 1 : stage - 1);
@@ -405,7 +433,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
             const int r = L::krow(g);
             const unsigned char* ra = kt + (u * 16 + r) * DP;
             const unsigned char* rb = ra + 8 * DP;
-#pragma unroll
+#pragma unroll (NT >= 3 ? 1 : L::KL)
             for (int q = 0; q < L::KL; ++q) {
                 const int at = (L::k_chunk(t, q) ^ L::swz(r)) << 4;
                 const uint4 wa = *(const uint4*)(ra + at), wb = *(const uint4*)(rb + at);
@@ -622,12 +650,12 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
 }
 
 // What is left once the units are done, in one launch of 128-thread CTAs.
-//   CTAs below `joins`: one (item, row) each whose item several warps worked on. The lanes weigh the parts by their
-//     maxima, the four warps each add up a quarter of them, and the sums meet in shared memory: always in the
-//     same order.
+//   CTAs below `joins`: the rows of items that several warps worked on, a row a warp, or a row a CTA where there are
+//     many parts (the warps' sums then meet in shared memory). The lanes weigh the parts by their maxima; the
+//     order of the sums is fixed.
 //   CTAs from there on (scores kept): KEYS_PER_CTA cached rows of one (sequence, kv head): score_in + the sum over the
 //     query rows of exp(s - lse), from the scores the first kernel wrote and the rows' (max, sum) parts.
-constexpr int KEYS_PER_CTA = 1024;
+constexpr int KEYS_PER_CTA = 512;
 
 // A row's parts summed by one warp: (m, l) with sum of 2^score = l 2^m. Parts that saw no key have maximum -inf; those
 // of a row of NaN have sum and maximum NaN, and make l NaN.
@@ -648,92 +676,120 @@ __device__ __forceinline__ float2 row_lse2(const MmaP& p, const int2 range, int 
     return make_float2(m, l);
 }
 
-template <int DP>
+template <int DP, int SPAN>
 __global__ void __launch_bounds__(128) kv8_finish_kernel(const __grid_constant__ MmaP p, int rows, unsigned joins) {
     cudaGridDependencySynchronize();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per_seq = (int)p.c.Hkv * p.row_tiles;
     if (blockIdx.x < joins) {
-        const unsigned per_item = min(rows, p.R);
-        const unsigned item = blockIdx.x / per_item;
-        const int r = (int)(blockIdx.x - item * per_item);
+        // SPAN warps a row
+        constexpr int PER = DP / 32, RPC = 4 / SPAN;
+        const unsigned per_item = min(rows, p.R), rx = blockIdx.x * RPC + (RPC > 1 ? warp : 0);
+        const unsigned item = rx / per_item;
+        const int r = (int)(rx - item * per_item), part = RPC > 1 ? 0 : warp;
         const int b = (int)(item / (unsigned)per_seq), rest = (int)(item - (unsigned)b * per_seq);
         const int hk = rest / p.row_tiles, tile = rest - hk * p.row_tiles, gr = tile * rows + r;
-        if (gr >= p.R) return;
-        const int2 range = p.meta[item];
-        if (range.x == range.y) return;
+        const bool live = b < p.c.B && gr < p.R;
+        const int2 range = live ? p.meta[item] : make_int2(0, 0);
+        if (range.x == range.y) return;  // the whole CTA with SPAN 4
         const float2 all = row_lse2(p, range, rows, r);
-        constexpr int PER = DP / 32;
         float acc[PER] = {};
-        // parts of this warp: k = range.x + warp, + 4, ...; 4 at a time, the loads of all before their use
-        for (int k0 = range.x + warp; k0 <= range.y; k0 += 16) {
+        // this warp's parts: k = range.x + part, + SPAN, ...; 4 at a time, the loads of all before their use
+        for (int k0 = range.x + part; k0 <= range.y; k0 += 4 * SPAN) {
             float x[4][PER], w[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int k = min(k0 + 4 * q, range.y);
+                const int k = min(k0 + SPAN * q, range.y);
                 const int64_t slot = (2 * (int64_t)k + (k == range.x)) * rows + r;
-                const float m = p.part_ml[slot].x;
-                w[q] = k0 + 4 * q <= range.y ? ex2f(m - all.x) : 0.0f;
+                w[q] = p.part_ml[slot].x;
 #pragma unroll
                 for (int i = 0; i < PER; ++i) x[q][i] = p.part_o[slot * DP + i * 32 + lane];
             }
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int q = 0; q < 4; ++q) {
+                const float f = k0 + SPAN * q <= range.y ? ex2f(w[q] - all.x) : 0.0f;
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
-                    if (w[q] != 0.0f) acc[i] = fmaf(x[q][i], w[q], acc[i]);
+                    if (f != 0.0f) acc[i] = fmaf(x[q][i], f, acc[i]);
+            }
         }
-        __shared__ float sum[4][DP];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) sum[warp][i * 32 + lane] = acc[i];
-        __syncthreads();
         const float inv = all.y > 0.0f || !(all.y == all.y) ? 1.0f / all.y : 0.0f;
         const int i = gr / p.G, h = hk * p.G + (gr - i * p.G);
         const int64_t at = b * p.o.sb + h * p.o.sh + (int64_t)i * p.o.ss;
-        for (int d = threadIdx.x; d < p.c.D; d += 128) {
-            const float y = ((sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d])) * inv;
+        if constexpr (SPAN > 1) {
+            __shared__ float sum[4][DP];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) sum[warp][k * 32 + lane] = acc[k];
+            __syncthreads();
+            if (warp) return;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) acc[k] = (sum[0][k * 32 + lane] + sum[1][k * 32 + lane]) + (sum[2][k * 32 + lane] + sum[3][k * 32 + lane]);
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int d = k * 32 + lane;
+            if (d >= p.c.D) continue;
+            const float y = acc[k] * inv;
             if (p.dtype == F32) ((float*)p.o.p)[at + d] = y;
             else if (p.dtype == F16) ((__half*)p.o.p)[at + d] = __float2half_rn(y);
             else ((__nv_bfloat16*)p.o.p)[at + d] = __float2bfloat16_rn(y);
         }
-        if (p.lse && threadIdx.x == 0)
+        if (p.lse && lane == 0)
             p.lse[((int64_t)b * p.H + h) * p.Lq + i] = all.y == 0.0f ? -INFINITY : (all.x + log2f(all.y)) * 0.6931471805599453f;
         return;
     }
     // one row tile, so the item is the (sequence, kv head)
     const unsigned per_head = (unsigned)((p.c.Smax + KEYS_PER_CTA - 1) / KEYS_PER_CTA);
-    const unsigned x = blockIdx.x - joins, item = x / per_head;
-    const int k0 = (int)(x - item * per_head) * KEYS_PER_CTA;
+    const unsigned idx = blockIdx.x - joins, item = idx / per_head;
+    const int k0 = (int)(idx - item * per_head) * KEYS_PER_CTA;
     const int64_t b = item / (unsigned)p.c.Hkv;
     const int len = (int)clamp64(p.c.lens[b], 0, p.c.Smax);
     if (k0 >= len) return;
+    // the scores of up to four rows and the old sums are on their way while the rows' log-sum-exp is put together
+    constexpr int KPT = KEYS_PER_CTA / 128;
+    const float* s = p.s_out + (int64_t)item * p.c.Smax * p.R;
+    const int64_t at = (int64_t)item * p.c.Smax;
+    float4 x[KPT];
+    float old[KPT];
+#pragma unroll
+    for (int q = 0; q < KPT; ++q) {
+        const int k = k0 + q * 128 + threadIdx.x;
+        x[q] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (k < len) {
+            const float* row = s + (int64_t)k * p.R;
+            if ((p.R & 3) == 0) {
+                x[q] = *(const float4*)row;
+            } else {
+                x[q].x = row[0];
+                if (p.R > 1) x[q].y = row[1];
+                if (p.R > 2) x[q].z = row[2];
+                if (p.R > 3) x[q].w = row[3];
+            }
+            old[q] = p.score_in[at + k];
+        }
+    }
     __shared__ float lse2[32];
     const int2 range = p.meta[item];
-    for (int r = warp; r < p.R; r += 4) {
-        float z;
-        if (range.x == range.y) {
+    for (int r = warp; r < 32; r += 4) {
+        float z = -INFINITY;
+        if (r < p.R && range.x == range.y) {
             const int i = r / p.G, h = (int)(item - (unsigned)b * p.c.Hkv) * p.G + (r - i * p.G);
             z = p.lse[(b * p.H + h) * p.Lq + i] * 1.4426950408889634f;
-        } else {
+        } else if (r < p.R) {
             const float2 ml = row_lse2(p, range, rows, r);
             z = ml.y == 0.0f ? -INFINITY : ml.x + log2f(ml.y);
         }
         if (lane == 0) lse2[r] = z == -INFINITY ? INFINITY : z;  // a row that attends nothing gives no weight
     }
     __syncthreads();
-    const float* s = p.s_out + (int64_t)item * p.c.Smax * p.R;
-    for (int k = k0 + threadIdx.x; k < min(k0 + KEYS_PER_CTA, len); k += 128) {
+#pragma unroll
+    for (int q = 0; q < KPT; ++q) {
+        const int k = k0 + q * 128 + threadIdx.x;
+        if (k >= len) continue;
+        float w = (ex2f(x[q].x - lse2[0]) + ex2f(x[q].y - lse2[1])) + (ex2f(x[q].z - lse2[2]) + ex2f(x[q].w - lse2[3]));
         const float* row = s + (int64_t)k * p.R;
-        float w = 0.0f;
-        if ((p.R & 3) == 0) {
-            for (int r = 0; r < p.R; r += 4) {
-                const float4 v = *(const float4*)(row + r);
-                w += (ex2f(v.x - lse2[r]) + ex2f(v.y - lse2[r + 1])) + (ex2f(v.z - lse2[r + 2]) + ex2f(v.w - lse2[r + 3]));
-            }
-        } else {
-            for (int r = 0; r < p.R; ++r) w += ex2f(row[r] - lse2[r]);
-        }
-        p.score_out[(int64_t)item * p.c.Smax + k] = p.score_in[(int64_t)item * p.c.Smax + k] + w;
+        for (int r = 4; r < p.R; ++r) w += ex2f(row[r] - lse2[r]);
+        p.score_out[at + k] = old[q] + w;
     }
 }
 
@@ -765,14 +821,17 @@ int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
     kern<<<n_sm, C::WARPS * 32, C::SMEM, st>>>(p);
     bool bad = cuda_failed(cudaGetLastError(), "kv8_attention launch");
     if (!bad) {
+        // rows to join; with many parts each (few items) four warps share a row
         const int64_t joins = items * std::min(8 * NT, p.R);
+        const bool shared_rows = warps > 8 * items;
+        const int64_t ctas = shared_rows ? joins : (joins + 3) / 4;
         const int64_t sums = p.score_out ? p.c.B * p.c.Hkv * ((p.c.Smax + KEYS_PER_CTA - 1) / KEYS_PER_CTA) : 0;
-        if (joins + sums > INT32_MAX) {
+        if (ctas + sums > INT32_MAX || joins > INT32_MAX) {
             set_error("kv8_attention: too many query rows");
             bad = true;
         } else {
-            bad = !launch_behind("kv8_attention: finish launch", kv8_finish_kernel<DP>, dim3((unsigned)(joins + sums)), 128, st, 0, p,
-                                 8 * NT, (unsigned)joins);
+            bad = !launch_behind("kv8_attention: finish launch", shared_rows ? kv8_finish_kernel<DP, 4> : kv8_finish_kernel<DP, 1>,
+                                 dim3((unsigned)(ctas + sums)), 128, st, 0, p, 8 * NT, (unsigned)ctas);
         }
     }
     cudaFreeAsync(scratch, st);
