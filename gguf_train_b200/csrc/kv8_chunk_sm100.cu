@@ -5,14 +5,16 @@
 //   kv8_widen_kernel  K, V codes -> f16 (exact: int8 and e4m3 both fit), rows past the length zero, head size
 //                     padded to DP; q -> f16 rows r = i * G + g of each (sequence, kv head), normalised by a power
 //                     of two per row as in kv8_mma.cuh; the scales of every 16 keys as (sk, log2 sv, 1 / sv).
-//   kv8_chunk_kernel  one CTA per SM claims items (sequence, kv head, pair of 128-row tiles, part of the keys),
-//                     heaviest first. Twelve warps: TMA producer, MMA issuer, two idle, and four softmax warps per
+//   kv8_chunk_kernel  one CTA per SM claims items (sequence, kv head, pair of 128-row tiles) from a counter, the
+//                     longest sequences first and a head's pairs together, so that the CTAs running at a time share
+//                     few heads' K and V through L2; the last items are claimed in parts of their keys, so that
+//                     the SMs end together. Twelve warps: TMA producer, MMA issuer, two idle, and four softmax warps per
 //                     tile, one row a thread, which ping-pong with the tensor core:
 //                       S_t = Q_t K_j^T (M = N = 128, K = DP),  O_t += P_t V_j (A = P_t from TMEM, V read MN-major).
 //                     Scores become log2 units with their 16 keys' scale, V's scale is folded into the exponent
 //                     (P' = 2^(s + log2 sv - M + 8), M raised when a block exceeds it by 2^7) and the row sum
 //                     takes P' / sv, so scales cost three packed operations per 16 keys and no accuracy.
-//   kv8_chunk_join_kernel  joins the parts where the keys were split (few items on many SMs).
+//   kv8_chunk_join_kernel  joins those parts.
 // The tile pair reuses each K/V tile for 256 rows; the second kernel is bound by the tensor core and the
 // exponentials. Every wait is bounded: a timeout records a status code, drains the CTA's own copies and MMAs,
 // frees TMEM and returns.
@@ -35,6 +37,7 @@ using namespace sm100;
 
 constexpr int BM = 128, BN = 128, NTHREADS = 384, REG_LO = 104, REG_HI = 200;
 constexpr uint32_t TMEM_COLS = 512;
+constexpr int TAIL_SPLITS = 4;
 
 template <int D>
 struct ChunkCfg {
@@ -49,7 +52,8 @@ struct ChunkCfg {
 struct ChunkP {
     gtb_kv8 c;
     Rows3 q, o;
-    int dtype, G, R, pairs, splits;
+    int dtype, G, R, pairs;
+    int whole, tail, splits;     // items claimed whole, items claimed in `splits` parts each
     int64_t b0, nb;              // sequences of this launch
     int64_t H, Lq;
     float scale_log2;
@@ -59,18 +63,37 @@ struct ChunkP {
     __half *k16, *v16, *q16;     // [nb * Hkv][Spad | Rpad][DP]
     float4* scl;                 // [nb * Hkv][Spad / 16]: sk, log2 sv, 1 / sv
     float* qmul;                 // [nb * Hkv][Rpad]
-    float* part_o;               // [item][split][256][DP], splits > 1
-    float2* part_ml;             // [item][split][256]
+    float* part_o;               // [tail item][split][256][DP]
+    float2* part_ml;             // [tail item][split][256]
+    int* order;                  // [nb]: sequences, longest first
     int* claim;
     int* status;
 };
 
-// Rows of codes to f16, q to normalised f16: one warp per row of 32-row groups; blockIdx.y = (sequence, kv head)
+// Rows of codes to f16, q to normalised f16: one warp per row of 32-row groups; blockIdx.y = (sequence, kv head). The last
+// CTA of the first row orders the sequences and zeroes the counter.
 template <int FMT, int DP>
 __global__ void __launch_bounds__(256) kv8_widen_kernel(const __grid_constant__ ChunkP p) {
     const gtb_kv8& c = p.c;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.claim = 0;
+    if (blockIdx.x == gridDim.x - 1) {
+        if (blockIdx.y != 0) return;
+        if (threadIdx.x == 0) *p.claim = 0;
+        const int n = (int)p.nb;
+        for (int i = threadIdx.x; i < n; i += 256) {
+            int rank = i;  // more sequences than are worth comparing stay as they come
+            if (n <= 2048) {
+                const int own = c.lens[p.b0 + i];
+                rank = 0;
+                for (int k = 0; k < n; ++k) {
+                    const int other = c.lens[p.b0 + k];
+                    rank += other > own || (other == own && k < i);
+                }
+            }
+            p.order[rank] = i;
+        }
+        return;
+    }
     const int k_ctas = (int)(p.Spad / 64);
     const int64_t lbh = blockIdx.y, b = p.b0 + lbh / c.Hkv, hk = lbh % c.Hkv, bh = b * c.Hkv + hk;
     const int len = (int)clamp64(c.lens[b], 0, c.Smax);
@@ -78,15 +101,20 @@ __global__ void __launch_bounds__(256) kv8_widen_kernel(const __grid_constant__ 
         // 64 rows of K and V; a thread makes 16 codes into 32 bytes
         const int r0 = blockIdx.x * 64;
         if (r0 >= (len + BN - 1) / BN * BN) return;  // no tile reads them
-        constexpr int CPR = DP / 16;
-        for (int e = threadIdx.x; e < 2 * 64 * CPR; e += 256) {
-            const int v = e >= 64 * CPR, x = v ? e - 64 * CPR : e, row = r0 + x / CPR, ch = x % CPR;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (row < len && ch * 16 < c.D) w = *(const uint4*)((const uint8_t*)(v ? c.v : c.k) + (bh * c.Smax + row) * c.D + ch * 16);
-            const uint32_t u[4] = {prep_word<FMT>(w.x), prep_word<FMT>(w.y), prep_word<FMT>(w.z), prep_word<FMT>(w.w)};
-            uint4* dst = (uint4*)((v ? p.v16 : p.k16) + (lbh * p.Spad + row) * DP + ch * 16);
-            dst[0] = make_uint4(expand<FMT, 0>(u[0]), expand<FMT, 1>(u[0]), expand<FMT, 0>(u[1]), expand<FMT, 1>(u[1]));
-            dst[1] = make_uint4(expand<FMT, 0>(u[2]), expand<FMT, 1>(u[2]), expand<FMT, 0>(u[3]), expand<FMT, 1>(u[3]));
+        constexpr int CPR = DP / 8, STEPS = 2 * 64 * CPR / 256;  // 8 codes -> 16 bytes a step
+        uint2 w[STEPS];
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            const int e = k * 256 + threadIdx.x, v = e >= 64 * CPR, x = v ? e - 64 * CPR : e, row = r0 + x / CPR, ch = x % CPR;
+            w[k] = make_uint2(0, 0);
+            if (row < len && ch * 8 < c.D) w[k] = *(const uint2*)((const uint8_t*)(v ? c.v : c.k) + (bh * c.Smax + row) * c.D + ch * 8);
+        }
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+            const int e = k * 256 + threadIdx.x, v = e >= 64 * CPR, x = v ? e - 64 * CPR : e, row = r0 + x / CPR, ch = x % CPR;
+            const uint32_t u0 = prep_word<FMT>(w[k].x), u1 = prep_word<FMT>(w[k].y);
+            *(uint4*)((v ? p.v16 : p.k16) + (lbh * p.Spad + row) * DP + ch * 8) =
+                make_uint4(expand<FMT, 0>(u0), expand<FMT, 1>(u0), expand<FMT, 0>(u1), expand<FMT, 1>(u1));
         }
         if (threadIdx.x < 4) {
             const int k = r0 + threadIdx.x * 16;
@@ -135,7 +163,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* s
     return __all_sync(0xffffffffu, ok);
 }
 
-template <int D>
+// GROUPS: scales in a 128-key block (1, 2, 4 or 8: blocks of 128, 64, 32 or 16 tokens)
+template <int D, int GROUPS>
 __global__ void __launch_bounds__(NTHREADS, 1)
 kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ ChunkP p) {
@@ -160,32 +189,33 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     int* abort_flag = (int*)(tmem_slot + 1);
     int* item_slot = abort_flag + 1;     // [2]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int heads = (int)(p.nb * p.c.Hkv), n_items = heads * p.pairs * p.splits;
+    const int n_items = p.whole + p.tail * p.splits;
 
-    // Item i = (pair of tiles, last first; part of the keys; sequence x kv head fastest). nblk[t]: key blocks of tile
-    // t in this part; j0: the part's first block; n: blocks to load.
+    // Item i. nblk[t]: key blocks of tile t in this part; j0: the part's first block; n: blocks to load.
     struct Item {
-        int bh, pair, split, row0[2], nblk[2], j0, n, len, cnt;
+        int bh, slot, row0[2], nblk[2], j0, n, len, cnt;
     };
     auto item_of = [&](int i) {
         Item it;
-        const int rest = i / heads;
-        it.bh = i - rest * heads;
-        it.pair = p.pairs - 1 - rest / p.splits;
-        it.split = rest % p.splits;
-        const int64_t b = p.b0 + it.bh / p.c.Hkv;
+        const bool part = i >= p.whole;
+        it.slot = part ? i - p.whole : -1;
+        const int item = part ? p.whole + it.slot / p.splits : i, split = part ? it.slot % p.splits : 0, splits = part ? p.splits : 1;
+        const int per_seq = (int)p.c.Hkv * p.pairs, sq = item / per_seq, rest = item - sq * per_seq, hk = rest / p.pairs;
+        const int lb = p.order[sq], pair = p.pairs - 1 - (rest - hk * p.pairs);
+        it.bh = lb * (int)p.c.Hkv + hk;
+        const int64_t b = p.b0 + lb;
         it.len = (int)clamp64(p.c.lens[b], 0, p.c.Smax);
         it.cnt = p.counts ? (int)clamp64(p.counts[b], 0, p.Lq) : (int)p.Lq;
         int blk[2];
         for (int t = 0; t < 2; ++t) {
-            it.row0[t] = it.pair * 2 * BM + t * BM;
+            it.row0[t] = pair * 2 * BM + t * BM;
             const int last = min(it.row0[t] + BM, it.cnt * p.G) - 1;  // last row that has a query
             const int lim = last < it.row0[t] ? -1 : it.len - it.cnt + last / p.G;
             blk[t] = lim < 0 ? 0 : lim / BN + 1;
         }
         const int all = max(blk[0], blk[1]);
-        it.j0 = (int)((int64_t)all * it.split / p.splits);
-        const int j1 = (int)((int64_t)all * (it.split + 1) / p.splits);
+        it.j0 = (int)((int64_t)all * split / splits);
+        const int j1 = (int)((int64_t)all * (split + 1) / splits);
         it.n = 0;
         for (int t = 0; t < 2; ++t) {
             it.nblk[t] = max(0, min(j1, blk[t]) - it.j0);
@@ -392,47 +422,86 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     for (int e = 0; e < 128; ++e)
                         if (kv0 + e > lim) x[e] = -INFINITY;
                 }
-                // largest s + log2 sv of the block: per 16 keys the scale is one
+                // the block's scales: read once where they fit in registers
+                constexpr int GK = 128 / GROUPS;  // keys a scale covers
+                float g_mul[GROUPS <= 2 ? GROUPS : 1], g_add[GROUPS <= 2 ? GROUPS : 1], g_inv[GROUPS <= 2 ? GROUPS : 1];
+                auto scale_of_group = [&](int g, float& mul, float& add, float& inv) {
+                    const float4 z = __ldg(sc + g * (GK / 16));
+                    mul = fmaxf(qmul * z.x, 1e-37f);
+                    add = z.y;
+                    inv = z.z;
+                };
+                if constexpr (GROUPS <= 2) {
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g) scale_of_group(g, g_mul[g], g_add[g], g_inv[g]);
+                }
+                // largest s + log2 sv of the block
                 const float m_start = m_used;
                 float cm = -INFINITY;
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    const float4 z = __ldg(sc + g);
-                    const float* y = x + 16 * g;
+                for (int g = 0; g < GROUPS; ++g) {
+                    const float* y = x + GK * g;
                     float a = fmax3(y[0], y[1], y[2]), b = fmax3(y[3], y[4], y[5]), d = fmax3(y[6], y[7], y[8]);
                     a = fmax3(a, y[9], y[10]);
                     b = fmax3(b, y[11], y[12]);
                     d = fmax3(d, y[13], y[14]);
-                    a = fmax3(fmax3(a, b, d), y[15], y[15]);
-                    cm = fmaxf(cm, fmaf(a, fmaxf(qmul * z.x, 1e-37f), z.y));
+                    a = fmaxf(a, y[15]);
+#pragma unroll
+                    for (int e = 16; e + 5 < GK; e += 6) {
+                        a = fmax3(a, y[e], y[e + 1]);
+                        b = fmax3(b, y[e + 2], y[e + 3]);
+                        d = fmax3(d, y[e + 4], y[e + 5]);
+                    }
+#pragma unroll
+                    for (int e = 16 + (GK - 16) / 6 * 6; e < GK; ++e) a = fmaxf(a, y[e]);
+                    float mul, add, inv;
+                    if constexpr (GROUPS <= 2) {
+                        mul = g_mul[g];
+                        add = g_add[g];
+                    } else {
+                        scale_of_group(g, mul, add, inv);
+                    }
+                    cm = fmaxf(cm, fmaf(fmax3(a, b, d), mul, add));
                 }
                 if (cm > m_used + RAISE) m_used = cm;  // never while the row has no finite score
                 const bool grew = m_used != m_start;
                 const float off = m_used == -INFINITY ? 0.0f : SHIFT - m_used;
                 float block_sum = 0.0f;
+                uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
-                for (int g2 = 0; g2 < 4; ++g2) {
+                for (int c = 0; c < 4; ++c) {
                     uint32_t pk[16];
+                    constexpr int STEP = GK < 32 ? GK : 32;  // keys of the chunk that share a scale
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float4 z = __ldg(sc + 2 * g2 + h);
-                        const float mul = fmaxf(qmul * z.x, 1e-37f), add = z.y + off;
-                        const uint64_t mul2 = f2_pack(mul, mul), add2 = f2_pack(add, add);
-                        uint64_t sum2 = 0ull;
-#pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            const int at = 32 * g2 + 16 * h + e;
-                            float a0, a1;
-                            f2_unpack(f2_fma(f2_pack(x[at], x[at + 1]), mul2, add2), a0, a1);
-                            const float p0 = ex2(a0), p1 = ex2(a1);
-                            sum2 = f2_add(sum2, f2_pack(p0, p1));
-                            pk[8 * h + e / 2] = pack_f16(p0, p1);
+                    for (int h = 0; h < 32; h += STEP) {
+                        const int key = 32 * c + h, g = key / GK;
+                        float mul, add, inv;
+                        if constexpr (GROUPS <= 2) {
+                            mul = g_mul[g];
+                            add = g_add[g];
+                            inv = g_inv[g];
+                        } else {
+                            scale_of_group(g, mul, add, inv);
                         }
-                        float s0, s1;
-                        f2_unpack(sum2, s0, s1);
-                        block_sum = fmaf(s0 + s1, z.z, block_sum);
+                        add += off;
+                        const uint64_t mul2 = f2_pack(mul, mul), add2 = f2_pack(add, add);
+#pragma unroll
+                        for (int e = 0; e < STEP; e += 2) {
+                            float a0, a1;
+                            f2_unpack(f2_fma(f2_pack(x[key + e], x[key + e + 1]), mul2, add2), a0, a1);
+                            const float p0 = ex2(a0), p1 = ex2(a1);
+                            sum2[(e >> 1) & 1] = f2_add(sum2[(e >> 1) & 1], f2_pack(p0, p1));
+                            pk[(h + e) / 2] = pack_f16(p0, p1);
+                        }
+                        if ((key + STEP) % GK == 0) {  // the end of a scale's keys
+                            float s0, s1, s2, s3;
+                            f2_unpack(sum2[0], s0, s1);
+                            f2_unpack(sum2[1], s2, s3);
+                            block_sum = fmaf((s0 + s1) + (s2 + s3), inv, block_sum);
+                            sum2[0] = sum2[1] = 0ull;
+                        }
                     }
-                    tmem_st16(s_tmem + 32 * g2, pk);
+                    tmem_st16(s_tmem + 32 * c, pk);
                 }
                 if (__any_sync(0xffffffffu, grew && j > 0)) {
                     // PV_t(j-1) is complete: it was issued before S_t(j), whose completion we have seen
@@ -455,7 +524,7 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (!ok) break;
             u += nb;
             // results: the row's values, or its part of them; zeros for a row that attends nothing
-            const bool whole = p.splits == 1;
+            const bool whole = it.slot < 0;
             if (nb > 0) {
                 if (*(volatile int*)abort_flag) ok = false;
                 ok = __all_sync(0xffffffffu, ok) && warp_wait(&o_final[t], nf & 1, p.status, 133);
@@ -466,7 +535,7 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const int64_t b = p.b0 + it.bh / p.c.Hkv;
             const int h = (it.bh % (int)p.c.Hkv) * p.G + (row - qi * p.G);
             const int64_t at = b * p.o.sb + (int64_t)h * p.o.sh + (int64_t)qi * p.o.ss;
-            const int64_t prow = (((int64_t)(it.bh * p.pairs + it.pair) * p.splits + it.split) * 2 + t) * BM + r;
+            const int64_t prow = ((int64_t)it.slot * 2 + t) * BM + r;
             const float m_out = m_used == -INFINITY ? -INFINITY : m_used - SHIFT;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
@@ -519,24 +588,24 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
 }
 
-// One warp per row joins its parts
+// Joins the parts of a tail item: blockIdx.x the item, 8 rows a CTA, one a warp
 template <int D>
 __global__ void __launch_bounds__(256) kv8_chunk_join_kernel(const __grid_constant__ ChunkP p) {
     cudaGridDependencySynchronize();
-    const int lane = threadIdx.x & 31;
-    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t bh = w / p.R;
-    const int row = (int)(w - bh * p.R);
-    if (bh >= p.nb * p.c.Hkv) return;
-    const int64_t b = p.b0 + bh / p.c.Hkv;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per_seq = (int)p.c.Hkv * p.pairs, item = p.whole + (int)blockIdx.x, sq = item / per_seq, rest = item - sq * per_seq;
+    const int hk = rest / p.pairs, pair = p.pairs - 1 - (rest - hk * p.pairs);
+    const int64_t b = p.b0 + p.order[sq], first = (int64_t)blockIdx.x * p.splits * 2 * BM;
     const int cnt = p.counts ? (int)clamp64(p.counts[b], 0, p.Lq) : (int)p.Lq;
-    const int pair = row / (2 * BM), qi = row / p.G, h = (int)(bh % p.c.Hkv) * p.G + (row - qi * p.G);
-    const int64_t first = ((bh * p.pairs + pair) * p.splits * 2) * BM + row % (2 * BM);  // + split * 2 * BM
+    const int lr = blockIdx.y * 8 + warp, row = pair * 2 * BM + lr;
+    if (row >= p.R) return;
+    const int qi = row / p.G, h = hk * p.G + (row - qi * p.G);
     float m = -INFINITY, l = 0.0f, acc[D / 32] = {};
-    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[first + (int64_t)s * 2 * BM].x);
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part_ml[first + (int64_t)s * 2 * BM + lr].x);
     if (m == -INFINITY) m = 0.0f;
+#pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
-        const int64_t at = first + (int64_t)s * 2 * BM;
+        const int64_t at = first + (int64_t)s * 2 * BM + lr;
         const float2 ml = p.part_ml[at];
         const float f = ex2f(ml.x - m);
         l = fmaf(ml.y, f, l);
@@ -557,13 +626,13 @@ __global__ void __launch_bounds__(256) kv8_chunk_join_kernel(const __grid_consta
     if (p.lse && lane == 0) p.lse[(b * p.H + h) * p.Lq + qi] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
-template <int D>
+template <int D, int GROUPS>
 int set_up() {
     static std::atomic<uint64_t> ready{0};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 64 && (ready.load(std::memory_order_relaxed) >> dev & 1)) return 0;
-    auto kern = kv8_chunk_kernel<D>;
+    auto kern = kv8_chunk_kernel<D, GROUPS>;
     if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkCfg<D>::SMEM), "kv8_attention: shared memory"))
         return -1;
     // setmaxnreg.inc waits until the block's registers cover the split: refuse a build with fewer
@@ -586,9 +655,9 @@ bool map_rows(CUtensorMap* tm, void* data, int64_t heads, int64_t rows, int64_t 
     return make_tma_map_4d(tm, t, D, false, 128);
 }
 
-template <int D>
+template <int D, int GROUPS>
 int run(const Kv8AttnArgs& a, float* lse, int n_sm, cudaStream_t st) {
-    if (set_up<D>()) return -1;
+    if (set_up<D, GROUPS>()) return -1;
     ChunkP p{};
     p.c = a.c;
     p.q = a.q;
@@ -612,20 +681,27 @@ int run(const Kv8AttnArgs& a, float* lse, int n_sm, cudaStream_t st) {
     const int64_t Hkv = a.c.Hkv;
     const int64_t per_seq = Hkv * (p.Spad * D * 4 + p.Spad + p.Rpad * (D * 2 + 4));
     const int64_t nb = std::max<int64_t>(1, std::min<int64_t>(a.c.B, (2ll << 30) / std::max<int64_t>(per_seq, 1)));
-    // split the keys where there are too few items for the SMs, down to 512 keys a part
     const int64_t items = nb * Hkv * p.pairs;
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((2 * n_sm + items - 1) / items, p.Spad / 512));
-    if (items >= n_sm) p.splits = 1;
-    if (items * p.splits > INT32_MAX / 2 || nb * Hkv > 65535) {
+    if (items > INT32_MAX / 16 || nb * Hkv > 65535) {
         set_error("kv8_attention: too many work items");
         return -1;
     }
+    // the last items, one for two SMs, go in quarters; all of them in more parts where there are fewer items than that.
+    // No part is shorter than 512 keys at full length.
+    const int64_t most = std::max<int64_t>(1, p.Spad / 512);
+    auto plan = [&](int64_t n) {
+        p.splits = (int)std::min<int64_t>(most, n >= n_sm ? TAIL_SPLITS : (TAIL_SPLITS * n_sm + n - 1) / n);
+        p.tail = p.splits <= 1 ? 0 : n >= n_sm ? n_sm / 2 : (int)n;
+        p.whole = (int)n - p.tail;
+    };
+    plan(items);
     const int64_t heads = nb * Hkv;
     const int64_t b_kv = up(heads * p.Spad * D * 2), b_q = up(heads * p.Rpad * D * 2), b_s = up(heads * p.Spad), b_m = up(heads * p.Rpad * 4);
-    const int64_t prows = p.splits > 1 ? items * p.splits * 2 * BM : 0;
-    const int64_t b_po = up(prows * D * 4), b_pm = up(prows * 8);
+    // (a last launch with fewer sequences has at most n_sm items, in parts as many)
+    const int64_t prows = std::max<int64_t>((int64_t)p.tail * p.splits, std::min<int64_t>(n_sm * (TAIL_SPLITS + 1), n_sm * most)) * 2 * BM;
+    const int64_t b_po = up(prows * D * 4), b_pm = up(prows * 8), b_o = up(nb * 4);
     char* mem = nullptr;
-    if (cuda_failed(cudaMallocAsync((void**)&mem, 2 * b_kv + b_q + b_s + b_m + b_po + b_pm + 1024, st), "kv8_attention: scratch allocation"))
+    if (cuda_failed(cudaMallocAsync((void**)&mem, 2 * b_kv + b_q + b_s + b_m + b_po + b_pm + b_o + 1024, st), "kv8_attention: scratch allocation"))
         return -1;
     char* at = mem;
     auto take = [&](int64_t n) { char* r = at; at += n; return (void*)r; };
@@ -636,6 +712,7 @@ int run(const Kv8AttnArgs& a, float* lse, int n_sm, cudaStream_t st) {
     p.qmul = (float*)take(b_m);
     p.part_o = (float*)take(b_po);
     p.part_ml = (float2*)take(b_pm);
+    p.order = (int*)take(b_o);
     p.claim = (int*)take(1024);
     bool bad = false;
     for (int64_t b0 = 0; b0 < a.c.B && !bad; b0 += nb) {
@@ -647,16 +724,17 @@ int run(const Kv8AttnArgs& a, float* lse, int n_sm, cudaStream_t st) {
             bad = true;
             break;
         }
-        const dim3 grid((unsigned)(p.Spad / 64 + p.Rpad / 32), (unsigned)h);
+        plan(h * p.pairs);
+        const dim3 grid((unsigned)(p.Spad / 64 + p.Rpad / 32 + 1), (unsigned)h);
         if (a.c.format == GTB_KV8_INT8) kv8_widen_kernel<GTB_KV8_INT8, D><<<grid, 256, 0, st>>>(p);
         else kv8_widen_kernel<GTB_KV8_E4M3, D><<<grid, 256, 0, st>>>(p);
         bad = cuda_failed(cudaGetLastError(), "kv8_attention: widen launch");
         if (bad) break;
-        const int64_t n = h * p.pairs * p.splits;
-        bad = !launch_behind("kv8_attention: chunk launch", kv8_chunk_kernel<D>, dim3((unsigned)std::min<int64_t>(n, n_sm)), NTHREADS, st,
-                             ChunkCfg<D>::SMEM, mq, mk, mv, p);
-        if (!bad && p.splits > 1)
-            bad = !launch_behind("kv8_attention: join launch", kv8_chunk_join_kernel<D>, dim3((unsigned)((h * p.R + 7) / 8)), 256, st, 0, p);
+        bad = !launch_behind("kv8_attention: chunk launch", kv8_chunk_kernel<D, GROUPS>,
+                             dim3((unsigned)std::min<int64_t>(p.whole + (int64_t)p.tail * p.splits, n_sm)), NTHREADS, st, ChunkCfg<D>::SMEM,
+                             mq, mk, mv, p);
+        if (!bad && p.tail)
+            bad = !launch_behind("kv8_attention: join launch", kv8_chunk_join_kernel<D>, dim3((unsigned)p.tail, 2 * BM / 8), 256, st, 0, p);
     }
     cudaFreeAsync(mem, st);
     return bad ? -1 : 0;
@@ -670,7 +748,12 @@ bool chunk_supported(const Kv8AttnArgs& a) {
 }
 
 int launch_chunk(const Kv8AttnArgs& a, float* lse, int n_sm, cudaStream_t st) {
-    return a.c.D <= 64 ? run<64>(a, lse, n_sm, st) : run<128>(a, lse, n_sm, st);
+    switch (a.c.block) {
+        case 16: return a.c.D <= 64 ? run<64, 8>(a, lse, n_sm, st) : run<128, 8>(a, lse, n_sm, st);
+        case 32: return a.c.D <= 64 ? run<64, 4>(a, lse, n_sm, st) : run<128, 4>(a, lse, n_sm, st);
+        case 64: return a.c.D <= 64 ? run<64, 2>(a, lse, n_sm, st) : run<128, 2>(a, lse, n_sm, st);
+        default: return a.c.D <= 64 ? run<64, 1>(a, lse, n_sm, st) : run<128, 1>(a, lse, n_sm, st);
+    }
 }
 
 }  // namespace kv8
