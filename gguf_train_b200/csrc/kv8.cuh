@@ -56,48 +56,60 @@ __device__ __noinline__ uint8_t quantise8(float x, float s) {
     return Code8<FMT>::nearest(y);
 }
 
-// The same codes without a division each: x * (1 / s) is within a few ulp of the quotient, so it rounds to the
-// same code unless it lies that close to the middle between two; those (one in some thousands) and anything
-// not finite take quantise8. Scales near either end of f32 take it throughout.
+// The same codes without a division each. x (1 / s), a little up and a little down, bracket the quotient as the
+// division would round it; where both round to one code, that is the code. The others (next to the middle between two
+// codes: one in some ten thousand, more where values repeat) are divided. The caller sees to values that are
+// not finite; scales near either end of f32 divide throughout.
 struct Quantiser {
-    float s, inv;
-    bool plain;
-    __device__ explicit Quantiser(float scale) : s(scale), inv(0.0f), plain(!(scale > 1e-30f && scale < 1e30f)) {
-        if (!plain) inv = __frcp_rn(scale);
+    float s, up, down;
+    bool ends;
+    __device__ explicit Quantiser(float scale) : s(scale), up(0.0f), down(0.0f), ends(!(scale > 1e-30f && scale < 1e30f)) {
+        if (!ends) {
+            const float inv = __frcp_rn(scale);
+            up = inv * (1.0f + 0x1p-20f);
+            down = inv * (1.0f - 0x1p-20f);
+        }
+    }
+    // for values f x (f > 0): the same with f taken into the factor
+    __device__ void times(float f) {
+        up *= f;
+        down *= f;
+        ends |= !(f > 1e-30f && up < 1e30f);
     }
 };
 
 template <int FMT>
-__device__ __forceinline__ uint32_t quantise8x4(const float* x, const Quantiser& z) {
-    if (!z.plain) {
-        const float y0 = x[0] * z.inv, y1 = x[1] * z.inv, y2 = x[2] * z.inv, y3 = x[3] * z.inv;
-        if constexpr (FMT == GTB_KV8_INT8) {
-            constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the nearest integer's
-            const float r0 = y0 + MAGIC, r1 = y1 + MAGIC, r2 = y2 + MAGIC, r3 = y3 + MAGIC;
-            const float d = fmaxf(fmaxf(fabsf(y0 - (r0 - MAGIC)), fabsf(y1 - (r1 - MAGIC))),
-                                  fmaxf(fabsf(y2 - (r2 - MAGIC)), fabsf(y3 - (r3 - MAGIC))));
-            const float top = fmaxf(fmaxf(fabsf(y0), fabsf(y1)), fmaxf(fabsf(y2), fabsf(y3)));
-            // (fmaxf drops a NaN, so the sum asks for one)
-            if (d < 0.4999f && top < 127.4f && y0 + y1 + y2 + y3 == y0 + y1 + y2 + y3) {
-                const uint32_t lo = __byte_perm(__float_as_uint(r0), __float_as_uint(r1), 0x0040);
-                const uint32_t hi = __byte_perm(__float_as_uint(r2), __float_as_uint(r3), 0x0040);
-                return __byte_perm(lo, hi, 0x5410);
-            }
-        } else {
-            constexpr float UP = 1.0f + 0x1p-21f, DOWN = 1.0f - 0x1p-21f;
-            uint16_t a0, a1, b0, b1;
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a0) : "f"(y1 * DOWN), "f"(y0 * DOWN));
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a1) : "f"(y3 * DOWN), "f"(y2 * DOWN));
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b0) : "f"(y1 * UP), "f"(y0 * UP));
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b1) : "f"(y3 * UP), "f"(y2 * UP));
-            const float sum = y0 + y1 + y2 + y3;
-            if (a0 == b0 && a1 == b1 && sum - sum == 0.0f) return (uint32_t)a0 | ((uint32_t)a1 << 16);
-        }
-    }
+__device__ __forceinline__ uint32_t divide8x4(const float* x, float s) {
     uint32_t r = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r |= (uint32_t)quantise8<FMT>(x[i], z.s) << (8 * i);
+    for (int i = 0; i < 4; ++i) {
+        const float y = __fdiv_rn(x[i], s);
+        r |= (uint32_t)Code8<FMT>::nearest(fminf(fmaxf(y, -Code8<FMT>::TOP), Code8<FMT>::TOP)) << (8 * i);
+    }
     return r;
+}
+
+// Codes of finite x[0..3]; `exact` gives the numbers to divide by z.s where that is needed
+template <int FMT, typename Exact>
+__device__ __forceinline__ uint32_t quantise8x4(const float* x, const Quantiser& z, Exact&& exact) {
+    if constexpr (FMT == GTB_KV8_INT8) {
+        constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the nearest integer's
+        uint32_t a[4], diff = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            a[i] = __float_as_uint(fmaf(x[i], z.up, MAGIC));
+            diff |= a[i] ^ __float_as_uint(fmaf(x[i], z.down, MAGIC));
+        }
+        if (!z.ends && diff == 0) return __byte_perm(__byte_perm(a[0], a[1], 0x0040), __byte_perm(a[2], a[3], 0x0040), 0x5410);
+    } else {
+        uint16_t a0, a1, b0, b1;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a0) : "f"(x[1] * z.up), "f"(x[0] * z.up));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a1) : "f"(x[3] * z.up), "f"(x[2] * z.up));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b0) : "f"(x[1] * z.down), "f"(x[0] * z.down));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b1) : "f"(x[3] * z.down), "f"(x[2] * z.down));
+        if (!z.ends && a0 == b0 && a1 == b1) return (uint32_t)a0 | ((uint32_t)a1 << 16);
+    }
+    return exact();
 }
 
 // The four codes of a word as f32 values

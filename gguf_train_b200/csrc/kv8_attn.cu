@@ -101,8 +101,7 @@ int launch_kv8_attention(const Kv8AttnArgs& a, cudaStream_t st) {
         p.q = a.q;
         p.o = a.o;
         p.dtype = a.dtype;
-        const int64_t lead = a.dtype == F32 ? 16 : 8, es = a.dtype == F32 ? 4 : 2;
-        p.q_vec = ((uintptr_t)a.q.p % lead == 0) && a.q.sb * es % lead == 0 && a.q.sh * es % lead == 0 && a.q.ss * es % lead == 0;
+        p.q_vec = kv8::vector_rows(a.q, a.dtype);
         p.G = (int)(a.H / a.c.Hkv);
         p.R = p.G * (int)a.Lq;
         p.H = a.H;

@@ -3,6 +3,7 @@
 // lies in one row): 16 bytes of codes against 16 values.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gtb_common.cuh"
 #include "kv8.cuh"
@@ -20,10 +21,10 @@ __device__ __forceinline__ float block_max(float v, float* red) {
     return v;
 }
 
-// 16 values of a row as f32: 16-byte loads where the rows allow them
+// 16 values of a row: 16-byte loads where the rows allow them
 template <typename T, bool VEC>
 struct Chunk {
-    static constexpr int W = VEC ? 16 * sizeof(T) / 16 : 16;
+    static constexpr int W = VEC ? (int)sizeof(T) : 16;
     using Word = typename std::conditional<VEC, uint4, T>::type;
     Word w[W];
     __device__ void load(const T* p) {
@@ -34,51 +35,115 @@ struct Chunk {
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = Elem<T>::load((const T*)w + 4 * q + i);
     }
-    __device__ float amax() const {
-        float m = 0.0f, x[4];
+    // |x| of the largest finite value; `odd` if any is not finite
+    __device__ float amax(bool& odd) const {
+        float m = 0.0f;
+        if constexpr (VEC && sizeof(T) == 2) {
+            // the bits of |x| order as |x| does, two values a word; what is not finite comes last
+            uint32_t u = 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                u = __vmaxu2(u, w[i].x & 0x7fff7fffu);
+                u = __vmaxu2(u, w[i].y & 0x7fff7fffu);
+                u = __vmaxu2(u, w[i].z & 0x7fff7fffu);
+                u = __vmaxu2(u, w[i].w & 0x7fff7fffu);
+            }
+            const uint32_t top = max(u & 0xffffu, u >> 16);
+            if (top < (std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u)) {
+                const unsigned short b = (unsigned short)top;
+                return Elem<T>::load((const T*)&b);
+            }
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+            float x[4];
             values(q, x);
-            m = fmaxf(fmaxf(m, fmaxf(finite_abs(x[0]), finite_abs(x[1]))), fmaxf(finite_abs(x[2]), finite_abs(x[3])));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                odd |= !(fabsf(x[i]) <= 3.402823466e38f);
+                m = fmaxf(m, finite_abs(x[i]));
+            }
         }
         return m;
     }
     template <int FMT>
-    __device__ uint4 codes(const Quantiser& z) const {
-        float x[4];
-        uint4 r;
-        values(0, x); r.x = quantise8x4<FMT>(x, z);
-        values(1, x); r.y = quantise8x4<FMT>(x, z);
-        values(2, x); r.z = quantise8x4<FMT>(x, z);
-        values(3, x); r.w = quantise8x4<FMT>(x, z);
-        return r;
+    __device__ uint4 codes(const Quantiser& z, bool odd) const {
+        uint32_t r[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float x[4];
+            values(q, x);
+            if (odd || z.ends) {
+                r[q] = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[q] |= (uint32_t)quantise8<FMT>(x[i], z.s) << (8 * i);
+            } else {
+                r[q] = quantise8x4<FMT>(x, z, [&]() { return divide8x4<FMT>(x, z.s); });
+            }
+        }
+        return make_uint4(r[0], r[1], r[2], r[3]);
     }
 };
 
-// 16 codes at an old scale
+// 16 codes at an old scale (their values may be NaN only where a caller's own e4m3 codes are)
 template <int FMT>
 struct Codes16 {
     uint4 w;
-    __device__ float amax() const {  // of the codes' values, without the scale
+    // the largest finite |value|, without the scale
+    __device__ float amax(bool& odd) const {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-        float m = 0.0f, x[4];
+        if constexpr (FMT == GTB_KV8_INT8) {
+            // bytes as pairs of 16-bit integers, largest and smallest of all
+            uint32_t hi = 0, lo = 0;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            values8x4<FMT>(u[q], x);
-            m = fmaxf(fmaxf(m, fmaxf(finite_abs(x[0]), finite_abs(x[1]))), fmaxf(finite_abs(x[2]), finite_abs(x[3])));
+            for (int q = 0; q < 4; ++q) {
+                uint32_t a, b;  // bytes 0, 1 and 2, 3 with their signs (a selector of 8 + i repeats byte i's)
+                asm("prmt.b32 %0, %1, 0, 0x9180;" : "=r"(a) : "r"(u[q]));
+                asm("prmt.b32 %0, %1, 0, 0xb3a2;" : "=r"(b) : "r"(u[q]));
+                hi = __vimax3_s16x2(hi, a, b);
+                lo = __vimin3_s16x2(lo, a, b);
+            }
+            const int top = max((int)(int16_t)(hi & 0xffff), (int)(int16_t)(hi >> 16));
+            const int bot = min((int)(int16_t)(lo & 0xffff), (int)(int16_t)(lo >> 16));
+            odd |= bot < -127;  // a code that no quantiser gives, and that has to saturate
+            return (float)max(top, -bot);
+        } else {
+            // magnitudes order as their bits; 0x7f is NaN
+            uint32_t m = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) m = __vmaxu2(m, __vmaxu2(u[q] & 0x007f007fu, (u[q] >> 8) & 0x007f007fu));
+            const uint32_t top = max(m & 0xffffu, m >> 16);
+            if (top < 0x7fu) return Code8<FMT>::value((uint8_t)top);
+            odd = true;
+            float f = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float x[4];
+                values8x4<FMT>(u[q], x);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f = fmaxf(f, finite_abs(x[i]));
+            }
+            return f;
         }
-        return m;
     }
-    __device__ uint4 again(float s_old, const Quantiser& z) const {
+    // codes of (code * s_old) / s; z: of s, its factors times s_old
+    __device__ uint4 again(float s_old, const Quantiser& z, bool odd) const {
         const uint32_t u[4] = {w.x, w.y, w.z, w.w};
         uint32_t r[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             float x[4];
             values8x4<FMT>(u[q], x);
+            if (odd || z.ends) {
+                r[q] = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __fmul_rn(x[i], s_old);
-            r[q] = quantise8x4<FMT>(x, z);
+                for (int i = 0; i < 4; ++i) r[q] |= (uint32_t)quantise8<FMT>(__fmul_rn(x[i], s_old), z.s) << (8 * i);
+            } else {
+                r[q] = quantise8x4<FMT>(x, z, [&]() {
+                    const float y[4] = {__fmul_rn(x[0], s_old), __fmul_rn(x[1], s_old), __fmul_rn(x[2], s_old), __fmul_rn(x[3], s_old)};
+                    return divide8x4<FMT>(y, z.s);
+                });
+            }
         }
         return make_uint4(r[0], r[1], r[2], r[3]);
     }
@@ -109,6 +174,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
     const float s_old = j * bt < pos ? *scale : 0.0f;
     Chunk<T, VEC> kept[KEEP];
     float m = 0.0f;
+    bool odd = false;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const unsigned e = threadIdx.x + i * blockDim.x, r = e / cpr;
@@ -116,31 +182,38 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
     }
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
-        if (threadIdx.x + i * blockDim.x < n_new) m = fmaxf(m, kept[i].amax());
+        if (threadIdx.x + i * blockDim.x < n_new) m = fmaxf(m, kept[i].amax(odd));
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n_new; e += blockDim.x) {
         const unsigned r = e / cpr;
         Chunk<T, VEC> t;
         t.load(src + r * x.ss + (e - r * cpr) * 16);
-        m = fmaxf(m, t.amax());
+        m = fmaxf(m, t.amax(odd));
     }
     const float s = fmaxf(s_old, scale_of<FMT>(block_max(m, red)));
     const Quantiser z(s);
     if (s > s_old) {
         uint4* held = (uint4*)codes;
         const unsigned n_old = (unsigned)(r0 - j * bt) * cpr;
-        for (unsigned e = threadIdx.x; e < n_old; e += blockDim.x) held[e] = Codes16<FMT>{held[e]}.again(s_old, z);
+        Quantiser zo = z;
+        zo.times(s_old);
+        for (unsigned e = threadIdx.x; e < n_old; e += blockDim.x) {
+            const Codes16<FMT> w{held[e]};
+            bool nan = false;
+            w.amax(nan);
+            held[e] = w.again(s_old, zo, nan);
+        }
     }
     uint4* dst = (uint4*)(codes + (int64_t)(r0 - j * bt) * c.D);
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const unsigned e = threadIdx.x + i * blockDim.x;
-        if (e < n_new) dst[e] = kept[i].template codes<FMT>(z);
+        if (e < n_new) dst[e] = kept[i].template codes<FMT>(z, odd);
     }
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n_new; e += blockDim.x) {
         const unsigned r = e / cpr;
         Chunk<T, VEC> t;
         t.load(src + r * x.ss + (e - r * cpr) * 16);
-        dst[e] = t.template codes<FMT>(z);
+        dst[e] = t.template codes<FMT>(z, odd);
     }
     if (threadIdx.x == 0) *scale = s;
 }
@@ -347,6 +420,7 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__
     uint4* dst = (uint4*)(is_v ? a.dst.v : a.dst.k) + (bh * a.dst.Smax + r0) * cpr;
     Codes16<FMT> w[KEEP];
     float s_old[KEEP], m = 0.0f;
+    bool odd = false;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const unsigned e = threadIdx.x + i * blockDim.x, r = e / cpr;
@@ -359,21 +433,27 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__
     }
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
-        if (threadIdx.x + i * blockDim.x < n) m = fmaxf(m, finite_abs(__fmul_rn(w[i].amax(), s_old[i])));
+        if (threadIdx.x + i * blockDim.x < n) m = fmaxf(m, finite_abs(__fmul_rn(w[i].amax(odd), s_old[i])));
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n; e += blockDim.x) {
         const unsigned r = e / cpr, row = kept[r];
-        m = fmaxf(m, finite_abs(__fmul_rn(Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.amax(), sscale[row / bs])));
+        m = fmaxf(m, finite_abs(__fmul_rn(Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.amax(odd), sscale[row / bs])));
     }
     const float s = scale_of<FMT>(block_max(m, red));
     const Quantiser z(s);
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const unsigned e = threadIdx.x + i * blockDim.x;
-        if (e < n) dst[e] = w[i].again(s_old[i], z);
+        if (e < n) {
+            Quantiser zo = z;
+            zo.times(s_old[i]);
+            dst[e] = w[i].again(s_old[i], zo, odd);
+        }
     }
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n; e += blockDim.x) {
         const unsigned r = e / cpr, row = kept[r];
-        dst[e] = Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.again(sscale[row / bs], z);
+        Quantiser zo = z;
+        zo.times(sscale[row / bs]);
+        dst[e] = Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.again(sscale[row / bs], zo, odd);
     }
     if (threadIdx.x == 0) (is_v ? a.dst.v_scale : a.dst.k_scale)[bh * ((a.dst.Smax + bd - 1) / bd) + j] = s;
 }

@@ -52,7 +52,7 @@ struct ChunkCfg {
 struct ChunkP {
     gtb_kv8 c;
     Rows3 q, o;
-    int dtype, G, R, pairs;
+    int dtype, q_vec, G, R, pairs;
     int whole, tail, splits;     // items claimed whole, items claimed in `splits` parts each
     int64_t b0, nb;              // sequences of this launch
     int64_t H, Lq;
@@ -70,7 +70,7 @@ struct ChunkP {
     int* status;
 };
 
-// Rows of codes to f16, q to normalised f16: one warp per row of 32-row groups; blockIdx.y = (sequence, kv head). The last
+// Rows of codes (64 of K and V a CTA) to f16, rows of q (32) to normalised f16; blockIdx.y = (sequence, kv head). The last
 // CTA of the first row orders the sequences and zeroes the counter.
 template <int FMT, int DP>
 __global__ void __launch_bounds__(256) kv8_widen_kernel(const __grid_constant__ ChunkP p) {
@@ -128,27 +128,25 @@ __global__ void __launch_bounds__(256) kv8_widen_kernel(const __grid_constant__ 
         }
         return;
     }
-    // 32 rows of q, a warp each four
-    const int g0 = ((int)blockIdx.x - k_ctas) * 32;
-    for (int rr = warp; rr < 32; rr += 8) {
-        const int r = g0 + rr, i = r / p.G, h = (int)hk * p.G + (r - i * p.G);
-        const int64_t es = p.dtype == F32 ? 4 : 2;
-        const unsigned char* row = (const unsigned char*)p.q.p + (b * p.q.sb + h * p.q.sh + (int64_t)i * p.q.ss) * es;
-        float x[DP / 32], m = 0.0f;
+    // 32 rows of q, four values a lane
+    constexpr int LPR = DP / 4, RPW = 32 / LPR, STEPS = 4 / RPW;  // lanes of a row, rows a warp takes at once
+    const int g0 = ((int)blockIdx.x - k_ctas) * 32 + warp * 4 + lane / LPR, d = (lane % LPR) * 4;
+    float x[STEPS][4];
 #pragma unroll
-        for (int k = 0; k < DP / 32; ++k) {
-            const int d = 2 * lane + (k & 1) + 64 * (k >> 1);
-            x[k] = r < p.R && d < c.D ? load_any<float>(row, d, p.dtype) : 0.0f;
-            m = fmaxf(m, finite_abs(x[k]));
-        }
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int k = 0; k < STEPS; ++k) {
+        const int r = g0 + k * RPW, i = r / p.G, h = (int)hk * p.G + (r - i * p.G);
+        load_q4(p, b * p.q.sb + h * p.q.sh + (int64_t)i * p.q.ss + d, r < p.R && d < c.D, x[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+        float m = fmaxf(fmaxf(finite_abs(x[k][0]), finite_abs(x[k][1])), fmaxf(finite_abs(x[k][2]), finite_abs(x[k][3])));
+        for (int o = LPR / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         int e = (int)(__float_as_uint(m) >> 23) - 127;
         e = m >= 1.17549435e-38f ? min(max(e, -126), 126) : 0;
         const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        __half2* dst = (__half2*)(p.q16 + (lbh * p.Rpad + r) * DP);
-#pragma unroll
-        for (int k = 0; k < DP / 64; ++k) dst[lane + 32 * k] = __floats2half2_rn(x[2 * k] * down, x[2 * k + 1] * down);
-        if (lane == 0) p.qmul[lbh * p.Rpad + r] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
+        const int64_t row = lbh * p.Rpad + g0 + k * RPW;
+        *(uint2*)(p.q16 + row * DP + d) = make_uint2(pack_f16(x[k][0] * down, x[k][1] * down), pack_f16(x[k][2] * down, x[k][3] * down));
+        if (d == 0) p.qmul[row] = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale_log2;
     }
 }
 
@@ -663,6 +661,7 @@ int run(const Kv8AttnArgs& a, float* lse, int n_sm, cudaStream_t st) {
     p.q = a.q;
     p.o = a.o;
     p.dtype = a.dtype;
+    p.q_vec = vector_rows(a.q, a.dtype);
     p.G = (int)(a.H / a.c.Hkv);
     p.R = p.G * (int)a.Lq;
     p.pairs = (p.R + 2 * BM - 1) / (2 * BM);

@@ -147,7 +147,8 @@ struct Lay<256> {
 };
 
 // Four values of a query row as f32, 0 where it has none; in one load where every row starts on 16 (f32) or 8 bytes
-__device__ __forceinline__ void load_q4(const MmaP& p, int64_t at, bool live, float* x) {
+template <typename P>
+__device__ __forceinline__ void load_q4(const P& p, int64_t at, bool live, float* x) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = 0.0f;
     if (!live) return;
@@ -848,6 +849,12 @@ int launch_mma_rows(const MmaP& p, int n_sm, cudaStream_t st) {
         return wide ? launch_mma<DP, FMT, 4, 2>(p, n_sm, st) : launch_mma<DP, FMT, 4, 1>(p, n_sm, st);
     }
     return -1;
+}
+
+// Whether load_q4 may take four values at once
+inline int vector_rows(const Rows3& q, int dtype) {
+    const int64_t lead = dtype == F32 ? 16 : 8, es = dtype == F32 ? 4 : 2;
+    return (uintptr_t)q.p % lead == 0 && q.sb * es % lead == 0 && q.sh * es % lead == 0 && q.ss * es % lead == 0;
 }
 
 // Whether the first kernel should keep its scores for the weights: R f32 scores a key written and read against the
