@@ -48,7 +48,7 @@ __device__ __forceinline__ float scale_of(float amax) {
 
 // The code of x at scale s: round(x / s), saturating; 0 for NaN and for a zero scale
 template <int FMT>
-__device__ __noinline__ uint8_t quantise8(float x, float s) {
+__device__ __forceinline__ uint8_t quantise8(float x, float s) {
     if (!(s > 0.0f)) return 0;
     float y = __fdiv_rn(x, s);
     if (!(y == y)) return 0;
@@ -79,19 +79,16 @@ struct Quantiser {
 };
 
 template <int FMT>
-__device__ __forceinline__ uint32_t divide8x4(const float* x, float s) {
-    uint32_t r = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float y = __fdiv_rn(x[i], s);
-        r |= (uint32_t)Code8<FMT>::nearest(fminf(fmaxf(y, -Code8<FMT>::TOP), Code8<FMT>::TOP)) << (8 * i);
-    }
-    return r;
+__device__ __noinline__ uint32_t divide8x4(float x0, float x1, float x2, float x3, float s) {
+    return (uint32_t)quantise8<FMT>(x0, s) | (uint32_t)quantise8<FMT>(x1, s) << 8 | (uint32_t)quantise8<FMT>(x2, s) << 16 |
+           (uint32_t)quantise8<FMT>(x3, s) << 24;
 }
 
-// Codes of finite x[0..3]; `exact` gives the numbers to divide by z.s where that is needed
-template <int FMT, typename Exact>
-__device__ __forceinline__ uint32_t quantise8x4(const float* x, const Quantiser& z, Exact&& exact) {
+// Codes of x[0..3] * f at scale z.s, z made for values x f (f = 1: as they are); `odd`: some may not be finite
+template <int FMT>
+__device__ __forceinline__ uint32_t quantise8x4(const float* x, const Quantiser& z, float f, bool odd) {
+    uint32_t r;
+    bool same;
     if constexpr (FMT == GTB_KV8_INT8) {
         constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the nearest integer's
         uint32_t a[4], diff = 0;
@@ -100,16 +97,20 @@ __device__ __forceinline__ uint32_t quantise8x4(const float* x, const Quantiser&
             a[i] = __float_as_uint(fmaf(x[i], z.up, MAGIC));
             diff |= a[i] ^ __float_as_uint(fmaf(x[i], z.down, MAGIC));
         }
-        if (!z.ends && diff == 0) return __byte_perm(__byte_perm(a[0], a[1], 0x0040), __byte_perm(a[2], a[3], 0x0040), 0x5410);
+        same = diff == 0;
+        r = __byte_perm(__byte_perm(a[0], a[1], 0x0040), __byte_perm(a[2], a[3], 0x0040), 0x5410);
     } else {
         uint16_t a0, a1, b0, b1;
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a0) : "f"(x[1] * z.up), "f"(x[0] * z.up));
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a1) : "f"(x[3] * z.up), "f"(x[2] * z.up));
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b0) : "f"(x[1] * z.down), "f"(x[0] * z.down));
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b1) : "f"(x[3] * z.down), "f"(x[2] * z.down));
-        if (!z.ends && a0 == b0 && a1 == b1) return (uint32_t)a0 | ((uint32_t)a1 << 16);
+        same = a0 == b0 && a1 == b1;
+        r = (uint32_t)a0 | ((uint32_t)a1 << 16);
     }
-    return exact();
+    if (!same || odd || z.ends)
+        r = divide8x4<FMT>(__fmul_rn(x[0], f), __fmul_rn(x[1], f), __fmul_rn(x[2], f), __fmul_rn(x[3], f), z.s);
+    return r;
 }
 
 // The four codes of a word as f32 values

@@ -11,6 +11,13 @@
 namespace gtb {
 namespace {
 
+// Row of chunk e of a block (e < 128 * 16 + 1, cpr <= 16 chunks a row): a product with ceil(2^16 / cpr), exact there
+struct RowOf {
+    unsigned mul;
+    explicit RowOf(int64_t D) : mul((unsigned)(65536 / (D / 16) + (65536 % (D / 16) != 0))) {}
+    __device__ unsigned operator()(unsigned e) const { return e * mul >> 16; }
+};
+
 __device__ __forceinline__ float block_max(float v, float* red) {
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     if (blockDim.x == 32) return v;
@@ -73,13 +80,7 @@ struct Chunk {
         for (int q = 0; q < 4; ++q) {
             float x[4];
             values(q, x);
-            if (odd || z.ends) {
-                r[q] = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) r[q] |= (uint32_t)quantise8<FMT>(x[i], z.s) << (8 * i);
-            } else {
-                r[q] = quantise8x4<FMT>(x, z, [&]() { return divide8x4<FMT>(x, z.s); });
-            }
+            r[q] = quantise8x4<FMT>(x, z, 1.0f, odd);
         }
         return make_uint4(r[0], r[1], r[2], r[3]);
     }
@@ -134,16 +135,7 @@ struct Codes16 {
         for (int q = 0; q < 4; ++q) {
             float x[4];
             values8x4<FMT>(u[q], x);
-            if (odd || z.ends) {
-                r[q] = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) r[q] |= (uint32_t)quantise8<FMT>(__fmul_rn(x[i], s_old), z.s) << (8 * i);
-            } else {
-                r[q] = quantise8x4<FMT>(x, z, [&]() {
-                    const float y[4] = {__fmul_rn(x[0], s_old), __fmul_rn(x[1], s_old), __fmul_rn(x[2], s_old), __fmul_rn(x[3], s_old)};
-                    return divide8x4<FMT>(y, z.s);
-                });
-            }
+            r[q] = quantise8x4<FMT>(x, z, s_old, odd);
         }
         return make_uint4(r[0], r[1], r[2], r[3]);
     }
@@ -152,7 +144,7 @@ struct Codes16 {
 // One CTA per (touched block, sequence x kv head, K or V). The new rows stay in registers between the largest
 // value and the codes (KEEP chunks a thread; what does not fit is read again, from L2).
 template <typename T, int FMT, bool VEC, int KEEP>
-__global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a, unsigned blocks) {
+__global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a, unsigned blocks, RowOf row_of) {
     __shared__ float red[8];
     const gtb_kv8& c = a.c;
     const unsigned bhx = blockIdx.x / blocks, jx = blockIdx.x - bhx * blocks;
@@ -164,27 +156,27 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
     const int cnt = a.counts ? (int)clamp64(a.counts[b], 0, a.n) : (int)a.n;
     const int end = (int)min((int64_t)pos + cnt, c.Smax);
     if ((int64_t)pos + cnt > c.Smax && jx == 0 && threadIdx.x == 0) atomicCAS(a.status, 0, 61);
-    const int j = pos / bt + (int)jx;
+    const int shift = 31 - __clz(bt), j = (pos >> shift) + (int)jx;
     const int r0 = max(j * bt, pos), r1 = (int)min((int64_t)(j + 1) * bt, (int64_t)end);  // new rows of this block
     if (r0 >= r1) return;
     const unsigned cpr = (unsigned)c.D / 16, n_new = (unsigned)(r1 - r0) * cpr;
     const T* src = (const T*)x.p + b * x.sb + hk * x.sh + (int64_t)(r0 - pos) * x.ss;
     uint8_t* codes = (uint8_t*)(is_v ? c.v : c.k) + (bh * c.Smax + (int64_t)j * bt) * c.D;
-    float* scale = (is_v ? c.v_scale : c.k_scale) + bh * ((c.Smax + bt - 1) / bt) + j;
+    float* scale = (is_v ? c.v_scale : c.k_scale) + bh * ((c.Smax + bt - 1) >> shift) + j;
     const float s_old = j * bt < pos ? *scale : 0.0f;
     Chunk<T, VEC> kept[KEEP];
     float m = 0.0f;
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
-        const unsigned e = threadIdx.x + i * blockDim.x, r = e / cpr;
+        const unsigned e = threadIdx.x + i * blockDim.x, r = row_of(e);
         if (e < n_new) kept[i].load(src + r * x.ss + (e - r * cpr) * 16);
     }
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
         if (threadIdx.x + i * blockDim.x < n_new) m = fmaxf(m, kept[i].amax(odd));
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n_new; e += blockDim.x) {
-        const unsigned r = e / cpr;
+        const unsigned r = row_of(e);
         Chunk<T, VEC> t;
         t.load(src + r * x.ss + (e - r * cpr) * 16);
         m = fmaxf(m, t.amax(odd));
@@ -210,7 +202,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
         if (e < n_new) dst[e] = kept[i].template codes<FMT>(z, odd);
     }
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n_new; e += blockDim.x) {
-        const unsigned r = e / cpr;
+        const unsigned r = row_of(e);
         Chunk<T, VEC> t;
         t.load(src + r * x.ss + (e - r * cpr) * 16);
         dst[e] = t.template codes<FMT>(z, odd);
@@ -234,7 +226,8 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ K
     const unsigned cpr = (unsigned)c.D / 16, rows = 256 / cpr;  // rows a CTA covers at a time
     const unsigned row = threadIdx.x / cpr, chunk = threadIdx.x - row * cpr;
     if (row >= rows) return;
-    const int64_t nb = (c.Smax + c.block - 1) / c.block;
+    const int shift = 31 - __clz(c.block);
+    const int64_t nb = (c.Smax + c.block - 1) >> shift;
     for (int64_t p = blockIdx.y; p < 2 * c.B * c.Hkv; p += gridDim.y) {
         const bool is_v = p >= c.B * c.Hkv;
         const int64_t bh = is_v ? p - c.B * c.Hkv : p;
@@ -250,7 +243,7 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ K
             const int64_t t = t0 + i * rows, r = start + t;
             const bool live = t < a.n && r >= 0 && r < c.Smax;
             w[i] = live ? codes[r * cpr] : make_uint4(0, 0, 0, 0);
-            s[i] = live ? scale[(unsigned)r / (unsigned)c.block] : 0.0f;
+            s[i] = live ? scale[r >> shift] : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < READ_ROWS; ++i) {
@@ -400,13 +393,13 @@ __global__ void __launch_bounds__(SEL_THREADS) kv8_select_kernel(const __grid_co
 // One CTA per (destination block, sequence x kv head, K or V): the kept rows' values, their largest, the new
 // scale, the new codes. As in the append, KEEP chunks a thread stay in registers.
 template <int FMT, int KEEP>
-__global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__ Kv8EvictArgs a, unsigned blocks) {
+__global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__ Kv8EvictArgs a, unsigned blocks, RowOf row_of) {
     __shared__ float red[8];
     cudaGridDependencySynchronize();  // the kept rows and the new lengths are there
     const unsigned bhx = blockIdx.x / blocks, j = blockIdx.x - bhx * blocks;
     const int64_t bh = bhx;
     const bool is_v = blockIdx.y != 0;
-    const unsigned bs = a.src.block, bd = a.dst.block;
+    const unsigned bs = a.src.block, bd = a.dst.block, shift = 31 - __clz((int)bs);
     const int newlen = a.dst.lens[bhx / (unsigned)a.src.Hkv];
     const int r0 = (int)(j * bd), r1 = min(r0 + (int)bd, newlen);
     const int32_t* kept = a.kept + bh * a.budget + r0;
@@ -416,27 +409,27 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__
     if (r0 >= r1) return;
     const unsigned cpr = (unsigned)a.src.D / 16, n = (unsigned)(r1 - r0) * cpr;
     const uint4* src = (const uint4*)(is_v ? a.src.v : a.src.k) + bh * a.src.Smax * cpr;
-    const float* sscale = (is_v ? a.src.v_scale : a.src.k_scale) + bh * ((a.src.Smax + bs - 1) / bs);
+    const float* sscale = (is_v ? a.src.v_scale : a.src.k_scale) + bh * ((a.src.Smax + bs - 1) >> shift);
     uint4* dst = (uint4*)(is_v ? a.dst.v : a.dst.k) + (bh * a.dst.Smax + r0) * cpr;
     Codes16<FMT> w[KEEP];
     float s_old[KEEP], m = 0.0f;
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
-        const unsigned e = threadIdx.x + i * blockDim.x, r = e / cpr;
+        const unsigned e = threadIdx.x + i * blockDim.x, r = row_of(e);
         s_old[i] = 0.0f;
         if (e < n) {
             const unsigned row = kept[r];
             w[i].w = src[(int64_t)row * cpr + (e - r * cpr)];
-            s_old[i] = sscale[row / bs];
+            s_old[i] = sscale[row >> shift];
         }
     }
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
         if (threadIdx.x + i * blockDim.x < n) m = fmaxf(m, finite_abs(__fmul_rn(w[i].amax(odd), s_old[i])));
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n; e += blockDim.x) {
-        const unsigned r = e / cpr, row = kept[r];
-        m = fmaxf(m, finite_abs(__fmul_rn(Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.amax(odd), sscale[row / bs])));
+        const unsigned r = row_of(e), row = kept[r];
+        m = fmaxf(m, finite_abs(__fmul_rn(Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.amax(odd), sscale[row >> shift])));
     }
     const float s = scale_of<FMT>(block_max(m, red));
     const Quantiser z(s);
@@ -450,12 +443,12 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__
         }
     }
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n; e += blockDim.x) {
-        const unsigned r = e / cpr, row = kept[r];
+        const unsigned r = row_of(e), row = kept[r];
         Quantiser zo = z;
-        zo.times(sscale[row / bs]);
-        dst[e] = Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.again(sscale[row / bs], zo, odd);
+        zo.times(sscale[row >> shift]);
+        dst[e] = Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.again(sscale[row >> shift], zo, odd);
     }
-    if (threadIdx.x == 0) (is_v ? a.dst.v_scale : a.dst.k_scale)[bh * ((a.dst.Smax + bd - 1) / bd) + j] = s;
+    if (threadIdx.x == 0) (is_v ? a.dst.v_scale : a.dst.k_scale)[bh * ((a.dst.Smax + bd - 1) >> (31 - __clz((int)bd))) + j] = s;
 }
 
 // Threads for `chunks` of work in a CTA: a power of two, two chunks a thread where there are enough
@@ -483,8 +476,12 @@ int append_t(const Kv8AppendArgs& a, cudaStream_t st) {
         vec = vec && ((uintptr_t)r->p & 15) == 0 && r->sb % N == 0 && r->sh % N == 0 && r->ss % N == 0;
     const int threads = threads_for(std::min<int64_t>(a.n, a.c.block) * (a.c.D / 16));
     const dim3 grid((unsigned)n, 2);
-    if (vec) kv8_append_kernel<T, FMT, true, sizeof(T) == 4 ? 2 : 4><<<grid, threads, 0, st>>>(a, (unsigned)blocks);
-    else kv8_append_kernel<T, FMT, false, 2><<<grid, threads, 0, st>>>(a, (unsigned)blocks);
+    // chunks a thread keeps: two cover a block of 64 tokens x 128, four one of 128 x 128
+    const bool few = std::min<int64_t>(a.n, a.c.block) * (a.c.D / 16) <= 2 * threads;
+    auto go = [&](auto kern) { kern<<<grid, threads, 0, st>>>(a, (unsigned)blocks, RowOf(a.c.D)); };
+    if (!vec) go(kv8_append_kernel<T, FMT, false, 1>);
+    else if (few || sizeof(T) == 4) go(kv8_append_kernel<T, FMT, true, 2>);
+    else go(kv8_append_kernel<T, FMT, true, 4>);
     return cuda_failed(cudaGetLastError(), "kv8_append launch") ? -1 : 0;
 }
 
@@ -516,7 +513,9 @@ bool gather(const Kv8EvictArgs& a, cudaStream_t st) {
     const int64_t blocks = (rows + a.dst.block - 1) / a.dst.block, n = blocks * a.src.B * a.src.Hkv;
     if (!grid_fits(n, "kv8_evict")) return false;
     const int threads = threads_for(std::min<int64_t>(a.budget, a.dst.block) * (a.src.D / 16));
-    return launch_behind("kv8_evict: gather launch", kv8_gather_kernel<FMT, 4>, dim3((unsigned)n, 2), threads, st, 0, a, (unsigned)blocks);
+    const bool few = std::min<int64_t>(a.budget, a.dst.block) * (a.src.D / 16) <= 2 * threads;
+    return launch_behind("kv8_evict: gather launch", few ? kv8_gather_kernel<FMT, 2> : kv8_gather_kernel<FMT, 4>, dim3((unsigned)n, 2),
+                         threads, st, 0, a, (unsigned)blocks, RowOf(a.src.D));
 }
 
 }  // namespace

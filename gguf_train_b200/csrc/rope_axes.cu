@@ -5,7 +5,7 @@
 //
 // HBM bound: every value is read and written once. A CTA takes TOK tokens of one sequence and a share of the
 // heads: it forms the tokens' (cos, sin) table once in shared memory, then each thread keeps the part of the table
-// that belongs to its 16 bytes of a row in registers and walks the heads with 16-byte accesses, four rows in
+// that belongs to its 16 bytes of a row in registers and walks the heads with 16-byte accesses, two rows in
 // flight.
 
 #include <algorithm>
@@ -30,21 +30,28 @@ struct Vec {
     T v[N];
 };
 
-constexpr int THREADS = 256, FLIGHT = 4;
+constexpr int THREADS = 256, FLIGHT = 2;
 
 // A thread owns one piece of a row: V values, and in mode 2 their V partners P further on (V = 16 bytes, or one
 // value where sizes, strides or alignment allow no more). Pieces per row: the rotated ones first, then the
 // dims that pass through.
 template <typename T, int V, int MODE>
-__global__ void __launch_bounds__(THREADS) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a, int tok, int rot, int pieces,
+__global__ void __launch_bounds__(THREADS, 4) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a, int tok, int rot, int pieces,
                                                             int groups, int heads_per_group) {
     extern __shared__ float2 tab[];  // [tok][pairs]
     const int64_t s0 = (int64_t)blockIdx.x * tok, b = blockIdx.z;
     const int P = a.pairs;
+    // (a parameter indexed by lane is read a lane at a time, so each pair's frequency and axis are read once)
+    __shared__ uint64_t turn[ROPE_MAX_PAIRS];
+    __shared__ int64_t axis[ROPE_MAX_PAIRS];
+    if (threadIdx.x < P) {
+        turn[threadIdx.x] = a.tab.turn[threadIdx.x];
+        axis[threadIdx.x] = a.tab.axis[threadIdx.x] * a.pos_axis + b * a.pos_batch + s0;
+    }
+    __syncthreads();
     for (int e = threadIdx.x; e < tok * P; e += THREADS) {
         const int sl = e / P, i = e - sl * P;
-        if (s0 + sl < a.S)
-            tab[e] = turn_of(a.pos[a.tab.axis[i] * a.pos_axis + b * a.pos_batch + s0 + sl], a.tab.turn[i], a.sin_sign);
+        if (s0 + sl < a.S) tab[e] = turn_of(a.pos[axis[i] + sl], turn[i], a.sin_sign);
     }
     __syncthreads();
     // thread -> (head group within the CTA, token, piece)
