@@ -18,13 +18,20 @@ struct RowOf {
     __device__ unsigned operator()(unsigned e) const { return e * mul >> 16; }
 };
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+// The CTA's largest x and largest y
+__device__ __forceinline__ float2 block_max(float2 v, float2* red) {
+    for (int o = 16; o; o >>= 1) {
+        v.x = fmaxf(v.x, __shfl_xor_sync(0xffffffffu, v.x, o));
+        v.y = fmaxf(v.y, __shfl_xor_sync(0xffffffffu, v.y, o));
+    }
     if (blockDim.x == 32) return v;
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     v = red[threadIdx.x & 31 & ((blockDim.x >> 5) - 1)];  // blockDim a power of two
-    for (int o = (int)(blockDim.x >> 6); o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = (int)(blockDim.x >> 6); o; o >>= 1) {
+        v.x = fmaxf(v.x, __shfl_xor_sync(0xffffffffu, v.x, o));
+        v.y = fmaxf(v.y, __shfl_xor_sync(0xffffffffu, v.y, o));
+    }
     return v;
 }
 
@@ -141,16 +148,14 @@ struct Codes16 {
     }
 };
 
-// One CTA per (touched block, sequence x kv head, K or V). The new rows stay in registers between the largest
-// value and the codes (KEEP chunks a thread; what does not fit is read again, from L2).
+// One CTA per (touched block, sequence x kv head), K and V together. The new rows stay in registers between the largest
+// value and the codes (KEEP chunks of each a thread; what does not fit is read again, from L2).
 template <typename T, int FMT, bool VEC, int KEEP>
 __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a, unsigned blocks, RowOf row_of) {
-    __shared__ float red[8];
+    __shared__ float2 red[8];
     const gtb_kv8& c = a.c;
     const unsigned bhx = blockIdx.x / blocks, jx = blockIdx.x - bhx * blocks;
-    const bool is_v = blockIdx.y != 0;
     const int64_t bh = bhx, b = bhx / (unsigned)c.Hkv, hk = bh - b * c.Hkv;
-    const Rows3& x = is_v ? a.v : a.k;
     const int bt = c.block;
     const int pos = (int)clamp64(c.lens[b], 0, c.Smax);
     const int cnt = a.counts ? (int)clamp64(a.counts[b], 0, a.n) : (int)a.n;
@@ -160,54 +165,79 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
     const int r0 = max(j * bt, pos), r1 = (int)min((int64_t)(j + 1) * bt, (int64_t)end);  // new rows of this block
     if (r0 >= r1) return;
     const unsigned cpr = (unsigned)c.D / 16, n_new = (unsigned)(r1 - r0) * cpr;
-    const T* src = (const T*)x.p + b * x.sb + hk * x.sh + (int64_t)(r0 - pos) * x.ss;
-    uint8_t* codes = (uint8_t*)(is_v ? c.v : c.k) + (bh * c.Smax + (int64_t)j * bt) * c.D;
-    float* scale = (is_v ? c.v_scale : c.k_scale) + bh * ((c.Smax + bt - 1) >> shift) + j;
-    const float s_old = j * bt < pos ? *scale : 0.0f;
-    Chunk<T, VEC> kept[KEEP];
-    float m = 0.0f;
+    const T* src_k = (const T*)a.k.p + b * a.k.sb + hk * a.k.sh + (int64_t)(r0 - pos) * a.k.ss;
+    const T* src_v = (const T*)a.v.p + b * a.v.sb + hk * a.v.sh + (int64_t)(r0 - pos) * a.v.ss;
+    const int64_t at = (bh * c.Smax + (int64_t)j * bt) * c.D, sat = bh * ((c.Smax + bt - 1) >> shift) + j;
+    const bool had = j * bt < pos;
+    const float2 s_old = had ? make_float2(c.k_scale[sat], c.v_scale[sat]) : make_float2(0.0f, 0.0f);
+    Chunk<T, VEC> kk[KEEP], kv[KEEP];
+    float2 m = make_float2(0.0f, 0.0f);
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
-        const unsigned e = threadIdx.x + i * blockDim.x, r = row_of(e);
-        if (e < n_new) kept[i].load(src + r * x.ss + (e - r * cpr) * 16);
+        const unsigned e = threadIdx.x + i * blockDim.x, r = row_of(e), d = (e - r * cpr) * 16;
+        if (e < n_new) {
+            kk[i].load(src_k + r * a.k.ss + d);
+            kv[i].load(src_v + r * a.v.ss + d);
+        }
     }
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
-        if (threadIdx.x + i * blockDim.x < n_new) m = fmaxf(m, kept[i].amax(odd));
+        if (threadIdx.x + i * blockDim.x < n_new) {
+            m.x = fmaxf(m.x, kk[i].amax(odd));
+            m.y = fmaxf(m.y, kv[i].amax(odd));
+        }
+#pragma unroll 1
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n_new; e += blockDim.x) {
-        const unsigned r = row_of(e);
+        const unsigned r = row_of(e), d = (e - r * cpr) * 16;
         Chunk<T, VEC> t;
-        t.load(src + r * x.ss + (e - r * cpr) * 16);
-        m = fmaxf(m, t.amax(odd));
+        t.load(src_k + r * a.k.ss + d);
+        m.x = fmaxf(m.x, t.amax(odd));
+        t.load(src_v + r * a.v.ss + d);
+        m.y = fmaxf(m.y, t.amax(odd));
     }
-    const float s = fmaxf(s_old, scale_of<FMT>(block_max(m, red)));
-    const Quantiser z(s);
-    if (s > s_old) {
-        uint4* held = (uint4*)codes;
-        const unsigned n_old = (unsigned)(r0 - j * bt) * cpr;
+    m = block_max(m, red);
+    const float2 s = make_float2(fmaxf(s_old.x, scale_of<FMT>(m.x)), fmaxf(s_old.y, scale_of<FMT>(m.y)));
+    const Quantiser zk(s.x), zv(s.y);
+    // the rows already held, where their scale grew
+    auto requantise = [&](void* codes, float from, const Quantiser& z) {
         Quantiser zo = z;
-        zo.times(s_old);
+        zo.times(from);
+        uint4* held = (uint4*)((uint8_t*)codes + at);
+        const unsigned n_old = (unsigned)(r0 - j * bt) * cpr;
+#pragma unroll 1
         for (unsigned e = threadIdx.x; e < n_old; e += blockDim.x) {
             const Codes16<FMT> w{held[e]};
             bool nan = false;
             w.amax(nan);
-            held[e] = w.again(s_old, zo, nan);
+            held[e] = w.again(from, zo, nan);
         }
-    }
-    uint4* dst = (uint4*)(codes + (int64_t)(r0 - j * bt) * c.D);
+    };
+    if (had && s.x > s_old.x) requantise(c.k, s_old.x, zk);
+    if (had && s.y > s_old.y) requantise(c.v, s_old.y, zv);
+    const int64_t to = at + (int64_t)(r0 - j * bt) * c.D;
+    uint4 *dst_k = (uint4*)((uint8_t*)c.k + to), *dst_v = (uint4*)((uint8_t*)c.v + to);
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const unsigned e = threadIdx.x + i * blockDim.x;
-        if (e < n_new) dst[e] = kept[i].template codes<FMT>(z, odd);
+        if (e < n_new) {
+            dst_k[e] = kk[i].template codes<FMT>(zk, odd);
+            dst_v[e] = kv[i].template codes<FMT>(zv, odd);
+        }
     }
+#pragma unroll 1
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n_new; e += blockDim.x) {
-        const unsigned r = row_of(e);
+        const unsigned r = row_of(e), d = (e - r * cpr) * 16;
         Chunk<T, VEC> t;
-        t.load(src + r * x.ss + (e - r * cpr) * 16);
-        dst[e] = t.template codes<FMT>(z, odd);
+        t.load(src_k + r * a.k.ss + d);
+        dst_k[e] = t.template codes<FMT>(zk, odd);
+        t.load(src_v + r * a.v.ss + d);
+        dst_v[e] = t.template codes<FMT>(zv, odd);
     }
-    if (threadIdx.x == 0) *scale = s;
+    if (threadIdx.x == 0) {
+        c.k_scale[sat] = s.x;
+        c.v_scale[sat] = s.y;
+    }
 }
 
 __global__ void kv8_advance_kernel(const Kv8AppendArgs a) {
@@ -390,65 +420,83 @@ __global__ void __launch_bounds__(SEL_THREADS) kv8_select_kernel(const __grid_co
     }
 }
 
-// One CTA per (destination block, sequence x kv head, K or V): the kept rows' values, their largest, the new
-// scale, the new codes. As in the append, KEEP chunks a thread stay in registers.
+// One CTA per (destination block, sequence x kv head), K and V together: the kept rows' values, their largest, the new
+// scale, the new codes. As in the append, KEEP chunks of each a thread stay in registers.
 template <int FMT, int KEEP>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__ Kv8EvictArgs a, unsigned blocks, RowOf row_of) {
-    __shared__ float red[8];
+    __shared__ float2 red[8];
     cudaGridDependencySynchronize();  // the kept rows and the new lengths are there
     const unsigned bhx = blockIdx.x / blocks, j = blockIdx.x - bhx * blocks;
     const int64_t bh = bhx;
-    const bool is_v = blockIdx.y != 0;
-    const unsigned bs = a.src.block, bd = a.dst.block, shift = 31 - __clz((int)bs);
+    const int bs = a.src.block, bd = a.dst.block, shift = 31 - __clz(bs);
     const int newlen = a.dst.lens[bhx / (unsigned)a.src.Hkv];
-    const int r0 = (int)(j * bd), r1 = min(r0 + (int)bd, newlen);
+    const int r0 = (int)(j * bd), r1 = min(r0 + bd, newlen);
     const int32_t* kept = a.kept + bh * a.budget + r0;
-    if (!is_v && a.score_out)
+    if (a.score_out)
         for (int64_t r = r0 + threadIdx.x; r < min((int64_t)r0 + bd, a.dst.Smax); r += blockDim.x)
             a.score_out[bh * a.dst.Smax + r] = r < newlen ? a.score[bh * a.src.Smax + kept[r - r0]] : 0.0f;
     if (r0 >= r1) return;
     const unsigned cpr = (unsigned)a.src.D / 16, n = (unsigned)(r1 - r0) * cpr;
-    const uint4* src = (const uint4*)(is_v ? a.src.v : a.src.k) + bh * a.src.Smax * cpr;
-    const float* sscale = (is_v ? a.src.v_scale : a.src.k_scale) + bh * ((a.src.Smax + bs - 1) >> shift);
-    uint4* dst = (uint4*)(is_v ? a.dst.v : a.dst.k) + (bh * a.dst.Smax + r0) * cpr;
-    Codes16<FMT> w[KEEP];
-    float s_old[KEEP], m = 0.0f;
+    const uint4 *src_k = (const uint4*)a.src.k + bh * a.src.Smax * cpr, *src_v = (const uint4*)a.src.v + bh * a.src.Smax * cpr;
+    const int64_t ns = bh * ((a.src.Smax + bs - 1) >> shift), to = (bh * a.dst.Smax + r0) * cpr;
+    const float *sk = a.src.k_scale + ns, *sv = a.src.v_scale + ns;
+    uint4 *dst_k = (uint4*)a.dst.k + to, *dst_v = (uint4*)a.dst.v + to;
+    Codes16<FMT> wk[KEEP], wv[KEEP];
+    float2 s_old[KEEP], m = make_float2(0.0f, 0.0f);
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const unsigned e = threadIdx.x + i * blockDim.x, r = row_of(e);
-        s_old[i] = 0.0f;
+        s_old[i] = make_float2(0.0f, 0.0f);
         if (e < n) {
             const unsigned row = kept[r];
-            w[i].w = src[(int64_t)row * cpr + (e - r * cpr)];
-            s_old[i] = sscale[row >> shift];
+            const int64_t at = (int64_t)row * cpr + (e - r * cpr);
+            wk[i].w = src_k[at];
+            wv[i].w = src_v[at];
+            s_old[i] = make_float2(sk[row >> shift], sv[row >> shift]);
         }
     }
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
-        if (threadIdx.x + i * blockDim.x < n) m = fmaxf(m, finite_abs(__fmul_rn(w[i].amax(odd), s_old[i])));
+        if (threadIdx.x + i * blockDim.x < n) {
+            m.x = fmaxf(m.x, finite_abs(__fmul_rn(wk[i].amax(odd), s_old[i].x)));
+            m.y = fmaxf(m.y, finite_abs(__fmul_rn(wv[i].amax(odd), s_old[i].y)));
+        }
+#pragma unroll 1
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n; e += blockDim.x) {
         const unsigned r = row_of(e), row = kept[r];
-        m = fmaxf(m, finite_abs(__fmul_rn(Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.amax(odd), sscale[row >> shift])));
+        const int64_t at = (int64_t)row * cpr + (e - r * cpr);
+        m.x = fmaxf(m.x, finite_abs(__fmul_rn(Codes16<FMT>{src_k[at]}.amax(odd), sk[row >> shift])));
+        m.y = fmaxf(m.y, finite_abs(__fmul_rn(Codes16<FMT>{src_v[at]}.amax(odd), sv[row >> shift])));
     }
-    const float s = scale_of<FMT>(block_max(m, red));
-    const Quantiser z(s);
+    m = block_max(m, red);
+    const float2 s = make_float2(scale_of<FMT>(m.x), scale_of<FMT>(m.y));
+    const Quantiser zk(s.x), zv(s.y);
+    auto again = [&](const Codes16<FMT>& w, float from, const Quantiser& z) {
+        Quantiser zo = z;
+        zo.times(from);
+        return w.again(from, zo, odd);
+    };
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const unsigned e = threadIdx.x + i * blockDim.x;
         if (e < n) {
-            Quantiser zo = z;
-            zo.times(s_old[i]);
-            dst[e] = w[i].again(s_old[i], zo, odd);
+            dst_k[e] = again(wk[i], s_old[i].x, zk);
+            dst_v[e] = again(wv[i], s_old[i].y, zv);
         }
     }
+#pragma unroll 1
     for (unsigned e = threadIdx.x + KEEP * blockDim.x; e < n; e += blockDim.x) {
         const unsigned r = row_of(e), row = kept[r];
-        Quantiser zo = z;
-        zo.times(sscale[row >> shift]);
-        dst[e] = Codes16<FMT>{src[(int64_t)row * cpr + (e - r * cpr)]}.again(sscale[row >> shift], zo, odd);
+        const int64_t at = (int64_t)row * cpr + (e - r * cpr);
+        dst_k[e] = again(Codes16<FMT>{src_k[at]}, sk[row >> shift], zk);
+        dst_v[e] = again(Codes16<FMT>{src_v[at]}, sv[row >> shift], zv);
     }
-    if (threadIdx.x == 0) (is_v ? a.dst.v_scale : a.dst.k_scale)[bh * ((a.dst.Smax + bd - 1) >> (31 - __clz((int)bd))) + j] = s;
+    if (threadIdx.x == 0) {
+        const int64_t nd = bh * ((a.dst.Smax + bd - 1) >> (31 - __clz(bd))) + j;
+        a.dst.k_scale[nd] = s.x;
+        a.dst.v_scale[nd] = s.y;
+    }
 }
 
 // Threads for `chunks` of work in a CTA: a power of two, two chunks a thread where there are enough
@@ -475,12 +523,13 @@ int append_t(const Kv8AppendArgs& a, cudaStream_t st) {
     for (const Rows3* r : {&a.k, &a.v})
         vec = vec && ((uintptr_t)r->p & 15) == 0 && r->sb % N == 0 && r->sh % N == 0 && r->ss % N == 0;
     const int threads = threads_for(std::min<int64_t>(a.n, a.c.block) * (a.c.D / 16));
-    const dim3 grid((unsigned)n, 2);
+    const dim3 grid((unsigned)n);
     // chunks a thread keeps: two cover a block of 64 tokens x 128, four one of 128 x 128
     const bool few = std::min<int64_t>(a.n, a.c.block) * (a.c.D / 16) <= 2 * threads;
     auto go = [&](auto kern) { kern<<<grid, threads, 0, st>>>(a, (unsigned)blocks, RowOf(a.c.D)); };
     if (!vec) go(kv8_append_kernel<T, FMT, false, 1>);
-    else if (few || sizeof(T) == 4) go(kv8_append_kernel<T, FMT, true, 2>);
+    else if (sizeof(T) == 4) go(kv8_append_kernel<T, FMT, true, 1>);
+    else if (few) go(kv8_append_kernel<T, FMT, true, 2>);
     else go(kv8_append_kernel<T, FMT, true, 4>);
     return cuda_failed(cudaGetLastError(), "kv8_append launch") ? -1 : 0;
 }
@@ -514,7 +563,7 @@ bool gather(const Kv8EvictArgs& a, cudaStream_t st) {
     if (!grid_fits(n, "kv8_evict")) return false;
     const int threads = threads_for(std::min<int64_t>(a.budget, a.dst.block) * (a.src.D / 16));
     const bool few = std::min<int64_t>(a.budget, a.dst.block) * (a.src.D / 16) <= 2 * threads;
-    return launch_behind("kv8_evict: gather launch", few ? kv8_gather_kernel<FMT, 2> : kv8_gather_kernel<FMT, 4>, dim3((unsigned)n, 2),
+    return launch_behind("kv8_evict: gather launch", few ? kv8_gather_kernel<FMT, 2> : kv8_gather_kernel<FMT, 4>, dim3((unsigned)n),
                          threads, st, 0, a, (unsigned)blocks, RowOf(a.src.D));
 }
 
