@@ -6,6 +6,9 @@
 // warp that finishes an item alone writes the result; otherwise it leaves (out, max, sum) for
 // kv8_finish_kernel.
 //
+// Where the cache is short and the items few (one_cta()), a CTA takes an item instead: its warps take its units in turn
+// and meet in shared memory, and everything is done in one launch.
+//
 // A warp streams its units through its own ring in shared memory with 16-byte asynchronous copies (rows
 // past the length arrive as zeros: nothing stored there can reach a result). Codes become f16 in registers,
 // exactly (int8 and e4m3 both fit), and feed mma.m16n8k16 as the A operand:
@@ -50,6 +53,7 @@ struct MmaP {
     const float* score_in;    // nullable, with score_out: the rows' weights are wanted (one row tile)
     float* score_out;
     float* s_out;             // then: scores (log2 units) [b, hk][key][R]
+    int one;                  // a CTA per item
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -202,6 +206,7 @@ struct MmaCfg {
     static_assert(STAGES >= 2, "a stage in work and one in flight");
     static constexpr int WARP_SMEM = STAGES * STAGE + QBYTES;
     static constexpr int SMEM = WARPS * WARP_SMEM;
+    static_assert(WARP_SMEM >= 8 * NT * (DP * 4 + 8), "a warp's results fit where its ring was");
 };
 
 template <int DP, int FMT, int NT, int NS>
@@ -219,9 +224,23 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
     auto len_of = [&](int64_t b) { return (int)clamp64(c.lens[b], 0, c.Smax); };
     auto units_in = [&](int len) { return max(1, (len + UNIT - 1) / UNIT); };
 
-    // units before each thread's share of the sequences
-    const int64_t share = (c.B + blockDim.x - 1) / blockDim.x;
-    {
+    struct Cursor {
+        int b, len, units, item, unit;
+    };
+    Cursor wk;
+    int64_t U = 0, NW = 0, wid = 0, u0 = 0;
+    int n_units;
+    const int step = p.one ? C::WARPS : 1;
+    if (p.one) {
+        wk.b = (int)blockIdx.x / per_seq;
+        wk.item = (int)blockIdx.x - wk.b * per_seq;
+        wk.len = len_of(wk.b);
+        wk.units = units_in(wk.len);
+        wk.unit = warp;
+        n_units = warp < wk.units ? (wk.units - 1 - warp) / C::WARPS + 1 : 0;
+    } else {
+        // units before each thread's share of the sequences
+        const int64_t share = (c.B + blockDim.x - 1) / blockDim.x;
         int64_t n = 0;
         for (int64_t b = threadIdx.x * share; b < min(c.B, (threadIdx.x + 1) * share); ++b) n += units_in(len_of(b));
         int64_t x = n;
@@ -237,44 +256,38 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
         seg[threadIdx.x + 1] = (before + x) * per_seq;
         if (threadIdx.x == 0) seg[0] = 0;
         __syncthreads();
+        U = seg[blockDim.x];
+        // no more warps than units, so that every warp below NW has some; neighbours in different CTAs
+        NW = min((int64_t)gridDim.x * C::WARPS, U);
+        wid = (int64_t)warp * gridDim.x + blockIdx.x;
+        if (wid >= NW) return;
+        u0 = wid * U / NW;
+        n_units = (int)((wid + 1) * U / NW - u0);
+        // where unit u0 is: its sequence, the item in it, the unit in the item
+        int lo = 0, hi = blockDim.x;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (seg[mid] <= u0) lo = mid;
+            else hi = mid;
+        }
+        wk.b = (int)(lo * share);
+        int64_t base = seg[lo];
+        wk.len = len_of(wk.b);
+        for (;;) {
+            const int64_t all = (int64_t)units_in(wk.len) * per_seq;
+            if (base + all > u0) break;
+            base += all;
+            wk.len = len_of(++wk.b);
+        }
+        wk.units = units_in(wk.len);
+        wk.item = (int)((u0 - base) / wk.units);
+        wk.unit = (int)((u0 - base) - (int64_t)wk.item * wk.units);
     }
-    const int64_t U = seg[blockDim.x];
-    // no more warps than units, so that every warp below NW has some; neighbours in different CTAs
-    const int64_t NW = min((int64_t)gridDim.x * C::WARPS, U);
-    const int64_t wid = (int64_t)warp * gridDim.x + blockIdx.x;
-    if (wid >= NW) return;
-    const int64_t u0 = wid * U / NW;
-    const int n_units = (int)((wid + 1) * U / NW - u0);
-
-    // where unit u0 is: its sequence, the item in it, the unit in the item
-    int lo = 0, hi = blockDim.x;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (seg[mid] <= u0) lo = mid;
-        else hi = mid;
-    }
-    int b = (int)(lo * share);
-    int64_t base = seg[lo];
-    int len = len_of(b);
-    for (;;) {
-        const int64_t n = (int64_t)units_in(len) * per_seq;
-        if (base + n > u0) break;
-        base += n;
-        len = len_of(++b);
-    }
-    struct Cursor {
-        int b, len, units, item, unit;
-    };
-    Cursor wk;
-    wk.b = b;
-    wk.len = len;
-    wk.units = units_in(len);
-    wk.item = (int)((u0 - base) / wk.units);
-    wk.unit = (int)((u0 - base) - (int64_t)wk.item * wk.units);
     Cursor ld = wk;
     // to the next unit; whether that is in another item
     auto advance = [&](Cursor& k) {
-        if (++k.unit < k.units) return false;
+        k.unit += step;
+        if (k.unit < k.units || p.one) return false;
         k.unit = 0;
         if (++k.item == per_seq) {
             k.item = 0;
@@ -344,7 +357,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
     int lim[NT][2];                  // keys each row may attend
     int lim_min = 0;                 // smallest over the tile's rows
     uint32_t qr[C::QREG ? C::KSTEPS : 1][2];
-    bool fresh = true, head_split = wk.unit != 0;
+    bool fresh = true, head_split = !p.one && wk.unit != 0;
 
     int stage = 0;
     for (int it = 0; it < n_units; ++it) {
@@ -588,7 +601,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
         stage = stage + 1 == C::STAGES ? 0 : stage + 1;
 
         const bool item_done = wk.unit + 1 == wk.units;
-        if (item_done || it + 1 == n_units) {
+        if (!p.one && (item_done || it + 1 == n_units)) {
             const int hk = wk.item / p.row_tiles, tile = wk.item - hk * p.row_tiles;
             const bool whole = item_done && !head_split;
             if (!head_split && lane == 0) {
@@ -648,6 +661,82 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
         advance(wk);
     }
     cp_wait<0>();
+    if (!p.one) return;
+
+    // the warps' (out, max, sum) side by side in shared memory, a row a warp at a time from there
+    __syncthreads();
+    float* mine = (float*)ws;
+    float2* ml = (float2*)(mine + ROWS * DP);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float x = n_units ? l[n][e] : 0.0f;
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            const int r = n * 8 + 2 * t + e;
+            if (n_units) {
+#pragma unroll
+                for (int vl = 0; vl < L::VL; ++vl)
+#pragma unroll
+                    for (int k = 0; k < L::V_BYTES; k += 2) {
+                        const int j = (vl * L::V_BYTES + k) / 2;
+                        *(float2*)(mine + r * DP + L::v_byte(g, vl) + k) = make_float2(o[n][j][e], o[n][j][e + 2]);
+                    }
+            }
+            if (g == 0) ml[r] = make_float2(x == 0.0f ? -INFINITY : x == x ? M[n][e] - SHIFT : x, x);
+        }
+    __syncthreads();
+    const int hk = wk.item / p.row_tiles, tile = wk.item - hk * p.row_tiles;
+    __shared__ float lse2[ROWS];
+    for (int r = warp; r < ROWS; r += C::WARPS) {
+        const int gr = tile * ROWS + r;
+        if (gr >= p.R) break;
+        const float2 part = lane < C::WARPS ? ((const float2*)((const float*)(smem + lane * C::WARP_SMEM) + ROWS * DP))[r] : make_float2(-INFINITY, 0.0f);
+        float m = part.x;
+#pragma unroll
+        for (int o2 = 16; o2; o2 >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
+        if (m == -INFINITY) m = 0.0f;
+        const float f = ex2f(part.x - m);
+        float sum = part.y * f;
+#pragma unroll
+        for (int o2 = 16; o2; o2 >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
+        float acc[DP / 32] = {};
+        for (int w = 0; w < C::WARPS; ++w) {
+            const float fw = __shfl_sync(0xffffffffu, f, w);
+            if (w >= wk.units) break;  // warps that had no unit
+            const float* other = (const float*)(smem + w * C::WARP_SMEM) + r * DP;
+#pragma unroll
+            for (int k = 0; k < DP / 32; ++k) acc[k] = fmaf(other[k * 32 + lane], fw, acc[k]);
+        }
+        const float inv = sum > 0.0f || !(sum == sum) ? 1.0f / sum : 0.0f;
+        const int i = gr / p.G, h = hk * p.G + (gr - i * p.G);
+        const int64_t at = wk.b * p.o.sb + h * p.o.sh + (int64_t)i * p.o.ss;
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k) {
+            const int d = k * 32 + lane;
+            if (d >= c.D) continue;
+            const float y = acc[k] * inv;
+            if (p.dtype == F32) ((float*)p.o.p)[at + d] = y;
+            else if (p.dtype == F16) ((__half*)p.o.p)[at + d] = __float2half_rn(y);
+            else ((__nv_bfloat16*)p.o.p)[at + d] = __float2bfloat16_rn(y);
+        }
+        if (lane == 0) {
+            const float z = sum == 0.0f ? -INFINITY : m + log2f(sum);
+            if (p.lse) p.lse[(wk.b * p.H + h) * p.Lq + i] = z * 0.6931471805599453f;
+            lse2[r] = z == -INFINITY ? INFINITY : z;
+        }
+    }
+    if (!p.score_out) return;
+    __syncthreads();  // and every score is written
+    const int64_t head = (int64_t)wk.b * c.Hkv + hk;
+    for (int k = threadIdx.x; k < wk.len; k += blockDim.x) {
+        const float* row = p.s_out + (head * c.Smax + k) * p.R;
+        float w = 0.0f;
+        for (int r = 0; r < p.R; ++r) w += ex2f(row[r] - lse2[r]);
+        p.score_out[head * c.Smax + k] = p.score_in[head * c.Smax + k] + w;
+    }
 }
 
 // What is left once the units are done, in one launch of 128-thread CTAs.
@@ -794,6 +883,10 @@ __global__ void __launch_bounds__(128) kv8_finish_kernel(const __grid_constant__
     }
 }
 
+// A CTA per item: up to 2048 cached rows (a few units a warp; beyond, the other SMs' help outweighs the second launch) and
+// at most two items an SM (more keep every SM busy without it, and waste fewer warps)
+inline bool one_cta(int64_t items, int64_t Smax, int n_sm) { return Smax <= 2048 && items <= 2 * n_sm; }
+
 template <int DP, int FMT, int NT, int NS>
 int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
     using C = MmaCfg<DP, NT, NS>;
@@ -808,11 +901,19 @@ int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
     }
     p.row_tiles = (p.R + 8 * NT - 1) / (8 * NT);
     const int64_t items = p.c.B * p.c.Hkv * p.row_tiles;
+    const size_t s_bytes = p.score_out ? (size_t)p.c.B * p.c.Hkv * p.c.Smax * p.R * sizeof(float) : 0;
+    if (one_cta(items, p.c.Smax, n_sm)) {
+        p.one = 1;
+        if (s_bytes && cuda_failed(cudaMallocAsync((void**)&p.s_out, s_bytes, st), "kv8_attention: scratch allocation")) return -1;
+        kern<<<(unsigned)items, C::WARPS * 32, C::SMEM, st>>>(p);
+        const bool failed = cuda_failed(cudaGetLastError(), "kv8_attention launch");
+        if (s_bytes) cudaFreeAsync(p.s_out, st);
+        return failed ? -1 : 0;
+    }
     const int64_t warps = (int64_t)n_sm * C::WARPS;
     const size_t slots = 2 * (size_t)warps * 8 * NT;
     const size_t meta_bytes = ((size_t)items * sizeof(int2) + 255) & ~(size_t)255;
     const size_t part_bytes = slots * (sizeof(float2) + DP * sizeof(float));
-    const size_t s_bytes = p.score_out ? (size_t)p.c.B * p.c.Hkv * p.c.Smax * p.R * sizeof(float) : 0;
     void* scratch = nullptr;
     if (cuda_failed(cudaMallocAsync(&scratch, meta_bytes + part_bytes + s_bytes, st), "kv8_attention: scratch allocation")) return -1;
     p.meta = (int2*)scratch;

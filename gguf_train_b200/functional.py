@@ -585,7 +585,7 @@ def rope(input: torch.Tensor, positions: torch.Tensor, n_dims: int | None = None
 def _rope_axes_all(pos, sections, mode, flags, freq_base, freq_scale, backward, xs):
     """The rotated xs (one or two), contiguous, in one launch."""
     xs = [x if x.stride(3) == 1 else x.contiguous() for x in xs]
-    outs = tuple(x.new_empty(x.shape) for x in xs)
+    outs = tuple(torch.empty_like(x, memory_format=torch.contiguous_format) for x in xs)
     code = _DTYPE_CODE[xs[0].dtype]
     t = [_C.tensor4(z, code) for pair in zip(xs, outs) for z in pair]
     two = len(xs) == 2
@@ -595,6 +595,9 @@ def _rope_axes_all(pos, sections, mode, flags, freq_base, freq_scale, backward, 
                               torch._C._cuda_getCurrentRawStream(xs[0].device.index))
     _C.check_rc(rc, "rope_axes")
     return outs
+
+
+_ROPE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 class RoPEAxesFn(torch.autograd.Function):
@@ -634,26 +637,30 @@ def rope_axes(input: torch.Tensor, positions: torch.Tensor, sections, k: torch.T
     instead repeats ggml's f32 accumulation of one axis."""
     xs = (input,) if k is None else (input, k)
     _require_cuda("rope_axes", positions, *xs)
-    for x in xs:
-        if x.ndim != 4:
-            raise RuntimeError(f"rope_axes: expected (batch, heads, seq_len, head_dim), got {list(x.shape)}")
-        if x.dtype not in (torch.float32, torch.float16, torch.bfloat16) or x.dtype != input.dtype:
+    if input.ndim != 4 or input.dtype not in _ROPE_DTYPES:
+        raise RuntimeError(f"rope_axes: input must be (batch, heads, seq_len, head_dim) in f32, f16 or bf16, got "
+                           f"{list(input.shape)} in {input.dtype}")
+    B, H, S, D = input.shape
+    if k is not None:
+        if k.dtype != input.dtype:
             raise RuntimeError("rope_axes: input and k must be f32, f16 or bf16, of one type")
-        if x.device != positions.device:
-            raise RuntimeError("rope_axes: input, k and positions must be on one device")
-        if (x.shape[0], x.shape[2], x.shape[3]) != (input.shape[0], input.shape[2], input.shape[3]):
-            raise RuntimeError(f"rope_axes: input {list(input.shape)} and k {list(x.shape)} do not fit together")
-    sections = tuple(int(n) for n in sections)
-    B, S, A = input.shape[0], input.shape[2], len(sections)
-    if positions.shape[-1] != S or tuple(positions.shape[:-1]) not in ((A,), (A, B), (A, 1)):
-        raise RuntimeError(f"rope_axes: positions must be ({A}, {S}) or ({A}, {B}, {S}) for {A} sections, got "
-                           f"{list(positions.shape)}")
+        if k.ndim != 4 or k.shape[0] != B or k.shape[2] != S or k.shape[3] != D:
+            raise RuntimeError(f"rope_axes: input {list(input.shape)} and k {list(k.shape)} do not fit together")
+    dev = positions.device
+    if input.device != dev or (k is not None and k.device != dev):
+        raise RuntimeError("rope_axes: input, k and positions must be on one device")
+    sections = tuple(map(int, sections))
+    A = len(sections)
+    ps = positions.shape
+    if len(ps) not in (2, 3) or ps[0] != A or ps[-1] != S or (len(ps) == 3 and ps[1] not in (1, B)):
+        raise RuntimeError(f"rope_axes: positions must be ({A}, {S}) or ({A}, {B}, {S}) for {A} sections, got {list(ps)}")
     if positions.dtype != torch.int32:
         raise RuntimeError("rope_axes: positions must be int32")
-    positions = positions if S <= 1 or positions.stride(-1) == 1 else positions.contiguous()
+    if S > 1 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
     flags = (_C.GTB_ROPE_INTERLEAVED if interleaved else 0) | (_C.GTB_ROPE_PER_AXIS if per_axis else 0)
     args = (positions, (ctypes.c_int32 * max(A, 1))(*sections), int(mode), flags, float(freq_base), float(freq_scale))
-    if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+    if torch.is_grad_enabled() and (input.requires_grad or (k is not None and k.requires_grad)):
         return RoPEAxesFn.apply(*args, *xs)
     outs = _rope_axes_all(*args, False, xs)
     return outs[0] if k is None else outs

@@ -139,7 +139,7 @@ def kv8_read(cache: KV8Cache, start: torch.Tensor | None, n: int, dtype=torch.fl
     B, Hkv, _, D = cache.k.shape
     if int(n) < 0:
         raise RuntimeError(f"kv8_read: the number of rows must not be negative, got {n}")
-    k = torch.empty((B, Hkv, int(n), D), dtype=dtype, device=cache.k.device)
+    k = cache.k_scale.new_empty((B, Hkv, int(n), D), dtype=dtype)
     v = torch.empty_like(k)
     rc = _C.lib.gtb_kv8_read(ctypes.byref(cache._native), _counts("kv8_read", start, B), _t4(k), _t4(v),
                              _stream(k.device))
@@ -171,7 +171,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, scale: float | None = None, 
         if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (B, Hkv, cap) or not t.is_contiguous()):
             raise RuntimeError(f"kv8_attention: score must be a contiguous float32 tensor ({B}, {Hkv}, {cap})")
     q = _unit_inner(q)
-    out = q.new_empty(q.shape)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty(q.shape[:3], dtype=torch.float32) if need_lse else None
     s_in = None if score is None else score.data_ptr()
     s_out = s_in if score_out is None else score_out.data_ptr()

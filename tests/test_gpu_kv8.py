@@ -275,6 +275,15 @@ SHAPES = [
     (2, 4, 4, 257, 64, 300, 16, [300, 280]),
     (1, 3, 1, 200, 48, 260, 32, [231]),
     (1, 2, 2, 64, 256, 190, 64, [190]),
+    # caches of more than 2048 rows: the keys of a head are split over the SMs and joined
+    (1, 4, 1, 1, 128, 4100, 64, [4099]),
+    (2, 8, 8, 1, 64, 3000, 16, [3000, 5]),
+    (1, 10, 1, 1, 128, 2300, 32, [2222]),
+    (2, 4, 1, 5, 128, 2600, 128, [2600, 2049]),
+    (1, 8, 1, 4, 64, 2100, 32, [2100]),
+    (1, 2, 1, 30, 80, 2200, 16, [2195]),
+    (1, 1, 1, 3, 256, 2500, 64, [2500]),
+    (1, 3, 1, 5, 240, 2100, 32, [2100]),
 ]
 
 
