@@ -189,7 +189,7 @@ struct MmaCfg {
     static constexpr bool QREG = NT * NS == 1 && DP <= 128;
     static constexpr int KSTEPS = DP / 16;
     static constexpr int OREGS = NT * DP / 4;
-    static constexpr int SUB = OREGS > 32 ? 1 : 2;    // 16-key products per unit
+    static constexpr int SUB = OREGS > 16 ? 1 : 2;    // 16-key products per unit
     static constexpr int UNIT = 16 * SUB;
     static constexpr int STAGE = 2 * UNIT * DP + 16;  // K rows, V rows, scales (k, v of each 16 keys)
     static constexpr int QBYTES = QREG ? 0 : KSTEPS * NT * NS * 32 * 8 + NT * 32;
