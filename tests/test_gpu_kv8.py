@@ -275,6 +275,8 @@ SHAPES = [
     (2, 4, 4, 257, 64, 300, 16, [300, 280]),
     (1, 3, 1, 200, 48, 260, 32, [231]),
     (1, 2, 2, 64, 256, 190, 64, [190]),
+    (2, 4, 1, 70, 256, 300, 32, [300, 71]),
+    (1, 8, 1, 90, 64, 700, 128, [700]),
     # caches of more than 2048 rows: the keys of a head are split over the SMs and joined
     (1, 4, 1, 1, 128, 4100, 64, [4099]),
     (2, 8, 8, 1, 64, 3000, 16, [3000, 5]),
