@@ -5,6 +5,7 @@
 
 #include "gtb_common.cuh"
 #include "kv8.h"
+#include "sm100_ptx.cuh"
 
 namespace gtb {
 
@@ -91,11 +92,17 @@ __device__ __forceinline__ uint32_t quantise8x4(const float* x, const Quantiser&
     bool same;
     if constexpr (FMT == GTB_KV8_INT8) {
         constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low byte is the nearest integer's
+        const uint64_t up = sm100::f2_pack(z.up, z.up), down = sm100::f2_pack(z.down, z.down), magic = sm100::f2_pack(MAGIC, MAGIC);
         uint32_t a[4], diff = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a[i] = __float_as_uint(fmaf(x[i], z.up, MAGIC));
-            diff |= a[i] ^ __float_as_uint(fmaf(x[i], z.down, MAGIC));
+        for (int i = 0; i < 4; i += 2) {  // two at a time
+            const uint64_t v = sm100::f2_pack(x[i], x[i + 1]);
+            float a0, a1, b0, b1;
+            sm100::f2_unpack(sm100::f2_fma(v, up, magic), a0, a1);
+            sm100::f2_unpack(sm100::f2_fma(v, down, magic), b0, b1);
+            a[i] = __float_as_uint(a0);
+            a[i + 1] = __float_as_uint(a1);
+            diff |= (a[i] ^ __float_as_uint(b0)) | (a[i + 1] ^ __float_as_uint(b1));
         }
         same = diff == 0;
         r = __byte_perm(__byte_perm(a[0], a[1], 0x0040), __byte_perm(a[2], a[3], 0x0040), 0x5410);
@@ -119,7 +126,11 @@ __device__ __forceinline__ void values8x4(uint32_t w, float* x) {
     if constexpr (FMT == GTB_KV8_INT8) {
         const uint32_t u = w ^ 0x80808080u;  // code + 128 as a byte; 0x4B000000 | byte is 2^23 + byte
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + i)) - 8388736.0f;
+        for (int i = 0; i < 4; i += 2)
+            sm100::f2_unpack(sm100::f2_add(sm100::f2_pack(__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 + i)),
+                                                          __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441 + i))),
+                                           sm100::f2_pack(-8388736.0f, -8388736.0f)),
+                             x[i], x[i + 1]);
     } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {

@@ -499,10 +499,12 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__
     }
 }
 
-// Threads for `chunks` of work in a CTA: a power of two, two chunks a thread where there are enough
-int threads_for(int64_t chunks) {
+constexpr int GATHER_KEEP = 4;
+
+// Threads for `chunks` of work in a CTA: a power of two, `each` chunks a thread where there are enough
+int threads_for(int64_t chunks, int each) {
     int t = 32;
-    while (t < 256 && t * 2 < chunks) t *= 2;
+    while (t < 256 && t * each < chunks) t *= 2;
     return t;
 }
 
@@ -522,7 +524,7 @@ int append_t(const Kv8AppendArgs& a, cudaStream_t st) {
     bool vec = true;
     for (const Rows3* r : {&a.k, &a.v})
         vec = vec && ((uintptr_t)r->p & 15) == 0 && r->sb % N == 0 && r->sh % N == 0 && r->ss % N == 0;
-    const int threads = threads_for(std::min<int64_t>(a.n, a.c.block) * (a.c.D / 16));
+    const int threads = threads_for(std::min<int64_t>(a.n, a.c.block) * (a.c.D / 16), 2);
     const dim3 grid((unsigned)n);
     // chunks a thread keeps: two cover a block of 64 tokens x 128, four one of 128 x 128
     const bool few = std::min<int64_t>(a.n, a.c.block) * (a.c.D / 16) <= 2 * threads;
@@ -561,9 +563,9 @@ bool gather(const Kv8EvictArgs& a, cudaStream_t st) {
     const int64_t rows = a.score_out ? a.dst.Smax : a.budget;
     const int64_t blocks = (rows + a.dst.block - 1) / a.dst.block, n = blocks * a.src.B * a.src.Hkv;
     if (!grid_fits(n, "kv8_evict")) return false;
-    const int threads = threads_for(std::min<int64_t>(a.budget, a.dst.block) * (a.src.D / 16));
-    const bool few = std::min<int64_t>(a.budget, a.dst.block) * (a.src.D / 16) <= 2 * threads;
-    return launch_behind("kv8_evict: gather launch", few ? kv8_gather_kernel<FMT, 2> : kv8_gather_kernel<FMT, 4>, dim3((unsigned)n),
+    const int64_t chunks = std::min<int64_t>(a.budget, a.dst.block) * (a.src.D / 16);
+    const int threads = threads_for(chunks, GATHER_KEEP);
+    return launch_behind("kv8_evict: gather launch", kv8_gather_kernel<FMT, GATHER_KEEP>, dim3((unsigned)n),
                          threads, st, 0, a, (unsigned)blocks, RowOf(a.src.D));
 }
 

@@ -901,6 +901,13 @@ int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
     }
     p.row_tiles = (p.R + 8 * NT - 1) / (8 * NT);
     const int64_t items = p.c.B * p.c.Hkv * p.row_tiles;
+    // rows to join, at most, and CTAs that sum weights
+    const int64_t joins = items * std::min(8 * NT, p.R);
+    const int64_t sums = p.score_out ? p.c.B * p.c.Hkv * ((p.c.Smax + KEYS_PER_CTA - 1) / KEYS_PER_CTA) : 0;
+    if (joins + sums > INT32_MAX) {
+        set_error("kv8_attention: too many query rows");
+        return -1;
+    }
     const size_t s_bytes = p.score_out ? (size_t)p.c.B * p.c.Hkv * p.c.Smax * p.R * sizeof(float) : 0;
     if (one_cta(items, p.c.Smax, n_sm)) {
         p.one = 1;
@@ -923,18 +930,11 @@ int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
     kern<<<n_sm, C::WARPS * 32, C::SMEM, st>>>(p);
     bool bad = cuda_failed(cudaGetLastError(), "kv8_attention launch");
     if (!bad) {
-        // rows to join; with many parts each (few items) four warps share a row
-        const int64_t joins = items * std::min(8 * NT, p.R);
+        // with many parts each (few items) four warps share a row
         const bool shared_rows = warps > 8 * items;
         const int64_t ctas = shared_rows ? joins : (joins + 3) / 4;
-        const int64_t sums = p.score_out ? p.c.B * p.c.Hkv * ((p.c.Smax + KEYS_PER_CTA - 1) / KEYS_PER_CTA) : 0;
-        if (ctas + sums > INT32_MAX || joins > INT32_MAX) {
-            set_error("kv8_attention: too many query rows");
-            bad = true;
-        } else {
-            bad = !launch_behind("kv8_attention: finish launch", shared_rows ? kv8_finish_kernel<DP, 4> : kv8_finish_kernel<DP, 1>,
-                                 dim3((unsigned)(ctas + sums)), 128, st, 0, p, 8 * NT, (unsigned)ctas);
-        }
+        bad = !launch_behind("kv8_attention: finish launch", shared_rows ? kv8_finish_kernel<DP, 4> : kv8_finish_kernel<DP, 1>,
+                             dim3((unsigned)(ctas + sums)), 128, st, 0, p, 8 * NT, (unsigned)ctas);
     }
     cudaFreeAsync(scratch, st);
     return bad ? -1 : 0;

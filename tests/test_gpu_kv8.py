@@ -276,6 +276,10 @@ SHAPES = [
     (1, 3, 1, 200, 48, 260, 32, [231]),
     (1, 2, 2, 64, 256, 190, 64, [190]),
     (2, 4, 1, 70, 256, 300, 32, [300, 71]),
+    (6, 8, 2, 5, 128, 400, 64, [0, 1, 127, 128, 129, 400]),
+    (3, 4, 1, 16, 64, 1000, 16, [1000, 15, 640]),
+    (2, 4, 2, 9, 48, 260, 32, [260, 131]),
+    (2, 20, 1, 3, 112, 5000, 128, [5000, 3]),
     (1, 8, 1, 90, 64, 700, 128, [700]),
     # caches of more than 2048 rows: the keys of a head are split over the SMs and joined
     (1, 4, 1, 1, 128, 4100, 64, [4099]),
