@@ -14,9 +14,13 @@
 //                     Scores become log2 units with their 16 keys' scale, V's scale is folded into the exponent
 //                     (P' = 2^(s + log2 sv - M + 8), M raised when a block exceeds it by 2^7) and the row sum
 //                     takes P' / sv, so scales cost three packed operations per 16 keys and no accuracy.
+//                     P' becomes f16 for the second product: 11 bits, where the 16-bit outputs keep 8 or 11; the row
+//                     sum is of the f32 values.
 //   kv8_chunk_join_kernel  joins those parts.
-// The tile pair reuses each K/V tile for 256 rows; the second kernel is bound by the tensor core and the
-// exponentials. Every wait is bounded: a timeout records a status code, drains the CTA's own copies and MMAs,
+// The tile pair reuses each K/V tile for 256 rows; the second kernel is bound by the softmax warps' chain from scores
+// to weights (tensor pipe 49 % busy). 4 sequences, 1021 tokens x 32 heads of 128 against 4k to 8k cached: 40 us to
+// widen (its bytes at HBM rate), 400 for the products (0.57 of the bf16 GEMM rate), 13 for the join; on kv8_mma.cuh
+// 2.6 ms. Every wait is bounded: a timeout records a status code, drains the CTA's own copies and MMAs,
 // frees TMEM and returns.
 
 #include <algorithm>
@@ -37,6 +41,8 @@ using namespace sm100;
 
 constexpr int BM = 128, BN = 128, NTHREADS = 384, REG_LO = 104, REG_HI = 200;
 constexpr uint32_t TMEM_COLS = 512;
+// Parts of each of the last items: 1021 tokens of 4 sequences with 1 / 2 / 4 / 8 471 / 459 / 451 / 467 us, 333 tokens
+// 263 / 240 / 222 / 238
 constexpr int TAIL_SPLITS = 4;
 
 template <int D>
@@ -685,19 +691,32 @@ int run(const Kv8AttnArgs& a, float* lse, int n_sm, cudaStream_t st) {
         set_error("kv8_attention: too many work items");
         return -1;
     }
-    // the last items, one for two SMs, go in quarters; all of them in more parts where there are fewer items than that.
-    // No part is shorter than 512 keys at full length.
-    const int64_t most = std::max<int64_t>(1, p.Spad / 512);
+    // Parts of the keys, none shorter than 512 at full length. With an item for every SM the last ones, one for two SMs, go
+    // in quarters. With fewer, all go in as many parts as make the shortest schedule: waves of parts of 1 / splits each, and
+    // 0.04 of an item for a part's start and its share of the join (8192 cached tokens, us: 128 items in 1 / 2 / 4 parts
+    // 166 / 180 / 192, 88 in 1 / 3 / 5 163 / 135 / 135, 32 in 1 / 4 / 16 148 / 75 / 90, 8 in 1 / 4 / 16 149 / 64 / 44).
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(p.Spad / 512, n_sm));
     auto plan = [&](int64_t n) {
-        p.splits = (int)std::min<int64_t>(most, n >= n_sm ? TAIL_SPLITS : (TAIL_SPLITS * n_sm + n - 1) / n);
+        p.splits = (int)std::min<int64_t>(most, TAIL_SPLITS);
+        if (n < n_sm) {
+            double best = 1e30;
+            for (int s = 1; s <= most; ++s) {
+                const double cost = (double)((n * s + n_sm - 1) / n_sm) * (1.0 / s + 0.04);
+                if (cost < best) {
+                    best = cost;
+                    p.splits = s;
+                }
+            }
+        }
         p.tail = p.splits <= 1 ? 0 : n >= n_sm ? n_sm / 2 : (int)n;
         p.whole = (int)n - p.tail;
+        return (int64_t)p.tail * p.splits;
     };
-    plan(items);
+    // (the last launch may have fewer sequences)
+    const int64_t parts = std::max(plan(items), a.c.B % nb ? plan(a.c.B % nb * Hkv * p.pairs) : 0);
     const int64_t heads = nb * Hkv;
     const int64_t b_kv = up(heads * p.Spad * D * 2), b_q = up(heads * p.Rpad * D * 2), b_s = up(heads * p.Spad), b_m = up(heads * p.Rpad * 4);
-    // (a last launch with fewer sequences has at most n_sm items, in parts as many)
-    const int64_t prows = std::max<int64_t>((int64_t)p.tail * p.splits, std::min<int64_t>(n_sm * (TAIL_SPLITS + 1), n_sm * most)) * 2 * BM;
+    const int64_t prows = parts * 2 * BM;
     const int64_t b_po = up(prows * D * 4), b_pm = up(prows * 8), b_o = up(nb * 4);
     char* mem = nullptr;
     if (cuda_failed(cudaMallocAsync((void**)&mem, 2 * b_kv + b_q + b_s + b_m + b_po + b_pm + b_o + 1024, st), "kv8_attention: scratch allocation"))

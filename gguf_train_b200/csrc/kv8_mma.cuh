@@ -183,13 +183,21 @@ __device__ __forceinline__ void load_q4(const P& p, int64_t at, bool live, float
 }
 
 // Units, warps and stages. More warps hide the dependent chain of a unit (scores, exponentials, second product); their
-// number is what the registers (O alone takes NT DP / 4) and two stages of each warp's ring allow.
+// number is what the registers (O alone takes NT DP / 4) and two stages of each warp's ring allow: 64 sequences of 1k to 32k
+// tokens, 32 heads of 128 over 8, with 12 warps of 168 registers 0.42 ms, with 8 0.48 ms; 16 of 128 are slower again.
+// A unit of two products halves the waits and joins a key, where its scores fit into the registers left and the ring keeps
+// its warps. One / two products, us, 32 sequences of 100 to 8k tokens (G = 4; e4m3, 64-token blocks):
+//   heads of 64, bf16: 8 rows 44.8 / 41.8, 16 62.5 / 54.6, 24 76.0 / 66.7, 32 94.2 / 111;   f32: 24 83.6 / 80.3, 32 101 / 133
+//   128, bf16: 12 rows 86.3 / 89.1, 20 126 / 119, 32 156 / 150;   f32: 8 rows 73.2 / 67.9, 16 94.0 / 94.4, 20 137 / 145
+//   256, bf16: 8 rows 132 / 137, 16 171 / 218
+// and 8 rows of 128 in bf16, with q in registers, 383 / 402 for the 64 sequences above.
 template <int DP, int NT, int NS>
 struct MmaCfg {
     static constexpr bool QREG = NT * NS == 1 && DP <= 128;
     static constexpr int KSTEPS = DP / 16;
     static constexpr int OREGS = NT * DP / 4;
-    static constexpr int SUB = OREGS > 16 ? 1 : 2;    // 16-key products per unit
+    static constexpr bool PAIR = OREGS <= 64 ? OREGS <= 16 || (OREGS <= 48 && !QREG) : NS == 1 && DP <= 128;
+    static constexpr int SUB = PAIR ? 2 : 1;          // 16-key products per unit
     static constexpr int UNIT = 16 * SUB;
     static constexpr int STAGE = 2 * UNIT * DP + 16;  // K rows, V rows, scales (k, v of each 16 keys)
     static constexpr int QBYTES = QREG ? 0 : KSTEPS * NT * NS * 32 * 8 + NT * 32;
@@ -883,9 +891,14 @@ __global__ void __launch_bounds__(128) kv8_finish_kernel(const __grid_constant__
     }
 }
 
-// A CTA per item: up to 2048 cached rows (a few units a warp; beyond, the other SMs' help outweighs the second launch) and
-// at most two items an SM (more keep every SM busy without it, and waste fewer warps)
-inline bool one_cta(int64_t items, int64_t Smax, int n_sm) { return Smax <= 2048 && items <= 2 * n_sm; }
+// A CTA per item, without scratch and a second launch, where an SM's items come to 2^17 codes of K at most: there its own
+// bandwidth costs less than the join. Measured one CTA an item / split over the SMs, us on the device, heads of 128:
+// 64 items of 1024 keys 14.8 / 20.1, of 2048 21.8 / 22.8; 288 of 512 19.9 / 24.9, of 1024 29.0 / 26.4; 32 with weights of
+// 1024 17.2 / 19.4, of 2048 25.7 / 21.4. Heads of 64: 64 of 2048 13.4 / 18.0, 288 of 2048 27.4 / 25.4. More items than two an
+// SM fill every SM by themselves (512 of 256: 28.3 / 23.5).
+inline bool one_cta(int64_t items, int64_t Smax, int64_t D, int n_sm) {
+    return items <= 2 * n_sm && (items > n_sm ? 2 : 1) * Smax * D <= 1 << 17;
+}
 
 template <int DP, int FMT, int NT, int NS>
 int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
@@ -909,7 +922,7 @@ int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
         return -1;
     }
     const size_t s_bytes = p.score_out ? (size_t)p.c.B * p.c.Hkv * p.c.Smax * p.R * sizeof(float) : 0;
-    if (one_cta(items, p.c.Smax, n_sm)) {
+    if (one_cta(items, p.c.Smax, p.c.D, n_sm)) {
         p.one = 1;
         if (s_bytes && cuda_failed(cudaMallocAsync((void**)&p.s_out, s_bytes, st), "kv8_attention: scratch allocation")) return -1;
         kern<<<(unsigned)items, C::WARPS * 32, C::SMEM, st>>>(p);
@@ -930,7 +943,8 @@ int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
     kern<<<n_sm, C::WARPS * 32, C::SMEM, st>>>(p);
     bool bad = cuda_failed(cudaGetLastError(), "kv8_attention launch");
     if (!bad) {
-        // with many parts each (few items) four warps share a row
+        // with many parts each (few items) four warps share a row; a warp a row / four, us: 2 sequences of 1k to 32k tokens
+        // 77 / 57, 64 382 / 385, 32 drafts of 5 tokens 116 / 122
         const bool shared_rows = warps > 8 * items;
         const int64_t ctas = shared_rows ? joins : (joins + 3) / 4;
         bad = !launch_behind("kv8_attention: finish launch", shared_rows ? kv8_finish_kernel<DP, 4> : kv8_finish_kernel<DP, 1>,
@@ -958,9 +972,11 @@ inline int vector_rows(const Rows3& q, int dtype) {
     return (uintptr_t)q.p % lead == 0 && q.sb * es % lead == 0 && q.sh * es % lead == 0 && q.ss * es % lead == 0;
 }
 
-// Whether the first kernel should keep its scores for the weights: R f32 scores a key written and read against the
-// key's D codes read again.
-inline bool keep_scores(int R, int64_t D) { return 8 * (int64_t)R <= D && R <= (D > 128 ? 16 : 32); }
+// Whether the first kernel should keep its scores (4 R bytes a key of scratch) for the weights, in the second: all rows of
+// a head are then one tile. Otherwise the products are formed again (kv8_weigh_sm100.cu). Kept / formed again, us, 16
+// sequences of 2k to 16k tokens, 8 kv heads: 4 rows of 128 87 / 623, 32 rows 369 / 703, of f32 398 / 746; 32 rows of 64
+// 309 / 543; 16 rows of 256 236 / 925 (the second figures before that kernel took two CTAs an SM).
+inline bool keep_scores(int R, int64_t D) { return R <= (D > 128 ? 16 : 32); }
 
 int launch_mma_64(const MmaP& p, int n_sm, cudaStream_t st);
 int launch_mma_128(const MmaP& p, int n_sm, cudaStream_t st);

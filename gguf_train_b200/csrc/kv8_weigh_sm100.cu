@@ -4,7 +4,10 @@
 //   S^T (128 keys x NQ rows) = K (A, from shared memory) Q^T (B, a tile of rows that TMA brings).
 // The keys are the TMEM lanes, so a thread sums one key's weights over the columns of every tile, in registers and in
 // a fixed order. Two tiles are in flight, each with its own buffer and its own four warps, so the tensor core works on
-// one while the other's exponentials run; those (one per key and row) bound the kernel: 16 a clock and SM.
+// one while the other's exponentials run, and two CTAs share an SM where their tiles fit, so that one's start (codes
+// to f16, first tile) hides behind the other. The exponentials, one per key and row at 16 a clock and SM, and the
+// additions around them bound it where rows are many, a CTA's start where they are few. 1021 tokens x 32 heads of 128
+// against 4 x 4k to 8k cached: 0.44 ms (0.58 with one CTA an SM); 36 rows a head, 16 sequences of 2k to 16k: 0.24 ms (0.52).
 // q is brought to f16 as in kv8_mma.cuh, f32 q as two numbers whose products add up in the accumulator.
 
 #include <algorithm>
@@ -34,6 +37,7 @@ struct WeighCfg {
     static constexpr int OFF_SUM = OFF_ROW + 8 * NQ * 8, OFF_BAR = OFF_SUM + BM * 4;
     static constexpr int SMEM = OFF_BAR + 9 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "shared memory");
+    static constexpr int CTAS = 2 * (SMEM + 1024) <= 228 * 1024 ? 2 : 1;  // an SM (each takes 256 columns of TMEM's 512)
 };
 
 struct WeighP {
@@ -96,7 +100,7 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(const __grid_constant__ W
 }
 
 template <int DP, int FMT, int NS>
-__global__ void __launch_bounds__(NTHREADS, 1) kv8_weigh_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ WeighP p) {
+__global__ void __launch_bounds__(NTHREADS, WeighCfg<DP, NS>::CTAS) kv8_weigh_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ WeighP p) {
     using C = WeighCfg<DP, NS>;
     constexpr int NQ = C::NQ;
     const int per_head = (int)((p.c.Smax + BM - 1) / BM);
@@ -215,12 +219,13 @@ __global__ void __launch_bounds__(NTHREADS, 1) kv8_weigh_kernel(const __grid_con
             if (!ok) break;
             tc_fence_after();
             const bool edge = k0 + BM - 1 > len - cnt + row0 / p.G;  // some key past the first row's last
+            const int chunks = min(NQ / 32, (rows_end - row0 + 31) / 32);  // with a row in them
 #pragma unroll 1
-            for (int c = 0; c < NQ / 32; ++c) {
+            for (int c = 0; c < chunks; ++c) {
                 uint32_t raw[32];
                 tmem_ld32(s_tmem + c * 32, raw);
                 tmem_ld_wait();
-                if (c == NQ / 32 - 1) {
+                if (c == chunks - 1) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&s_free[wg]);
