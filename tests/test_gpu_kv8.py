@@ -310,6 +310,32 @@ def test_attention_with_counts(Lq):
     check_attention(q, cache, counts=[Lq, Lq, Lq, 0, max(1, Lq // 2)])
 
 
+# where the kernels change over, in long caches: full tiles of rows with weights, the first rows past a tile, many
+# rows in so few items that each is cut into parts (some of them past a sequence's end)
+EDGES = [
+    (1, 8, 1, 4, 128, 2600, 64, [2600]),
+    (2, 12, 1, 2, 64, 4200, 16, [4200, 31]),
+    (1, 3, 1, 11, 128, 2100, 32, [2099]),
+    (1, 32, 2, 1, 256, 1500, 128, [1500]),
+    (1, 17, 1, 1, 256, 1200, 16, [1200]),
+    (3, 4, 1, 33, 128, 8192, 64, [8192, 5, 0]),
+    (2, 8, 2, 40, 64, 5000, 128, [3000, 5000]),
+    (1, 1, 1, 300, 96, 9000, 16, [8999]),
+    (5, 4, 2, 129, 64, 1600, 32, [1600, 1100, 129, 70, 513]),
+]
+
+
+@pytest.mark.parametrize("fmt", FMTS, ids=["int8", "e4m3"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("shape", EDGES, ids=lambda s: "x".join(map(str, s[:7])))
+def test_attention_where_kernels_change_over(fmt, dt, shape):
+    B, H, Hkv, Lq, D, cap, block, lens = shape
+    cache = random_cache(B, Hkv, cap, D, block, fmt, lens, 31)
+    q = (torch.randn((B, Lq, H, D), device="cuda", generator=gen(32)) * 1.2).to(dt).transpose(1, 2)
+    check_attention(q, cache)
+    check_attention(q, cache, counts=[max(0, Lq - 3 * b) for b in range(B)])
+
+
 def test_attention_over_many_short_sequences_and_one_long():
     lens = [(37 * i) % 90 for i in range(300)] + [6000]
     cache = random_cache(301, 1, 6000, 64, 32, torch.int8, lens, 8)
