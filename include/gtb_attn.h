@@ -299,7 +299,7 @@ GTB_API int gtb_kv8_read(const gtb_kv8 *cache, const int32_t *start, gtb_tensor4
  * clamped to [0, Lq]; NULL: Lq) of the lens[b] tokens cached, query i < counts[b] attending rows
  * s <= lens[b] - counts[b] + i. A query at or past counts[b], or with no row to attend, gives 0 and lse -inf.
  *   q f32/f16/bf16, any strides with a unit innermost one; out (B,H,Lq,D) in q's dtype, contiguous, 16-byte
- *   aligned; *   lse NULL or (B,H,Lq) f32; scale <= 0 means 1/sqrt(D).
+ *   aligned; lse NULL or (B,H,Lq) f32; scale <= 0 means 1/sqrt(D).
  *   score_out NULL, or (B,Hkv,Smax) f32 that receives score_in (same shape, may be score_out itself) + the
  *   attention weight each row s < lens[b] got, summed over the kv head's query heads and all queries; other
  *   entries are not written. The sums run in a fixed order: the same bits on every run.
