@@ -22,6 +22,10 @@
 // * q becomes f16 after a power of two per row brings its largest value to [1, 2): bf16's 8 bits fit, and what
 //   falls below f16's smallest step is 2^-24 of that value. f32 q is split into two f16 numbers (NS = 2), and
 //   so is P', which is otherwise rounded to f16 once.
+// * One tile of 8 rows of 16-bit q over int8 codes (QINT) takes the codes as they are: that q times 2^21 is an integer of
+//   three digits to base 256 (what falls below its step is 2^-22 of the row's largest value), and
+//   mma.m16n8k32 sums each digit's products exactly. K's codes then need no conversion, 5 instructions in 4 of them:
+//   64 sequences of 1k to 32k tokens in a row 421 -> 380 us, where power, and with it instructions, sets the clock.
 // * M is raised only when a score exceeds it by 2^7 (P' carries a factor 2^8 and f16 ends at 2^16), so most
 //   units need neither shuffles nor a rescaling of O.
 #pragma once
@@ -76,6 +80,12 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16832(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -190,13 +200,16 @@ __device__ __forceinline__ void load_q4(const P& p, int64_t at, bool live, float
 //   heads of 64, bf16: 8 rows 44.8 / 41.8, 16 62.5 / 54.6, 24 76.0 / 66.7, 32 94.2 / 111;   f32: 24 83.6 / 80.3, 32 101 / 133
 //   128, bf16: 12 rows 86.3 / 89.1, 20 126 / 119, 32 156 / 150;   f32: 8 rows 73.2 / 67.9, 16 94.0 / 94.4, 20 137 / 145
 //   256, bf16: 8 rows 132 / 137, 16 171 / 218
-// and 8 rows of 128 in bf16, with q in registers, 383 / 402 for the 64 sequences above.
-template <int DP, int NT, int NS>
+// and 8 rows of 128 in bf16, with q in registers, for the 64 sequences above: int8 372 / 400 at full clock but 419 / 381 called
+// in a row, where the power cap lowers it and fewer instructions count; e4m3 393 / 396 and 406 / 389, but 87 / 91
+// for 16 sequences with weights, so one there.
+template <int DP, int FMT, int NT, int NS>
 struct MmaCfg {
-    static constexpr bool QREG = NT * NS == 1 && DP <= 128;
+    static constexpr bool QREG = NT * NS == 1 && DP <= 128;         // q in registers
+    static constexpr bool QINT = QREG && FMT == GTB_KV8_INT8;       // as integers
     static constexpr int KSTEPS = DP / 16;
     static constexpr int OREGS = NT * DP / 4;
-    static constexpr bool PAIR = OREGS <= 64 ? OREGS <= 16 || (OREGS <= 48 && !QREG) : NS == 1 && DP <= 128;
+    static constexpr bool PAIR = OREGS <= 64 ? OREGS <= 16 || (OREGS <= 48 && (!QREG || QINT)) : NS == 1 && DP <= 128;
     static constexpr int SUB = PAIR ? 2 : 1;          // 16-key products per unit
     static constexpr int UNIT = 16 * SUB;
     static constexpr int STAGE = 2 * UNIT * DP + 16;  // K rows, V rows, scales (k, v of each 16 keys)
@@ -218,8 +231,8 @@ struct MmaCfg {
 };
 
 template <int DP, int FMT, int NT, int NS>
-__global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_kernel(const __grid_constant__ MmaP p) {
-    using C = MmaCfg<DP, NT, NS>;
+__global__ void __launch_bounds__(MmaCfg<DP, FMT, NT, NS>::WARPS * 32, 1) kv8_mma_kernel(const __grid_constant__ MmaP p) {
+    using C = MmaCfg<DP, FMT, NT, NS>;
     using L = Lay<DP>;
     constexpr int ROWS = 8 * NT, OM = DP / 16, SUB = C::SUB, UNIT = C::UNIT;  // OM: products of 16 dims
     extern __shared__ __align__(16) unsigned char smem[];
@@ -364,7 +377,8 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
     float M[NT][2], l[NT][2], qmul[NT][2];
     int lim[NT][2];                  // keys each row may attend
     int lim_min = 0;                 // smallest over the tile's rows
-    uint32_t qr[C::QREG ? C::KSTEPS : 1][2];
+    constexpr int QWORDS = C::QINT ? 3 : 2;
+    uint32_t qr[C::QREG ? C::KSTEPS : 1][QWORDS];
     bool fresh = true, head_split = !p.one && wk.unit != 0;
 
     int stage = 0;
@@ -395,6 +409,27 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
                 e2 = m >= 1.17549435e-38f ? min(max(e2, -126), 126) : 0;
                 const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
                 const float mul = __uint_as_float((uint32_t)(127 + e2) << 23) * p.scale_log2;
+                if constexpr (C::QINT) {
+                    // digits of y 2^21 to base 256, -128 to 127 each, a plane a digit; a row with a value that is not finite
+                    // is NaN throughout
+                    bool odd = false;
+#pragma unroll
+                    for (int k = 0; k < C::KSTEPS; ++k) {
+                        qr[k][0] = qr[k][1] = qr[k][QWORDS - 1] = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            odd |= !(fabsf(x[k][e]) <= 3.402823466e38f);
+                            const int z = __float2int_rn(x[k][e] * down * 0x1p21f);
+                            const int z1 = (z + 128) >> 8, z2 = (z1 + 128) >> 8;  // z = (z2 256 + low(z1)) 256 + low(z)
+                            qr[k][0] |= (uint32_t)(z2 & 255) << (8 * e);
+                            qr[k][1] |= (uint32_t)(z1 & 255) << (8 * e);
+                            qr[k][QWORDS - 1] |= (uint32_t)(z & 255) << (8 * e);
+                        }
+                    }
+                    const unsigned rows_odd = __ballot_sync(0xffffffffu, odd);
+                    row_mul = rows_odd >> (lane & 28) & 15u ? __uint_as_float(0x7fc00000u) : mul * 0x1p-21f;
+                    continue;
+                }
                 if constexpr (C::QREG) row_mul = mul;
                 else if (t == 0) qm[n * 8 + g] = mul;
 #pragma unroll
@@ -455,25 +490,43 @@ __global__ void __launch_bounds__(MmaCfg<DP, NT, NS>::WARPS * 32, 1) kv8_mma_ker
             const int r = L::krow(g);
             const unsigned char* ra = kt + (u * 16 + r) * DP;
             const unsigned char* rb = ra + 8 * DP;
+            if constexpr (C::QINT) {
+                // the codes themselves against q's three digits: exact sums in 32 bits
+                int d[3][4] = {};
+#pragma unroll
+                for (int q = 0; q < L::KL; ++q) {
+                    const int at = (L::k_chunk(t, q) ^ L::swz(r)) << 4;
+                    const uint4 wa = *(const uint4*)(ra + at), wb = *(const uint4*)(rb + at);
+                    const uint32_t a0[4] = {wa.x, wb.x, wa.y, wb.y}, a1[4] = {wa.z, wb.z, wa.w, wb.w};
+#pragma unroll
+                    for (int z = 0; z < 3; ++z) {
+                        mma16832(d[z], a0, qr[q * 4][z % QWORDS], qr[q * 4 + 1][z % QWORDS]);
+                        mma16832(d[z], a1, qr[q * 4 + 2][z % QWORDS], qr[q * 4 + 3][z % QWORDS]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[u][0][e] = fmaf((float)(d[0][e] * 256 + d[1][e]), 256.0f, (float)d[2][e]);
+            } else {
 #pragma unroll (NT >= 3 ? 1 : L::KL)
-            for (int q = 0; q < L::KL; ++q) {
-                const int at = (L::k_chunk(t, q) ^ L::swz(r)) << 4;
-                const uint4 wa = *(const uint4*)(ra + at), wb = *(const uint4*)(rb + at);
-                const uint32_t xa[4] = {wa.x, wa.y, wa.z, wa.w}, xb[4] = {wb.x, wb.y, wb.z, wb.w};
+                for (int q = 0; q < L::KL; ++q) {
+                    const int at = (L::k_chunk(t, q) ^ L::swz(r)) << 4;
+                    const uint4 wa = *(const uint4*)(ra + at), wb = *(const uint4*)(rb + at);
+                    const uint32_t xa[4] = {wa.x, wa.y, wa.z, wa.w}, xb[4] = {wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t ya = prep_word<FMT>(xa[w]), yb = prep_word<FMT>(xb[w]);
-                    const uint32_t a[4] = {expand<FMT, 0>(ya), expand<FMT, 0>(yb), expand<FMT, 1>(ya), expand<FMT, 1>(yb)};
-                    const int k = q * 4 + w;
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t ya = prep_word<FMT>(xa[w]), yb = prep_word<FMT>(xb[w]);
+                        const uint32_t a[4] = {expand<FMT, 0>(ya), expand<FMT, 0>(yb), expand<FMT, 1>(ya), expand<FMT, 1>(yb)};
+                        const int k = q * 4 + w;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        if constexpr (C::QREG) {
-                            mma16816(s[u][n], a, qr[k][0], qr[k][1]);
-                        } else {
+                        for (int n = 0; n < NT; ++n) {
+                            if constexpr (C::QREG) {
+                                mma16816(s[u][n], a, qr[k][0], qr[k][1]);
+                            } else {
 #pragma unroll
-                            for (int z = 0; z < NS; ++z) {
-                                const uint2 bq = qf[((k * NT + n) * NS + z) * 32 + lane];
-                                mma16816(s[u][n], a, bq.x, bq.y);
+                                for (int z = 0; z < NS; ++z) {
+                                    const uint2 bq = qf[((k * NT + n) * NS + z) * 32 + lane];
+                                    mma16816(s[u][n], a, bq.x, bq.y);
+                                }
                             }
                         }
                     }
@@ -902,7 +955,7 @@ inline bool one_cta(int64_t items, int64_t Smax, int64_t D, int n_sm) {
 
 template <int DP, int FMT, int NT, int NS>
 int launch_mma(MmaP p, int n_sm, cudaStream_t st) {
-    using C = MmaCfg<DP, NT, NS>;
+    using C = MmaCfg<DP, FMT, NT, NS>;
     auto kern = kv8_mma_kernel<DP, FMT, NT, NS>;
     static std::atomic<uint64_t> ready{0};  // devices on which the attribute is set
     int dev = 0;
