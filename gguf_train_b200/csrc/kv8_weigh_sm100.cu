@@ -54,7 +54,8 @@ struct WeighP {
     int* status;
 };
 
-// 32 rows of q a CTA; blockIdx.y = (sequence, kv head)
+// 32 rows of q a CTA; blockIdx.y = (sequence, kv head). Rows past the sequence's queries become zeros, whatever they hold:
+// the weights kernel runs over them up to the end of a group of 32, and only a finite score plus -inf is weight 0.
 template <int DP, int NS>
 __global__ void __launch_bounds__(256) kv8_rows_kernel(const __grid_constant__ WeighP p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(const __grid_constant__ W
 #pragma unroll
         for (int w = 0; w < PER; ++w) {
             const int d = lane * 4 + w * 128;
-            load_q4(p, b * p.q.sb + h * p.q.sh + (int64_t)i * p.q.ss + d, r < p.R && d < p.c.D, x[w]);
+            load_q4(p, b * p.q.sb + h * p.q.sh + (int64_t)i * p.q.ss + d, r < p.R && i < cnt && d < p.c.D, x[w]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) m = fmaxf(m, finite_abs(x[w][e]));
         }
