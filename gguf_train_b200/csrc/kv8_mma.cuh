@@ -17,8 +17,8 @@
 // operands agree, so a thread reads 16 consecutive bytes of a row and calls them the elements its lane owns;
 // only P^T has to change layout (movmatrix, two per 16 keys and 8 rows).
 // * Scales: K's block scale multiplies the scores. V's is folded into the exponent, P' = 2^(s + log2 sv - M), so
-//   the second product accumulates across blocks without rescaling; the row sum takes P' / sv. sv below
-//   2^-100 counts as 2^-100.
+//   the second product accumulates across blocks without rescaling; the row sum takes P' / sv. sv below 2^-80 (zero
+//   above all: a block of zeros) counts as 2^-80: P' stays below 2^15, so no sum over 2^30 rows passes 2^125.
 // * q becomes f16 after a power of two per row brings its largest value to [1, 2): bf16's 8 bits fit, and what
 //   falls below f16's smallest step is 2^-24 of that value. f32 q is split into two f16 numbers (NS = 2), and
 //   so is P', which is otherwise rounded to f16 once.
@@ -39,7 +39,7 @@
 namespace gtb {
 namespace kv8 {
 
-constexpr float SV_MIN = 7.888609052210118e-31f;  // 2^-100
+constexpr float SV_MIN = 0x1p-80f;
 constexpr float RAISE = 7.0f, SHIFT = 8.0f, NONE = -1e30f;  // NONE: no key seen yet
 
 struct MmaP {
