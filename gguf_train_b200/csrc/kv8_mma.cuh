@@ -413,13 +413,14 @@ __global__ void __launch_bounds__(MmaCfg<DP, FMT, NT, NS>::WARPS * 32, 1) kv8_mm
                     // digits of y 2^21 to base 256, -128 to 127 each, a plane a digit; a row with a value that is not finite
                     // is NaN throughout
                     bool odd = false;
+                    const float lift = m < 0x1p127f ? 0x1p21f : 0x1p20f;  // `down` ends at 2^-126: y may reach 4 there
 #pragma unroll
                     for (int k = 0; k < C::KSTEPS; ++k) {
                         qr[k][0] = qr[k][1] = qr[k][QWORDS - 1] = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             odd |= !(fabsf(x[k][e]) <= 3.402823466e38f);
-                            const int z = __float2int_rn(x[k][e] * down * 0x1p21f);
+                            const int z = __float2int_rn(x[k][e] * down * lift);
                             const int z1 = (z + 128) >> 8, z2 = (z1 + 128) >> 8;  // z = (z2 256 + low(z1)) 256 + low(z)
                             qr[k][0] |= (uint32_t)(z2 & 255) << (8 * e);
                             qr[k][1] |= (uint32_t)(z1 & 255) << (8 * e);
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, FMT, NT, NS>::WARPS * 32, 1) kv8_mm
                         }
                     }
                     const unsigned rows_odd = __ballot_sync(0xffffffffu, odd);
-                    row_mul = rows_odd >> (lane & 28) & 15u ? __uint_as_float(0x7fc00000u) : mul * 0x1p-21f;
+                    row_mul = rows_odd >> (lane & 28) & 15u ? __uint_as_float(0x7fc00000u) : mul / lift;
                     continue;
                 }
                 if constexpr (C::QREG) row_mul = mul;
