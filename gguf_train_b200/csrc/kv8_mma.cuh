@@ -22,10 +22,13 @@
 // * q becomes f16 after a power of two per row brings its largest value to [1, 2): bf16's 8 bits fit, and what
 //   falls below f16's smallest step is 2^-24 of that value. f32 q is split into two f16 numbers (NS = 2), and
 //   so is P', which is otherwise rounded to f16 once.
-// * One tile of 8 rows of 16-bit q over int8 codes (QINT) takes the codes as they are: that q times 2^21 is an integer of
-//   three digits to base 256 (what falls below its step is 2^-22 of the row's largest value), and
-//   mma.m16n8k32 sums each digit's products exactly. K's codes then need no conversion, 5 instructions in 4 of them:
-//   64 sequences of 1k to 32k tokens in a row 421 -> 380 us, where power, and with it instructions, sets the clock.
+// * One tile of 8 rows of 16-bit q over int8 codes (QINT) takes the codes as they are: that q times 2^29 is an integer of
+//   four digits to base 256 (what falls below its step is 2^-30 of the row's largest value), and
+//   mma.m16n8k32 sums each digit's products exactly. The last digit is 0 in rows whose values all end at 2^-21 of the
+//   largest, most of them, and is multiplied only where it is not. K's codes then need no conversion, 5 instructions in 4 of
+//   them. Against f16 products, us: 64 sequences of 1k to 32k tokens called in a row 455 / 419 (f16 q, whose rows have a
+//   last digit more often, 455 / 433), where power, and with it instructions, sets the clock, but 393 / 412 at full
+//   clock; 16 of them 123 / 128, 16 with weights 94 / 90.
 // * M is raised only when a score exceeds it by 2^7 (P' carries a factor 2^8 and f16 ends at 2^16), so most
 //   units need neither shuffles nor a rescaling of O.
 #pragma once
@@ -213,7 +216,7 @@ struct MmaCfg {
     static constexpr int SUB = PAIR ? 2 : 1;          // 16-key products per unit
     static constexpr int UNIT = 16 * SUB;
     static constexpr int STAGE = 2 * UNIT * DP + 16;  // K rows, V rows, scales (k, v of each 16 keys)
-    static constexpr int QBYTES = QREG ? 0 : KSTEPS * NT * NS * 32 * 8 + NT * 32;
+    static constexpr int QBYTES = QINT ? KSTEPS * 128 : QREG ? 0 : KSTEPS * NT * NS * 32 * 8 + NT * 32;
     static constexpr int SPACE = 224 * 1024, MOST12 = 64;
     static constexpr int fit(int warps) { return (SPACE / warps - QBYTES) / STAGE; }
     static constexpr int pick() {
@@ -323,6 +326,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, FMT, NT, NS>::WARPS * 32, 1) kv8_mm
     unsigned char* ws = smem + warp * C::WARP_SMEM;
     const uint32_t ring = smem_addr(ws);
     uint2* qf = (uint2*)(ws + C::STAGES * C::STAGE);  // B operands of the rows, then their multipliers
+    uint32_t* q_last = (uint32_t*)qf;                  // (QINT) or the last digits
     float* qm = (float*)(qf + C::KSTEPS * NT * NS * 32);
     const int64_t nblk = (c.Smax + c.block - 1) / c.block;
     const int block_shift = 31 - __clz(c.block);
@@ -379,6 +383,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, FMT, NT, NS>::WARPS * 32, 1) kv8_mm
     int lim_min = 0;                 // smallest over the tile's rows
     constexpr int QWORDS = C::QINT ? 3 : 2;
     uint32_t qr[C::QREG ? C::KSTEPS : 1][QWORDS];
+    bool last_digit = false;         // (QINT) whether some row's is not 0
     bool fresh = true, head_split = !p.one && wk.unit != 0;
 
     int stage = 0;
@@ -410,25 +415,33 @@ __global__ void __launch_bounds__(MmaCfg<DP, FMT, NT, NS>::WARPS * 32, 1) kv8_mm
                 const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
                 const float mul = __uint_as_float((uint32_t)(127 + e2) << 23) * p.scale_log2;
                 if constexpr (C::QINT) {
-                    // digits of y 2^21 to base 256, -128 to 127 each, a plane a digit; a row with a value that is not finite
+                    // digits of y 2^29 to base 256, -128 to 127 each, a plane a digit; a row with a value that is not finite
                     // is NaN throughout
                     bool odd = false;
-                    const float lift = m < 0x1p127f ? 0x1p21f : 0x1p20f;  // `down` ends at 2^-126: y may reach 4 there
+                    uint32_t any = 0;
+                    const float lift = m < 0x1p127f ? 0x1p29f : 0x1p28f;  // `down` ends at 2^-126: y may reach 4 there
 #pragma unroll
                     for (int k = 0; k < C::KSTEPS; ++k) {
+                        uint32_t low = 0;
                         qr[k][0] = qr[k][1] = qr[k][QWORDS - 1] = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            odd |= !(fabsf(x[k][e]) <= 3.402823466e38f);
-                            const int z = __float2int_rn(x[k][e] * down * lift);
-                            const int z1 = (z + 128) >> 8, z2 = (z1 + 128) >> 8;  // z = (z2 256 + low(z1)) 256 + low(z)
-                            qr[k][0] |= (uint32_t)(z2 & 255) << (8 * e);
-                            qr[k][1] |= (uint32_t)(z1 & 255) << (8 * e);
-                            qr[k][QWORDS - 1] |= (uint32_t)(z & 255) << (8 * e);
+                            const bool finite = fabsf(x[k][e]) <= 3.402823466e38f;
+                            odd |= !finite;
+                            const int z = finite ? __float2int_rn(x[k][e] * down * lift) : 0;
+                            // z = ((z3 256 + low(z2)) 256 + low(z1)) 256 + low(z)
+                            const int z1 = (z + 128) >> 8, z2 = (z1 + 128) >> 8, z3 = (z2 + 128) >> 8;
+                            qr[k][0] |= (uint32_t)(z3 & 255) << (8 * e);
+                            qr[k][1] |= (uint32_t)(z2 & 255) << (8 * e);
+                            qr[k][QWORDS - 1] |= (uint32_t)(z1 & 255) << (8 * e);
+                            low |= (uint32_t)(z & 255) << (8 * e);
                         }
+                        q_last[k * 32 + lane] = low;  // (a lane reads its own)
+                        any |= low;
                     }
+                    last_digit = __any_sync(0xffffffffu, any != 0);
                     const unsigned rows_odd = __ballot_sync(0xffffffffu, odd);
-                    row_mul = rows_odd >> (lane & 28) & 15u ? __uint_as_float(0x7fc00000u) : mul / lift;
+                    row_mul = rows_odd >> (lane & 28) & 15u ? __uint_as_float(0x7fc00000u) : mul * 256.0f / lift;
                     continue;
                 }
                 if constexpr (C::QREG) row_mul = mul;
@@ -492,7 +505,7 @@ __global__ void __launch_bounds__(MmaCfg<DP, FMT, NT, NS>::WARPS * 32, 1) kv8_mm
             const unsigned char* ra = kt + (u * 16 + r) * DP;
             const unsigned char* rb = ra + 8 * DP;
             if constexpr (C::QINT) {
-                // the codes themselves against q's three digits: exact sums in 32 bits
+                // the codes themselves against q's digits: exact sums in 32 bits
                 int d[3][4] = {};
 #pragma unroll
                 for (int q = 0; q < L::KL; ++q) {
@@ -507,6 +520,20 @@ __global__ void __launch_bounds__(MmaCfg<DP, FMT, NT, NS>::WARPS * 32, 1) kv8_mm
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[u][0][e] = fmaf((float)(d[0][e] * 256 + d[1][e]), 256.0f, (float)d[2][e]);
+                if (last_digit) {
+                    int z[4] = {};
+#pragma unroll
+                    for (int q = 0; q < L::KL; ++q) {
+                        const int at = (L::k_chunk(t, q) ^ L::swz(r)) << 4;
+                        const uint4 wa = *(const uint4*)(ra + at), wb = *(const uint4*)(rb + at);
+                        const uint32_t a0[4] = {wa.x, wb.x, wa.y, wb.y}, a1[4] = {wa.z, wb.z, wa.w, wb.w};
+                        const uint32_t* low = q_last + q * 128 + lane;
+                        mma16832(z, a0, low[0], low[32]);
+                        mma16832(z, a1, low[64], low[96]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[u][0][e] = fmaf((float)z[e], 0x1p-8f, s[u][0][e]);
+                }
             } else {
 #pragma unroll (NT >= 3 ? 1 : L::KL)
                 for (int q = 0; q < L::KL; ++q) {
