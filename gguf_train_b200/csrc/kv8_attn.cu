@@ -12,6 +12,10 @@ namespace gtb {
 
 namespace {
 
+// Kept scores take 4 R bytes for every row of capacity: at most this much at a time. A call that needs more runs in groups
+// of sequences; where one sequence alone needs more, the weights kernel forms the products again.
+constexpr int64_t SCORES_MAX = 1ll << 30;
+
 // score_out = score_in below the lengths: what the weights come to where there is no query
 __global__ void kv8_copy_scores_kernel(const gtb_kv8 c, const float* __restrict__ in, float* __restrict__ out) {
     for (int64_t bh = blockIdx.y; bh < c.B * c.Hkv; bh += gridDim.y) {
@@ -53,12 +57,40 @@ int launch_kv8_attention(const Kv8AttnArgs& a, cudaStream_t st) {
         p.scale_log2 = a.scale * 1.4426950408889634f;
         p.counts = a.counts;
         p.lse = lse;
+        // sequences a launch: all of them, or as many as the kept scores of fit into SCORES_MAX
+        int64_t group = a.c.B;
         kept = a.score_out && a.c.Smax > 0 && kv8::keep_scores(p.R, a.c.D);
         if (kept) {
             p.score_in = a.score_in;
             p.score_out = a.score_out;
+            const int64_t fit = SCORES_MAX / (a.c.Hkv * a.c.Smax * p.R * (int64_t)sizeof(float));
+            kept = fit > 0;
+            if (kept && fit < group) {
+                const int64_t launches = (group + fit - 1) / fit;
+                group = (group + launches - 1) / launches;
+            }
         }
-        rc = a.c.D <= 64 ? kv8::launch_mma_64(p, n_sm, st) : a.c.D <= 128 ? kv8::launch_mma_128(p, n_sm, st) : kv8::launch_mma_256(p, n_sm, st);
+        if (!kept) p.score_in = p.score_out = nullptr;
+        for (int64_t b0 = 0; b0 < a.c.B && !rc; b0 += group) {
+            kv8::MmaP g = p;
+            g.c.B = std::min(group, a.c.B - b0);
+            const int64_t rows0 = b0 * a.c.Hkv * a.c.Smax, blocks0 = b0 * a.c.Hkv * ((a.c.Smax + a.c.block - 1) / a.c.block);
+            const int64_t es = a.dtype == F32 ? 4 : 2;
+            g.c.k = (char*)a.c.k + rows0 * a.c.D;
+            g.c.v = (char*)a.c.v + rows0 * a.c.D;
+            g.c.k_scale = a.c.k_scale + blocks0;
+            g.c.v_scale = a.c.v_scale + blocks0;
+            g.c.lens = a.c.lens + b0;
+            g.q.p = (char*)a.q.p + b0 * a.q.sb * es;
+            g.o.p = (char*)a.o.p + b0 * a.o.sb * es;
+            if (g.counts) g.counts += b0;
+            if (g.lse) g.lse += b0 * a.H * a.Lq;
+            if (kept) {
+                g.score_in += rows0;
+                g.score_out += rows0;
+            }
+            rc = a.c.D <= 64 ? kv8::launch_mma_64(g, n_sm, st) : a.c.D <= 128 ? kv8::launch_mma_128(g, n_sm, st) : kv8::launch_mma_256(g, n_sm, st);
+        }
     }
     if (!rc && a.score_out && !kept && a.c.Smax > 0) {
         if (rows > 0) {

@@ -305,7 +305,9 @@ GTB_API int gtb_kv8_read(const gtb_kv8 *cache, const int32_t *start, gtb_tensor4
  *   entries are not written. The sums run in a fixed order: the same bits on every run.
  * A v_scale below 2^-80 (a largest value below 1.1e-22) counts as 2^-80, and the v_scales of a head's blocks that hold
  * other values than zeros may lie up to 2^120 apart.
- * Scratch comes from the stream-ordered allocator. */
+ * Scratch comes from the stream-ordered allocator: up to 1 GB for the scores (or, where query rows
+ * are many, the f16 queries) that score_out is made from, up to 2 GB (or what one sequence takes: 2 bytes a code of its
+ * capacity) for f16 copies of K and V where query rows are many, and some MB. */
 GTB_API int gtb_kv8_attention(const gtb_tensor4 *q, const gtb_kv8 *cache, float scale, const int32_t *counts,
                               const float *score_in, float *score_out, gtb_tensor4 *out, float *lse, void *stream);
 
