@@ -116,7 +116,7 @@ def _configure(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.gtb_attn_merge.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64,
                                    c_int64, c_void_p]
     lib.gtb_attn_merge.restype = c_int
-    lib.gtb_rope_axes.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, ctypes.POINTER(c_int32), c_int, c_int, c_int,
+    lib.gtb_rope_axes.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_int, c_int,
                                   c_float, c_float, c_int, c_void_p]
     lib.gtb_rope_axes.restype = c_int
     lib.gtb_kv8_append.argtypes = [PKV8, c_void_p, c_void_p, c_void_p, c_int, c_void_p]
