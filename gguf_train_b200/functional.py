@@ -605,24 +605,45 @@ _ROPE_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 class RoPEAxesFn(torch.autograd.Function):
     """rope_axes as an autograd Function: apply(pos, sections, mode, flags, freq_base, freq_scale, *xs) (sections int32
     numbers, or their bytes) -> the rotated xs (one, or q and k, in one launch). The backward rotates the gradients by
-    -angle, again in one launch; nothing but the positions is saved."""
+    -angle, again in one launch; nothing but the positions is saved. Where it is to be differentiated in turn
+    (create_graph) it is this Function again, of the other sign: the map is linear."""
 
     @staticmethod
     def forward(ctx, pos, sections, mode, flags, freq_base, freq_scale, *xs):
         if not isinstance(sections, bytes):
             sections = struct.pack(f"{len(sections)}i", *sections)
-        ctx.args = (sections, mode, flags, freq_base, freq_scale)
+        return RoPEAxesFn._rotate(ctx, pos, (sections, mode, flags, freq_base, freq_scale), False, xs)
+
+    @staticmethod
+    def _rotate(ctx, pos, args, back, xs):
+        ctx.args, ctx.back = args, back
         ctx.save_for_backward(pos)
-        outs = _rope_axes_all(pos, *ctx.args, False, xs)
+        outs = _rope_axes_all(pos, *args, back, xs)
         return outs if len(outs) > 1 else outs[0]
 
     @staticmethod
     def backward(ctx, *grads):
         (pos,) = ctx.saved_tensors
-        need = ctx.needs_input_grad[6:]
+        first = len(ctx.needs_input_grad) - len(grads)
+        need = ctx.needs_input_grad[first:]
         live = [g for g, n in zip(grads, need) if g is not None and n]
-        outs = iter(_rope_axes_all(pos, *ctx.args, True, live) if live else ())
-        return (None,) * 6 + tuple(next(outs) if g is not None and n else None for g, n in zip(grads, need))
+        if not live:
+            outs = ()
+        elif torch.is_grad_enabled():
+            outs = (RoPEAxesFn if ctx.back else _RoPEAxesBackFn).apply(pos, *ctx.args, *live)
+            outs = outs if len(live) > 1 else (outs,)
+        else:
+            outs = _rope_axes_all(pos, *ctx.args, not ctx.back, live)
+        outs = iter(outs)
+        return (None,) * first + tuple(next(outs) if g is not None and n else None for g, n in zip(grads, need))
+
+
+class _RoPEAxesBackFn(RoPEAxesFn):
+    """The rotation by -angle."""
+
+    @staticmethod
+    def forward(ctx, pos, sections, mode, flags, freq_base, freq_scale, *xs):
+        return RoPEAxesFn._rotate(ctx, pos, (sections, mode, flags, freq_base, freq_scale), True, xs)
 
 
 def rope_axes(input: torch.Tensor, positions: torch.Tensor, sections, k: torch.Tensor | None = None, mode: int = 2,
