@@ -560,19 +560,36 @@ def _rope_run(x, positions, n_dims, mode, freq_base, freq_scale, backward):
 
 class RoPEFn(torch.autograd.Function):
     """gguf_train's RoPEFn (_functions.py:1906-1919): forward gt_rope, backward gt_rope_backward (the
-    rotation by -angle), both on the device."""
+    rotation by -angle), both on the device. Where the backward is to be differentiated in turn (create_graph) it is
+    this Function again, of the other sign: the map is linear."""
 
     @staticmethod
     def forward(ctx, x, pos, n_dims: int, mode: int, n_ctx_orig: int, freq_base: float, freq_scale: float):
-        ctx.args = (n_dims, mode, float(freq_base), float(freq_scale))
+        return RoPEFn._rotate(ctx, x, pos, (n_dims, mode, float(freq_base), float(freq_scale)), False)
+
+    @staticmethod
+    def _rotate(ctx, x, pos, args, back):
+        ctx.args, ctx.back = args, back
         ctx.save_for_backward(pos)
-        return _rope_run(x, pos, n_dims, mode, freq_base, freq_scale, False)
+        return _rope_run(x, pos, *args, back)
 
     @staticmethod
     def backward(ctx, grad_out):
         (pos,) = ctx.saved_tensors
         n_dims, mode, fb, fs = ctx.args
-        return _rope_run(grad_out, pos, n_dims, mode, fb, fs, True), None, None, None, None, None, None
+        if torch.is_grad_enabled():
+            dx = (RoPEFn if ctx.back else _RoPEBackFn).apply(grad_out, pos, n_dims, mode, 0, fb, fs)
+        else:
+            dx = _rope_run(grad_out, pos, n_dims, mode, fb, fs, not ctx.back)
+        return dx, None, None, None, None, None, None
+
+
+class _RoPEBackFn(RoPEFn):
+    """The rotation by -angle."""
+
+    @staticmethod
+    def forward(ctx, x, pos, n_dims: int, mode: int, n_ctx_orig: int, freq_base: float, freq_scale: float):
+        return RoPEFn._rotate(ctx, x, pos, (n_dims, mode, float(freq_base), float(freq_scale)), True)
 
 
 def rope(input: torch.Tensor, positions: torch.Tensor, n_dims: int | None = None, mode: int = 0, n_ctx_orig: int = 0,

@@ -25,16 +25,18 @@ def dense(f, shape):
 
 
 def maps():
-    from gguf_train_b200 import rope_axes
+    from gguf_train_b200 import rope, rope_axes
 
     pos = torch.tensor([[0, 3, 7], [5, 1, 90]], dtype=torch.int32, device="cuda")
+    one = torch.tensor([0, 4, 33], dtype=torch.int32, device="cuda")
     return {
         "rope_axes": lambda x: rope_axes(x, pos, (2, 4)),
         "rope_axes interleaved": lambda x: rope_axes(x, pos, (4, 4), mode=0, interleaved=True),
+        "rope": lambda x: rope(x, one, mode=2),
     }
 
 
-@pytest.mark.parametrize("which", ["rope_axes", "rope_axes interleaved"])
+@pytest.mark.parametrize("which", ["rope_axes", "rope_axes interleaved", "rope"])
 def test_second_derivative(which):
     """f = sum(y^3) + sum(x^2), y = L x: the gradient is L^T 3 y^2 + 2 x, its derivative along w L^T (6 y (L w)) + 2 w."""
     f = maps()[which]
