@@ -41,8 +41,8 @@ def _unit_inner(t: torch.Tensor) -> torch.Tensor:
 
 def _same_device(name: str, cache: "KV8Cache", *ts) -> None:
     for t in ts:
-        if t is not None and t.device != cache.k.device:
-            raise RuntimeError(f"{name}: a tensor is on {t.device}, the cache on {cache.k.device}")
+        if t is not None and t.device != cache._k.device:
+            raise RuntimeError(f"{name}: a tensor is on {t.device}, the cache on {cache._k.device}")
 
 
 def _counts(name: str, counts, batch: int):
@@ -53,13 +53,34 @@ def _counts(name: str, counts, batch: int):
     return counts.data_ptr()
 
 
+def _tensor(name: str):
+    """A tensor of a cache. One put in its place has to be like it; the native handle follows."""
+    slot = "_" + name
+
+    def get(self) -> torch.Tensor:
+        return getattr(self, slot)
+
+    def put(self, t: torch.Tensor) -> None:
+        old = getattr(self, slot)
+        if not isinstance(t, torch.Tensor) or t.shape != old.shape or t.dtype != old.dtype or t.device != old.device or \
+                not t.is_contiguous():
+            raise RuntimeError(f"KV8Cache: {name} can only be replaced by a contiguous {old.dtype} tensor of shape "
+                               f"{list(old.shape)} on {old.device}; make a new KV8Cache for others")
+        setattr(self._native, name, t.data_ptr())
+        setattr(self, slot, t)
+
+    return property(get, put)
+
+
 class KV8Cache:
     """The tensors of an 8-bit cache: k, v (B, Hkv, capacity, D) int8 or float8_e4m3fn codes; k_scale, v_scale
     (B, Hkv, ceil(capacity / block)) float32; lens (B) int32, the rows each sequence holds. All contiguous, on
-    one CUDA device; D a multiple of 16 up to 256, block 16, 32, 64 or 128. The handle keeps the tensors'
-    addresses: change their contents freely, but make a new handle for other tensors."""
+    one CUDA device; D a multiple of 16 up to 256, block 16, 32, 64 or 128. Their contents may be changed freely, and
+    a tensor may be replaced by one of the same shape and type (cache.lens = cache.lens - rejected)."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "lens", "block", "_native")
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_lens", "_block", "_native")
+    k, v, k_scale, v_scale, lens = map(_tensor, ("k", "v", "k_scale", "v_scale", "lens"))
+    block = property(lambda self: self._block, doc="tokens that share a scale")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                  lens: torch.Tensor, block: int) -> None:
@@ -83,7 +104,7 @@ class KV8Cache:
                 raise RuntimeError("KV8Cache: all tensors must be contiguous")
             if t.device != k.device:
                 raise RuntimeError("KV8Cache: all tensors must be on one device")
-        self.k, self.v, self.k_scale, self.v_scale, self.lens, self.block = k, v, k_scale, v_scale, lens, block
+        self._k, self._v, self._k_scale, self._v_scale, self._lens, self._block = k, v, k_scale, v_scale, lens, block
         self._native = _C.KV8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), lens.data_ptr(), B,
                               Hkv, cap, D, block, _FORMAT[k.dtype])
 
@@ -117,7 +138,7 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, counts: torch.
     cache."""
     _require_cuda("kv8_append", k, v, counts)
     _same_device("kv8_append", cache, k, v, counts)
-    B, Hkv, _, D = cache.k.shape
+    B, Hkv, _, D = cache._k.shape
     if k.ndim != 4 or k.shape != v.shape or (k.shape[0], k.shape[1], k.shape[3]) != (B, Hkv, D):
         raise RuntimeError(f"kv8_append: k and v must be ({B}, {Hkv}, n, {D}), got {list(k.shape)} and {list(v.shape)}")
     if k.dtype not in _CODE or v.dtype != k.dtype:
@@ -136,10 +157,10 @@ def kv8_read(cache: KV8Cache, start: torch.Tensor | None, n: int, dtype=torch.fl
     _same_device("kv8_read", cache, start)
     if dtype not in _CODE:
         raise RuntimeError("kv8_read: dtype must be f32, f16 or bf16")
-    B, Hkv, _, D = cache.k.shape
+    B, Hkv, _, D = cache._k.shape
     if int(n) < 0:
         raise RuntimeError(f"kv8_read: the number of rows must not be negative, got {n}")
-    k = cache.k_scale.new_empty((B, Hkv, int(n), D), dtype=dtype)
+    k = cache._k_scale.new_empty((B, Hkv, int(n), D), dtype=dtype)
     v = torch.empty_like(k)
     rc = _C.lib.gtb_kv8_read(ctypes.byref(cache._native), _counts("kv8_read", start, B), _t4(k), _t4(v),
                              _stream(k.device))
@@ -160,7 +181,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, scale: float | None = None, 
     cache.lens[b]. It is what kv8_evict goes by."""
     _require_cuda("kv8_attention", q, counts, score, score_out)
     _same_device("kv8_attention", cache, q, counts, score, score_out)
-    B, Hkv, cap, D = cache.k.shape
+    B, Hkv, cap, D = cache._k.shape
     if q.ndim != 4 or q.shape[0] != B or q.shape[3] != D:
         raise RuntimeError(f"kv8_attention: q must be ({B}, H, Lq, {D}), got {list(q.shape)}")
     if q.dtype not in _CODE:
@@ -193,14 +214,14 @@ def kv8_evict(cache: KV8Cache, score: torch.Tensor, budget: int, recent: int = 0
     source rows (B, Hkv, budget) int32, -1 past the length. Keys keep the rotation they were stored with."""
     _require_cuda("kv8_evict", score, score_out)
     _same_device("kv8_evict", cache, score, score_out)
-    B, Hkv, cap, D = cache.k.shape
+    B, Hkv, cap, D = cache._k.shape
     budget, recent = int(budget), int(recent)
     if budget < 1 or not 0 <= recent <= budget:
         raise RuntimeError(f"kv8_evict: budget must be at least 1 and recent between 0 and budget, got {budget} and {recent}")
     if score.dtype != torch.float32 or tuple(score.shape) != (B, Hkv, cap) or not score.is_contiguous():
         raise RuntimeError(f"kv8_evict: score must be a contiguous float32 tensor ({B}, {Hkv}, {cap})")
     if out is None:
-        out = KV8Cache.empty(B, Hkv, budget, D, cache.block, cache.k.dtype, cache.k.device)
+        out = KV8Cache.empty(B, Hkv, budget, D, cache._block, cache._k.dtype, cache._k.device)
     if score_out is None:
         score_out = torch.empty((B, Hkv, out.capacity), dtype=torch.float32, device=score.device)
     elif score_out.dtype != torch.float32 or tuple(score_out.shape) != (B, Hkv, out.capacity) or not score_out.is_contiguous():
