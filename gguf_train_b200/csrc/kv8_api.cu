@@ -140,6 +140,7 @@ bool rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags,
     thread_local RopeKey last;
     thread_local RopeAxesTable table;
     thread_local int last_pairs;
+    thread_local bool made = false;  // `table` is that of `last` (an empty key is a caller's too)
     RopeKey key;
     if (sections && n_axes >= 1 && n_axes <= 4) std::copy(sections, sections + n_axes, key.sections);
     key.n_axes = n_axes;
@@ -147,10 +148,11 @@ bool rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags,
     key.base = freq_base;
     key.scale = freq_scale;
     key.D = D;
-    if (!(key == last)) {
-        last = RopeKey{};
+    if (!made || !(key == last)) {
+        made = false;
         if (!make_rope_table(ctx, sections, n_axes, flags, freq_base, freq_scale, D, table, last_pairs)) return false;
         last = key;
+        made = true;
     }
     t = table;
     pairs = last_pairs;
