@@ -2,6 +2,7 @@
 // checks and the bundles the launchers take.
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <exception>
 
@@ -78,7 +79,7 @@ int guarded(const char* ctx, F&& f) {
     return -1;
 }
 
-// axis and frequency of each pair (64 powers: 3 us, so the last one made stays with the thread)
+// axis and frequency of each pair (64 powers: 4 us, so the last one made stays with the thread)
 bool make_rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags, float freq_base, float freq_scale,
                 int64_t D, RopeAxesTable& t, int& pairs) {
     if (!sections || n_axes < 1 || n_axes > 4) return fail(ctx, "there must be 1 to 4 sections");
@@ -96,6 +97,7 @@ bool make_rope_table(const char* ctx, const int32_t* sections, int n_axes, int f
     if (!(freq_base > 0.0f) || !std::isfinite(freq_base) || !std::isfinite(freq_scale))
         return fail(ctx, "freq_base must be positive and finite, and freq_scale finite");
     pairs = (int)P;
+    const long double log2_base = std::log2((long double)freq_base);
     int used[4] = {};
     int block = 0, left = sections[0];
     for (int i = 0; i < pairs; ++i) {
@@ -108,13 +110,16 @@ bool make_rope_table(const char* ctx, const int32_t* sections, int n_axes, int f
             a = block;
             --left;
         }
-        const double e = (flags & GTB_ROPE_PER_AXIS) ? (double)used[a] / std::max(1, sections[a]) : (double)i / (double)P;
+        const long double e = (flags & GTB_ROPE_PER_AXIS) ? (long double)used[a] / std::max(1, sections[a]) : (long double)i / P;
         ++used[a];
-        const double turns = (double)freq_scale * std::pow((double)freq_base, -e) / 6.283185307179586476925287;
-        // the fraction of a turn per position, rounded to 2^-64; whole turns per position drop out
-        double frac = turns - std::floor(turns);
-        const double hi = std::floor(std::ldexp(frac, 32));
-        const double lo = std::nearbyint(std::ldexp(std::ldexp(frac, 32) - hi, 32));
+        // (base^-e as 2^(-e log2 base): where e log2 base is large, and with it its rounding, the power is small)
+        const long double turns = freq_scale * std::exp2(-e * log2_base) / 6.283185307179586476925286766559005768L;
+        // the fraction of a turn per position, rounded to 2^-64; whole turns per position drop out. A position multiplies the
+        // error by up to 2^31, so f64's 53 bits would not do (2^-25 of a turn there)
+        static_assert(LDBL_MANT_DIG >= 64, "the fraction takes 64 bits");
+        const long double frac = turns - std::floor(turns);
+        const long double hi = std::floor(std::ldexp(frac, 32));
+        const long double lo = std::nearbyint(std::ldexp(std::ldexp(frac, 32) - hi, 32));
         t.turn[i] = ((uint64_t)hi << 32) + (uint64_t)lo;
         t.axis[i] = (uint8_t)a;
     }

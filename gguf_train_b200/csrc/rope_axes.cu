@@ -1,7 +1,8 @@
 // Rotary position embedding with several position axes, of one tensor or of q and k in one launch.
 // The angle of pair i of token (b, s) is pos[axis(i)][b][s] * f(i). Its value modulo a turn is all that the
 // sine and cosine see, so the frequency is kept as turns per position in 64-bit fixed point: the integer
-// product position * turn modulo 2^64 drops the whole turns exactly, at any int32 position.
+// product position * turn modulo 2^64 drops the whole turns exactly, and what is left is right to 2^-31 of a turn at any
+// int32 position. It becomes f32 (half a turn at most: to 2^-26) for sine and cosine.
 //
 // HBM bound: every value is read and written once. A CTA takes TOK tokens of one sequence and a share of the
 // heads: it forms the tokens' (cos, sin) table once in shared memory, then each thread keeps the part of the table

@@ -675,8 +675,8 @@ def rope_axes(input: torch.Tensor, positions: torch.Tensor, sections, k: torch.T
     has pairs left, else axis 0). Pair i turns by freq_base^(-i / P) a position, or with `per_axis` each axis
     runs through its own frequencies, freq_base^(-j / sections[a]). Differentiable in input and k.
 
-    Angles are formed modulo a turn in 64-bit fixed point, so positions may be any int32 without loss; rope()
-    instead repeats ggml's f32 accumulation of one axis."""
+    Angles are formed modulo a turn in 64-bit fixed point, right to 2^-31 of a turn at any int32 position, and then
+    rounded to f32; rope() instead repeats ggml's f32 accumulation of one axis."""
     xs = (input,) if k is None else (input, k)
     _require_cuda("rope_axes", positions, *xs)
     if input.ndim != 4 or input.dtype not in _ROPE_DTYPES:

@@ -251,9 +251,10 @@ GTB_API int gtb_attn_merge(float *o_acc, float *lse_acc, const void *o_part, con
  *   has freq_scale * freq_base^(-j / sections[a]).
  *   mode 0 (pairs 2i, 2i+1) or 2 (pairs i, i + P); dims >= 2 P pass through; backward != 0 rotates by
  *   -angle (the gradient).
- * Angles are turns in 64-bit fixed point (position x frequency modulo one turn, exact to 2^-33 of a turn
- * for any int32 position), so long positions lose nothing; gtb_rope instead follows ggml's f32
- * accumulation, and the two differ by that rounding where they can express the same rotation. */
+ * Angles are turns in 64-bit fixed point: position x frequency modulo one turn is right to 2^-31 of a turn at any int32
+ * position (frequencies up to 1 radian a position) and then rounded to f32 (2^-26 of a turn at most), so long positions
+ * lose nothing against short ones; gtb_rope instead follows ggml's f32 accumulation, and the two differ by that rounding
+ * where they can express the same rotation. */
 #define GTB_ROPE_INTERLEAVED 1
 #define GTB_ROPE_PER_AXIS 2
 GTB_API int gtb_rope_axes(const gtb_tensor4 *x, gtb_tensor4 *out, const gtb_tensor4 *k, gtb_tensor4 *k_out,
