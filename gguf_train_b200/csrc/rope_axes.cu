@@ -134,6 +134,10 @@ __global__ void __launch_bounds__(THREADS, 4) rope_axes_kernel(const __grid_cons
 
 template <typename T, int V, int MODE>
 int launch(const RopeAxesArgs& a, cudaStream_t st) {
+    int dev = 0, n_sm = 0;
+    if (cuda_failed(cudaGetDevice(&dev), "rope_axes") ||
+        cuda_failed(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev), "rope_axes"))
+        return -1;
     const int64_t heads = a.heads[0] + a.heads[1];
     const int rot = V == 1 ? a.pairs : MODE == 2 ? a.pairs / V : 2 * a.pairs / V;
     const int pieces = rot + (a.D - 2 * a.pairs) / V;
@@ -143,7 +147,7 @@ int launch(const RopeAxesArgs& a, cudaStream_t st) {
     int groups = std::max(1, THREADS / (tok * pieces));  // head groups side by side in the CTA
     const int64_t blocks = (a.S + tok - 1) / tok * a.B;
     // enough CTAs for 8 per SM, but no fewer than FLIGHT heads a thread
-    int64_t split = std::max<int64_t>(1, std::min<int64_t>((heads + groups * FLIGHT - 1) / (groups * FLIGHT), (148 * 8 + blocks - 1) / blocks));
+    int64_t split = std::max<int64_t>(1, std::min<int64_t>((heads + groups * FLIGHT - 1) / (groups * FLIGHT), (n_sm * 8 + blocks - 1) / blocks));
     int64_t hpg = (heads + groups * split - 1) / (groups * split);
     split = (heads + groups * hpg - 1) / (groups * hpg);
     const size_t smem = sizeof(float2) * tok * a.pairs;
