@@ -282,7 +282,7 @@ GTB_API int gtb_kv8_attention(const gtb_tensor4* q, const gtb_kv8* cache, float 
         if (!score_in != !score_out) return fail(ctx, "score_in and score_out go together"), -1;
         if (std::isnan(scale) || std::isinf(scale)) return fail(ctx, "scale must be finite"), -1;
         const bool no_rows = count(*q) == 0;
-        if (no_rows && (!score_out || score_in == score_out)) return 0;
+        if (no_rows && (!score_out || score_in == score_out || cache->B == 0)) return 0;
         if (!no_rows && (!check_device_ptr(q->data, ctx, "q") || !check_device_ptr(out->data, ctx, "out"))) return -1;
         if (!no_rows && lse && !check_device_ptr(lse, ctx, "lse")) return -1;
         if (counts && !check_device_ptr(counts, ctx, "counts")) return -1;
