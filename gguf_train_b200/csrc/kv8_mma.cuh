@@ -43,7 +43,7 @@ namespace gtb {
 namespace kv8 {
 
 constexpr float SV_MIN = 0x1p-80f;
-constexpr float RAISE = 7.0f, SHIFT = 8.0f, NONE = -1e30f;  // NONE: no key seen yet
+constexpr float RAISE = 7.0f, SHIFT = 8.0f, NONE = -3.402823466e38f;  // NONE: no key seen yet (finite: -inf - NONE is -inf)
 
 struct MmaP {
     gtb_kv8 c;

@@ -304,6 +304,7 @@ GTB_API int gtb_kv8_read(const gtb_kv8 *cache, const int32_t *start, gtb_tensor4
  *   score_out NULL, or (B,Hkv,Smax) f32 that receives score_in (same shape, may be score_out itself) + the
  *   attention weight each row s < lens[b] got, summed over the kv head's query heads and all queries; other
  *   entries are not written. The sums run in a fixed order: the same bits on every run.
+ * A weight is 2^(score - log-sum-exp) of f32 numbers: off by about |score| 2^-22 of itself (scores in powers of 2).
  * A v_scale below 2^-80 (a largest value below 1.1e-22) counts as 2^-80, and the v_scales of a head's blocks that hold
  * other values than zeros may lie up to 2^120 apart.
  * Scratch comes from the stream-ordered allocator: up to 1 GB for the scores (or, where query rows
