@@ -44,6 +44,7 @@ constexpr uint32_t TMEM_COLS = 512;
 // Parts of each of the last items: 1021 tokens of 4 sequences with 1 / 2 / 4 / 8 471 / 459 / 451 / 467 us, 333 tokens
 // 263 / 240 / 222 / 238
 constexpr int TAIL_SPLITS = 4;
+constexpr float LARGE = 0x1p20f;  // f32 holds a score above to 2^-4 at best
 
 template <int D>
 struct ChunkCfg {
@@ -407,6 +408,7 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const int lim0 = it.row0[t] / p.G + it.len - it.cnt;        // ... the tile's first row
             const float qmul = p.qmul[(int64_t)it.bh * p.Rpad + row];
             const float4* scl = p.scl + (int64_t)it.bh * (p.Spad / 16) + it.j0 * 8;
+            const float large_from = valid ? LARGE : INFINITY;         // (padding changes no other row's rounding)
             float m_used = -INFINITY, lsum = 0.0f;
             for (int j = 0; j < nb; ++j) {
                 ok = warp_wait(&s_full[t], (u + j) & 1, p.status, 131);
@@ -468,6 +470,22 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                     cm = fmaxf(cm, fmaf(fmax3(a, b, d), mul, add));
                 }
                 if (cm > m_used + RAISE) m_used = cm;  // never while the row has no finite score
+                // Scores so large that x * mul + (add - m), rounded once, would be off m's own rounding by more than P' has
+                // room for: they are rounded as m was, and then differ from it exactly
+                const bool large = __any_sync(0xffffffffu, fabsf(m_used) > large_from && m_used != -INFINITY);
+                if (large) {
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g) {
+                        float mul, add, inv;
+                        scale_of_group(g, mul, add, inv);
+#pragma unroll
+                        for (int e = 0; e < GK; ++e) x[GK * g + e] = fmaf(x[GK * g + e], mul, add);
+                        if constexpr (GROUPS <= 2) {
+                            g_mul[g] = 1.0f;
+                            g_add[g] = 0.0f;
+                        }
+                    }
+                }
                 const bool grew = m_used != m_start;
                 const float off = m_used == -INFINITY ? 0.0f : SHIFT - m_used;
                 float block_sum = 0.0f;
@@ -486,6 +504,10 @@ kv8_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                             inv = g_inv[g];
                         } else {
                             scale_of_group(g, mul, add, inv);
+                            if (large) {
+                                mul = 1.0f;
+                                add = 0.0f;
+                            }
                         }
                         add += off;
                         const uint64_t mul2 = f2_pack(mul, mul), add2 = f2_pack(add, add);

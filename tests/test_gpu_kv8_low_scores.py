@@ -15,7 +15,7 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("fmt", [torch.int8, torch.float8_e4m3fn], ids=["int8", "e4m3"])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("size", [1e3, 1e34, 1e37])
-@pytest.mark.parametrize("Lq,cap", [(1, 100), (1, 5000), (5, 5000), (40, 300)])
+@pytest.mark.parametrize("Lq,cap", [(1, 100), (1, 5000), (5, 5000), (40, 300), (80, 300)])
 def test_rows_of_low_scores(fmt, dt, size, Lq, cap):
     from gguf_train_b200 import KV8Cache, _C, kv8_attention
 
