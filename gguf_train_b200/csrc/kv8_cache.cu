@@ -151,8 +151,8 @@ struct Codes16 {
 
 // One CTA per (touched block, sequence x kv head), K and V together. The new rows stay in registers between the largest
 // value and the codes (KEEP chunks of each a thread; what does not fit is read again, from L2). 8 sequences, up to 4099
-// tokens, 8 heads of 128, f16 to e4m3 blocks of 32: 26 us, bound by HBM and by the conversions' issue slots together; with
-// 2 / 4 chunks kept the append and a read of it take 75 / 86 us (fewer threads a block hide less).
+// tokens, 8 heads of 128, f16 to e4m3 blocks of 32: 31 us for 110 MB (3.6 TB/s), bound by the conversions' issue slots (70 %
+// busy); with 2 / 4 chunks kept the append and a read of it take 75 / 86 us (fewer threads a block hide less).
 template <typename T, int FMT, bool VEC, int KEEP>
 __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__ Kv8AppendArgs a, unsigned blocks, RowOf row_of) {
     __shared__ float2 red[8];
@@ -252,7 +252,7 @@ __global__ void kv8_advance_kernel(const Kv8AppendArgs a) {
 }
 
 // A thread reads chunks of READ_ROWS rows of one (sequence, kv head, K or V) and writes their values. HBM bound: the
-// read after the append above 38 us (5.7 TB/s), 16 x 4096 tokens x 8 heads of 128 to bf16 70 us (5.8 TB/s).
+// read after the append above 39 us (5.2 TB/s), 16 x 4096 tokens x 8 heads of 128 to bf16 72 us (5.6 TB/s).
 constexpr int READ_ROWS = 4;
 template <typename T, int FMT>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const __grid_constant__ Kv8ReadArgs a) {
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(SEL_THREADS) kv8_select_kernel(const __grid_co
 
 // One CTA per (destination block, sequence x kv head), K and V together: the kept rows' values, their largest, the new
 // scale, the new codes. As in the append, KEEP chunks of each a thread stay in registers. 16 sequences to 4096 rows,
-// 8 heads of 128: 92 us, bound by the conversions (ALU 63 % busy) rather than by its 0.27 GB (41 us).
+// 8 heads of 128: 93 us, bound by the conversions (ALU 65 %, issue slots 69 % busy) rather than by its 0.27 GB (41 us).
 template <int FMT, int KEEP>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(const __grid_constant__ Kv8EvictArgs a, unsigned blocks, RowOf row_of) {
     __shared__ float2 red[8];

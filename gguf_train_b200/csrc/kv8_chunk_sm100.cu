@@ -18,9 +18,9 @@
 //                     sum is of the f32 values.
 //   kv8_chunk_join_kernel  joins those parts.
 // The tile pair reuses each K/V tile for 256 rows; the second kernel is bound by the softmax warps' chain from scores
-// to weights (tensor pipe 49 % busy). 4 sequences, 1021 tokens x 32 heads of 128 against 4k to 8k cached: 40 us to
-// widen (its bytes at HBM rate), 400 for the products (0.57 of the bf16 GEMM rate), 13 for the join; on kv8_mma.cuh
-// 2.6 ms. Every wait is bounded: a timeout records a status code, drains the CTA's own copies and MMAs,
+// to weights (tensor pipe and exponentials 48 to 49 % busy each). 4 sequences, 1021 tokens x 32 heads of 128 against 4k to
+// 8k cached: 46 us to widen, 400 to 428 for the products (0.54 to 0.58 of the bf16 GEMM rate), 13 for the join; on
+// kv8_mma.cuh 2.7 ms. Every wait is bounded: a timeout records a status code, drains the CTA's own copies and MMAs,
 // frees TMEM and returns.
 
 #include <algorithm>

@@ -7,7 +7,7 @@
 // one while the other's exponentials run, and two CTAs share an SM where their tiles fit, so that one's start (codes
 // to f16, first tile) hides behind the other. The exponentials, one per key and row at 16 a clock and SM, and the
 // additions around them bound it where rows are many, a CTA's start where they are few. 1021 tokens x 32 heads of 128
-// against 4 x 4k to 8k cached: 0.44 ms (0.58 with one CTA an SM); 36 rows a head, 16 sequences of 2k to 16k: 0.24 ms (0.52).
+// against 4 x 4k to 8k cached: 0.44 ms (0.58 with one CTA an SM); 36 rows a head, 16 sequences of 2k to 16k: 0.30 ms.
 // q is brought to f16 as in kv8_mma.cuh, f32 q as two numbers whose products add up in the accumulator.
 
 #include <algorithm>

@@ -7,7 +7,7 @@
 // HBM bound: every value is read and written once. A CTA takes TOK tokens of one sequence and a share of the
 // heads: it forms the tokens' (cos, sin) table once in shared memory, then each thread keeps the part of the table
 // that belongs to its 16 bytes of a row in registers and walks the heads with 16-byte accesses, two rows in
-// flight. Measured: 8 x 4096 tokens, 32 + 8 heads of 128, bf16 115 us, 5.9 TB/s (166 with one row in flight and three CTAs
+// flight. Measured: 8 x 4096 tokens, 32 + 8 heads of 128, bf16 115 us, 5.8 TB/s (166 with one row in flight and three CTAs
 // an SM); 6 x 2047 tokens, 16 + 16 heads of 80, f32 43 us, 5.9 TB/s; one token of 64 sequences is a launch, 4 us.
 
 #include <algorithm>
