@@ -75,6 +75,16 @@ class KV8(ctypes.Structure):
 PKV8 = ctypes.POINTER(KV8)
 
 
+class Latent(ctypes.Structure):
+    """gtb_latent: a cache of latents and rotary keys (include/gtb_attn.h)."""
+
+    _fields_ = [("rows", c_void_p), ("lens", c_void_p), ("B", c_int64), ("Smax", c_int64), ("R", ctypes.c_int32),
+                ("Dr", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+PLATENT = ctypes.POINTER(Latent)
+
+
 def _configure(lib: ctypes.CDLL) -> ctypes.CDLL:
     # raw-pointer ABI (gtb_attn.h)
     lib.gtb_sdpa_fwd.argtypes = [P4, P4, P4, P4, c_float, c_int, P4, c_void_p, c_void_p]
@@ -127,6 +137,10 @@ def _configure(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.gtb_kv8_attention.restype = c_int
     lib.gtb_kv8_evict.argtypes = [PKV8, c_void_p, c_int64, c_int64, PKV8, c_void_p, c_void_p, c_void_p]
     lib.gtb_kv8_evict.restype = c_int
+    lib.gtb_latent_append.argtypes = [PLATENT, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float, c_float, c_int, c_void_p]
+    lib.gtb_latent_append.restype = c_int
+    lib.gtb_latent_attention.argtypes = [c_void_p, PLATENT, PLATENT, c_float, c_void_p, c_void_p, c_void_p, c_void_p]
+    lib.gtb_latent_attention.restype = c_int
     lib.gtb_last_error.argtypes = []
     lib.gtb_last_error.restype = c_char_p
     lib.gtb_clear_error.argtypes = []

@@ -15,6 +15,7 @@ from . import handles
 from .functional import (FlashAttentionFn, RoPEAxesFn, RoPEFn, decode_q8_0, dequantize_q8_0, q8_0_append, quantize_q8_0,
                          rope, rope_axes, scaled_dot_product_attention, sdpa_from_host)
 from .kv8 import KV8Cache, kv8_append, kv8_attention, kv8_evict, kv8_read
+from .latent import LatentCache, latent_append, latent_attention, latent_sdpa
 from .modules import MultiheadAttention
 
 __all__ = [
@@ -39,4 +40,8 @@ __all__ = [
     "kv8_attention",
     "kv8_evict",
     "kv8_read",
+    "LatentCache",
+    "latent_append",
+    "latent_attention",
+    "latent_sdpa",
 ]

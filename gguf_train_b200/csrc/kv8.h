@@ -64,6 +64,9 @@ struct RopeAxesTable {
     uint64_t turn[ROPE_MAX_PAIRS];
     uint8_t axis[ROPE_MAX_PAIRS];
 };
+// the table of gtb_rope_axes's arguments (kv8_api.cu); false: refused, with the message set
+bool rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags, float freq_base, float freq_scale, int64_t D,
+                RopeAxesTable& t, int& pairs);
 struct RopeAxesArgs {
     RopeAxesTable tab;
     Rows3 x[2], y[2];

@@ -140,6 +140,8 @@ struct RopeKey {
     }
 };
 
+}  // namespace
+
 bool rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags, float freq_base, float freq_scale, int64_t D,
                 RopeAxesTable& t, int& pairs) {
     thread_local RopeKey last;
@@ -164,7 +166,6 @@ bool rope_table(const char* ctx, const int32_t* sections, int n_axes, int flags,
     return true;
 }
 
-}  // namespace
 }  // namespace gtb
 
 using namespace gtb;

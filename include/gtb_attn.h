@@ -324,6 +324,43 @@ GTB_API int gtb_kv8_attention(const gtb_tensor4 *q, const gtb_kv8 *cache, float 
 GTB_API int gtb_kv8_evict(const gtb_kv8 *src, const float *score, int64_t budget, int64_t recent, const gtb_kv8 *dst,
                           float *score_out, int32_t *kept, void *stream);
 
+/* A cache for latent attention: of each token one latent vector of R values, from which every head's keys and values
+ * are made, and one rotary key of Dr values that the heads share. New exports; the reference has no such attention.
+ *   rows: (B,Smax,R+Dr) contiguous f16 or bf16, 16-byte aligned, a row the latent followed by the rotary key; lens:
+ *   device int32 (B), rows held of each sequence (values outside [0, Smax] are read as the nearest end). R a
+ *   multiple of 64 from 64 to 512, Dr a multiple of 16 from 16 to 64; Smax below 2^30.
+ * Rows at and past lens[b] may hold anything (NaN included): no call lets them into a result. */
+typedef struct gtb_latent {
+    void *rows;
+    int32_t *lens;
+    int64_t B, Smax;
+    int32_t R, Dr;
+    int32_t dtype;
+} gtb_latent;
+
+/* Append rows: latent (B,1,n,R) and k_rope (B,1,n,Dr), f32/f16/bf16 (one dtype, any strides with a unit innermost one);
+ * the first counts[b] of them (device int32, clamped to [0, n]; NULL: n) go to rows lens[b] .. of sequence b, rounded
+ * once to the cache's type. With rope_mode 0 (pairs 2i, 2i+1) or 2 (pairs i, i + Dr/2) the rotary key is first rotated,
+ * in f32, for position offset[0] + lens[b] + i (offset: device int32, the lens of a prefix, or NULL: 0), its pairs'
+ * frequencies freq_scale * freq_base^(-2i / Dr) and angles those of gtb_rope_axes; with -1 it is taken as given.
+ * With advance != 0 a second kernel sets lens[b] = min(lens[b] + counts[b], Smax). Rows that would land past Smax are
+ * dropped and leave status 62 (gtb_device_status). */
+GTB_API int gtb_latent_append(const gtb_latent *cache, const gtb_tensor4 *latent, const gtb_tensor4 *k_rope,
+                              const int32_t *counts, const int32_t *offset, int rope_mode, float freq_base,
+                              float freq_scale, int advance, void *stream);
+
+/* Attention in the absorbed form: q (B,H,Lq,R+Dr) in the cache's dtype, its first R values the query taken through the
+ * keys' up-projection, the other Dr the rotated ones. The queries are the last counts[b] (device int32, clamped to
+ * [0, Lq]; NULL: Lq) of the lens[b] tokens cached, and query i < counts[b] attends every row of the prefix and rows
+ * s <= lens[b] - counts[b] + i of its sequence: score = scale * q . row, out (B,H,Lq,R) = sum of weight * latent
+ * (the values' up-projection is the caller's next product). A query at or past counts[b], or with no row to attend,
+ * gives 0 and lse -inf.
+ *   prefix: NULL, or a cache of one sequence (B = 1, same R, Dr and dtype) whose rows come before every sequence's own:
+ *   they are read once for the whole batch. q 16-byte aligned, any strides that are multiples of 8 with a unit
+ *   innermost one; out contiguous, 16-byte aligned; lse NULL or (B,H,Lq) f32; scale positive. */
+GTB_API int gtb_latent_attention(const gtb_tensor4 *q, const gtb_latent *cache, const gtb_latent *prefix, float scale,
+                                 const int32_t *counts, gtb_tensor4 *out, float *lse, void *stream);
+
 /* Kernel family of the calling thread's last gtb_sdpa_fwd / gtb_sdpa_fwd_rope / gtb_sdpa_bwd call:
  * "tcgen05" (tensor cores, TMA), "tcgen05+rope" (the same with q rotated inside the kernel),
  * "f32_tiled" (fp32 with head size 64, register-blocked on the CUDA cores) or "simt" (one warp per
