@@ -1,0 +1,847 @@
+// Absorbed latent attention on tcgen05: one latent row a token is the key of every head and, without its rotary part, the
+// value, so a cached row is read once for all of a sequence's query rows.
+//
+// A tile of 64 cached rows (TMA, 64-column panels with 128-byte swizzle) meets up to 64 query rows, transposed:
+//     S^T = C Q^T        (M = 64 keys, N = query rows, K = R + Dr; both operands K-major)
+//     O^T += C^T P^T     (M = 128 latent dims a product, N = query rows, K = 64 keys; both operands MN-major)
+// The query rows are the N side because a decode step has few (heads x tokens, padded to 16) and N can be small, and because
+// O of 64 rows x 512 dims then takes 4 x 64 of TMEM's 512 columns (as M side it would take all of them for
+// 128 rows, and leave none for S). The same tile in shared memory is the A operand of both products. P^T goes
+// through 8 KB of shared memory, rows = keys.
+//
+// Warps: 0 TMA producer, 1 TMEM owner and MMA issuer (one thread), 2-3 idle, 4-11 softmax and epilogue. S^T uses 16 lanes
+// of each TMEM quadrant; a softmax warp reads its quadrant's 16 keys in the 16x256b shape (a thread has two keys of
+// four column pairs), warps 4-7 the even groups of 8 columns, 8-11 the odd ones. The exponent's offset of a query row is
+// raised only when a score exceeds it by more than 2^8, so most tiles need no maximum: one vote over the block (a
+// barrier with a reduction) finds that no row grew. Sums stay with each thread until a segment's end.
+// MMA order S(0) S(1) PV(0) S(2) PV(1) ...: the next tile's scores are formed while this one's weights are.
+//
+// Work: an item is a block of query rows (tokens x heads of one sequence) over the rows it attends. All items' tiles
+// in a row are cut into equal shares, one a CTA, so ragged lengths balance and a long sequence is split where there are
+// few; an item that more than one CTA worked on is joined by a second kernel from f32 partial results. Behind a shared
+// prefix, rows of several sequences make up an item of their own over the prefix (where a sequence alone fills
+// an item, the prefix's tiles simply come first in its own), and every row is joined.
+//
+// Rows past a sequence's end are zeroed in shared memory before the second product (a weight of 0 would make NaN of
+// them). Every mbarrier wait is bounded; the softmax warps, which also meet at block barriers, go on without
+// waiting after a timeout so that none is left behind.
+
+#include <algorithm>
+
+#include "gtb_common.cuh"
+#include "latent.h"
+#include "sdpa_args.h"
+#include "sm100_ptx.cuh"
+
+namespace gtb {
+namespace {
+
+using namespace sm100;
+
+constexpr int KT = 64;                 // cached rows a tile
+constexpr int NR = 64;                 // query rows an item, at most
+constexpr int PANEL = KT * 128;        // bytes of 64 rows x 64 columns
+constexpr int NTHREADS = 384;
+constexpr int NSOFT = 256;             // threads of the softmax warps
+constexpr int MAX_STAGES = 4;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr uint32_t O_COL = 2 * NR;     // S^T buffers at 0 and 64, O^T of dims 128 t .. at O_COL + 64 t
+constexpr int SMEM_MAX = 232448;
+
+struct Bars {
+    uint64_t q_full, q_empty, pv_done, o_empty, p_full, drain;
+    uint64_t k_full[MAX_STAGES], k_empty[MAX_STAGES], s_full[2];
+    uint32_t tmem;
+    int abort;
+};
+
+struct Extra {                 // what lies behind the operands in shared memory
+    Bars bars;
+    int64_t line, warp_sum[NTHREADS / 32];  // finding the CTA's share
+    int first_item, first_tile;
+    float exch[4][NR];         // a quadrant's maxima, later its sums
+    float alpha[NR];           // factor of a row's sums; at the end 1 / sum
+    int lim[NR];               // last own row a query row attends; DEAD: it attends nothing
+    int out_row[NR];           // row of the output, -1: none
+};
+
+constexpr int DEAD = INT_MIN;
+
+struct Params {
+    const int32_t *lens, *counts, *prefix_lens;  // counts, prefix_lens nullable
+    int64_t Smax, prefix_max;
+    int B, H, Lq, R, Dr;
+    int hh, ii, n_h, n_rt;     // heads and tokens of an item, items along the heads, items a sequence
+    int bb, n_pre;             // sequences of a prefix item (0: the prefix's tiles belong to the own items), prefix items
+    int panels, stages;
+    float scale_log2;
+    void* o;
+    float* lse;
+    float* part_o;             // [slot][row][R]
+    float2* part_ml;           // [slot][row]: offset, sum
+    int64_t* item_pos;         // first tile of an own item on the line (split prefix only)
+    int2* cta_item;            // item and tile within it that a CTA begins at
+    int64_t* line;             // [0] tiles in all, [1] CTAs in use
+    int own_rows;              // rows a slot of an own item
+    int64_t own_base;          // first float of own slots in part_o (split prefix)
+    int* status;
+};
+
+static_assert(3 * 9 * PANEL + PANEL + (int)sizeof(Extra) + 1024 <= SMEM_MAX, "two stages of the largest rows");
+
+struct Item {
+    int b, i0, h0;             // first sequence, token, head
+    int nb, ni, nh;            // extent in them (box sizes)
+    int len, cnt;              // of an own item's sequence
+    int nt_pre, nt;            // tiles over the prefix; tiles in all (at least 1)
+    bool pre, empty;           // an item over the prefix alone; no rows to attend
+    __device__ __forceinline__ int rows() const { return nb * ni * nh; }
+};
+
+__device__ __forceinline__ int prefix_rows(const Params& p) {
+    return p.prefix_lens ? (int)min((int64_t)max(p.prefix_lens[0], 0), p.prefix_max) : 0;
+}
+
+// items over the prefix alone: only where there are rows in it
+__device__ __forceinline__ int prefix_items(const Params& p, int P) { return p.bb && P > 0 ? p.n_pre : 0; }
+
+__device__ __forceinline__ Item item_of(const Params& p, int k, int P, int np) {
+    Item it;
+    it.nh = p.hh;
+    it.ni = p.ii;
+    const int pt = (P + KT - 1) / KT;
+    if (k < np) {
+        it.pre = true;
+        it.empty = false;
+        it.b = k * p.bb;
+        it.i0 = it.h0 = 0;
+        it.nb = p.bb;
+        it.len = it.cnt = 0;
+        it.nt_pre = it.nt = pt;
+        return it;
+    }
+    k -= np;
+    it.pre = false;
+    it.nb = 1;
+    it.b = k / p.n_rt;
+    const int rt = k - it.b * p.n_rt, ti = rt / p.n_h;
+    it.i0 = ti * p.ii;
+    it.h0 = (rt - ti * p.n_h) * p.hh;
+    it.len = (int)min((int64_t)max(p.lens[it.b], 0), p.Smax);
+    it.cnt = p.counts ? min(max(p.counts[it.b], 0), p.Lq) : p.Lq;
+    const bool live = it.i0 < it.cnt;
+    const int keys = live ? max(0, it.len - it.cnt + min(it.i0 + p.ii, it.cnt)) : 0;
+    it.nt_pre = live && !p.bb ? pt : 0;
+    it.nt = it.nt_pre + (keys + KT - 1) / KT;
+    it.empty = it.nt == 0;
+    it.nt = max(it.nt, 1);
+    return it;
+}
+
+__device__ __forceinline__ int64_t share(int64_t line, int n, int c) { return line * c / n; }
+
+// query row `col` of an item: (sequence, token, head), false where there is none
+__device__ __forceinline__ bool row_of(const Params& p, const Item& it, int col, int& b, int& i, int& h) {
+    const int r = col / it.nh;
+    h = it.h0 + col - r * it.nh;
+    const int s = r / it.ni;
+    i = it.i0 + r - s * it.ni;
+    b = it.b + s;
+    return s < it.nb && h < p.H && i < p.Lq && b < p.B;
+}
+
+// slot of CTA c's partial result of item k, in floats of part_o and rows of part_ml
+__device__ __forceinline__ void slot_of(const Params& p, int k, int np, int c, bool head, int64_t& o, int64_t& ml) {
+    if (!p.bb) {  // a CTA leaves at most two: of the item it begins within, and of the one that it ends within
+        const int64_t s = 2 * c + (head ? 1 : 0);
+        o = s * p.own_rows * p.R;
+        ml = s * NR;
+    } else {      // (a step along the line changes the item or the CTA: k + c names the segment)
+        o = k < np ? (int64_t)(k + c) * NR * p.R : p.own_base + (int64_t)(k - np + c) * p.own_rows * p.R;
+        ml = (int64_t)(k + c) * NR;
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
+}
+
+// 16 lanes x 8 columns of 32 bits: thread t gets (lane t/4, columns 2 (t%4), +1) and (lane t/4 + 8, the same columns)
+__device__ __forceinline__ void tmem_ld_16x8(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr));
+}
+
+__device__ __forceinline__ void soft_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(NSOFT) : "memory"); }
+__device__ __forceinline__ bool soft_any(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v), "n"(NSOFT)
+        : "memory");
+    return r != 0;
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(NTHREADS, 1)
+latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQp,
+                   const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmCp,
+                   const __grid_constant__ Params p) {
+    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const int op_bytes = p.panels * PANEL;  // Q, and a stage of cached rows
+    unsigned char* sQ = smem;
+    unsigned char* sC = smem + op_bytes;
+    unsigned char* sP = sC + p.stages * op_bytes;
+    Extra& ex = *(Extra*)(sP + PANEL);
+    Bars& bar = ex.bars;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
+    const int P = prefix_rows(p), np = prefix_items(p, P);
+    const int n_items = np + p.B * p.n_rt;
+
+    // ---------------------------------------------------------------- this CTA's share of the line of tiles
+    if (threadIdx.x == 0) ex.line = 0;
+    __syncthreads();
+    {
+        int64_t mine = 0;
+        for (int k = threadIdx.x; k < n_items; k += NTHREADS) mine += item_of(p, k, P, np).nt;
+        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
+        if (lane == 0) atomicAdd((unsigned long long*)&ex.line, (unsigned long long)mine);
+    }
+    __syncthreads();
+    const int64_t line = ex.line;
+    const int n_cta = (int)min((int64_t)gridDim.x, line);
+    if (cta == 0 && threadIdx.x == 0) {
+        p.line[0] = line;
+        p.line[1] = n_cta;
+    }
+    if (cta >= n_cta) return;
+    const int64_t begin = share(line, n_cta, cta), end = share(line, n_cta, cta + 1);
+    {
+        int64_t before = 0;
+        for (int k0 = 0;; k0 += NTHREADS) {
+            const int k = k0 + (int)threadIdx.x;
+            const int64_t n = k < n_items ? item_of(p, k, P, np).nt : 0;
+            int64_t incl = n;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(~0u, incl, o);
+                if (lane >= o) incl += y;
+            }
+            if (lane == 31) ex.warp_sum[warp] = incl;
+            __syncthreads();
+            int64_t total = 0;
+            for (int w = 0; w < NTHREADS / 32; ++w) {
+                if (w < warp) incl += ex.warp_sum[w];
+                total += ex.warp_sum[w];
+            }
+            incl += before;
+            if (begin >= incl - n && begin < incl) {
+                ex.first_item = k;
+                ex.first_tile = (int)(begin - (incl - n));
+            }
+            before += total;
+            __syncthreads();
+            if (begin < before) break;  // (begin < line: found by the last round)
+        }
+    }
+    const int k_first = ex.first_item, off_first = ex.first_tile;
+    if (threadIdx.x == 0) p.cta_item[cta] = make_int2(k_first, off_first);
+
+    if (threadIdx.x == 0) {
+        mbar_init(&bar.q_full, 1);
+        mbar_init(&bar.q_empty, 1);
+        mbar_init(&bar.pv_done, 1);
+        mbar_init(&bar.o_empty, NSOFT);
+        mbar_init(&bar.p_full, NSOFT);
+        mbar_init(&bar.drain, 1);
+        for (int s = 0; s < MAX_STAGES; ++s) { mbar_init(&bar.k_full[s], 1); mbar_init(&bar.k_empty[s], 1); }
+        for (int s = 0; s < 2; ++s) mbar_init(&bar.s_full[s], 1);
+        bar.abort = 0;
+        fence_mbar_init();
+    }
+    // query rows that no load fills stay zero (their columns are computed and dropped)
+    for (int e = threadIdx.x; e < op_bytes / 16; e += NTHREADS) ((uint4*)sQ)[e] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+    if (warp == 1) tmem_alloc(&bar.tmem, TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar.tmem;
+    volatile int* abort_flag = &bar.abort;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0) {
+            prefetch_tmap(&tmQ);
+            prefetch_tmap(&tmC);
+            bool ok = true;
+            int u = 0, nseg = 0;  // tiles and segments started
+            int64_t pos = begin;
+            for (int k = k_first, off = off_first; pos < end && ok; ++k, off = 0) {
+                const Item it = item_of(p, k, P, np);
+                const int n = (int)min((int64_t)(it.nt - off), end - pos);
+                pos += n;
+                if (it.empty) continue;
+                for (int t = off; t < off + n && ok; ++t, ++u) {
+                    const int s = u % p.stages;
+                    if (u >= p.stages) ok = mbar_wait(&bar.k_empty[s], ((u / p.stages) - 1) & 1, p.status, 71);
+                    if (!ok || *abort_flag) { ok = false; break; }
+                    mbar_expect_tx(&bar.k_full[s], op_bytes);
+                    const bool pre = t < it.nt_pre;
+                    const CUtensorMap* tm = pre ? &tmCp : &tmC;
+                    const int row = (pre ? t : t - it.nt_pre) * KT, b = pre ? 0 : it.b;
+                    for (int a = 0; a < p.panels; ++a)
+                        tma_load_4d(sC + s * op_bytes + a * PANEL, tm, a * 64, row, b, 0, &bar.k_full[s]);
+                    if (t == off) {  // the segment's query rows, once the last one's have been read
+                        if (nseg > 0) ok = mbar_wait(&bar.q_empty, (nseg - 1) & 1, p.status, 72);
+                        if (!ok || *abort_flag) { ok = false; ++u; break; }
+                        mbar_expect_tx(&bar.q_full, it.rows() * 128 * p.panels);
+                        for (int a = 0; a < p.panels; ++a)
+                            tma_load_4d(sQ + a * PANEL, it.pre ? &tmQp : &tmQ, a * 64, it.h0, it.i0, it.b, &bar.q_full);
+                        ++nseg;
+                    }
+                }
+            }
+            if (!ok) *abort_flag = 1;
+            if (*abort_flag) {  // our copies in flight end before the CTA does
+                if (nseg > 0) mbar_wait(&bar.q_full, (nseg - 1) & 1, nullptr, 0);
+                for (int v = max(0, u - p.stages); v < u; ++v) mbar_wait(&bar.k_full[v % p.stages], (v / p.stages) & 1, nullptr, 0);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            const uint64_t qd = desc_sw128(smem_u32(sQ), 16, 1024);
+            const uint64_t cd = desc_sw128(smem_u32(sC), 16, 1024);
+            const uint64_t vd = desc_sw128(smem_u32(sC), PANEL, 1024);
+            const uint64_t pd = desc_sw128(smem_u32(sP), PANEL, 1024);
+            const int k_steps = (p.R + p.Dr) / 16, m_tiles = (p.R + 127) / 128;
+            bool ok = true;
+            int u = 0, nseg = 0;
+            int64_t pos = begin;
+            auto issue_s = [&](int v, uint32_t n16) -> bool {
+                const int s = v % p.stages;
+                if (!mbar_wait(&bar.k_full[s], (v / p.stages) & 1, p.status, 73)) return false;
+                tc_fence_after();
+                const uint32_t idesc = idesc_f16(KT, 0, BF16, false) | (n16 >> 3 << 17);
+                const uint64_t a = desc_advance(cd, s * op_bytes);
+                for (int kk = 0; kk < k_steps; ++kk) {
+                    const uint32_t o = (uint32_t)((kk >> 2) * PANEL + (kk & 3) * 32);
+                    mma_ss(tmem + (v & 1) * NR, desc_advance(a, o), desc_advance(qd, o), idesc, kk > 0);
+                }
+                mma_commit(&bar.s_full[v & 1]);
+                return true;
+            };
+            for (int k = k_first, off = off_first; pos < end && ok; ++k, off = 0) {
+                const Item it = item_of(p, k, P, np);
+                const int n = (int)min((int64_t)(it.nt - off), end - pos);
+                pos += n;
+                if (it.empty) continue;
+                const uint32_t n16 = (it.rows() + 15) & ~15;
+                const uint32_t idesc_pv = idesc_f16_amn(128, 0, BF16, true) | (n16 >> 3 << 17);
+                ok = mbar_wait(&bar.q_full, nseg & 1, p.status, 74) && issue_s(u, n16);
+                if (ok && n == 1) mma_commit(&bar.q_empty);
+                for (int t = 0; t < n && ok; ++t, ++u) {
+                    if (t + 1 < n) {
+                        ok = issue_s(u + 1, n16);
+                        if (!ok) break;
+                        if (t + 2 == n) mma_commit(&bar.q_empty);
+                    }
+                    ok = mbar_wait(&bar.p_full, u & 1, p.status, 75);
+                    // the segment's first product overwrites O^T: the last one's epilogue must have read it
+                    if (ok && t == 0 && nseg > 0) ok = mbar_wait(&bar.o_empty, (nseg - 1) & 1, p.status, 76);
+                    if (!ok || *abort_flag) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t a = desc_advance(vd, (u % p.stages) * op_bytes);
+                    for (int m = 0; m < m_tiles; ++m)
+                        for (int kk = 0; kk < KT / 16; ++kk)
+                            mma_ss(tmem + O_COL + m * NR, desc_advance(a, m * 2 * PANEL + kk * 2048), desc_advance(pd, kk * 2048),
+                                   idesc_pv, t > 0 || kk > 0);
+                    mma_commit(&bar.k_empty[u % p.stages]);
+                    mma_commit(&bar.pv_done);
+                }
+                ++nseg;
+            }
+            if (!ok) *abort_flag = 1;
+            if (*abort_flag) {
+                mma_commit(&bar.drain);
+                mbar_wait(&bar.drain, 0, nullptr, 0);
+            }
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ softmax, rescaling, epilogue
+        const int st = (int)threadIdx.x - 128, quad = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+        const int key0 = quad * 16 + (lane >> 2);          // this thread's keys of a tile: key0, key0 + 8
+        const int cpair = 2 * (lane & 3);                  // its columns of a group: cpair, cpair + 1
+        const int m_tiles = (p.R + 127) / 128;
+        bool ok = true;
+        int u = 0;
+        int64_t pos = begin;
+        for (int k = k_first, off = off_first; pos < end; ++k, off = 0) {
+            const Item it = item_of(p, k, P, np);
+            const int n = (int)min((int64_t)(it.nt - off), end - pos);
+            const int64_t item_start = pos - off;
+            pos += n;
+            const int gl = (it.rows() + 15) / 16;          // groups of 8 columns of this warp: 2 j + half, j < gl
+            soft_sync();                                   // the last segment's lim, out_row, alpha have been read
+            if (st < NR) {
+                int b, i, h;
+                const bool is = row_of(p, it, st, b, i, h);
+                ex.out_row[st] = is ? (b * p.H + h) * p.Lq + i : -1;
+                ex.lim[st] = !is || it.pre ? INT_MAX : i >= it.cnt ? DEAD : it.len - it.cnt + i;
+            }
+            if (st == 0 && p.bb && !it.pre && off == 0) p.item_pos[k - np] = item_start;
+            soft_sync();
+            const int lim_min = it.len - it.cnt + it.i0;   // smallest limit of a live row
+            float m[4][2], l[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m[j][0] = m[j][1] = -INFINITY, l[j][0] = l[j][1] = 0.0f;
+            for (int t = off; t < off + n && !it.empty; ++t, ++u) {
+                const bool pre = t < it.nt_pre;
+                const int row0 = (pre ? t : t - it.nt_pre) * KT;
+                const int valid = (pre ? P : it.len) - row0;  // cached rows of the tile
+                if (ok) ok = warp_wait(&bar.s_full[u & 1], (u >> 1) & 1, p.status, 77);
+                tc_fence_after();
+                uint32_t raw[4][4];
+                float (*x)[4] = (float(*)[4])raw;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j < gl) tmem_ld_16x8(tmem + lane_addr + (u & 1) * NR + 8 * (2 * j + half), raw[j]);
+                tmem_ld_wait();
+                if (pre ? valid < KT : row0 + KT - 1 > lim_min) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j >= gl) continue;
+                        const int c = 8 * (2 * j + half) + cpair;
+                        // (rows that attend nothing take the others' way and are dropped at the end)
+                        const int l0 = pre ? P - 1 : max(ex.lim[c], -1), l1 = pre ? P - 1 : max(ex.lim[c + 1], -1);
+                        if (row0 + key0 > l0) x[j][0] = -INFINITY;
+                        if (row0 + key0 > l1) x[j][1] = -INFINITY;
+                        if (row0 + key0 + 8 > l0) x[j][2] = -INFINITY;
+                        if (row0 + key0 + 8 > l1) x[j][3] = -INFINITY;
+                    }
+                }
+                bool grow = false;
+                float top[4][2];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= gl) continue;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        top[j][c] = fmaxf(x[j][c], x[j][c + 2]) * p.scale_log2;
+                        grow = grow || top[j][c] > m[j][c] + 8.0f;
+                    }
+                }
+                if (soft_any(grow)) {
+                    // the rows' maxima over the tile: over the thread's two keys, the warp's 16, the four quadrants
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j >= gl) continue;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float v = top[j][c];
+                            v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
+                            v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
+                            v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
+                            if (lane < 4) ex.exch[quad][8 * (2 * j + half) + cpair + c] = v;
+                        }
+                    }
+                    soft_sync();
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j >= gl) continue;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const int col = 8 * (2 * j + half) + cpair + c;
+                            const float v = fmaxf(fmaxf(ex.exch[0][col], ex.exch[1][col]), fmaxf(ex.exch[2][col], ex.exch[3][col]));
+                            const float mn = fmaxf(m[j][c], v);
+                            const float al = mn == m[j][c] ? 1.0f : ex2(m[j][c] - mn);
+                            m[j][c] = mn;
+                            l[j][c] *= al;
+                            if (quad == 0 && lane < 4) ex.alpha[col] = al;
+                        }
+                    }
+                    if (t > off) {  // O^T takes the same factors, once the last tile's product has been added
+                        if (ok) ok = warp_wait(&bar.pv_done, (u - 1) & 1, p.status, 78);
+                        soft_sync();
+                        tc_fence_after();
+                        for (int mt = half; mt < m_tiles; mt += 2) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if (j >= gl) continue;
+                                uint32_t v[16];
+                                tmem_ldx<16>(tmem + lane_addr + O_COL + mt * NR + 16 * j, v);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int c = 0; c < 16; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * ex.alpha[16 * j + c]);
+                                tmem_st16(tmem + lane_addr + O_COL + mt * NR + 16 * j, v);
+                            }
+                        }
+                        tmem_st_wait();
+                    }
+                }
+                uint32_t w[4][2];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= gl) continue;
+                    const float n0 = m[j][0] == -INFINITY ? 0.0f : -m[j][0], n1 = m[j][1] == -INFINITY ? 0.0f : -m[j][1];
+                    const float e0 = ex2(fmaf(x[j][0], p.scale_log2, n0)), e1 = ex2(fmaf(x[j][1], p.scale_log2, n1));
+                    const float e2 = ex2(fmaf(x[j][2], p.scale_log2, n0)), e3 = ex2(fmaf(x[j][3], p.scale_log2, n1));
+                    l[j][0] += e0 + e2;
+                    l[j][1] += e1 + e3;
+                    w[j][0] = pack2<BF16>(e0, e1);
+                    w[j][1] = pack2<BF16>(e2, e3);
+                }
+                if (u > 0 && ok) ok = warp_wait(&bar.pv_done, (u - 1) & 1, p.status, 79);  // P's buffer is free
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= gl) continue;
+                    unsigned char* d = sP + key0 * 128 + (((2 * j + half) ^ (key0 & 7)) << 4) + cpair * 2;
+                    *(uint32_t*)d = w[j][0];
+                    *(uint32_t*)(d + 8 * 128) = w[j][1];
+                }
+                if (valid < KT) {  // rows past the end: 0 in the second product, whatever they hold
+                    unsigned char* base = sC + (u % p.stages) * op_bytes;
+                    const int first = max(valid, 0), per = (KT - first) * 8;
+                    for (int e = st; e < per * (p.R / 64); e += NSOFT) {
+                        const int a = e / per, r = e - a * per;
+                        *(uint4*)(base + a * PANEL + first * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                }
+                fence_proxy_async_smem();
+                tc_fence_before();
+                mbar_arrive(&bar.p_full);
+            }
+            // ---- the segment's rows: sums over the quadrants, then O^T a latent dim a lane
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (j >= gl) continue;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float v = l[j][c];
+                    v += __shfl_xor_sync(~0u, v, 4);
+                    v += __shfl_xor_sync(~0u, v, 8);
+                    v += __shfl_xor_sync(~0u, v, 16);
+                    if (lane < 4) ex.exch[quad][8 * (2 * j + half) + cpair + c] = v;
+                    if (quad == 0 && lane < 4) ex.alpha[8 * (2 * j + half) + cpair + c] = m[j][c];
+                }
+            }
+            soft_sync();
+            const bool whole = !p.bb && off == 0 && n == it.nt;
+            int64_t so, sml;
+            slot_of(p, k, np, cta, off == 0, so, sml);
+            float lsum = 0.0f, mrow = -INFINITY;
+            if (st < NR) {
+                mrow = ex.alpha[st];
+                lsum = (ex.exch[0][st] + ex.exch[1][st]) + (ex.exch[2][st] + ex.exch[3][st]);
+                if (ex.lim[st] == DEAD || it.empty || st >= gl * 16) lsum = 0.0f, mrow = -INFINITY;
+            }
+            soft_sync();
+            if (st < NR && ex.out_row[st] >= 0) {
+                ex.alpha[st] = lsum > 0.0f ? 1.0f / lsum : 0.0f;
+                if (whole) {
+                    if (p.lse && ok) p.lse[ex.out_row[st]] = lsum > 0.0f ? (mrow + log2f(lsum)) * 0.69314718055994531f : -INFINITY;
+                } else if (ok) {
+                    p.part_ml[sml + st] = make_float2(mrow, lsum);
+                }
+            }
+            if (!it.empty && ok) ok = warp_wait(&bar.pv_done, (u - 1) & 1, p.status, 80);
+            soft_sync();
+            tc_fence_after();
+            for (int mt = half; mt < m_tiles; mt += 2) {
+                const int d = mt * 128 + quad * 32 + lane;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (j >= gl) continue;
+                    uint32_t v[16];
+                    tmem_ldx<16>(tmem + lane_addr + O_COL + mt * NR + 16 * j, v);
+                    tmem_ld_wait();
+                    if (d >= p.R || !ok) continue;
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const int col = 16 * j + c, row = ex.out_row[col];
+                        if (row < 0) continue;
+                        if (whole) {
+                            const float inv = ex.alpha[col];  // 0: nothing attended, whatever O^T holds
+                            Elem<T>::store((T*)p.o + (int64_t)row * p.R + d, inv == 0.0f ? 0.0f : __uint_as_float(v[c]) * inv);
+                        } else if (!it.empty) {
+                            p.part_o[so + (int64_t)col * p.R + d] = __uint_as_float(v[c]);
+                        }
+                    }
+                }
+            }
+            tc_fence_before();
+            if (!it.empty) mbar_arrive(&bar.o_empty);
+        }
+        if (!ok) *abort_flag = 1;
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+// Rows whose item more than one CTA worked on. A block has a query row; its warps share the row's dims (128 a warp) and,
+// where there are warps left, the parts.
+constexpr int JOIN_WARPS = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) latent_join_kernel(const __grid_constant__ Params p) {
+    __shared__ float4 sum[JOIN_WARPS][32];
+    const int P = prefix_rows(p), np = prefix_items(p, P), n_cta = (int)p.line[1];
+    const int64_t line = p.line[0];
+    // parts: CTAs c0 .. c1 of item k, column col; with a split prefix those of the prefix's item come first
+    int c0[2], c1[2], k[2], col[2], n_src = 0, b, i, h;
+    auto cta_at = [&](int64_t x) {  // the CTA whose share holds tile x
+        int c = (int)min((int64_t)n_cta - 1, x * n_cta / line);
+        while (c + 1 < n_cta && share(line, n_cta, c + 1) <= x) ++c;
+        while (share(line, n_cta, c) > x) --c;
+        return c;
+    };
+    bool dead;
+    if (!p.bb) {
+        const int c = (int)blockIdx.x + 1;  // the share's first tile lies within an item that began before
+        if (c >= n_cta) return;
+        const int2 at = p.cta_item[c];
+        const int64_t start = share(line, n_cta, c) - at.y;
+        if (at.y == 0 || share(line, n_cta, c - 1) > start) return;
+        const Item it = item_of(p, at.x, P, np);
+        if (!row_of(p, it, blockIdx.y, b, i, h)) return;
+        dead = i >= it.cnt;
+        k[0] = at.x;
+        col[0] = blockIdx.y;
+        c0[0] = c - 1;
+        c1[0] = cta_at(start + it.nt - 1);
+        n_src = 1;
+    } else {
+        const int64_t row = blockIdx.x;     // (b, i, h)
+        h = (int)(row % p.H);
+        i = (int)(row / p.H % p.Lq);
+        b = (int)(row / ((int64_t)p.H * p.Lq));
+        const Item it = item_of(p, np + b, P, np);
+        dead = i >= it.cnt;
+        const int pt = (P + KT - 1) / KT;
+        if (np > 0) {
+            k[0] = b / p.bb;
+            col[0] = ((b % p.bb) * p.Lq + i) * p.H + h;
+            c0[0] = cta_at((int64_t)k[0] * pt);
+            c1[0] = cta_at((int64_t)k[0] * pt + pt - 1);
+            n_src = 1;
+        }
+        if (!it.empty) {
+            const int64_t start = p.item_pos[b];
+            k[n_src] = np + b;
+            col[n_src] = i * p.H + h;
+            c0[n_src] = cta_at(start);
+            c1[n_src] = cta_at(start + it.nt - 1);
+            ++n_src;
+        }
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int chunks = (p.R + 127) / 128, groups = JOIN_WARPS / chunks;
+    const int chunk = warp % chunks, group = warp / chunks, d = chunk * 128 + lane * 4;
+    const int64_t orow = ((int64_t)b * p.H + h) * p.Lq + i;
+    float m = -INFINITY;
+    for (int s = 0; s < n_src; ++s)
+        for (int c = c0[s] + lane; c <= c1[s]; c += 32) {
+            int64_t o, ml;
+            slot_of(p, k[s], np, c, c == c0[s], o, ml);
+            m = fmaxf(m, p.part_ml[ml + col[s]].x);
+        }
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    float l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    int turn = 0;
+    for (int s = 0; s < n_src; ++s)
+#pragma unroll 4
+        for (int c = c0[s]; c <= c1[s]; ++c, ++turn) {
+            int64_t o, ml;
+            slot_of(p, k[s], np, c, c == c0[s], o, ml);
+            const float2 v = p.part_ml[ml + col[s]];
+            const float f = v.y > 0.0f ? exp2f(v.x - m) : 0.0f;  // (a part without a weight holds nothing)
+            l += v.y * f;
+            if (group < groups && turn % groups == group && d < p.R && f > 0.0f) {
+                const float4 y = *(const float4*)(p.part_o + o + (int64_t)col[s] * p.R + d);
+                acc.x = fmaf(y.x, f, acc.x);
+                acc.y = fmaf(y.y, f, acc.y);
+                acc.z = fmaf(y.z, f, acc.z);
+                acc.w = fmaf(y.w, f, acc.w);
+            }
+        }
+    sum[warp][lane] = acc;
+    __syncthreads();
+    const bool none = dead || !(l > 0.0f);
+    if (group == 0 && d < p.R) {
+        for (int g = 1; g < groups; ++g) {
+            const float4 y = sum[g * chunks + chunk][lane];
+            acc.x += y.x;
+            acc.y += y.y;
+            acc.z += y.z;
+            acc.w += y.w;
+        }
+        const float inv = none ? 0.0f : 1.0f / l;
+        __align__(8) T w[4];
+        const float a[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) Elem<T>::store(w + e, none ? 0.0f : a[e] * inv);
+        *(uint2*)((T*)p.o + orow * p.R + d) = *(const uint2*)w;
+    }
+    if (p.lse && threadIdx.x == 0) p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+}
+
+// nothing cached and nothing before it: zeros and -inf
+__global__ void latent_nothing_kernel(uint16_t* o, int64_t n, float* lse, int64_t rows) {
+    const int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = e; i < n; i += step) o[i] = 0;
+    for (int64_t i = e; lse && i < rows; i += step) lse[i] = -INFINITY;
+}
+
+// 4-D map of 16-bit values with a 64-column box and 128-byte swizzle; sizes and strides (elements) from the second dimension on
+bool make_map(CUtensorMap* tm, const void* base, bool bf16, int64_t cols, const int64_t (&size)[3], const int64_t (&stride)[3],
+              const int (&box)[3]) {
+    auto enc = encode_fn();
+    if (!enc) {
+        set_error("latent_attention: cuTensorMapEncodeTiled is unavailable");
+        return false;
+    }
+    cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)size[0], (cuuint64_t)size[1], (cuuint64_t)size[2]}, st[3];
+    for (int i = 0; i < 3; ++i) {
+        const int64_t bytes = (size[i] == 1 ? (cols + 7) / 8 * 8 : stride[i]) * 2;  // (a dimension of size 1 is never stepped)
+        if (bytes <= 0 || bytes % 16 || bytes >= (1ll << 40)) {
+            set_error("latent_attention: a stride is not a positive multiple of 16 bytes below 2^40");
+            return false;
+        }
+        st[i] = (cuuint64_t)bytes;
+    }
+    const cuuint32_t bx[4] = {64, (cuuint32_t)box[0], (cuuint32_t)box[1], (cuuint32_t)box[2]}, es[4] = {1, 1, 1, 1};
+    const CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void*)base, dims, st,
+                           bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_errorf("latent_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
+        return false;
+    }
+    return true;
+}
+
+template <bool BF16>
+int launch(const LatentAttnArgs& a, cudaStream_t st) {
+    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    const char* ctx = "latent_attention";
+    int dev = 0, n_sm = 0;
+    if (cuda_failed(cudaGetDevice(&dev), ctx) || cuda_failed(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev), ctx))
+        return -1;
+    Params p{};
+    p.lens = a.c.lens;
+    p.counts = a.counts;
+    p.Smax = a.c.Smax;
+    p.B = (int)a.c.B;
+    p.H = (int)a.H;
+    p.Lq = (int)a.Lq;
+    p.R = a.c.R;
+    p.Dr = a.c.Dr;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.o = a.o;
+    p.lse = a.lse;
+    p.status = a.status;
+    if (a.prefix.rows) {
+        p.prefix_lens = a.prefix.lens;
+        p.prefix_max = a.prefix.Smax;
+    }
+    // rows of an item: all heads of as many tokens as fit, or a part of the heads of one token, in equal parts
+    p.n_h = (p.H + NR - 1) / NR;
+    p.hh = (p.H + p.n_h - 1) / p.n_h;
+    const int fit = p.n_h > 1 ? 1 : NR / p.hh, n_i = (p.Lq + fit - 1) / fit;
+    p.ii = (p.Lq + n_i - 1) / n_i;
+    p.n_rt = n_i * p.n_h;
+    p.own_rows = p.hh * p.ii;
+    // a prefix gets items of its own where those can take the rows of several sequences
+    if (a.prefix.rows && n_i == 1 && p.n_h == 1 && 2 * p.own_rows <= NR && p.B > 1) {
+        const int most = NR / p.own_rows, n = (p.B + most - 1) / most;
+        p.bb = (p.B + n - 1) / n;
+        p.n_pre = (p.B + p.bb - 1) / p.bb;
+    }
+    const int64_t items = (int64_t)p.B * p.n_rt + p.n_pre;
+    if (items > INT32_MAX / 2) {
+        set_error("latent_attention: too many query rows");
+        return -1;
+    }
+    p.panels = p.R / 64 + 1;
+    const int op = p.panels * PANEL, fixed = op + PANEL + (int)sizeof(Extra) + 1024;
+    p.stages = std::min(MAX_STAGES, (SMEM_MAX - fixed) / op);
+    const size_t smem = fixed + p.stages * op;
+
+    const int64_t tiles_seq = (a.c.Smax + KT - 1) / KT + (p.prefix_lens ? (p.prefix_max + KT - 1) / KT : 0);
+    const int grid = (int)std::min<int64_t>(n_sm, items * std::max<int64_t>(tiles_seq, 1));
+
+    CUtensorMap mq, mqp, mc, mcp;
+    const int64_t D = p.R + p.Dr, qs[3] = {p.H, p.Lq, p.B}, qt[3] = {a.q.sh, a.q.ss, a.q.sb};
+    if (!make_map(&mq, a.q.p, BF16, D, qs, qt, {p.hh, p.ii, 1})) return -1;
+    mqp = mq;
+    if (p.bb && !make_map(&mqp, a.q.p, BF16, D, qs, qt, {p.hh, p.ii, p.bb})) return -1;
+    if (a.c.Smax > 0 && !make_map(&mc, a.c.rows, BF16, D, {a.c.Smax, a.c.B, 1}, {D, a.c.Smax * D, D}, {KT, 1, 1})) return -1;
+    if (a.prefix.rows && !make_map(&mcp, a.prefix.rows, BF16, D, {a.prefix.Smax, 1, 1}, {D, D, D}, {KT, 1, 1})) return -1;
+    if (a.c.Smax == 0) mc = a.prefix.rows ? mcp : mq;  // (never read: there are no own tiles)
+    if (!a.prefix.rows) mcp = mc;
+
+    // workspace: the line's data, then the parts
+    const int64_t slots_pre = p.bb ? p.n_pre + grid : 0, slots_own = p.bb ? (int64_t)p.B * p.n_rt + grid : 2 * (int64_t)grid;
+    p.own_base = slots_pre * NR * p.R;
+    const int64_t n_o = p.own_base + slots_own * p.own_rows * p.R;
+    const int64_t n_ml = (p.bb ? items + grid : 2 * (int64_t)grid) * NR;
+    auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+    const int64_t o_line = 0, o_cta = 256, o_pos = o_cta + up(grid * 8), o_ml = o_pos + up(p.bb ? (int64_t)p.B * 8 : 0),
+                  o_o = o_ml + up(n_ml * 8), total = o_o + up(n_o * 4);
+    char* ws = nullptr;
+    if (cuda_failed(cudaMallocAsync((void**)&ws, total, st), "latent_attention: workspace")) return -1;
+    p.line = (int64_t*)(ws + o_line);
+    p.cta_item = (int2*)(ws + o_cta);
+    p.item_pos = (int64_t*)(ws + o_pos);
+    p.part_ml = (float2*)(ws + o_ml);
+    p.part_o = (float*)(ws + o_o);
+
+    int rc = 0;
+    auto kern = latent_attn_kernel<BF16>;
+    if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), ctx)) rc = -1;
+    if (!rc) {
+        kern<<<grid, NTHREADS, smem, st>>>(mq, mqp, mc, mcp, p);
+        if (cuda_failed(cudaGetLastError(), "latent_attention launch")) rc = -1;
+    }
+    if (!rc && (p.bb || grid > 1)) {
+        const dim3 g = p.bb ? dim3((unsigned)((int64_t)p.B * p.H * p.Lq)) : dim3(grid - 1, p.own_rows);
+        latent_join_kernel<T><<<g, JOIN_WARPS * 32, 0, st>>>(p);
+        if (cuda_failed(cudaGetLastError(), "latent_attention join launch")) rc = -1;
+    }
+    cudaFreeAsync(ws, st);
+    return rc;
+}
+
+}  // namespace
+
+int launch_latent_attention(const LatentAttnArgs& a, cudaStream_t st) {
+    if (a.c.Smax == 0 && !a.prefix.rows) {
+        const int64_t rows = a.c.B * a.H * a.Lq, n = rows * a.c.R;
+        latent_nothing_kernel<<<(unsigned)std::min<int64_t>(1184, (n + 255) / 256), 256, 0, st>>>((uint16_t*)a.o, n, a.lse, rows);
+        return cuda_failed(cudaGetLastError(), "latent_attention launch") ? -1 : 0;
+    }
+    return a.c.dtype == BF16 ? launch<true>(a, st) : launch<false>(a, st);
+}
+
+}  // namespace gtb
