@@ -14,7 +14,8 @@
 // four column pairs), warps 4-7 the even groups of 8 columns, 8-11 the odd ones. The exponent's offset of a query row is
 // raised only when a score exceeds it by more than 2^8, so most tiles need no maximum: one vote over the block (a
 // barrier with a reduction) finds that no row grew. Sums stay with each thread until a segment's end.
-// MMA order S(0) S(1) PV(0) S(2) PV(1) ...: the next tile's scores are formed while this one's weights are.
+// The next tile's scores are formed while this one's weights are, unless its load is late: then the second product comes first and
+// frees its stage. Panels are loaded and freed in two groups, as the second product goes through them.
 //
 // Work: an item is a block of query rows (tokens x heads of one sequence) over the rows it attends. All items' tiles
 // in a row are cut into equal shares, one a CTA, so ragged lengths balance and a long sequence is split where there are
@@ -43,14 +44,15 @@ constexpr int NR = 64;                 // query rows an item, at most
 constexpr int PANEL = KT * 128;        // bytes of 64 rows x 64 columns
 constexpr int NTHREADS = 384;
 constexpr int NSOFT = 256;             // threads of the softmax warps
-constexpr int MAX_STAGES = 4;
+constexpr int MAX_STAGES = 6;
+constexpr int GROUPS = 2;              // panels 0 .. 3 and the others: what is loaded, and freed, at once
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t O_COL = 2 * NR;     // S^T buffers at 0 and 64, O^T of dims 128 t .. at O_COL + 64 t
 constexpr int SMEM_MAX = 232448;
 
 struct Bars {
     uint64_t q_full, q_empty, pv_done, o_empty, p_full, drain;
-    uint64_t k_full[MAX_STAGES], k_empty[MAX_STAGES], s_full[2];
+    uint64_t k_full[MAX_STAGES][GROUPS], k_empty[MAX_STAGES][GROUPS], s_full[2];
     uint32_t tmem;
     int abort;
 };
@@ -73,7 +75,7 @@ struct Params {
     int B, H, Lq, R, Dr;
     int hh, ii, n_h, n_rt;     // heads and tokens of an item, items along the heads, items a sequence
     int bb, n_pre;             // sequences of a prefix item (0: the prefix's tiles belong to the own items), prefix items
-    int panels, stages;
+    int panels, stages, slack;
     float scale_log2;
     void* o;
     float* lse;
@@ -87,7 +89,7 @@ struct Params {
     int* status;
 };
 
-static_assert(3 * 9 * PANEL + PANEL + (int)sizeof(Extra) + 1024 <= SMEM_MAX, "two stages of the largest rows");
+static_assert(3 * 9 * PANEL + PANEL + (int)sizeof(Extra) <= SMEM_MAX, "two stages of the largest rows");
 
 struct Item {
     int b, i0, h0;             // first sequence, token, head
@@ -181,6 +183,28 @@ __device__ __forceinline__ void tmem_ld_16x8(uint32_t taddr, uint32_t* r) {
                  : "r"(taddr));
 }
 
+// The lane that issues the MMA warp's products and commits. The whole warp goes through the loops around them without diverging,
+// on values that are the same in every lane for the compiler too (votes and reductions), so that descriptors
+// are formed in uniform registers, where the instruction takes its operands from. (One lane in loops of its own: 106 cycles a
+// product whatever its size; this way the unit's own 33 and 50.)
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(~0u, v); }  // of a value that all lanes have
+
+// The low words of the descriptors (address, leading byte offset) come in registers; the high ones are the same for all operands here
+// (stride byte offset 1024, version, 128-byte swizzle).
+constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void mma(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI)
+        : "memory");
+}
+
 __device__ __forceinline__ void soft_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(NSOFT) : "memory"); }
 __device__ __forceinline__ bool soft_any(bool v) {
     uint32_t r;
@@ -201,6 +225,10 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    if (smem - smem_raw > p.slack) {  // (the largest rows leave less than the alignment may take; it takes nothing)
+        if (threadIdx.x == 0) atomicCAS(p.status, 0, 70);
+        return;
+    }
     const int op_bytes = p.panels * PANEL;  // Q, and a stage of cached rows
     unsigned char* sQ = smem;
     unsigned char* sC = smem + op_bytes;
@@ -267,7 +295,10 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         mbar_init(&bar.o_empty, NSOFT);
         mbar_init(&bar.p_full, NSOFT);
         mbar_init(&bar.drain, 1);
-        for (int s = 0; s < MAX_STAGES; ++s) { mbar_init(&bar.k_full[s], 1); mbar_init(&bar.k_empty[s], 1); }
+        for (int s = 0; s < MAX_STAGES * GROUPS; ++s) {
+            mbar_init(&bar.k_full[0][0] + s, 1);
+            mbar_init(&bar.k_empty[0][0] + s, 1);
+        }
         for (int s = 0; s < 2; ++s) mbar_init(&bar.s_full[s], 1);
         bar.abort = 0;
         fence_mbar_init();
@@ -287,8 +318,9 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (lane == 0) {
             prefetch_tmap(&tmQ);
             prefetch_tmap(&tmC);
+            const int groups = p.panels > 5 ? 2 : 1;
             bool ok = true;
-            int u = 0, nseg = 0;  // tiles and segments started
+            int u = 0, nseg = 0, loads = 0;  // tiles and segments started, groups loaded
             int64_t pos = begin;
             for (int k = k_first, off = off_first; pos < end && ok; ++k, off = 0) {
                 const Item it = item_of(p, k, P, np);
@@ -297,17 +329,22 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 if (it.empty) continue;
                 for (int t = off; t < off + n && ok; ++t, ++u) {
                     const int s = u % p.stages;
-                    if (u >= p.stages) ok = mbar_wait(&bar.k_empty[s], ((u / p.stages) - 1) & 1, p.status, 71);
-                    if (!ok || *abort_flag) { ok = false; break; }
-                    mbar_expect_tx(&bar.k_full[s], op_bytes);
                     const bool pre = t < it.nt_pre;
                     const CUtensorMap* tm = pre ? &tmCp : &tmC;
                     const int row = (pre ? t : t - it.nt_pre) * KT, b = pre ? 0 : it.b;
-                    for (int a = 0; a < p.panels; ++a)
-                        tma_load_4d(sC + s * op_bytes + a * PANEL, tm, a * 64, row, b, 0, &bar.k_full[s]);
+                    for (int g = 0; g < groups; ++g) {
+                        if (u >= p.stages) ok = mbar_wait(&bar.k_empty[s][g], ((u / p.stages) - 1) & 1, p.status, 71);
+                        if (!ok || *abort_flag) { ok = false; break; }
+                        const int first = 4 * g, last = g + 1 < groups ? 4 : p.panels;
+                        mbar_expect_tx(&bar.k_full[s][g], (last - first) * PANEL);
+                        for (int a = first; a < last; ++a)
+                            tma_load_4d(sC + s * op_bytes + a * PANEL, tm, a * 64, row, b, 0, &bar.k_full[s][g]);
+                        ++loads;
+                    }
+                    if (!ok) break;
                     if (t == off) {  // the segment's query rows, once the last one's have been read
                         if (nseg > 0) ok = mbar_wait(&bar.q_empty, (nseg - 1) & 1, p.status, 72);
-                        if (!ok || *abort_flag) { ok = false; ++u; break; }
+                        if (!ok || *abort_flag) { ok = false; break; }
                         mbar_expect_tx(&bar.q_full, it.rows() * 128 * p.panels);
                         for (int a = 0; a < p.panels; ++a)
                             tma_load_4d(sQ + a * PANEL, it.pre ? &tmQp : &tmQ, a * 64, it.h0, it.i0, it.b, &bar.q_full);
@@ -318,68 +355,110 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (!ok) *abort_flag = 1;
             if (*abort_flag) {  // our copies in flight end before the CTA does
                 if (nseg > 0) mbar_wait(&bar.q_full, (nseg - 1) & 1, nullptr, 0);
-                for (int v = max(0, u - p.stages); v < u; ++v) mbar_wait(&bar.k_full[v % p.stages], (v / p.stages) & 1, nullptr, 0);
+                for (int v = max(0, loads - p.stages * groups); v < loads; ++v)
+                    mbar_wait(&bar.k_full[v / groups % p.stages][v % groups], (v / groups / p.stages) & 1, nullptr, 0);
             }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            const uint64_t qd = desc_sw128(smem_u32(sQ), 16, 1024);
-            const uint64_t cd = desc_sw128(smem_u32(sC), 16, 1024);
-            const uint64_t vd = desc_sw128(smem_u32(sC), PANEL, 1024);
-            const uint64_t pd = desc_sw128(smem_u32(sP), PANEL, 1024);
-            const int k_steps = (p.R + p.Dr) / 16, m_tiles = (p.R + 127) / 128;
-            bool ok = true;
-            int u = 0, nseg = 0;
-            int64_t pos = begin;
-            auto issue_s = [&](int v, uint32_t n16) -> bool {
-                const int s = v % p.stages;
-                if (!mbar_wait(&bar.k_full[s], (v / p.stages) & 1, p.status, 73)) return false;
+        const bool lead = elect_lane();
+        const uint32_t tm = uniform(tmem);
+        const uint32_t qd = (uint32_t)desc_sw128(smem_u32(sQ), 16, 1024), cd = (uint32_t)desc_sw128(smem_u32(sC), 16, 1024);
+        const uint32_t vd = (uint32_t)desc_sw128(smem_u32(sC), PANEL, 1024), pd = (uint32_t)desc_sw128(smem_u32(sP), PANEL, 1024);
+        const int rope_steps = p.Dr / 16, m_tiles = (p.R + 127) / 128;
+        bool ok = true;
+        int nseg = 0, left = (int)uniform((uint32_t)(end - begin)), k = (int)uniform(k_first), off = (int)uniform(off_first);
+        int s_stage = 0, s_phase = 0, pv_stage = 0;  // stage and phase of the next scores, stage of the next second product
+        int u = 0;                                   // tiles whose second product is issued
+        auto issue_s = [&](int v, uint32_t idesc) -> bool {
+            const uint32_t a = uniform(cd + s_stage * (op_bytes >> 4)), dst = tm + (v & 1) * NR;
+            for (int g = 0; 4 * g < p.panels - 1; ++g) {
+                if (!warp_wait(&bar.k_full[s_stage][g], s_phase, p.status, 73)) return false;
                 tc_fence_after();
-                const uint32_t idesc = idesc_f16(KT, 0, BF16, false) | (n16 >> 3 << 17);
-                const uint64_t a = desc_advance(cd, s * op_bytes);
-                for (int kk = 0; kk < k_steps; ++kk) {
-                    const uint32_t o = (uint32_t)((kk >> 2) * PANEL + (kk & 3) * 32);
-                    mma_ss(tmem + (v & 1) * NR, desc_advance(a, o), desc_advance(qd, o), idesc, kk > 0);
-                }
-                mma_commit(&bar.s_full[v & 1]);
-                return true;
-            };
-            for (int k = k_first, off = off_first; pos < end && ok; ++k, off = 0) {
-                const Item it = item_of(p, k, P, np);
-                const int n = (int)min((int64_t)(it.nt - off), end - pos);
-                pos += n;
-                if (it.empty) continue;
-                const uint32_t n16 = (it.rows() + 15) & ~15;
-                const uint32_t idesc_pv = idesc_f16_amn(128, 0, BF16, true) | (n16 >> 3 << 17);
-                ok = mbar_wait(&bar.q_full, nseg & 1, p.status, 74) && issue_s(u, n16);
-                if (ok && n == 1) mma_commit(&bar.q_empty);
-                for (int t = 0; t < n && ok; ++t, ++u) {
-                    if (t + 1 < n) {
-                        ok = issue_s(u + 1, n16);
-                        if (!ok) break;
-                        if (t + 2 == n) mma_commit(&bar.q_empty);
+                if (lead) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (4 * g + i < p.panels - 1) {
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                const uint32_t o = (4 * g + i) * (PANEL >> 4) + kk * 2;
+                                mma(dst, a + o, qd + o, idesc, i > 0 || kk > 0 || g > 0);
+                            }
+                        }
                     }
-                    ok = mbar_wait(&bar.p_full, u & 1, p.status, 75);
-                    // the segment's first product overwrites O^T: the last one's epilogue must have read it
-                    if (ok && t == 0 && nseg > 0) ok = mbar_wait(&bar.o_empty, (nseg - 1) & 1, p.status, 76);
-                    if (!ok || *abort_flag) { ok = false; break; }
-                    tc_fence_after();
-                    const uint64_t a = desc_advance(vd, (u % p.stages) * op_bytes);
-                    for (int m = 0; m < m_tiles; ++m)
-                        for (int kk = 0; kk < KT / 16; ++kk)
-                            mma_ss(tmem + O_COL + m * NR, desc_advance(a, m * 2 * PANEL + kk * 2048), desc_advance(pd, kk * 2048),
-                                   idesc_pv, t > 0 || kk > 0);
-                    mma_commit(&bar.k_empty[u % p.stages]);
+                }
+            }
+            if (lead) {  // the rotary keys
+                for (int kk = 0; kk < rope_steps; ++kk) {
+                    const uint32_t o = (p.panels - 1) * (PANEL >> 4) + kk * 2;
+                    mma(dst, a + o, qd + o, idesc, 1);
+                }
+            }
+            if (lead) {
+                mma_commit(&bar.s_full[v & 1]);
+            }
+            if (++s_stage == p.stages) s_stage = 0, s_phase ^= 1;
+            return true;
+        };
+        for (; left > 0 && ok; ++k, off = 0) {
+            const Item it = item_of(p, k, P, np);
+            const int n = (int)uniform(min(it.nt - off, left));
+            left -= n;
+            if (uniform(it.empty)) continue;
+            const uint32_t n16 = uniform((it.rows() + 15) & ~15);
+            const uint32_t idesc_s = idesc_f16(KT, 0, BF16, false) | (n16 >> 3 << 17);
+            const uint32_t idesc_pv = idesc_f16_amn(128, 0, BF16, true) | (n16 >> 3 << 17);
+            ok = warp_wait(&bar.q_full, nseg & 1, p.status, 74) && issue_s(u, idesc_s);
+            if (ok && n == 1 && lead) mma_commit(&bar.q_empty);
+            for (int t = 0; t < n && ok; ++t, ++u) {
+                // the next tile's scores and this tile's second product, whichever can start first (waiting for the next
+                // tile's load here would keep this one's stage from the producer)
+                bool next = t + 1 < n;
+                auto issue_next = [&]() {
+                    ok = issue_s(u + 1, idesc_s);
+                    if (ok && t + 2 == n && lead) mma_commit(&bar.q_empty);
+                    next = false;
+                };
+                const long long t0 = clock64();
+                for (;;) {
+                    if (next && __all_sync(~0u, mbar_test(&bar.k_full[s_stage][0], s_phase))) issue_next();
+                    if (!ok || __all_sync(~0u, mbar_test(&bar.p_full, u & 1))) break;
+                    if (__any_sync(~0u, clock64() - t0 > WAIT_LIMIT)) {
+                        if (lead) atomicCAS(p.status, 0, 75);
+                        ok = false;
+                    }
+                }
+                // the segment's first product overwrites O^T: the last one's epilogue must have read it
+                if (ok && t == 0 && nseg > 0) ok = warp_wait(&bar.o_empty, (nseg - 1) & 1, p.status, 76);
+                if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t a = uniform(vd + pv_stage * (op_bytes >> 4));
+                if (lead) {
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        if (m < m_tiles) {
+#pragma unroll
+                            for (int kk = 0; kk < KT / 16; ++kk)
+                                mma(tm + O_COL + m * NR, a + m * (2 * PANEL >> 4) + kk * 128, pd + kk * 128, idesc_pv, t > 0 || kk > 0);
+                            if (m == 1 && m_tiles > 2) mma_commit(&bar.k_empty[pv_stage][0]);
+                        }
+                    }
+                    mma_commit(&bar.k_empty[pv_stage][(m_tiles - 1) >> 1]);
                     mma_commit(&bar.pv_done);
                 }
-                ++nseg;
+                if (++pv_stage == p.stages) pv_stage = 0;
+                if (next) {
+                    issue_next();
+                    if (!ok) break;
+                }
             }
-            if (!ok) *abort_flag = 1;
-            if (*abort_flag) {
-                mma_commit(&bar.drain);
-                mbar_wait(&bar.drain, 0, nullptr, 0);
-            }
+            ++nseg;
+        }
+        if (!ok) *abort_flag = 1;
+        __syncwarp();
+        if (__any_sync(~0u, *abort_flag)) {
+            if (lead) mma_commit(&bar.drain);
+            warp_wait(&bar.drain, 0, nullptr, 0);
         }
     } else if (warp >= 4) {
         // ------------------------------------------------------------ softmax, rescaling, epilogue
@@ -784,9 +863,10 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
         return -1;
     }
     p.panels = p.R / 64 + 1;
-    const int op = p.panels * PANEL, fixed = op + PANEL + (int)sizeof(Extra) + 1024;
+    const int op = p.panels * PANEL, fixed = op + PANEL + (int)sizeof(Extra);
     p.stages = std::min(MAX_STAGES, (SMEM_MAX - fixed) / op);
-    const size_t smem = fixed + p.stages * op;
+    const size_t smem = std::min(SMEM_MAX, fixed + p.stages * op + 1023);
+    p.slack = (int)smem - (fixed + p.stages * op);
 
     const int64_t tiles_seq = (a.c.Smax + KT - 1) / KT + (p.prefix_lens ? (p.prefix_max + KT - 1) / KT : 0);
     const int grid = (int)std::min<int64_t>(n_sm, items * std::max<int64_t>(tiles_seq, 1));
