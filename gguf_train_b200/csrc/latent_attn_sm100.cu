@@ -9,13 +9,13 @@
 // 128 rows, and leave none for S). The same tile in shared memory is the A operand of both products. P^T goes
 // through 8 KB of shared memory, rows = keys.
 //
-// Warps: 0 TMA producer, 1 TMEM owner and MMA issuer (one thread), 2-3 idle, 4-11 softmax and epilogue. S^T uses 16 lanes
+// Warps: 0 TMA producer, 1 issues the first products (and owns TMEM), 2 the second ones, 3 idle, 4-11 softmax and epilogue. S^T uses 16 lanes
 // of each TMEM quadrant; a softmax warp reads its quadrant's 16 keys in the 16x256b shape (a thread has two keys of
 // four column pairs), warps 4-7 the even groups of 8 columns, 8-11 the odd ones. The exponent's offset of a query row is
 // raised only when a score exceeds it by more than 2^8, so most tiles need no maximum: one vote over the block (a
 // barrier with a reduction) finds that no row grew. Sums stay with each thread until a segment's end.
-// The next tile's scores are formed while this one's weights are, unless its load is late: then the second product comes first and
-// frees its stage. Panels are loaded and freed in two groups, as the second product goes through them.
+// Two warps issue so that neither kind of product waits behind one of the other kind that cannot start yet. A tile's panels are loaded
+// and freed in two groups, as the second product goes through them.
 //
 // Work: an item is a block of query rows (tokens x heads of one sequence) over the rows it attends. All items' tiles
 // in a row are cut into equal shares, one a CTA, so ragged lengths balance and a long sequence is split where there are
@@ -51,7 +51,7 @@ constexpr uint32_t O_COL = 2 * NR;     // S^T buffers at 0 and 64, O^T of dims 1
 constexpr int SMEM_MAX = 232448;
 
 struct Bars {
-    uint64_t q_full, q_empty, pv_done, o_empty, p_full, drain;
+    uint64_t q_full, q_empty, pv_done, o_empty, p_full, drain[2], s_free[2];
     uint64_t k_full[MAX_STAGES][GROUPS], k_empty[MAX_STAGES][GROUPS], s_full[2];
     uint32_t tmem;
     int abort;
@@ -176,11 +176,22 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* s
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
 }
 
-// 16 lanes x 8 columns of 32 bits: thread t gets (lane t/4, columns 2 (t%4), +1) and (lane t/4 + 8, the same columns)
-__device__ __forceinline__ void tmem_ld_16x8(uint32_t taddr, uint32_t* r) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(taddr));
+// 16 lanes x 8 n columns of 32 bits (n 1 to 4): of each 8 columns, thread t gets (lane t/4, columns 2 (t%4), +1) and (lane t/4 + 8, the
+// same columns)
+__device__ __forceinline__ void tmem_ld_16(int n, uint32_t taddr, uint32_t* r) {
+    if (n == 1)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(taddr));
+    else if (n == 2)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                     : "r"(taddr));
+    else  // (of 3 too: the columns behind are allocated, and dropped)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                       "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                     : "r"(taddr));
 }
 
 // The lane that issues the MMA warp's products and commits. The whole warp goes through the loops around them without diverging,
@@ -292,14 +303,17 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         mbar_init(&bar.q_full, 1);
         mbar_init(&bar.q_empty, 1);
         mbar_init(&bar.pv_done, 1);
-        mbar_init(&bar.o_empty, NSOFT);
-        mbar_init(&bar.p_full, NSOFT);
-        mbar_init(&bar.drain, 1);
+        mbar_init(&bar.o_empty, NSOFT / 32);
+        mbar_init(&bar.p_full, NSOFT / 32);
         for (int s = 0; s < MAX_STAGES * GROUPS; ++s) {
             mbar_init(&bar.k_full[0][0] + s, 1);
             mbar_init(&bar.k_empty[0][0] + s, 1);
         }
-        for (int s = 0; s < 2; ++s) mbar_init(&bar.s_full[s], 1);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&bar.s_full[s], 1);
+            mbar_init(&bar.s_free[s], NSOFT / 32);
+            mbar_init(&bar.drain[s], 1);
+        }
         bar.abort = 0;
         fence_mbar_init();
     }
@@ -359,97 +373,80 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     mbar_wait(&bar.k_full[v / groups % p.stages][v % groups], (v / groups / p.stages) & 1, nullptr, 0);
             }
         }
-    } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA issuer
-        const bool lead = elect_lane();
+    } else if (warp < 3) {
+        // ------------------------------------------------------------ MMA issuers: 1 the scores, 2 the second products
+        const bool scores = warp == 1, lead = elect_lane();
         const uint32_t tm = uniform(tmem);
         const uint32_t qd = (uint32_t)desc_sw128(smem_u32(sQ), 16, 1024), cd = (uint32_t)desc_sw128(smem_u32(sC), 16, 1024);
         const uint32_t vd = (uint32_t)desc_sw128(smem_u32(sC), PANEL, 1024), pd = (uint32_t)desc_sw128(smem_u32(sP), PANEL, 1024);
         const int rope_steps = p.Dr / 16, m_tiles = (p.R + 127) / 128;
         bool ok = true;
         int nseg = 0, left = (int)uniform((uint32_t)(end - begin)), k = (int)uniform(k_first), off = (int)uniform(off_first);
-        int s_stage = 0, s_phase = 0, pv_stage = 0;  // stage and phase of the next scores, stage of the next second product
-        int u = 0;                                   // tiles whose second product is issued
-        auto issue_s = [&](int v, uint32_t idesc) -> bool {
-            const uint32_t a = uniform(cd + s_stage * (op_bytes >> 4)), dst = tm + (v & 1) * NR;
-            for (int g = 0; 4 * g < p.panels - 1; ++g) {
-                if (!warp_wait(&bar.k_full[s_stage][g], s_phase, p.status, 73)) return false;
-                tc_fence_after();
-                if (lead) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (4 * g + i < p.panels - 1) {
-#pragma unroll
-                            for (int kk = 0; kk < 4; ++kk) {
-                                const uint32_t o = (4 * g + i) * (PANEL >> 4) + kk * 2;
-                                mma(dst, a + o, qd + o, idesc, i > 0 || kk > 0 || g > 0);
-                            }
-                        }
-                    }
-                }
-            }
-            if (lead) {  // the rotary keys
-                for (int kk = 0; kk < rope_steps; ++kk) {
-                    const uint32_t o = (p.panels - 1) * (PANEL >> 4) + kk * 2;
-                    mma(dst, a + o, qd + o, idesc, 1);
-                }
-            }
-            if (lead) {
-                mma_commit(&bar.s_full[v & 1]);
-            }
-            if (++s_stage == p.stages) s_stage = 0, s_phase ^= 1;
-            return true;
-        };
+        int u = 0, stage = 0, phase = 0;  // tiles so far, the next one's stage and its phase
         for (; left > 0 && ok; ++k, off = 0) {
             const Item it = item_of(p, k, P, np);
             const int n = (int)uniform(min(it.nt - off, left));
             left -= n;
             if (uniform(it.empty)) continue;
             const uint32_t n16 = uniform((it.rows() + 15) & ~15);
-            const uint32_t idesc_s = idesc_f16(KT, 0, BF16, false) | (n16 >> 3 << 17);
-            const uint32_t idesc_pv = idesc_f16_amn(128, 0, BF16, true) | (n16 >> 3 << 17);
-            ok = warp_wait(&bar.q_full, nseg & 1, p.status, 74) && issue_s(u, idesc_s);
-            if (ok && n == 1 && lead) mma_commit(&bar.q_empty);
-            for (int t = 0; t < n && ok; ++t, ++u) {
-                // the next tile's scores and this tile's second product, whichever can start first (waiting for the next
-                // tile's load here would keep this one's stage from the producer)
-                bool next = t + 1 < n;
-                auto issue_next = [&]() {
-                    ok = issue_s(u + 1, idesc_s);
-                    if (ok && t + 2 == n && lead) mma_commit(&bar.q_empty);
-                    next = false;
-                };
-                const long long t0 = clock64();
-                for (;;) {
-                    if (next && __all_sync(~0u, mbar_test(&bar.k_full[s_stage][0], s_phase))) issue_next();
-                    if (!ok || __all_sync(~0u, mbar_test(&bar.p_full, u & 1))) break;
-                    if (__any_sync(~0u, clock64() - t0 > WAIT_LIMIT)) {
-                        if (lead) atomicCAS(p.status, 0, 75);
-                        ok = false;
-                    }
-                }
-                // the segment's first product overwrites O^T: the last one's epilogue must have read it
-                if (ok && t == 0 && nseg > 0) ok = warp_wait(&bar.o_empty, (nseg - 1) & 1, p.status, 76);
-                if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t a = uniform(vd + pv_stage * (op_bytes >> 4));
-                if (lead) {
+            if (scores) {
+                const uint32_t idesc = idesc_f16(KT, 0, BF16, false) | (n16 >> 3 << 17);
+                ok = warp_wait(&bar.q_full, nseg & 1, p.status, 74);
+                for (int t = 0; t < n && ok; ++t, ++u) {
+                    if (u >= 2) ok = warp_wait(&bar.s_free[u & 1], ((u >> 1) - 1) & 1, p.status, 75);
+                    if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
+                    const uint32_t a = uniform(cd + stage * (op_bytes >> 4)), dst = tm + (u & 1) * NR;
+                    for (int g = 0; 4 * g < p.panels - 1; ++g) {
+                        ok = warp_wait(&bar.k_full[stage][g], phase, p.status, 73);
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (lead) {
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) {
-                        if (m < m_tiles) {
+                            for (int i = 0; i < 4; ++i) {
+                                if (4 * g + i < p.panels - 1) {
 #pragma unroll
-                            for (int kk = 0; kk < KT / 16; ++kk)
-                                mma(tm + O_COL + m * NR, a + m * (2 * PANEL >> 4) + kk * 128, pd + kk * 128, idesc_pv, t > 0 || kk > 0);
-                            if (m == 1 && m_tiles > 2) mma_commit(&bar.k_empty[pv_stage][0]);
+                                    for (int kk = 0; kk < 4; ++kk) {
+                                        const uint32_t o = (4 * g + i) * (PANEL >> 4) + kk * 2;
+                                        mma(dst, a + o, qd + o, idesc, i > 0 || kk > 0 || g > 0);
+                                    }
+                                }
+                            }
                         }
                     }
-                    mma_commit(&bar.k_empty[pv_stage][(m_tiles - 1) >> 1]);
-                    mma_commit(&bar.pv_done);
-                }
-                if (++pv_stage == p.stages) pv_stage = 0;
-                if (next) {
-                    issue_next();
                     if (!ok) break;
+                    if (lead) {  // the rotary keys
+                        for (int kk = 0; kk < rope_steps; ++kk) {
+                            const uint32_t o = (p.panels - 1) * (PANEL >> 4) + kk * 2;
+                            mma(dst, a + o, qd + o, idesc, 1);
+                        }
+                        mma_commit(&bar.s_full[u & 1]);
+                        if (t + 1 == n) mma_commit(&bar.q_empty);
+                    }
+                    if (++stage == p.stages) stage = 0, phase ^= 1;
+                }
+            } else {
+                const uint32_t idesc = idesc_f16_amn(128, 0, BF16, true) | (n16 >> 3 << 17);
+                // the segment's first product overwrites O^T: the last one's epilogue must have read it
+                if (nseg > 0) ok = warp_wait(&bar.o_empty, (nseg - 1) & 1, p.status, 76);
+                for (int t = 0; t < n && ok; ++t, ++u) {
+                    ok = warp_wait(&bar.p_full, u & 1, p.status, 81);
+                    if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t a = uniform(vd + stage * (op_bytes >> 4));
+                    if (lead) {
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) {
+                            if (m < m_tiles) {
+#pragma unroll
+                                for (int kk = 0; kk < KT / 16; ++kk)
+                                    mma(tm + O_COL + m * NR, a + m * (2 * PANEL >> 4) + kk * 128, pd + kk * 128, idesc, t > 0 || kk > 0);
+                                if (m == 1 && m_tiles > 2) mma_commit(&bar.k_empty[stage][0]);
+                            }
+                        }
+                        mma_commit(&bar.k_empty[stage][(m_tiles - 1) >> 1]);
+                        mma_commit(&bar.pv_done);
+                    }
+                    if (++stage == p.stages) stage = 0;
                 }
             }
             ++nseg;
@@ -457,8 +454,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (!ok) *abort_flag = 1;
         __syncwarp();
         if (__any_sync(~0u, *abort_flag)) {
-            if (lead) mma_commit(&bar.drain);
-            warp_wait(&bar.drain, 0, nullptr, 0);
+            if (lead) mma_commit(&bar.drain[warp - 1]);
+            warp_wait(&bar.drain[warp - 1], 0, nullptr, 0);
         }
     } else if (warp >= 4) {
         // ------------------------------------------------------------ softmax, rescaling, epilogue
@@ -495,17 +492,18 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 const int valid = (pre ? P : it.len) - row0;  // cached rows of the tile
                 if (ok) ok = warp_wait(&bar.s_full[u & 1], (u >> 1) & 1, p.status, 77);
                 tc_fence_after();
-                uint32_t raw[4][4];
+                uint32_t raw[16];
                 float (*x)[4] = (float(*)[4])raw;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < gl) tmem_ld_16x8(tmem + lane_addr + (u & 1) * NR + 8 * (2 * j + half), raw[j]);
+                tmem_ld_16(gl, tmem + lane_addr + (u & 1) * NR + 8 * half * gl, raw);
                 tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.s_free[u & 1]);
                 if (pre ? valid < KT : row0 + KT - 1 > lim_min) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         if (j >= gl) continue;
-                        const int c = 8 * (2 * j + half) + cpair;
+                        const int c = 8 * (half * gl + j) + cpair;
                         // (rows that attend nothing take the others' way and are dropped at the end)
                         const int l0 = pre ? P - 1 : max(ex.lim[c], -1), l1 = pre ? P - 1 : max(ex.lim[c + 1], -1);
                         if (row0 + key0 > l0) x[j][0] = -INFINITY;
@@ -536,7 +534,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                             v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
                             v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
                             v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
-                            if (lane < 4) ex.exch[quad][8 * (2 * j + half) + cpair + c] = v;
+                            if (lane < 4) ex.exch[quad][8 * (half * gl + j) + cpair + c] = v;
                         }
                     }
                     soft_sync();
@@ -545,7 +543,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         if (j >= gl) continue;
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const int col = 8 * (2 * j + half) + cpair + c;
+                            const int col = 8 * (half * gl + j) + cpair + c;
                             const float v = fmaxf(fmaxf(ex.exch[0][col], ex.exch[1][col]), fmaxf(ex.exch[2][col], ex.exch[3][col]));
                             const float mn = fmaxf(m[j][c], v);
                             const float al = mn == m[j][c] ? 1.0f : ex2(m[j][c] - mn);
@@ -589,7 +587,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (j >= gl) continue;
-                    unsigned char* d = sP + key0 * 128 + (((2 * j + half) ^ (key0 & 7)) << 4) + cpair * 2;
+                    unsigned char* d = sP + key0 * 128 + (((half * gl + j) ^ (key0 & 7)) << 4) + cpair * 2;
                     *(uint32_t*)d = w[j][0];
                     *(uint32_t*)(d + 8 * 128) = w[j][1];
                 }
@@ -603,7 +601,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
                 fence_proxy_async_smem();
                 tc_fence_before();
-                mbar_arrive(&bar.p_full);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.p_full);
             }
             // ---- the segment's rows: sums over the quadrants, then O^T a latent dim a lane
 #pragma unroll
@@ -615,8 +614,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     v += __shfl_xor_sync(~0u, v, 4);
                     v += __shfl_xor_sync(~0u, v, 8);
                     v += __shfl_xor_sync(~0u, v, 16);
-                    if (lane < 4) ex.exch[quad][8 * (2 * j + half) + cpair + c] = v;
-                    if (quad == 0 && lane < 4) ex.alpha[8 * (2 * j + half) + cpair + c] = m[j][c];
+                    if (lane < 4) ex.exch[quad][8 * (half * gl + j) + cpair + c] = v;
+                    if (quad == 0 && lane < 4) ex.alpha[8 * (half * gl + j) + cpair + c] = m[j][c];
                 }
             }
             soft_sync();
@@ -664,7 +663,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
             }
             tc_fence_before();
-            if (!it.empty) mbar_arrive(&bar.o_empty);
+            __syncwarp();
+            if (!it.empty && lane == 0) mbar_arrive(&bar.o_empty);
         }
         if (!ok) *abort_flag = 1;
     }
