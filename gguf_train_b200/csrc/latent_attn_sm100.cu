@@ -28,6 +28,7 @@
 // waiting after a timeout so that none is left behind.
 
 #include <algorithm>
+#include <atomic>
 
 #include "gtb_common.cuh"
 #include "latent.h"
@@ -45,26 +46,26 @@ constexpr int PANEL = KT * 128;        // bytes of 64 rows x 64 columns
 constexpr int NTHREADS = 384;
 constexpr int NSOFT = 256;             // threads of the softmax warps
 constexpr int MAX_STAGES = 6;
-constexpr int GROUPS = 2;              // panels 0 .. 3 and the others: what is loaded, and freed, at once
+constexpr int GROUP = 4;               // panels of a tile's first group; the others (if there are more than 5) are a second one
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t O_COL = 2 * NR;     // S^T buffers at 0 and 64, O^T of dims 128 t .. at O_COL + 64 t
 constexpr int SMEM_MAX = 232448;
 
 struct Bars {
     uint64_t q_full, q_empty, pv_done, o_empty, p_full, drain[2], s_free[2];
-    uint64_t k_full[MAX_STAGES][GROUPS], k_empty[MAX_STAGES][GROUPS], s_full[2];
+    uint64_t k_full[2][MAX_STAGES], k_empty[2][MAX_STAGES], s_full[2];
     uint32_t tmem;
     int abort;
 };
 
 struct Extra {                 // what lies behind the operands in shared memory
+    float alpha[NR];           // factor of a row's sums; at the end 1 / sum
+    int out_row[NR];           // row of the output, -1: none
+    int lim[NR];               // last own row a query row attends; DEAD: it attends nothing
+    float exch[4][NR];         // a quadrant's maxima, later its sums
     Bars bars;
     int64_t line, warp_sum[NTHREADS / 32];  // finding the CTA's share
     int first_item, first_tile;
-    float exch[4][NR];         // a quadrant's maxima, later its sums
-    float alpha[NR];           // factor of a row's sums; at the end 1 / sum
-    int lim[NR];               // last own row a query row attends; DEAD: it attends nothing
-    int out_row[NR];           // row of the output, -1: none
 };
 
 constexpr int DEAD = INT_MIN;
@@ -75,16 +76,18 @@ struct Params {
     int B, H, Lq, R, Dr;
     int hh, ii, n_h, n_rt;     // heads and tokens of an item, items along the heads, items a sequence
     int bb, n_pre;             // sequences of a prefix item (0: the prefix's tiles belong to the own items), prefix items
-    int panels, stages, slack;
+    int panels, n_groups;
+    int q_pitch;               // bytes of a panel of Q
+    int group_bytes[2], stages[2], slack;
     float scale_log2;
     void* o;
     float* lse;
-    float* part_o;             // [slot][row][R]
+    float* part_o;             // [slot][dim][pitch], a row a column
     float2* part_ml;           // [slot][row]: offset, sum
-    int64_t* item_pos;         // first tile of an own item on the line (split prefix only)
-    int2* cta_item;            // item and tile within it that a CTA begins at
+    int4* joins;               // items that more than one CTA worked on, by the CTA that begins them; with a split prefix, by item:
+                               // item (-1: none), first CTA, last CTA
     int64_t* line;             // [0] tiles in all, [1] CTAs in use
-    int own_rows;              // rows a slot of an own item
+    int own_pitch;             // rows a slot of an own item, a multiple of 16
     int64_t own_base;          // first float of own slots in part_o (split prefix)
     int* status;
 };
@@ -142,6 +145,14 @@ __device__ __forceinline__ Item item_of(const Params& p, int k, int P, int np) {
 
 __device__ __forceinline__ int64_t share(int64_t line, int n, int c) { return line * c / n; }
 
+// the CTA whose share holds tile x
+__device__ __forceinline__ int cta_of(int64_t line, int n, int64_t x) {
+    int c = (int)min((int64_t)n - 1, x * n / line);
+    while (c + 1 < n && share(line, n, c + 1) <= x) ++c;
+    while (share(line, n, c) > x) --c;
+    return c;
+}
+
 // query row `col` of an item: (sequence, token, head), false where there is none
 __device__ __forceinline__ bool row_of(const Params& p, const Item& it, int col, int& b, int& i, int& h) {
     const int r = col / it.nh;
@@ -156,10 +167,10 @@ __device__ __forceinline__ bool row_of(const Params& p, const Item& it, int col,
 __device__ __forceinline__ void slot_of(const Params& p, int k, int np, int c, bool head, int64_t& o, int64_t& ml) {
     if (!p.bb) {  // a CTA leaves at most two: of the item it begins within, and of the one that it ends within
         const int64_t s = 2 * c + (head ? 1 : 0);
-        o = s * p.own_rows * p.R;
+        o = s * p.own_pitch * p.R;
         ml = s * NR;
     } else {      // (a step along the line changes the item or the CTA: k + c names the segment)
-        o = k < np ? (int64_t)(k + c) * NR * p.R : p.own_base + (int64_t)(k - np + c) * p.own_rows * p.R;
+        o = k < np ? (int64_t)(k + c) * NR * p.R : p.own_base + (int64_t)(k - np + c) * p.own_pitch * p.R;
         ml = (int64_t)(k + c) * NR;
     }
 }
@@ -240,10 +251,10 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (threadIdx.x == 0) atomicCAS(p.status, 0, 70);
         return;
     }
-    const int op_bytes = p.panels * PANEL;  // Q, and a stage of cached rows
     unsigned char* sQ = smem;
-    unsigned char* sC = smem + op_bytes;
-    unsigned char* sP = sC + p.stages * op_bytes;
+    unsigned char* sC = smem + p.panels * p.q_pitch;  // the stages of the first group, then of the second
+    unsigned char* sC1 = sC + p.stages[0] * p.group_bytes[0];
+    unsigned char* sP = sC1 + p.stages[1] * p.group_bytes[1];
     Extra& ex = *(Extra*)(sP + PANEL);
     Bars& bar = ex.bars;
 
@@ -252,26 +263,11 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const int n_items = np + p.B * p.n_rt;
 
     // ---------------------------------------------------------------- this CTA's share of the line of tiles
-    if (threadIdx.x == 0) ex.line = 0;
-    __syncthreads();
-    {
-        int64_t mine = 0;
-        for (int k = threadIdx.x; k < n_items; k += NTHREADS) mine += item_of(p, k, P, np).nt;
-        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
-        if (lane == 0) atomicAdd((unsigned long long*)&ex.line, (unsigned long long)mine);
-    }
-    __syncthreads();
-    const int64_t line = ex.line;
-    const int n_cta = (int)min((int64_t)gridDim.x, line);
-    if (cta == 0 && threadIdx.x == 0) {
-        p.line[0] = line;
-        p.line[1] = n_cta;
-    }
-    if (cta >= n_cta) return;
-    const int64_t begin = share(line, n_cta, cta), end = share(line, n_cta, cta + 1);
-    {
-        int64_t before = 0;
-        for (int k0 = 0;; k0 += NTHREADS) {
+    // (NTHREADS items a round; where that is all of them, their tiles are counted once)
+    int64_t line = 0, begin = 0, end = 0, before = 0;
+    int n_cta = 1;
+    for (int pass = n_items > NTHREADS ? 0 : 1; pass < 2; ++pass) {
+        for (int k0 = 0; k0 < n_items; k0 += NTHREADS) {
             const int k = k0 + (int)threadIdx.x;
             const int64_t n = k < n_items ? item_of(p, k, P, np).nt : 0;
             int64_t incl = n;
@@ -287,17 +283,30 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 total += ex.warp_sum[w];
             }
             incl += before;
-            if (begin >= incl - n && begin < incl) {
-                ex.first_item = k;
-                ex.first_tile = (int)(begin - (incl - n));
-            }
             before += total;
+            if (pass == 1) {
+                if (n_items <= NTHREADS) line = before;
+                if (k0 == 0) {
+                    n_cta = (int)min((int64_t)gridDim.x, line);
+                    if (cta == 0 && threadIdx.x == 0) {
+                        p.line[0] = line;
+                        p.line[1] = n_cta;
+                    }
+                    if (cta >= n_cta) return;
+                    begin = share(line, n_cta, cta);
+                    end = share(line, n_cta, cta + 1);
+                }
+                if (begin >= incl - n && begin < incl) {
+                    ex.first_item = k;
+                    ex.first_tile = (int)(begin - (incl - n));
+                }
+            }
             __syncthreads();
-            if (begin < before) break;  // (begin < line: found by the last round)
+            if (pass == 1 && begin < before) break;  // (begin < line: found by the last round)
         }
+        if (pass == 0) line = before, before = 0;
     }
     const int k_first = ex.first_item, off_first = ex.first_tile;
-    if (threadIdx.x == 0) p.cta_item[cta] = make_int2(k_first, off_first);
 
     if (threadIdx.x == 0) {
         mbar_init(&bar.q_full, 1);
@@ -305,7 +314,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         mbar_init(&bar.pv_done, 1);
         mbar_init(&bar.o_empty, NSOFT / 32);
         mbar_init(&bar.p_full, NSOFT / 32);
-        for (int s = 0; s < MAX_STAGES * GROUPS; ++s) {
+        for (int s = 0; s < 2 * MAX_STAGES; ++s) {
             mbar_init(&bar.k_full[0][0] + s, 1);
             mbar_init(&bar.k_empty[0][0] + s, 1);
         }
@@ -318,7 +327,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         fence_mbar_init();
     }
     // query rows that no load fills stay zero (their columns are computed and dropped)
-    for (int e = threadIdx.x; e < op_bytes / 16; e += NTHREADS) ((uint4*)sQ)[e] = make_uint4(0, 0, 0, 0);
+    for (int e = threadIdx.x; e < p.panels * p.q_pitch / 16; e += NTHREADS) ((uint4*)sQ)[e] = make_uint4(0, 0, 0, 0);
     fence_proxy_async_smem();
     if (warp == 1) tmem_alloc(&bar.tmem, TMEM_COLS);
     tc_fence_before();
@@ -332,28 +341,31 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (lane == 0) {
             prefetch_tmap(&tmQ);
             prefetch_tmap(&tmC);
-            const int groups = p.panels > 5 ? 2 : 1;
             bool ok = true;
-            int u = 0, nseg = 0, loads = 0;  // tiles and segments started, groups loaded
+            int nseg = 0, loads[2] = {0, 0};  // segments started, groups loaded
+            int stage[2] = {0, 0}, phase[2] = {1, 1};
             int64_t pos = begin;
             for (int k = k_first, off = off_first; pos < end && ok; ++k, off = 0) {
                 const Item it = item_of(p, k, P, np);
                 const int n = (int)min((int64_t)(it.nt - off), end - pos);
                 pos += n;
                 if (it.empty) continue;
-                for (int t = off; t < off + n && ok; ++t, ++u) {
-                    const int s = u % p.stages;
+                for (int t = off; t < off + n && ok; ++t) {
                     const bool pre = t < it.nt_pre;
                     const CUtensorMap* tm = pre ? &tmCp : &tmC;
                     const int row = (pre ? t : t - it.nt_pre) * KT, b = pre ? 0 : it.b;
-                    for (int g = 0; g < groups; ++g) {
-                        if (u >= p.stages) ok = mbar_wait(&bar.k_empty[s][g], ((u / p.stages) - 1) & 1, p.status, 71);
-                        if (!ok || *abort_flag) { ok = false; break; }
-                        const int first = 4 * g, last = g + 1 < groups ? 4 : p.panels;
-                        mbar_expect_tx(&bar.k_full[s][g], (last - first) * PANEL);
-                        for (int a = first; a < last; ++a)
-                            tma_load_4d(sC + s * op_bytes + a * PANEL, tm, a * 64, row, b, 0, &bar.k_full[s][g]);
-                        ++loads;
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        if (!ok || g >= p.n_groups) continue;
+                        const int s = stage[g];
+                        if (loads[g] >= p.stages[g]) ok = mbar_wait(&bar.k_empty[g][s], phase[g], p.status, 71);
+                        if (!ok || *abort_flag) { ok = false; continue; }
+                        mbar_expect_tx(&bar.k_full[g][s], p.group_bytes[g]);
+                        unsigned char* dst = (g ? sC1 : sC) + s * p.group_bytes[g];
+                        for (int a = 0; a < p.group_bytes[g] / PANEL; ++a)
+                            tma_load_4d(dst + a * PANEL, tm, (GROUP * g + a) * 64, row, b, 0, &bar.k_full[g][s]);
+                        ++loads[g];
+                        if (++stage[g] == p.stages[g]) stage[g] = 0, phase[g] ^= 1;
                     }
                     if (!ok) break;
                     if (t == off) {  // the segment's query rows, once the last one's have been read
@@ -361,7 +373,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         if (!ok || *abort_flag) { ok = false; break; }
                         mbar_expect_tx(&bar.q_full, it.rows() * 128 * p.panels);
                         for (int a = 0; a < p.panels; ++a)
-                            tma_load_4d(sQ + a * PANEL, it.pre ? &tmQp : &tmQ, a * 64, it.h0, it.i0, it.b, &bar.q_full);
+                            tma_load_4d(sQ + a * p.q_pitch, it.pre ? &tmQp : &tmQ, a * 64, it.h0, it.i0, it.b, &bar.q_full);
                         ++nseg;
                     }
                 }
@@ -369,20 +381,23 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (!ok) *abort_flag = 1;
             if (*abort_flag) {  // our copies in flight end before the CTA does
                 if (nseg > 0) mbar_wait(&bar.q_full, (nseg - 1) & 1, nullptr, 0);
-                for (int v = max(0, loads - p.stages * groups); v < loads; ++v)
-                    mbar_wait(&bar.k_full[v / groups % p.stages][v % groups], (v / groups / p.stages) & 1, nullptr, 0);
+                for (int g = 0; g < p.n_groups; ++g)
+                    for (int v = max(0, loads[g] - p.stages[g]); v < loads[g]; ++v)
+                        mbar_wait(&bar.k_full[g][v % p.stages[g]], (v / p.stages[g]) & 1, nullptr, 0);
             }
         }
     } else if (warp < 3) {
         // ------------------------------------------------------------ MMA issuers: 1 the scores, 2 the second products
         const bool scores = warp == 1, lead = elect_lane();
         const uint32_t tm = uniform(tmem);
-        const uint32_t qd = (uint32_t)desc_sw128(smem_u32(sQ), 16, 1024), cd = (uint32_t)desc_sw128(smem_u32(sC), 16, 1024);
-        const uint32_t vd = (uint32_t)desc_sw128(smem_u32(sC), PANEL, 1024), pd = (uint32_t)desc_sw128(smem_u32(sP), PANEL, 1024);
+        const uint32_t lead_off = scores ? 16 : PANEL;  // leading byte offset (K-major: unused)
+        const uint32_t qd = (uint32_t)desc_sw128(smem_u32(sQ), 16, 1024), pd = (uint32_t)desc_sw128(smem_u32(sP), PANEL, 1024);
+        const uint32_t cd[2] = {(uint32_t)desc_sw128(smem_u32(sC), lead_off, 1024), (uint32_t)desc_sw128(smem_u32(sC1), lead_off, 1024)};
+        const uint32_t q_step = p.q_pitch >> 4;
         const int rope_steps = p.Dr / 16, m_tiles = (p.R + 127) / 128;
         bool ok = true;
         int nseg = 0, left = (int)uniform((uint32_t)(end - begin)), k = (int)uniform(k_first), off = (int)uniform(off_first);
-        int u = 0, stage = 0, phase = 0;  // tiles so far, the next one's stage and its phase
+        int u = 0, stage[2] = {0, 0}, phase[2] = {0, 0};  // tiles so far, the next one's stages and their phases
         for (; left > 0 && ok; ++k, off = 0) {
             const Item it = item_of(p, k, P, np);
             const int n = (int)uniform(min(it.nt - off, left));
@@ -395,34 +410,35 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 for (int t = 0; t < n && ok; ++t, ++u) {
                     if (u >= 2) ok = warp_wait(&bar.s_free[u & 1], ((u >> 1) - 1) & 1, p.status, 75);
                     if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
-                    const uint32_t a = uniform(cd + stage * (op_bytes >> 4)), dst = tm + (u & 1) * NR;
-                    for (int g = 0; 4 * g < p.panels - 1; ++g) {
-                        ok = warp_wait(&bar.k_full[stage][g], phase, p.status, 73);
-                        if (!ok) break;
+                    const uint32_t dst = tm + (u & 1) * NR;
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        if (!ok || g >= p.n_groups) continue;
+                        ok = warp_wait(&bar.k_full[g][stage[g]], phase[g], p.status, 73);
+                        if (!ok) continue;
                         tc_fence_after();
+                        const uint32_t a = uniform(cd[g] + stage[g] * (p.group_bytes[g] >> 4)), q = qd + GROUP * g * q_step;
+                        const int n_val = min(GROUP, p.panels - 1 - GROUP * g);  // panels of latent values
                         if (lead) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if (4 * g + i < p.panels - 1) {
+                            for (int i = 0; i < GROUP; ++i) {
+                                if (i < n_val) {
 #pragma unroll
-                                    for (int kk = 0; kk < 4; ++kk) {
-                                        const uint32_t o = (4 * g + i) * (PANEL >> 4) + kk * 2;
-                                        mma(dst, a + o, qd + o, idesc, i > 0 || kk > 0 || g > 0);
-                                    }
+                                    for (int kk = 0; kk < 4; ++kk)
+                                        mma(dst, a + i * (PANEL >> 4) + kk * 2, q + i * q_step + kk * 2, idesc, i > 0 || kk > 0 || g > 0);
                                 }
                             }
+                            if (g + 1 == p.n_groups)  // the rotary keys
+                                for (int kk = 0; kk < rope_steps; ++kk)
+                                    mma(dst, a + n_val * (PANEL >> 4) + kk * 2, q + n_val * q_step + kk * 2, idesc, 1);
                         }
+                        if (++stage[g] == p.stages[g]) stage[g] = 0, phase[g] ^= 1;
                     }
                     if (!ok) break;
-                    if (lead) {  // the rotary keys
-                        for (int kk = 0; kk < rope_steps; ++kk) {
-                            const uint32_t o = (p.panels - 1) * (PANEL >> 4) + kk * 2;
-                            mma(dst, a + o, qd + o, idesc, 1);
-                        }
+                    if (lead) {
                         mma_commit(&bar.s_full[u & 1]);
                         if (t + 1 == n) mma_commit(&bar.q_empty);
                     }
-                    if (++stage == p.stages) stage = 0, phase ^= 1;
                 }
             } else {
                 const uint32_t idesc = idesc_f16_amn(128, 0, BF16, true) | (n16 >> 3 << 17);
@@ -432,21 +448,26 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     ok = warp_wait(&bar.p_full, u & 1, p.status, 81);
                     if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t a = uniform(vd + stage * (op_bytes >> 4));
+                    const uint32_t a0 = uniform(cd[0] + stage[0] * (p.group_bytes[0] >> 4));
+                    const uint32_t a1 = uniform(cd[1] + stage[1] * (p.group_bytes[1] >> 4));
                     if (lead) {
 #pragma unroll
                         for (int m = 0; m < 4; ++m) {
                             if (m < m_tiles) {
 #pragma unroll
                                 for (int kk = 0; kk < KT / 16; ++kk)
-                                    mma(tm + O_COL + m * NR, a + m * (2 * PANEL >> 4) + kk * 128, pd + kk * 128, idesc, t > 0 || kk > 0);
-                                if (m == 1 && m_tiles > 2) mma_commit(&bar.k_empty[stage][0]);
+                                    mma(tm + O_COL + m * NR, (m < 2 ? a0 : a1) + (m & 1) * (2 * PANEL >> 4) + kk * 128, pd + kk * 128, idesc,
+                                        t > 0 || kk > 0);
+                                if (m == 1 && p.n_groups > 1) mma_commit(&bar.k_empty[0][stage[0]]);
                             }
                         }
-                        mma_commit(&bar.k_empty[stage][(m_tiles - 1) >> 1]);
+                        if (p.n_groups > 1) mma_commit(&bar.k_empty[1][stage[1]]);
+                        else mma_commit(&bar.k_empty[0][stage[0]]);
                         mma_commit(&bar.pv_done);
                     }
-                    if (++stage == p.stages) stage = 0;
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+                        if (++stage[g] == p.stages[g]) stage[g] = 0;
                 }
             }
             ++nseg;
@@ -457,7 +478,23 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (lead) mma_commit(&bar.drain[warp - 1]);
             warp_wait(&bar.drain[warp - 1], 0, nullptr, 0);
         }
-    } else if (warp >= 4) {
+    } else if (warp == 3) {
+        // ------------------------------------------------------------ what the join kernel has to know
+        if (lane == 0) {
+            int4 mine = make_int4(-1, 0, 0, 0);
+            int64_t pos = begin;
+            for (int k = k_first, off = off_first; pos < end; ++k, off = 0) {
+                const Item it = item_of(p, k, P, np);
+                if (off == 0) {
+                    const int4 j = make_int4(it.empty ? -1 : k, cta, cta_of(line, n_cta, pos + it.nt - 1), 0);
+                    if (p.bb) p.joins[k] = j;
+                    else if (j.z > cta) mine = j;
+                }
+                pos += it.nt - off;
+            }
+            if (!p.bb) p.joins[cta] = mine;
+        }
+    } else {
         // ------------------------------------------------------------ softmax, rescaling, epilogue
         const int st = (int)threadIdx.x - 128, quad = warp & 3, half = (warp - 4) >> 2;
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
@@ -465,12 +502,11 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int cpair = 2 * (lane & 3);                  // its columns of a group: cpair, cpair + 1
         const int m_tiles = (p.R + 127) / 128;
         bool ok = true;
-        int u = 0;
+        int u = 0, stage[2] = {0, 0};
         int64_t pos = begin;
         for (int k = k_first, off = off_first; pos < end; ++k, off = 0) {
             const Item it = item_of(p, k, P, np);
             const int n = (int)min((int64_t)(it.nt - off), end - pos);
-            const int64_t item_start = pos - off;
             pos += n;
             const int gl = (it.rows() + 15) / 16;          // groups of 8 columns of this warp: 2 j + half, j < gl
             soft_sync();                                   // the last segment's lim, out_row, alpha have been read
@@ -480,7 +516,6 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 ex.out_row[st] = is ? (b * p.H + h) * p.Lq + i : -1;
                 ex.lim[st] = !is || it.pre ? INT_MAX : i >= it.cnt ? DEAD : it.len - it.cnt + i;
             }
-            if (st == 0 && p.bb && !it.pre && off == 0) p.item_pos[k - np] = item_start;
             soft_sync();
             const int lim_min = it.len - it.cnt + it.i0;   // smallest limit of a live row
             float m[4][2], l[4][2];
@@ -592,13 +627,16 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     *(uint32_t*)(d + 8 * 128) = w[j][1];
                 }
                 if (valid < KT) {  // rows past the end: 0 in the second product, whatever they hold
-                    unsigned char* base = sC + (u % p.stages) * op_bytes;
                     const int first = max(valid, 0), per = (KT - first) * 8;
                     for (int e = st; e < per * (p.R / 64); e += NSOFT) {
-                        const int a = e / per, r = e - a * per;
-                        *(uint4*)(base + a * PANEL + first * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+                        const int a = e / per, r = e - a * per, g = a >= GROUP && p.n_groups > 1;
+                        unsigned char* base = (g ? sC1 : sC) + stage[g] * p.group_bytes[g];
+                        *(uint4*)(base + (a - GROUP * g) * PANEL + first * 128 + r * 16) = make_uint4(0, 0, 0, 0);
                     }
                 }
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+                    if (++stage[g] == p.stages[g]) stage[g] = 0;
                 fence_proxy_async_smem();
                 tc_fence_before();
                 __syncwarp();
@@ -630,9 +668,9 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             soft_sync();
             if (st < NR && ex.out_row[st] >= 0) {
-                ex.alpha[st] = lsum > 0.0f ? 1.0f / lsum : 0.0f;
+                ex.alpha[st] = lsum == 0.0f ? 0.0f : 1.0f / lsum;  // (NaN stays NaN)
                 if (whole) {
-                    if (p.lse && ok) p.lse[ex.out_row[st]] = lsum > 0.0f ? (mrow + log2f(lsum)) * 0.69314718055994531f : -INFINITY;
+                    if (p.lse && ok) p.lse[ex.out_row[st]] = lsum == 0.0f ? -INFINITY : (mrow + log2f(lsum)) * 0.69314718055994531f;
                 } else if (ok) {
                     p.part_ml[sml + st] = make_float2(mrow, lsum);
                 }
@@ -640,6 +678,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (!it.empty && ok) ok = warp_wait(&bar.pv_done, (u - 1) & 1, p.status, 80);
             soft_sync();
             tc_fence_after();
+            const int pitch = it.pre ? NR : p.own_pitch;
             for (int mt = half; mt < m_tiles; mt += 2) {
                 const int d = mt * 128 + quad * 32 + lane;
 #pragma unroll
@@ -648,17 +687,43 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     uint32_t v[16];
                     tmem_ldx<16>(tmem + lane_addr + O_COL + mt * NR + 16 * j, v);
                     tmem_ld_wait();
-                    if (d >= p.R || !ok) continue;
+                    if (mt * 128 + quad * 32 >= p.R || !ok) continue;  // (the same for the warp)
+                    if (whole) {
+                        // 16 rows of one dim a lane become 4 rows of 4 dims: with the neighbour's and then with the
+                        // next pair's, each giving away the half of the rows that the other keeps
+                        uint32_t w[8];
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        const int col = 16 * j + c, row = ex.out_row[col];
-                        if (row < 0) continue;
-                        if (whole) {
-                            const float inv = ex.alpha[col];  // 0: nothing attended, whatever O^T holds
-                            Elem<T>::store((T*)p.o + (int64_t)row * p.R + d, inv == 0.0f ? 0.0f : __uint_as_float(v[c]) * inv);
-                        } else if (!it.empty) {
-                            p.part_o[so + (int64_t)col * p.R + d] = __uint_as_float(v[c]);
+                        for (int c = 0; c < 16; c += 4) {
+                            const float4 f = *(const float4*)(ex.alpha + 16 * j + c);  // 0: nothing attended, whatever O^T holds
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float g = e == 0 ? f.x : e == 1 ? f.y : e == 2 ? f.z : f.w;
+                                v[c + e] = __float_as_uint(g == 0.0f ? 0.0f : __uint_as_float(v[c + e]) * g);
+                            }
                         }
+                        const bool odd = lane & 1, far = lane & 2;
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const float mine = __uint_as_float(odd ? v[8 + c] : v[c]);
+                            const float other = __shfl_xor_sync(~0u, __uint_as_float(odd ? v[c] : v[8 + c]), 1);
+                            w[c] = odd ? pack2<BF16>(other, mine) : pack2<BF16>(mine, other);
+                        }
+                        uint2 y[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t mine = far ? w[4 + c] : w[c], other = __shfl_xor_sync(~0u, far ? w[c] : w[4 + c], 2);
+                            y[c] = far ? make_uint2(other, mine) : make_uint2(mine, other);
+                        }
+                        const int4 r = *(const int4*)(ex.out_row + 16 * j + 8 * odd + 4 * far);
+                        T* o = (T*)p.o + (d & ~3);
+                        if (r.x >= 0) *(uint2*)(o + (int64_t)r.x * p.R) = y[0];
+                        if (r.y >= 0) *(uint2*)(o + (int64_t)r.y * p.R) = y[1];
+                        if (r.z >= 0) *(uint2*)(o + (int64_t)r.z * p.R) = y[2];
+                        if (r.w >= 0) *(uint2*)(o + (int64_t)r.w * p.R) = y[3];
+                    } else if (!it.empty) {
+                        uint4* y = (uint4*)(p.part_o + so + (int64_t)d * pitch + 16 * j);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) y[c] = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
                     }
                 }
             }
@@ -677,112 +742,124 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
 }
 
-// Rows whose item more than one CTA worked on. A block has a query row; its warps share the row's dims (128 a warp) and,
-// where there are warps left, the parts.
-constexpr int JOIN_WARPS = 8;
+// Rows whose item more than one CTA worked on: a block has 8 of them (and 128 dims, 4 a lane), its warps take the parts in turn and
+// add theirs up in shared memory. Few bytes against the tiles'; what counts is that the parts' loads go out together.
+constexpr int JOIN_WARPS = 8, JOIN_ROWS = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) latent_join_kernel(const __grid_constant__ Params p) {
-    __shared__ float4 sum[JOIN_WARPS][32];
-    const int P = prefix_rows(p), np = prefix_items(p, P), n_cta = (int)p.line[1];
-    const int64_t line = p.line[0];
-    // parts: CTAs c0 .. c1 of item k, column col; with a split prefix those of the prefix's item come first
-    int c0[2], c1[2], k[2], col[2], n_src = 0, b, i, h;
-    auto cta_at = [&](int64_t x) {  // the CTA whose share holds tile x
-        int c = (int)min((int64_t)n_cta - 1, x * n_cta / line);
-        while (c + 1 < n_cta && share(line, n_cta, c + 1) <= x) ++c;
-        while (share(line, n_cta, c) > x) --c;
-        return c;
-    };
-    bool dead;
+    __shared__ float sum[JOIN_WARPS][JOIN_ROWS][128 + 4];
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the first kernel ends
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int P = prefix_rows(p), np = prefix_items(p, P);
+    // parts: CTAs c0 .. c1 of item k, its rows from `row` on; with a split prefix those of the prefix's item come first
+    int k[2], c0[2], n[2], row[2], n_src = 0;
+    const int col0 = (int)blockIdx.y * JOIN_ROWS;
+    Item it;
     if (!p.bb) {
-        const int c = (int)blockIdx.x + 1;  // the share's first tile lies within an item that began before
-        if (c >= n_cta) return;
-        const int2 at = p.cta_item[c];
-        const int64_t start = share(line, n_cta, c) - at.y;
-        if (at.y == 0 || share(line, n_cta, c - 1) > start) return;
-        const Item it = item_of(p, at.x, P, np);
-        if (!row_of(p, it, blockIdx.y, b, i, h)) return;
-        dead = i >= it.cnt;
-        k[0] = at.x;
-        col[0] = blockIdx.y;
-        c0[0] = c - 1;
-        c1[0] = cta_at(start + it.nt - 1);
+        if ((int64_t)blockIdx.x >= p.line[1]) return;
+        const int4 j = p.joins[blockIdx.x];
+        if (j.x < 0) return;
+        it = item_of(p, j.x, P, np);
+        k[0] = j.x, c0[0] = j.y, n[0] = j.z - j.y + 1, row[0] = col0;
         n_src = 1;
     } else {
-        const int64_t row = blockIdx.x;     // (b, i, h)
-        h = (int)(row % p.H);
-        i = (int)(row / p.H % p.Lq);
-        b = (int)(row / ((int64_t)p.H * p.Lq));
-        const Item it = item_of(p, np + b, P, np);
-        dead = i >= it.cnt;
-        const int pt = (P + KT - 1) / KT;
-        if (np > 0) {
-            k[0] = b / p.bb;
-            col[0] = ((b % p.bb) * p.Lq + i) * p.H + h;
-            c0[0] = cta_at((int64_t)k[0] * pt);
-            c1[0] = cta_at((int64_t)k[0] * pt + pt - 1);
-            n_src = 1;
-        }
-        if (!it.empty) {
-            const int64_t start = p.item_pos[b];
-            k[n_src] = np + b;
-            col[n_src] = i * p.H + h;
-            c0[n_src] = cta_at(start);
-            c1[n_src] = cta_at(start + it.nt - 1);
+        const int b = (int)blockIdx.x;
+        it = item_of(p, np + b, P, np);
+        for (int e = np > 0 ? 0 : 1; e < 2; ++e) {
+            const int4 j = p.joins[e == 0 ? b / p.bb : np + b];
+            if (j.x < 0) continue;
+            k[n_src] = j.x, c0[n_src] = j.y, n[n_src] = j.z - j.y + 1;
+            row[n_src] = (e == 0 ? (b % p.bb) * it.rows() : 0) + col0;
             ++n_src;
         }
     }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int chunks = (p.R + 127) / 128, groups = JOIN_WARPS / chunks;
-    const int chunk = warp % chunks, group = warp / chunks, d = chunk * 128 + lane * 4;
-    const int64_t orow = ((int64_t)b * p.H + h) * p.Lq + i;
-    float m = -INFINITY;
-    for (int s = 0; s < n_src; ++s)
-        for (int c = c0[s] + lane; c <= c1[s]; c += 32) {
-            int64_t o, ml;
-            slot_of(p, k[s], np, c, c == c0[s], o, ml);
-            m = fmaxf(m, p.part_ml[ml + col[s]].x);
-        }
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-    float l = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    int turn = 0;
-    for (int s = 0; s < n_src; ++s)
-#pragma unroll 4
-        for (int c = c0[s]; c <= c1[s]; ++c, ++turn) {
-            int64_t o, ml;
-            slot_of(p, k[s], np, c, c == c0[s], o, ml);
-            const float2 v = p.part_ml[ml + col[s]];
-            const float f = v.y > 0.0f ? exp2f(v.x - m) : 0.0f;  // (a part without a weight holds nothing)
-            l += v.y * f;
-            if (group < groups && turn % groups == group && d < p.R && f > 0.0f) {
-                const float4 y = *(const float4*)(p.part_o + o + (int64_t)col[s] * p.R + d);
-                acc.x = fmaf(y.x, f, acc.x);
-                acc.y = fmaf(y.y, f, acc.y);
-                acc.z = fmaf(y.z, f, acc.z);
-                acc.w = fmaf(y.w, f, acc.w);
+    const int rows = min(JOIN_ROWS, it.rows() - col0);
+    const int parts = (n_src > 0 ? n[0] : 0) + (n_src > 1 ? n[1] : 0);
+    auto part_of = [&](int q, int64_t& o, int64_t& ml, int& pitch) {  // part q's first row
+        const int s = q >= n[0], c = c0[s] + q - (s ? n[0] : 0);
+        slot_of(p, k[s], np, c, c == c0[s], o, ml);
+        pitch = k[s] < np ? NR : p.own_pitch;
+        o += row[s];
+        ml += row[s];
+    };
+    // each warp: the rows' largest offset and the sum in its terms, a row a lane & 7, 4 parts at a time
+    const int mine = lane & 7;
+    float m = -INFINITY, l = 0.0f;
+    for (int q = lane >> 3; q < parts; q += 4) {
+        int64_t o, ml;
+        int pitch;
+        part_of(q, o, ml, pitch);
+        if (mine < rows) {
+            const float2 v = p.part_ml[ml + mine];
+            if (v.y != 0.0f) {  // (a part without a weight holds nothing)
+                const float mn = fmaxf(m, v.x);
+                l = l * ex2(m - mn) + v.y * ex2(v.x - mn);
+                m = mn;
             }
         }
-    sum[warp][lane] = acc;
-    __syncthreads();
-    const bool none = dead || !(l > 0.0f);
-    if (group == 0 && d < p.R) {
-        for (int g = 1; g < groups; ++g) {
-            const float4 y = sum[g * chunks + chunk][lane];
-            acc.x += y.x;
-            acc.y += y.y;
-            acc.z += y.z;
-            acc.w += y.w;
+    }
+    for (int x = 8; x < 32; x <<= 1) {
+        const float om = __shfl_xor_sync(~0u, m, x), ol = __shfl_xor_sync(~0u, l, x), mn = fmaxf(m, om);
+        l = l == 0.0f ? ol : ol == 0.0f ? l : l * ex2(m - mn) + ol * ex2(om - mn);
+        m = mn;
+    }
+    const int d = (int)blockIdx.z * 128 + lane * 4;
+    float acc[JOIN_ROWS][4] = {};
+    for (int q = warp; q < parts; q += JOIN_WARPS) {
+        int64_t o, ml;
+        int pitch;
+        part_of(q, o, ml, pitch);
+        float f = 0.0f;
+        if (mine < rows) {
+            const float2 v = p.part_ml[ml + mine];
+            f = v.y == 0.0f ? 0.0f : ex2(v.x - m);
         }
-        const float inv = none ? 0.0f : 1.0f / l;
-        __align__(8) T w[4];
-        const float a[4] = {acc.x, acc.y, acc.z, acc.w};
+        const bool vec = ((o | pitch) & 3) == 0;
+        float y[4][JOIN_ROWS];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) Elem<T>::store(w + e, none ? 0.0f : a[e] * inv);
+        for (int e = 0; e < 4; ++e) {
+            if (d >= p.R) continue;
+            const float* x = p.part_o + o + (int64_t)(d + e) * pitch;
+            if (vec && rows == JOIN_ROWS) {
+                *(float4*)&y[e][0] = *(const float4*)x;
+                *(float4*)&y[e][4] = *(const float4*)(x + 4);
+            } else {
+#pragma unroll
+                for (int r = 0; r < JOIN_ROWS; ++r) y[e][r] = r < rows ? x[r] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < JOIN_ROWS; ++r) {
+            const float fr = __shfl_sync(~0u, f, r);
+            if (fr != 0.0f && d < p.R) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[r][e] = fmaf(y[e][r], fr, acc[r][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < JOIN_ROWS; ++r) *(float4*)&sum[warp][r][lane * 4] = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+    __syncthreads();
+    // a row a warp
+    const float mr = __shfl_sync(~0u, m, warp), lr = __shfl_sync(~0u, l, warp);
+    int b, i, h;
+    if (warp >= rows || !row_of(p, it, col0 + warp, b, i, h)) return;
+    const int64_t orow = ((int64_t)b * p.H + h) * p.Lq + i;
+    const bool none = i >= it.cnt || lr == 0.0f;
+    if (d < p.R) {
+        const float inv = none ? 0.0f : 1.0f / lr;
+        __align__(8) T w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float a = 0.0f;
+#pragma unroll
+            for (int g = 0; g < JOIN_WARPS; ++g) a += sum[g][warp][lane * 4 + e];
+            Elem<T>::store(w + e, none ? 0.0f : a * inv);
+        }
         *(uint2*)((T*)p.o + orow * p.R + d) = *(const uint2*)w;
     }
-    if (p.lse && threadIdx.x == 0) p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+    if (p.lse && lane == 0 && blockIdx.z == 0) p.lse[orow] = none ? -INFINITY : (mr + log2f(lr)) * 0.69314718055994531f;
 }
 
 // nothing cached and nothing before it: zeros and -inf
@@ -850,10 +927,11 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     const int fit = p.n_h > 1 ? 1 : NR / p.hh, n_i = (p.Lq + fit - 1) / fit;
     p.ii = (p.Lq + n_i - 1) / n_i;
     p.n_rt = n_i * p.n_h;
-    p.own_rows = p.hh * p.ii;
+    const int own_rows = p.hh * p.ii;
+    p.own_pitch = (own_rows + 15) & ~15;
     // a prefix gets items of its own where those can take the rows of several sequences
-    if (a.prefix.rows && n_i == 1 && p.n_h == 1 && 2 * p.own_rows <= NR && p.B > 1) {
-        const int most = NR / p.own_rows, n = (p.B + most - 1) / most;
+    if (a.prefix.rows && n_i == 1 && p.n_h == 1 && 2 * own_rows <= NR && p.B > 1) {
+        const int most = NR / own_rows, n = (p.B + most - 1) / most;
         p.bb = (p.B + n - 1) / n;
         p.n_pre = (p.B + p.bb - 1) / p.bb;
     }
@@ -863,10 +941,17 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
         return -1;
     }
     p.panels = p.R / 64 + 1;
-    const int op = p.panels * PANEL, fixed = op + PANEL + (int)sizeof(Extra);
-    p.stages = std::min(MAX_STAGES, (SMEM_MAX - fixed) / op);
-    const size_t smem = std::min(SMEM_MAX, fixed + p.stages * op + 1023);
-    p.slack = (int)smem - (fixed + p.stages * op);
+    p.n_groups = p.panels > GROUP + 1 ? 2 : 1;
+    p.group_bytes[0] = (p.n_groups > 1 ? GROUP : p.panels) * PANEL;
+    p.group_bytes[1] = p.panels * PANEL - p.group_bytes[0];
+    p.q_pitch = (p.bb ? NR : p.own_pitch) * 128;
+    const int fixed = p.panels * p.q_pitch + PANEL + (int)sizeof(Extra), tile = p.panels * PANEL;
+    p.stages[0] = p.stages[1] = std::min(MAX_STAGES, (SMEM_MAX - fixed) / tile);
+    // (what is left may hold one more first group: more loads in flight where there are few query rows)
+    if (p.n_groups > 1 && p.stages[0] < MAX_STAGES && SMEM_MAX - fixed - p.stages[0] * tile >= p.group_bytes[0]) ++p.stages[0];
+    const int used = fixed + p.stages[0] * p.group_bytes[0] + p.stages[1] * p.group_bytes[1];
+    const int smem = std::min(SMEM_MAX, used + 1023);
+    p.slack = smem - used;
 
     const int64_t tiles_seq = (a.c.Smax + KT - 1) / KT + (p.prefix_lens ? (p.prefix_max + KT - 1) / KT : 0);
     const int grid = (int)std::min<int64_t>(n_sm, items * std::max<int64_t>(tiles_seq, 1));
@@ -884,30 +969,39 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     // workspace: the line's data, then the parts
     const int64_t slots_pre = p.bb ? p.n_pre + grid : 0, slots_own = p.bb ? (int64_t)p.B * p.n_rt + grid : 2 * (int64_t)grid;
     p.own_base = slots_pre * NR * p.R;
-    const int64_t n_o = p.own_base + slots_own * p.own_rows * p.R;
-    const int64_t n_ml = (p.bb ? items + grid : 2 * (int64_t)grid) * NR;
+    const int64_t n_o = p.own_base + slots_own * p.own_pitch * p.R, n_ml = (p.bb ? items + grid : 2 * (int64_t)grid) * NR;
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-    const int64_t o_line = 0, o_cta = 256, o_pos = o_cta + up(grid * 8), o_ml = o_pos + up(p.bb ? (int64_t)p.B * 8 : 0),
-                  o_o = o_ml + up(n_ml * 8), total = o_o + up(n_o * 4);
+    const int64_t at_joins = 256, at_ml = at_joins + up((p.bb ? items : grid) * 16), at_o = at_ml + up(n_ml * 8);
     char* ws = nullptr;
-    if (cuda_failed(cudaMallocAsync((void**)&ws, total, st), "latent_attention: workspace")) return -1;
-    p.line = (int64_t*)(ws + o_line);
-    p.cta_item = (int2*)(ws + o_cta);
-    p.item_pos = (int64_t*)(ws + o_pos);
-    p.part_ml = (float2*)(ws + o_ml);
-    p.part_o = (float*)(ws + o_o);
+    if (cuda_failed(cudaMallocAsync((void**)&ws, at_o + up(n_o * 4), st), "latent_attention: workspace")) return -1;
+    p.line = (int64_t*)ws;
+    p.joins = (int4*)(ws + at_joins);
+    p.part_ml = (float2*)(ws + at_ml);
+    p.part_o = (float*)(ws + at_o);
 
     int rc = 0;
     auto kern = latent_attn_kernel<BF16>;
-    if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), ctx)) rc = -1;
+    static std::atomic<uint64_t> ready{0};  // devices (of the first 64) whose kernel may use this much shared memory
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(ready.load() & bit)) {
+        if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX), ctx)) rc = -1;
+        else ready.fetch_or(bit);
+    }
     if (!rc) {
         kern<<<grid, NTHREADS, smem, st>>>(mq, mqp, mc, mcp, p);
         if (cuda_failed(cudaGetLastError(), "latent_attention launch")) rc = -1;
     }
     if (!rc && (p.bb || grid > 1)) {
-        const dim3 g = p.bb ? dim3((unsigned)((int64_t)p.B * p.H * p.Lq)) : dim3(grid - 1, p.own_rows);
-        latent_join_kernel<T><<<g, JOIN_WARPS * 32, 0, st>>>(p);
-        if (cuda_failed(cudaGetLastError(), "latent_attention join launch")) rc = -1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(p.bb ? p.B : grid, (own_rows + JOIN_ROWS - 1) / JOIN_ROWS, (p.R + 127) / 128);
+        cfg.blockDim = dim3(JOIN_WARPS * 32);
+        cfg.stream = st;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        at[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        if (cuda_failed(cudaLaunchKernelEx(&cfg, latent_join_kernel<T>, p), "latent_attention join launch")) rc = -1;
     }
     cudaFreeAsync(ws, st);
     return rc;
