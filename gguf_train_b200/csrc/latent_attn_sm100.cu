@@ -65,7 +65,8 @@ struct Extra {                 // what lies behind the operands in shared memory
     float exch[4][NR];         // a quadrant's maxima, later its sums
     Bars bars;
     int64_t line, warp_sum[NTHREADS / 32];  // finding the CTA's share
-    int first_item, first_tile;
+    int first_item;
+    int64_t first_place;
 };
 
 constexpr int DEAD = INT_MIN;
@@ -77,12 +78,12 @@ struct Params {
     int hh, ii, n_h, n_rt;     // heads and tokens of an item, items along the heads, items a sequence
     int bb, n_pre;             // sequences of a prefix item (0: the prefix's tiles belong to the own items), prefix items
     int panels, n_groups;
-    int q_pitch;               // bytes of a panel of Q
+    int q_pitch, q_zero;       // bytes of a panel of Q; whether loads leave some of its rows
     int group_bytes[2], stages[2], slack;
     float scale_log2;
     void* o;
     float* lse;
-    float* part_o;             // [slot][dim][pitch], a row a column
+    float* part_o;             // [slot][row / 4][dim][row % 4]
     float2* part_ml;           // [slot][row]: offset, sum
     int4* joins;               // items that more than one CTA worked on, by the CTA that begins them; with a split prefix, by item:
                                // item (-1: none), first CTA, last CTA
@@ -93,6 +94,11 @@ struct Params {
 };
 
 static_assert(3 * 9 * PANEL + PANEL + (int)sizeof(Extra) <= SMEM_MAX, "two stages of the largest rows");
+
+// What an item costs besides its tiles (its query rows' load, the first tile's way through the empty pipeline, its output), in tiles:
+// (32 sequences of 100 to 8192 rows, drafts of 5 tokens of 20 heads: 48 us; with 0 places 59, 1 56, 6 47; 64 sequences of 1k to 32k 213,
+// 215, 213, 217)
+constexpr int LEAD = 3;
 
 struct Item {
     int b, i0, h0;             // first sequence, token, head
@@ -143,9 +149,11 @@ __device__ __forceinline__ Item item_of(const Params& p, int k, int P, int np) {
     return it;
 }
 
+// The line: each item takes LEAD places and one for each of its tiles; CTA c of n works on the tiles whose places are in
+// [share(c), share(c + 1)).
 __device__ __forceinline__ int64_t share(int64_t line, int n, int c) { return line * c / n; }
 
-// the CTA whose share holds tile x
+// the CTA whose share holds place x
 __device__ __forceinline__ int cta_of(int64_t line, int n, int64_t x) {
     int c = (int)min((int64_t)n - 1, x * n / line);
     while (c + 1 < n && share(line, n, c + 1) <= x) ++c;
@@ -214,7 +222,7 @@ __device__ __forceinline__ bool elect_lane() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
     return r != 0;
 }
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(~0u, v); }  // of a value that all lanes have
+__device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(~0u, v); }  // of a value that all lanes have
 
 // The low words of the descriptors (address, leading byte offset) come in registers; the high ones are the same for all operands here
 // (stride byte offset 1024, version, 128-byte swizzle).
@@ -262,14 +270,36 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     const int P = prefix_rows(p), np = prefix_items(p, P);
     const int n_items = np + p.B * p.n_rt;
 
-    // ---------------------------------------------------------------- this CTA's share of the line of tiles
-    // (NTHREADS items a round; where that is all of them, their tiles are counted once)
+    if (threadIdx.x == 0) {
+        mbar_init(&bar.q_full, 1);
+        mbar_init(&bar.q_empty, 1);
+        mbar_init(&bar.pv_done, 1);
+        mbar_init(&bar.o_empty, NSOFT / 32);
+        mbar_init(&bar.p_full, NSOFT / 32);
+        for (int s = 0; s < 2 * MAX_STAGES; ++s) {
+            mbar_init(&bar.k_full[0][0] + s, 1);
+            mbar_init(&bar.k_empty[0][0] + s, 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&bar.s_full[s], 1);
+            mbar_init(&bar.s_free[s], NSOFT / 32);
+            mbar_init(&bar.drain[s], 1);
+        }
+        bar.abort = 0;
+        fence_mbar_init();
+    }
+    // query rows that no load fills stay zero (their columns are computed and dropped)
+    for (int e = threadIdx.x; e < (p.q_zero ? p.panels * p.q_pitch / 16 : 0); e += NTHREADS) ((uint4*)sQ)[e] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async_smem();
+    if (warp == 1) tmem_alloc(&bar.tmem, TMEM_COLS);
+    // ---------------------------------------------------------------- this CTA's share of the line
+    // (NTHREADS items a round; where that is all of them, they are counted once)
     int64_t line = 0, begin = 0, end = 0, before = 0;
     int n_cta = 1;
     for (int pass = n_items > NTHREADS ? 0 : 1; pass < 2; ++pass) {
         for (int k0 = 0; k0 < n_items; k0 += NTHREADS) {
             const int k = k0 + (int)threadIdx.x;
-            const int64_t n = k < n_items ? item_of(p, k, P, np).nt : 0;
+            const int64_t n = k < n_items ? item_of(p, k, P, np).nt + LEAD : 0;
             int64_t incl = n;
             for (int o = 1; o < 32; o <<= 1) {
                 const int64_t y = __shfl_up_sync(~0u, incl, o);
@@ -292,13 +322,12 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         p.line[0] = line;
                         p.line[1] = n_cta;
                     }
-                    if (cta >= n_cta) return;
-                    begin = share(line, n_cta, cta);
-                    end = share(line, n_cta, cta + 1);
+                    begin = share(line, n_cta, min(cta, n_cta - 1));
+                    end = share(line, n_cta, min(cta, n_cta - 1) + 1);
                 }
                 if (begin >= incl - n && begin < incl) {
                     ex.first_item = k;
-                    ex.first_tile = (int)(begin - (incl - n));
+                    ex.first_place = incl - n;
                 }
             }
             __syncthreads();
@@ -306,35 +335,30 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         }
         if (pass == 0) line = before, before = 0;
     }
-    const int k_first = ex.first_item, off_first = ex.first_tile;
+    // from here on places count from the first item's first tile: tiles [off_first, ..) of item k_first, and on to place `last`
+    const int k_first = ex.first_item;
+    const int64_t first_place = ex.first_place;
+    const int off_first = max((int)(begin - first_place) - LEAD, 0), last = (int)(end - first_place) - LEAD;
+    const bool idle = cta >= n_cta;
 
-    if (threadIdx.x == 0) {
-        mbar_init(&bar.q_full, 1);
-        mbar_init(&bar.q_empty, 1);
-        mbar_init(&bar.pv_done, 1);
-        mbar_init(&bar.o_empty, NSOFT / 32);
-        mbar_init(&bar.p_full, NSOFT / 32);
-        for (int s = 0; s < 2 * MAX_STAGES; ++s) {
-            mbar_init(&bar.k_full[0][0] + s, 1);
-            mbar_init(&bar.k_empty[0][0] + s, 1);
-        }
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(&bar.s_full[s], 1);
-            mbar_init(&bar.s_free[s], NSOFT / 32);
-            mbar_init(&bar.drain[s], 1);
-        }
-        bar.abort = 0;
-        fence_mbar_init();
-    }
-    // query rows that no load fills stay zero (their columns are computed and dropped)
-    for (int e = threadIdx.x; e < p.panels * p.q_pitch / 16; e += NTHREADS) ((uint4*)sQ)[e] = make_uint4(0, 0, 0, 0);
-    fence_proxy_async_smem();
-    if (warp == 1) tmem_alloc(&bar.tmem, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = bar.tmem;
     volatile int* abort_flag = &bar.abort;
+    asm volatile("griddepcontrol.launch_dependents;");  // the join's blocks may take the SMs that this grid's leave
+    // A role's walk over the CTA's tiles: for_segments(f) calls f(item, its number, first tile, tiles)
+    auto for_segments = [&](auto uni, auto&& f) {
+        int to = uni(last), off = uni(off_first);
+        for (int k = uni(k_first); k < n_items && !idle; ++k, off = 0) {
+            const Item it = item_of(p, k, P, np);
+            const int n = uni(min(it.nt, to) - off);
+            if (n <= 0) break;
+            to -= uni(it.nt) + LEAD;
+            if (!f(it, k, off, n)) break;
+        }
+    };
+    auto plain = [](int v) { return v; };
 
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
@@ -344,12 +368,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             bool ok = true;
             int nseg = 0, loads[2] = {0, 0};  // segments started, groups loaded
             int stage[2] = {0, 0}, phase[2] = {1, 1};
-            int64_t pos = begin;
-            for (int k = k_first, off = off_first; pos < end && ok; ++k, off = 0) {
-                const Item it = item_of(p, k, P, np);
-                const int n = (int)min((int64_t)(it.nt - off), end - pos);
-                pos += n;
-                if (it.empty) continue;
+            for_segments(plain, [&](const Item& it, int, int off, int n) {
+                if (it.empty) return true;
                 for (int t = off; t < off + n && ok; ++t) {
                     const bool pre = t < it.nt_pre;
                     const CUtensorMap* tm = pre ? &tmCp : &tmC;
@@ -377,7 +397,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         ++nseg;
                     }
                 }
-            }
+                return ok;
+            });
             if (!ok) *abort_flag = 1;
             if (*abort_flag) {  // our copies in flight end before the CTA does
                 if (nseg > 0) mbar_wait(&bar.q_full, (nseg - 1) & 1, nullptr, 0);
@@ -389,20 +410,17 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     } else if (warp < 3) {
         // ------------------------------------------------------------ MMA issuers: 1 the scores, 2 the second products
         const bool scores = warp == 1, lead = elect_lane();
-        const uint32_t tm = uniform(tmem);
+        const uint32_t tm = (uint32_t)uniform((int)tmem);
         const uint32_t lead_off = scores ? 16 : PANEL;  // leading byte offset (K-major: unused)
         const uint32_t qd = (uint32_t)desc_sw128(smem_u32(sQ), 16, 1024), pd = (uint32_t)desc_sw128(smem_u32(sP), PANEL, 1024);
         const uint32_t cd[2] = {(uint32_t)desc_sw128(smem_u32(sC), lead_off, 1024), (uint32_t)desc_sw128(smem_u32(sC1), lead_off, 1024)};
         const uint32_t q_step = p.q_pitch >> 4;
         const int rope_steps = p.Dr / 16, m_tiles = (p.R + 127) / 128;
         bool ok = true;
-        int nseg = 0, left = (int)uniform((uint32_t)(end - begin)), k = (int)uniform(k_first), off = (int)uniform(off_first);
+        int nseg = 0;
         int u = 0, stage[2] = {0, 0}, phase[2] = {0, 0};  // tiles so far, the next one's stages and their phases
-        for (; left > 0 && ok; ++k, off = 0) {
-            const Item it = item_of(p, k, P, np);
-            const int n = (int)uniform(min(it.nt - off, left));
-            left -= n;
-            if (uniform(it.empty)) continue;
+        for_segments([](int v) { return uniform(v); }, [&](const Item& it, int, int, int n) {
+            if (uniform(it.empty)) return true;
             const uint32_t n16 = uniform((it.rows() + 15) & ~15);
             if (scores) {
                 const uint32_t idesc = idesc_f16(KT, 0, BF16, false) | (n16 >> 3 << 17);
@@ -471,7 +489,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
             }
             ++nseg;
-        }
+            return ok;
+        });
         if (!ok) *abort_flag = 1;
         __syncwarp();
         if (__any_sync(~0u, *abort_flag)) {
@@ -482,17 +501,17 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         // ------------------------------------------------------------ what the join kernel has to know
         if (lane == 0) {
             int4 mine = make_int4(-1, 0, 0, 0);
-            int64_t pos = begin;
-            for (int k = k_first, off = off_first; pos < end; ++k, off = 0) {
-                const Item it = item_of(p, k, P, np);
+            int64_t place = first_place + LEAD;  // of the item's first tile
+            for_segments(plain, [&](const Item& it, int k, int off, int) {
                 if (off == 0) {
-                    const int4 j = make_int4(it.empty ? -1 : k, cta, cta_of(line, n_cta, pos + it.nt - 1), 0);
+                    const int4 j = make_int4(it.empty ? -1 : k, cta, cta_of(line, n_cta, place + it.nt - 1), 0);
                     if (p.bb) p.joins[k] = j;
                     else if (j.z > cta) mine = j;
                 }
-                pos += it.nt - off;
-            }
-            if (!p.bb) p.joins[cta] = mine;
+                place += it.nt + LEAD;
+                return true;
+            });
+            if (!p.bb && !idle) p.joins[cta] = mine;
         }
     } else {
         // ------------------------------------------------------------ softmax, rescaling, epilogue
@@ -503,11 +522,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int m_tiles = (p.R + 127) / 128;
         bool ok = true;
         int u = 0, stage[2] = {0, 0};
-        int64_t pos = begin;
-        for (int k = k_first, off = off_first; pos < end; ++k, off = 0) {
-            const Item it = item_of(p, k, P, np);
-            const int n = (int)min((int64_t)(it.nt - off), end - pos);
-            pos += n;
+        for_segments(plain, [&](const Item& it, int k, int off, int n) {
             const int gl = (it.rows() + 15) / 16;          // groups of 8 columns of this warp: 2 j + half, j < gl
             soft_sync();                                   // the last segment's lim, out_row, alpha have been read
             if (st < NR) {
@@ -678,7 +693,6 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             if (!it.empty && ok) ok = warp_wait(&bar.pv_done, (u - 1) & 1, p.status, 80);
             soft_sync();
             tc_fence_after();
-            const int pitch = it.pre ? NR : p.own_pitch;
             for (int mt = half; mt < m_tiles; mt += 2) {
                 const int d = mt * 128 + quad * 32 + lane;
 #pragma unroll
@@ -721,16 +735,17 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         if (r.z >= 0) *(uint2*)(o + (int64_t)r.z * p.R) = y[2];
                         if (r.w >= 0) *(uint2*)(o + (int64_t)r.w * p.R) = y[3];
                     } else if (!it.empty) {
-                        uint4* y = (uint4*)(p.part_o + so + (int64_t)d * pitch + 16 * j);
+                        uint4* y = (uint4*)(p.part_o + so) + 4 * j * p.R + d;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) y[c] = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+                        for (int c = 0; c < 4; ++c) y[c * p.R] = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
                     }
                 }
             }
             tc_fence_before();
             __syncwarp();
             if (!it.empty && lane == 0) mbar_arrive(&bar.o_empty);
-        }
+            return true;
+        });
         if (!ok) *abort_flag = 1;
     }
 
@@ -776,22 +791,23 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) latent_join_kernel(const __gr
     }
     const int rows = min(JOIN_ROWS, it.rows() - col0);
     const int parts = (n_src > 0 ? n[0] : 0) + (n_src > 1 ? n[1] : 0);
-    auto part_of = [&](int q, int64_t& o, int64_t& ml, int& pitch) {  // part q's first row
+    auto part_of = [&](int q, const float*& o, const float2*& ml) -> int {  // part q, its first row
         const int s = q >= n[0], c = c0[s] + q - (s ? n[0] : 0);
-        slot_of(p, k[s], np, c, c == c0[s], o, ml);
-        pitch = k[s] < np ? NR : p.own_pitch;
-        o += row[s];
-        ml += row[s];
+        int64_t so, sml;
+        slot_of(p, k[s], np, c, c == c0[s], so, sml);
+        o = p.part_o + so;
+        ml = p.part_ml + sml + row[s];
+        return row[s];
     };
     // each warp: the rows' largest offset and the sum in its terms, a row a lane & 7, 4 parts at a time
     const int mine = lane & 7;
     float m = -INFINITY, l = 0.0f;
     for (int q = lane >> 3; q < parts; q += 4) {
-        int64_t o, ml;
-        int pitch;
-        part_of(q, o, ml, pitch);
+        const float* o;
+        const float2* ml;
+        part_of(q, o, ml);
         if (mine < rows) {
-            const float2 v = p.part_ml[ml + mine];
+            const float2 v = ml[mine];
             if (v.y != 0.0f) {  // (a part without a weight holds nothing)
                 const float mn = fmaxf(m, v.x);
                 l = l * ex2(m - mn) + v.y * ex2(v.x - mn);
@@ -807,26 +823,25 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) latent_join_kernel(const __gr
     const int d = (int)blockIdx.z * 128 + lane * 4;
     float acc[JOIN_ROWS][4] = {};
     for (int q = warp; q < parts; q += JOIN_WARPS) {
-        int64_t o, ml;
-        int pitch;
-        part_of(q, o, ml, pitch);
+        const float* o;
+        const float2* ml;
+        const int r0 = part_of(q, o, ml);
         float f = 0.0f;
         if (mine < rows) {
-            const float2 v = p.part_ml[ml + mine];
+            const float2 v = ml[mine];
             f = v.y == 0.0f ? 0.0f : ex2(v.x - m);
         }
-        const bool vec = ((o | pitch) & 3) == 0;
         float y[4][JOIN_ROWS];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (d >= p.R) continue;
-            const float* x = p.part_o + o + (int64_t)(d + e) * pitch;
-            if (vec && rows == JOIN_ROWS) {
-                *(float4*)&y[e][0] = *(const float4*)x;
-                *(float4*)&y[e][4] = *(const float4*)(x + 4);
+            if ((r0 & 3) == 0 && rows == JOIN_ROWS) {
+                *(float4*)&y[e][0] = *(const float4*)(o + ((int64_t)(r0 >> 2) * p.R + d + e) * 4);
+                *(float4*)&y[e][4] = *(const float4*)(o + ((int64_t)((r0 >> 2) + 1) * p.R + d + e) * 4);
             } else {
 #pragma unroll
-                for (int r = 0; r < JOIN_ROWS; ++r) y[e][r] = r < rows ? x[r] : 0.0f;
+                for (int r = 0; r < JOIN_ROWS; ++r)
+                    y[e][r] = r < rows ? o[((int64_t)((r0 + r) >> 2) * p.R + d + e) * 4 + ((r0 + r) & 3)] : 0.0f;
             }
         }
 #pragma unroll
@@ -945,6 +960,7 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     p.group_bytes[0] = (p.n_groups > 1 ? GROUP : p.panels) * PANEL;
     p.group_bytes[1] = p.panels * PANEL - p.group_bytes[0];
     p.q_pitch = (p.bb ? NR : p.own_pitch) * 128;
+    p.q_zero = own_rows % 16 != 0 || p.bb * own_rows % 16 != 0;
     const int fixed = p.panels * p.q_pitch + PANEL + (int)sizeof(Extra), tile = p.panels * PANEL;
     p.stages[0] = p.stages[1] = std::min(MAX_STAGES, (SMEM_MAX - fixed) / tile);
     // (what is left may hold one more first group: more loads in flight where there are few query rows)
@@ -954,7 +970,7 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     p.slack = smem - used;
 
     const int64_t tiles_seq = (a.c.Smax + KT - 1) / KT + (p.prefix_lens ? (p.prefix_max + KT - 1) / KT : 0);
-    const int grid = (int)std::min<int64_t>(n_sm, items * std::max<int64_t>(tiles_seq, 1));
+    const int grid = (int)std::min<int64_t>(n_sm, items * (std::max<int64_t>(tiles_seq, 1) + LEAD));
 
     CUtensorMap mq, mqp, mc, mcp;
     const int64_t D = p.R + p.Dr, qs[3] = {p.H, p.Lq, p.B}, qt[3] = {a.q.sh, a.q.ss, a.q.sb};
