@@ -141,6 +141,10 @@ def _configure(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.gtb_latent_append.restype = c_int
     lib.gtb_latent_attention.argtypes = [c_void_p, PLATENT, PLATENT, c_float, c_void_p, c_void_p, c_void_p, c_void_p]
     lib.gtb_latent_attention.restype = c_int
+    lib.gtb_latent_sdpa_fwd.argtypes = [c_void_p] * 5 + [c_float, c_int, c_void_p, c_void_p, c_void_p]
+    lib.gtb_latent_sdpa_fwd.restype = c_int
+    lib.gtb_latent_sdpa_bwd.argtypes = [c_void_p] * 8 + [c_float, c_int] + [c_void_p] * 5
+    lib.gtb_latent_sdpa_bwd.restype = c_int
     lib.gtb_last_error.argtypes = []
     lib.gtb_last_error.restype = c_char_p
     lib.gtb_clear_error.argtypes = []

@@ -37,4 +37,24 @@ struct LatentAttnArgs {
 };
 int launch_latent_attention(const LatentAttnArgs& a, cudaStream_t st);
 
+// Expanded latent attention: q, o, lse, g, dq (B, H, L, .), k, v, dk, dv (B, Hkv, S, .), the rotary keys and their gradient (B, 1, S, Dr)
+struct LatentSdpaArgs {
+    int64_t B, H, Hkv, L, S;
+    int Dn, Dr;              // Dv = Dn
+    gtb_tensor4 q, k, k_rope, v, o;
+    float* lse;              // (B, H, L); the forward's may be null
+    const int32_t* lens;     // nullable
+    float scale;
+    int causal;
+    gtb_tensor4 g, dq, dk, dk_rope, dv;  // backward only
+    int* status;
+};
+int launch_latent_sdpa_fwd(const LatentSdpaArgs& a, cudaStream_t st);
+int launch_latent_sdpa_bwd(const LatentSdpaArgs& a, cudaStream_t st);
+
+// tokens of sequence b that take part
+__device__ __forceinline__ int latent_tokens(const int32_t* lens, int b, int64_t n) {
+    return lens ? (int)min((int64_t)max(lens[b], 0), n) : (int)n;
+}
+
 }  // namespace gtb

@@ -56,6 +56,72 @@ int* status_of(const char* ctx) {
     return s;
 }
 
+bool tiled(const gtb_tensor4& t) {  // rows start on 16 bytes, as tile loads and vector stores need
+    if (!unit_inner(t) || ((uintptr_t)t.data & 15)) return false;
+    for (int i = 0; i < 3; ++i)
+        if (t.shape[i] > 1 && (t.stride[i] <= 0 || t.stride[i] % 8)) return false;
+    return true;
+}
+
+bool is_shape(const gtb_tensor4& t, int64_t a, int64_t b, int64_t c, int64_t d) {
+    return t.shape[0] == a && t.shape[1] == b && t.shape[2] == c && t.shape[3] == d;
+}
+
+// sizes, types and layout of the expanded form's inputs; `empty`: nothing to compute
+bool check_sdpa(const char* ctx, const gtb_tensor4* q, const gtb_tensor4* k, const gtb_tensor4* k_rope, const gtb_tensor4* v,
+                const int32_t* lens, float scale, LatentSdpaArgs& a, bool& empty) {
+    if (!q || !k || !k_rope || !v) return fail(ctx, "q, k, k_rope and v are required");
+    for (const gtb_tensor4* t : {q, k, k_rope, v}) {
+        for (int i = 0; i < 4; ++i)
+            if (t->shape[i] < 0 || t->shape[i] >= (int64_t)1 << 30) return fail(ctx, "sizes must be from 0 to below 2^30");
+        if ((t->dtype != F16 && t->dtype != BF16) || t->dtype != q->dtype) return fail(ctx, "q, k, k_rope and v must be f16 or bf16, of one type");
+    }
+    a.B = q->shape[0];
+    a.H = q->shape[1];
+    a.L = q->shape[2];
+    a.Hkv = k->shape[1];
+    a.S = k->shape[2];
+    if (k->shape[3] != 64 && k->shape[3] != 128) return fail(ctx, "k must have 64 or 128 values a head");
+    a.Dn = (int)k->shape[3];
+    if (q->shape[3] < a.Dn + 16 || q->shape[3] > a.Dn + 64 || q->shape[3] % 16)
+        return fail(ctx, "the rotary part must have a multiple of 16 values from 16 to 64");
+    a.Dr = (int)q->shape[3] - a.Dn;
+    if (k->shape[0] != a.B || !is_shape(*k_rope, a.B, 1, a.S, a.Dr) || !is_shape(*v, a.B, a.Hkv, a.S, a.Dn))
+        return fail(ctx, "q (B, H, L, Dn + Dr), k (B, Hkv, S, Dn), k_rope (B, 1, S, Dr) and v (B, Hkv, S, Dn) do not fit together");
+    if (a.Hkv == 0 ? a.H != 0 : a.H % a.Hkv) return fail(ctx, "num_heads must be divisible by num_kv_heads");
+    if (a.B > 65535 || a.H > 65535) return fail(ctx, "at most 65535 sequences and heads");
+    if (lens && a.L != a.S) return fail(ctx, "lengths need as many queries as keys");
+    if (!std::isfinite(scale) || !(scale > 0.0f)) return fail(ctx, "scale must be positive and finite");
+    a.q = *q;
+    a.k = *k;
+    a.k_rope = *k_rope;
+    a.v = *v;
+    a.lens = lens;
+    a.scale = scale;
+    empty = a.B * a.H == 0 || (a.L == 0 && a.S == 0);
+    if (empty) return true;
+    if (a.L == 0 || a.S == 0) return fail(ctx, "there must be queries and keys");
+    const char* names[4] = {"q", "k", "k_rope", "v"};
+    const gtb_tensor4* ts[4] = {q, k, k_rope, v};
+    for (int i = 0; i < 4; ++i) {
+        if (!check_device_ptr(ts[i]->data, ctx, names[i])) return false;
+        if (!tiled(*ts[i])) return fail(ctx, "rows must start on 16 bytes, with a unit innermost stride and positive others");
+    }
+    if (lens && !check_device_ptr(lens, ctx, "seq_lens")) return false;
+    a.status = status_of(ctx);
+    return a.status != nullptr;
+}
+
+bool check_result(const char* ctx, const gtb_tensor4* t, const gtb_tensor4& like, const char* name) {
+    if (!t || t->dtype != like.dtype || !is_shape(*t, like.shape[0], like.shape[1], like.shape[2], like.shape[3])) {
+        set_errorf("%s: %s has another shape or type than it should", ctx, name);
+        return false;
+    }
+    if (!check_device_ptr(t->data, ctx, name)) return false;
+    if (!tiled(*t)) return fail(ctx, "rows must start on 16 bytes, with a unit innermost stride and positive others");
+    return true;
+}
+
 }  // namespace
 }  // namespace gtb
 
@@ -145,6 +211,52 @@ GTB_API int gtb_latent_attention(const gtb_tensor4* q, const gtb_latent* cache, 
         LatentAttnArgs a{*cache, gtb_latent{}, rows3(*q), out->data, H, Lq, scale, counts, lse, status_of(ctx)};
         if (prefix && prefix->Smax > 0) a.prefix = *prefix;
         return a.status ? launch_latent_attention(a, (cudaStream_t)stream) : -1;
+    });
+}
+
+GTB_API int gtb_latent_sdpa_fwd(const gtb_tensor4* q, const gtb_tensor4* k, const gtb_tensor4* k_rope, const gtb_tensor4* v,
+                                const int32_t* seq_lens, float scale, int is_causal, gtb_tensor4* out, float* lse, void* stream) {
+    const char* ctx = "latent_sdpa";
+    return guarded(ctx, [&]() -> int {
+        LatentSdpaArgs a{};
+        bool empty = false;
+        if (!check_sdpa(ctx, q, k, k_rope, v, seq_lens, scale, a, empty)) return -1;
+        if (empty) return 0;
+        gtb_tensor4 like = *q;
+        like.shape[3] = a.Dn;
+        if (!check_result(ctx, out, like, "out")) return -1;
+        if (lse && !check_device_ptr(lse, ctx, "lse")) return -1;
+        a.o = *out;
+        a.lse = lse;
+        a.causal = is_causal != 0;
+        return launch_latent_sdpa_fwd(a, (cudaStream_t)stream);
+    });
+}
+
+GTB_API int gtb_latent_sdpa_bwd(const gtb_tensor4* grad_out, const gtb_tensor4* q, const gtb_tensor4* k, const gtb_tensor4* k_rope,
+                                const gtb_tensor4* v, const gtb_tensor4* out, const float* lse, const int32_t* seq_lens, float scale,
+                                int is_causal, gtb_tensor4* dq, gtb_tensor4* dk, gtb_tensor4* dk_rope, gtb_tensor4* dv, void* stream) {
+    const char* ctx = "latent_sdpa_bwd";
+    return guarded(ctx, [&]() -> int {
+        LatentSdpaArgs a{};
+        bool empty = false;
+        if (!check_sdpa(ctx, q, k, k_rope, v, seq_lens, scale, a, empty)) return -1;
+        if (empty) return 0;
+        gtb_tensor4 like = *q;
+        like.shape[3] = a.Dn;
+        if (!check_result(ctx, grad_out, like, "grad_out") || !check_result(ctx, out, like, "out") || !check_result(ctx, dq, *q, "dq") ||
+            !check_result(ctx, dk, *k, "dk") || !check_result(ctx, dk_rope, *k_rope, "dk_rope") || !check_result(ctx, dv, *v, "dv"))
+            return -1;
+        if (!check_device_ptr(lse, ctx, "lse")) return -1;
+        a.g = *grad_out;
+        a.o = *out;
+        a.lse = const_cast<float*>(lse);
+        a.causal = is_causal != 0;
+        a.dq = *dq;
+        a.dk = *dk;
+        a.dk_rope = *dk_rope;
+        a.dv = *dv;
+        return launch_latent_sdpa_bwd(a, (cudaStream_t)stream);
     });
 }
 

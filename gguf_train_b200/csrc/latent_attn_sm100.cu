@@ -32,6 +32,7 @@
 
 #include "gtb_common.cuh"
 #include "latent.h"
+#include "latent_mma.cuh"
 #include "sdpa_args.h"
 #include "sm100_ptx.cuh"
 
@@ -183,18 +184,6 @@ __device__ __forceinline__ void slot_of(const Params& p, int k, int np, int c, b
     }
 }
 
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    uint32_t r;
-    if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status, int code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code));
-}
-
 // 16 lanes x 8 n columns of 32 bits (n 1 to 4): of each 8 columns, thread t gets (lane t/4, columns 2 (t%4), +1) and (lane t/4 + 8, the
 // same columns)
 __device__ __forceinline__ void tmem_ld_16(int n, uint32_t taddr, uint32_t* r) {
@@ -211,28 +200,6 @@ __device__ __forceinline__ void tmem_ld_16(int n, uint32_t taddr, uint32_t* r) {
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
                        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
                      : "r"(taddr));
-}
-
-// The lane that issues the MMA warp's products and commits. The whole warp goes through the loops around them without diverging,
-// on values that are the same in every lane for the compiler too (votes and reductions), so that descriptors
-// are formed in uniform registers, where the instruction takes its operands from. (One lane in loops of its own: 106 cycles a
-// product whatever its size; this way the unit's own 33 and 50.)
-__device__ __forceinline__ bool elect_lane() {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-    return r != 0;
-}
-__device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(~0u, v); }  // of a value that all lanes have
-
-// The low words of the descriptors (address, leading byte offset) come in registers; the high ones are the same for all operands here
-// (stride byte offset 1024, version, 128-byte swizzle).
-constexpr uint32_t DESC_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
-__device__ __forceinline__ void mma(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI)
-        : "memory");
 }
 
 __device__ __forceinline__ void soft_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(NSOFT) : "memory"); }
@@ -443,12 +410,12 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                                 if (i < n_val) {
 #pragma unroll
                                     for (int kk = 0; kk < 4; ++kk)
-                                        mma(dst, a + i * (PANEL >> 4) + kk * 2, q + i * q_step + kk * 2, idesc, i > 0 || kk > 0 || g > 0);
+                                        mma_ss_lo(dst, a + i * (PANEL >> 4) + kk * 2, q + i * q_step + kk * 2, idesc, i > 0 || kk > 0 || g > 0);
                                 }
                             }
                             if (g + 1 == p.n_groups)  // the rotary keys
                                 for (int kk = 0; kk < rope_steps; ++kk)
-                                    mma(dst, a + n_val * (PANEL >> 4) + kk * 2, q + n_val * q_step + kk * 2, idesc, 1);
+                                    mma_ss_lo(dst, a + n_val * (PANEL >> 4) + kk * 2, q + n_val * q_step + kk * 2, idesc, 1);
                         }
                         if (++stage[g] == p.stages[g]) stage[g] = 0, phase[g] ^= 1;
                     }
@@ -474,7 +441,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                             if (m < m_tiles) {
 #pragma unroll
                                 for (int kk = 0; kk < KT / 16; ++kk)
-                                    mma(tm + O_COL + m * NR, (m < 2 ? a0 : a1) + (m & 1) * (2 * PANEL >> 4) + kk * 128, pd + kk * 128, idesc,
+                                    mma_ss_lo(tm + O_COL + m * NR, (m < 2 ? a0 : a1) + (m & 1) * (2 * PANEL >> 4) + kk * 128, pd + kk * 128, idesc,
                                         t > 0 || kk > 0);
                                 if (m == 1 && p.n_groups > 1) mma_commit(&bar.k_empty[0][stage[0]]);
                             }

@@ -1,0 +1,783 @@
+// Expanded latent attention backward on tcgen05. With w = exp(score - lse) recomputed tile by tile and
+// ds = w (g . v - g . out):   dv = w^T g,   [dk | dk_r] = scale ds^T [q_n | q_r],   dq = scale ds [k | k_r].
+//
+//   pre     a query row: -g . out and -lse log2 e (-inf for padded rows and rows that attend nothing: weights 0).
+//   dK/dV   one CTA a 128-key tile of one (batch, kv head), over its query heads' rows, 64 at a time:
+//             S^T = [K | K_r] Q^T, dP^T = V G^T        (M = 128 keys, N = 64 queries)
+//             dV += W^T G, dK += dS^T Q                (M = 128 keys, N = dims, K = 64; W^T, dS^T through shared memory)
+//           The rotary part of dK is the sum over all heads: each CTA writes its share in f32 and a last kernel adds the
+//           heads in order, so the bits are the same on every run.
+//   dQ      one CTA a 128-query tile, over 64 keys at a time:
+//             S = Q [K | K_r]^T, dP = G V^T            (M = 128 queries, N = 64 keys)
+//             dQ += dS [K | K_r]                       (N = dims, K = 64; dS from TMEM, over S)
+// A fused dQ (five products instead of seven) needs f32 sums in global memory by unordered additions, and TMEM that dK's 192 columns
+// do not leave. Products of N = 64 with both operands in shared memory are bound by its bandwidth (49.5 cycles instead of 32):
+// 64 is what TMEM holds of scores next to dV and dK (320 of 512 columns with Dn = 128).
+//
+// Warps: 0 TMA producer, 1 issues the score products (and owns TMEM), 2 the gradient products, 3 zeroes rows of padded tokens in a
+// loaded stage (their product with a weight of 0 would be NaN), 4-7 and 8-11 the weights of even and odd sub-tiles, a key (dK/dV)
+// or query (dQ) a thread. In the dK/dV kernel S^T and dP^T take turns in three 64-column buffers, freed as soon as they
+// are read. Every mbarrier wait is bounded.
+
+#include <algorithm>
+#include <atomic>
+
+#include "gtb_common.cuh"
+#include "latent.h"
+#include "latent_mma.cuh"
+#include "sdpa_args.h"
+
+namespace gtb {
+namespace {
+
+using namespace sm100;
+
+constexpr int BT = 128, SUB = 64;
+constexpr int NTHREADS = 384;
+constexpr int SB_UNITS = 4;  // (batch, head) units whose CTAs run together, heaviest tiles first, sharing their streams in L2
+constexpr uint32_t TMEM_COLS = 512;
+constexpr int SMEM_MAX = 232448;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Rows {
+    char* p;
+    int64_t s0, s1, s2;  // strides of batch, head, token (elements of 16 bits)
+    __device__ __forceinline__ uint16_t* at(int b, int h, int64_t i) const { return (uint16_t*)p + b * s0 + h * s1 + i * s2; }
+};
+
+struct Params {
+    int64_t L, S, Lpad;      // Lpad: L to a multiple of 64
+    int B, H, Hkv, group, Dr, rope_steps;
+    float scale, scale_log2;
+    int causal;
+    const int32_t* lens;
+    const float* lse;
+    float *nlse2, *ndelta;   // (B, H, Lpad)
+    float* dkr_part;         // (B, Hkv, S, Dr)
+    Rows o, g, dq, dk, dv, dkr;
+    int* status;
+};
+
+// ------------------------------------------------------------------ pre
+
+template <int DN, bool BF16>
+__global__ void __launch_bounds__(256) latent_bwd_pre_kernel(const __grid_constant__ Params p) {
+    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    constexpr int LANES = DN / 8, RPW = 32 / LANES, FLIGHT = 2;  // lanes a row, rows a warp at a time, loads in flight
+    const int lane = threadIdx.x & 31, sub = lane / LANES, c = lane % LANES;
+    const int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (RPW * FLIGHT), n = (int64_t)p.B * p.H * p.Lpad;
+    uint4 ov[FLIGHT], gv[FLIGHT];
+    int64_t row[FLIGHT];
+    bool live[FLIGHT];
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+        row[f] = row0 + f * RPW + sub;
+        ov[f] = gv[f] = make_uint4(0, 0, 0, 0);
+        live[f] = false;
+        if (row[f] >= n) continue;
+        const int64_t bh = row[f] / p.Lpad, l = row[f] - bh * p.Lpad;
+        const int b = (int)(bh / p.H), h = (int)(bh - (int64_t)b * p.H);
+        live[f] = l < latent_tokens(p.lens, b, p.L);
+        if (!live[f]) continue;
+        ov[f] = *(const uint4*)(p.o.at(b, h, l) + c * 8);
+        gv[f] = *(const uint4*)(p.g.at(b, h, l) + c * 8);
+    }
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+        const T *x = (const T*)&ov[f], *y = (const T*)&gv[f];
+        float acc = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc = fmaf(Elem<T>::load(x + e), Elem<T>::load(y + e), acc);
+#pragma unroll
+        for (int s = LANES / 2; s; s >>= 1) acc += __shfl_xor_sync(~0u, acc, s);
+        if (c == 0 && row[f] < n) {
+            const int64_t bh = row[f] / p.Lpad, l = row[f] - bh * p.Lpad;
+            const float lse = live[f] ? p.lse[bh * p.L + l] : -INFINITY;
+            p.nlse2[row[f]] = lse == -INFINITY ? -INFINITY : -lse * LOG2E;
+            p.ndelta[row[f]] = -acc;
+        }
+    }
+}
+
+// the heads' shares of the rotary keys' gradient, added in order: 4 values a thread
+template <bool BF16>
+__global__ void __launch_bounds__(256) latent_bwd_rope_kernel(const __grid_constant__ Params p) {
+    const int per = p.Dr / 4;
+    const int64_t n = (int64_t)p.B * p.S * per, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += step) {
+        const int64_t bs = e / per, b = bs / p.S, s = bs - b * p.S;
+        const int c = (int)(e - bs * per);
+        float4 a = make_float4(0, 0, 0, 0);
+        const float* x = p.dkr_part + (b * p.Hkv * p.S + s) * p.Dr + 4 * c;
+#pragma unroll 8
+        for (int h = 0; h < p.Hkv; ++h) {
+            const float4 y = *(const float4*)(x + (int64_t)h * p.S * p.Dr);
+            a.x += y.x;
+            a.y += y.y;
+            a.z += y.z;
+            a.w += y.w;
+        }
+        *(uint2*)(p.dkr.at((int)b, 0, s) + 4 * c) = make_uint2(pack2<BF16>(a.x, a.y), pack2<BF16>(a.z, a.w));
+    }
+}
+
+// ------------------------------------------------------------------ shared by both kernels
+
+// tile and (batch, head) unit of this CTA: superblocks of SB_UNITS units, their tiles outer, the units inner
+__device__ __forceinline__ void place(int tiles, int units, int& tile, int& unit) {
+    const int lin = (int)blockIdx.x, per = SB_UNITS * tiles, sb = lin / per, r = lin - sb * per;
+    const int size = min(SB_UNITS, units - sb * SB_UNITS);
+    tile = r / size;
+    unit = sb * SB_UNITS + r - tile * size;
+}
+
+// 16 accumulator columns of one row, times mul, as 16-bit values
+template <bool BF16>
+__device__ __forceinline__ void store_row16(uint16_t* dst, const uint32_t* v, float mul) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) w[i / 2] = pack2<BF16>(__uint_as_float(v[i]) * mul, __uint_as_float(v[i + 1]) * mul);
+    ((uint4*)dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    ((uint4*)dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+// rows [first, 64) of n 64-column slabs of 64 rows become zeros, by one warp
+__device__ __forceinline__ void zero_rows(unsigned char* base, int n, int first, int lane) {
+    const int per = (SUB - first) * 8;
+    for (int e = lane; e < per * n; e += 32) {
+        const int a = e / per;
+        *(uint4*)(base + a * (SUB * 128) + first * 128 + (e - a * per) * 16) = make_uint4(0, 0, 0, 0);
+    }
+}
+
+template <int DN>
+struct Sizes {
+    static constexpr int PANELS = DN / 64 + 1;
+    static constexpr int SLAB = BT * 128, SLAB64 = SUB * 128;     // a 64-column slab of 128 and of 64 rows
+    static constexpr int KTILE = PANELS * SLAB, VTILE = (DN / 64) * SLAB;
+    static constexpr int STAGE = (2 * PANELS - 1) * SLAB64;        // 64 rows of Q and G, or of K and V
+};
+
+// ------------------------------------------------------------------ dK, dV
+
+template <int DN>
+struct KvSmem {
+    using Z = Sizes<DN>;
+    static constexpr int OFF_V = Z::KTILE, OFF_ST = OFF_V + Z::VTILE;
+    static constexpr int OFF_W = OFF_ST + 2 * Z::STAGE, OFF_DS = OFF_W + 2 * BT * SUB * 2;
+    static constexpr int OFF_ROW = OFF_DS + 2 * BT * SUB * 2;      // [stage][-lse2, -delta][64]
+    static constexpr int OFF_BAR = OFF_ROW + 2 * 2 * SUB * 4;
+    static constexpr int USED = OFF_BAR + 256;
+    static constexpr int ALLOC = USED + 1023 < SMEM_MAX ? USED + 1023 : SMEM_MAX;
+    static_assert(USED <= SMEM_MAX, "shared memory");
+};
+
+struct KvBars {
+    uint64_t kv_full, st_full[2], st_empty[2], r_full[3], r_free[3], w_full[2], w_free[2], fix[2], fixed[2], final_, drain[2];
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(KvBars) <= 256, "barrier block");
+
+template <int DN, bool BF16>
+__global__ void __launch_bounds__(NTHREADS, 1)
+latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmR,
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
+    using Z = Sizes<DN>;
+    using M = KvSmem<DN>;
+    constexpr uint32_t DK_COL = DN, RING = 320;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    if (smem - smem_raw > M::ALLOC - M::USED) {
+        if (threadIdx.x == 0) atomicCAS(p.status, 0, 100);
+        return;
+    }
+    KvBars& bar = *(KvBars*)(smem + M::OFF_BAR);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int jt, unit;
+    place((int)((p.S + BT - 1) / BT), p.B * p.Hkv, jt, unit);
+    const int b = unit / p.Hkv, hk = unit - b * p.Hkv, key0 = jt * BT;
+    const int nL = latent_tokens(p.lens, b, p.L), nS = latent_tokens(p.lens, b, p.S);
+    const int i0 = p.causal ? key0 / SUB : 0;  // first sub-tile with a query that sees this key tile
+    const int nq = max(0, (nL + SUB - 1) / SUB - i0), nit = key0 < nS ? p.group * nq : 0;
+
+    if (threadIdx.x == 0) {
+        mbar_init(&bar.kv_full, 1);
+        mbar_init(&bar.final_, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.st_full[i], 1);
+            mbar_init(&bar.st_empty[i], 1);
+            mbar_init(&bar.w_full[i], 4);
+            mbar_init(&bar.w_free[i], 1);
+            mbar_init(&bar.fix[i], 1);
+            mbar_init(&bar.fixed[i], 1);
+            mbar_init(&bar.drain[i], 1);
+        }
+        for (int i = 0; i < 3; ++i) {
+            mbar_init(&bar.r_full[i], 1);
+            mbar_init(&bar.r_free[i], 4);
+        }
+        bar.abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc(&bar.tmem, TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar.tmem;
+    volatile int* abort_flag = &bar.abort;
+    // sub-tile `it`: its query head and first query
+    auto head_of = [&](int it) { return hk * p.group + it / nq; };
+    auto first_of = [&](int it) { return (i0 + it % nq) * SUB; };
+    auto padded = [&](int it) { return p.lens && first_of(it) + SUB > nL; };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0 && nit > 0) {
+            prefetch_tmap(&tmQ);
+            prefetch_tmap(&tmG);
+            mbar_expect_tx(&bar.kv_full, Z::KTILE + Z::VTILE);
+            for (int a = 0; a < DN / 64; ++a) {
+                tma_load_4d(smem + a * Z::SLAB, &tmK, a * 64, key0, hk, b, &bar.kv_full);
+                tma_load_4d(smem + M::OFF_V + a * Z::SLAB, &tmV, a * 64, key0, hk, b, &bar.kv_full);
+            }
+            tma_load_4d(smem + (DN / 64) * Z::SLAB, &tmR, 0, key0, 0, b, &bar.kv_full);
+            bool ok = true;
+            int it = 0;
+            for (; it < nit; ++it) {
+                const int st = it & 1, h = head_of(it), q = first_of(it);
+                if (it >= 2) ok = mbar_wait(&bar.st_empty[st], ((it >> 1) - 1) & 1, p.status, 101);
+                if (!ok || *abort_flag) { ok = false; break; }
+                unsigned char* d = smem + M::OFF_ST + st * Z::STAGE;
+                mbar_expect_tx(&bar.st_full[st], Z::STAGE + 2 * SUB * 4);
+                for (int a = 0; a < Z::PANELS; ++a) tma_load_4d(d + a * Z::SLAB64, &tmQ, a * 64, q, h, b, &bar.st_full[st]);
+                for (int a = 0; a < DN / 64; ++a) tma_load_4d(d + (Z::PANELS + a) * Z::SLAB64, &tmG, a * 64, q, h, b, &bar.st_full[st]);
+                const int64_t r = ((int64_t)b * p.H + h) * p.Lpad + q;
+                bulk_load(smem + M::OFF_ROW + st * 512, p.nlse2 + r, 256, &bar.st_full[st]);
+                bulk_load(smem + M::OFF_ROW + st * 512 + 256, p.ndelta + r, 256, &bar.st_full[st]);
+            }
+            if (!ok) *abort_flag = 1;
+            if (*abort_flag) {  // our copies in flight end before the CTA does
+                mbar_wait(&bar.kv_full, 0, nullptr, 0);
+                for (int n = max(0, it - 2); n < it; ++n) mbar_wait(&bar.st_full[n & 1], (n >> 1) & 1, nullptr, 0);
+            }
+        }
+    } else if (warp < 3) {
+        // ------------------------------------------------------------ MMA issuers: 1 the scores, 2 the gradients
+        const bool lead = elect_lane();
+        const uint32_t tm = (uint32_t)uniform((int)tmem);
+        const int n_it = uniform(nit);
+        bool ok = true;
+        if (warp == 1) {
+            constexpr uint32_t IDESC = idesc_f16(BT, SUB, BF16, false);
+            const uint32_t kd = desc_lo(smem_u32(smem), 16), vd = desc_lo(smem_u32(smem + M::OFF_V), 16);
+            const uint32_t sd = desc_lo(smem_u32(smem + M::OFF_ST), 16);
+            if (n_it > 0) ok = warp_wait(&bar.kv_full, 0, p.status, 102);
+            int slot = 0, round = 0, n_fix[2] = {0, 0};  // the ring buffer to fill next and how often it has been
+            for (int it = 0; it < n_it && ok; ++it) {
+                const int st = it & 1;
+                ok = warp_wait(&bar.st_full[st], (it >> 1) & 1, p.status, 103);
+                if (ok && padded(it)) {
+                    if (lead) mbar_arrive(&bar.fix[st]);
+                    ok = warp_wait(&bar.fixed[st], n_fix[st]++ & 1, p.status, 104);
+                }
+                const uint32_t q = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), g = q + (Z::PANELS * Z::SLAB64 >> 4);
+#pragma unroll
+                for (int which = 0; which < 2; ++which) {
+                    if (ok && round > 0) ok = warp_wait(&bar.r_free[slot], (round - 1) & 1, p.status, 105);
+                    if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; continue; }
+                    tc_fence_after();
+                    const uint32_t dst = tm + RING + slot * SUB;
+                    if (lead) {
+                        if (which == 0) {
+#pragma unroll
+                            for (int kk = 0; kk < DN / 16; ++kk)
+                                mma_ss_lo(dst, kd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, q + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC,
+                                          kk > 0);
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk)
+                                if (kk < p.rope_steps)
+                                    mma_ss_lo(dst, kd + (DN / 64) * (Z::SLAB >> 4) + kk * 2, q + (DN / 64) * (Z::SLAB64 >> 4) + kk * 2, IDESC, 1);
+                        } else {
+#pragma unroll
+                            for (int kk = 0; kk < DN / 16; ++kk)
+                                mma_ss_lo(dst, vd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, g + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC,
+                                          kk > 0);
+                        }
+                        mma_commit(&bar.r_full[slot]);
+                    }
+                    if (++slot == 3) slot = 0, ++round;
+                }
+            }
+        } else {
+            const uint32_t idesc_k = idesc_f16(BT, 0, BF16, true) | (uint32_t)(DN + 16 * p.rope_steps) >> 3 << 17;
+            constexpr uint32_t IDESC_V = idesc_f16(BT, DN, BF16, true);
+            const uint32_t wd = desc_lo(smem_u32(smem + M::OFF_W), 16), sd = desc_lo(smem_u32(smem + M::OFF_ST), Z::SLAB64);
+            for (int it = 0; it < n_it && ok; ++it) {
+                const int st = it & 1;
+                ok = warp_wait(&bar.w_full[st], (it >> 1) & 1, p.status, 106);
+                if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t q = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), g = q + (Z::PANELS * Z::SLAB64 >> 4);
+                const uint32_t w = (uint32_t)uniform((int)(wd + st * (BT * SUB * 2 >> 4))), ds = w + (2 * BT * SUB * 2 >> 4);
+                if (lead) {
+#pragma unroll
+                    for (int kk = 0; kk < SUB / 16; ++kk) mma_ss_lo(tm, w + kk * 2, g + kk * 128, IDESC_V, it > 0 || kk > 0);
+#pragma unroll
+                    for (int kk = 0; kk < SUB / 16; ++kk) mma_ss_lo(tm + DK_COL, ds + kk * 2, q + kk * 128, idesc_k, it > 0 || kk > 0);
+                    mma_commit(&bar.w_free[st]);
+                    mma_commit(&bar.st_empty[st]);
+                    if (it + 1 == n_it) mma_commit(&bar.final_);
+                }
+            }
+        }
+        if (!ok) *abort_flag = 1;
+        __syncwarp();
+        if (__any_sync(~0u, *abort_flag)) {
+            if (lead) mma_commit(&bar.drain[warp - 1]);
+            warp_wait(&bar.drain[warp - 1], 0, nullptr, 0);
+        }
+    } else if (warp == 3) {
+        // ------------------------------------------------------------ rows of padded tokens become zeros
+        bool ok = true;
+        int n_fix[2] = {0, 0};
+        for (int it = 0; it < nit && ok; ++it) {
+            if (!padded(it)) continue;
+            const int st = it & 1;
+            ok = warp_wait(&bar.fix[st], n_fix[st]++ & 1, p.status, 107);
+            if (!ok) break;
+            zero_rows(smem + M::OFF_ST + st * Z::STAGE, 2 * Z::PANELS - 1, max(0, nL - first_of(it)), lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.fixed[st]);
+        }
+        if (!ok) *abort_flag = 1;
+    } else {
+        // ------------------------------------------------------------ weights: warpgroup wg takes the sub-tiles it % 2 == wg
+        const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, key = key0 + r;
+        const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+        unsigned char* w_row = smem + M::OFF_W + wg * (BT * SUB * 2) + r * 128;
+        unsigned char* ds_row = smem + M::OFF_DS + wg * (BT * SUB * 2) + r * 128;
+        const float* nl = (const float*)(smem + M::OFF_ROW + wg * 512);
+        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
+        bool ok = true;
+        for (int it = wg; it < nit; it += 2) {
+            const int n = 2 * it, s0 = n % 3, s1 = (n + 1) % 3, q0 = first_of(it);
+            ok = warp_wait(&bar.st_full[wg], (it >> 1) & 1, p.status, 108);  // the rows' lse and delta
+            if (ok) ok = warp_wait(&bar.r_full[s0], (n / 3) & 1, p.status, 109);
+            if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            uint32_t ra[64], rb[64];
+            tmem_ld32(tmem + lane_addr + RING + s0 * SUB, ra);
+            tmem_ld32(tmem + lane_addr + RING + s0 * SUB + 32, ra + 32);
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.r_free[s0]);
+#pragma unroll
+            for (int i = 0; i < SUB; i += 2) {
+                float a0, a1;
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(ra[i]), __uint_as_float(ra[i + 1])), sc2, *(const uint64_t*)(nl + i)), a0, a1);
+                ra[i] = __float_as_uint(ex2(a0));
+                ra[i + 1] = __float_as_uint(ex2(a1));
+            }
+            if (p.causal && q0 < key0 + BT - 1) {
+#pragma unroll
+                for (int i = 0; i < SUB; ++i)
+                    if (key > q0 + i) ra[i] = 0u;
+            }
+            ok = warp_wait(&bar.r_full[s1], ((n + 1) / 3) & 1, p.status, 110);
+            if (!ok) break;
+            tc_fence_after();
+            tmem_ld32(tmem + lane_addr + RING + s1 * SUB, rb);
+            tmem_ld32(tmem + lane_addr + RING + s1 * SUB + 32, rb + 32);
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.r_free[s1]);
+            if (it >= 2) ok = warp_wait(&bar.w_free[wg], ((it >> 1) - 1) & 1, p.status, 111);
+            if (!ok) break;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {  // 16 bytes of W^T and of dS^T: 8 queries
+                uint32_t wv[4], dv[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 8 * j + 2 * e;
+                    const float p0 = __uint_as_float(ra[i]), p1 = __uint_as_float(ra[i + 1]);
+                    float d0, d1;
+                    f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack(__uint_as_float(rb[i]), __uint_as_float(rb[i + 1])),
+                                                             *(const uint64_t*)(nl + SUB + i))), d0, d1);
+                    wv[e] = pack2<BF16>(p0, p1);
+                    dv[e] = pack2<BF16>(d0, d1);
+                }
+                *(uint4*)(w_row + ((j ^ (r & 7)) << 4)) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
+                *(uint4*)(ds_row + ((j ^ (r & 7)) << 4)) = make_uint4(dv[0], dv[1], dv[2], dv[3]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.w_full[wg]);
+        }
+        if (nit > 0 && ok) ok = warp_wait(&bar.final_, 0, p.status, 112);
+        if (!ok) *abort_flag = 1;
+        if (ok && !__any_sync(~0u, *abort_flag)) {
+            tc_fence_after();
+            const bool live = nit > 0 && key < nS;  // others: no query sees the key, or it is a padded one
+            constexpr int PARTS = 2 * DN / 16;       // 16-column parts of dV and dK; the rotary ones behind them
+            const int parts = PARTS + p.Dr / 16;
+            for (int c = wg; c < parts; c += 2) {
+                uint32_t v[16];
+                tmem_ldx<16>(tmem + lane_addr + c * 16, v);
+                tmem_ld_wait();
+                if (!live) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = 0u;
+                }
+                if (key >= p.S) {
+                } else if (c < DN / 16) {
+                    store_row16<BF16>(p.dv.at(b, hk, key) + c * 16, v, 1.0f);
+                } else if (c < PARTS) {
+                    store_row16<BF16>(p.dk.at(b, hk, key) + c * 16 - DN, v, p.scale);
+                } else {
+                    float4* d = (float4*)(p.dkr_part + (((int64_t)b * p.Hkv + hk) * p.S + key) * p.Dr + (c - PARTS) * 16);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        d[i] = make_float4(__uint_as_float(v[4 * i]) * p.scale, __uint_as_float(v[4 * i + 1]) * p.scale,
+                                           __uint_as_float(v[4 * i + 2]) * p.scale, __uint_as_float(v[4 * i + 3]) * p.scale);
+                }
+                __syncwarp();
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+// ------------------------------------------------------------------ dQ
+
+constexpr int Q_STAGES = 3;
+
+template <int DN>
+struct QSmem {
+    using Z = Sizes<DN>;
+    static constexpr int OFF_G = Z::KTILE, OFF_ST = OFF_G + Z::VTILE;
+    static constexpr int OFF_BAR = OFF_ST + Q_STAGES * Z::STAGE;
+    static constexpr int USED = OFF_BAR + 256;
+    static constexpr int ALLOC = USED + 1023;
+    static_assert(ALLOC <= SMEM_MAX, "shared memory");
+};
+
+struct QBars {
+    uint64_t q_full, st_full[Q_STAGES], st_empty[Q_STAGES], s_full[2], ds_full[2], ds_free[2], fix, fixed, final_, drain[2];
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(QBars) <= 256, "barrier block");
+
+template <int DN, bool BF16>
+__global__ void __launch_bounds__(NTHREADS, 1)
+latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
+                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmR,
+                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
+    using Z = Sizes<DN>;
+    using M = QSmem<DN>;
+    constexpr uint32_t S_COL = 256, DP_COL = 384;  // dQ from 0; S and dP of sub-tile h at + 64 h
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    QBars& bar = *(QBars*)(smem + M::OFF_BAR);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int tile, unit;
+    const int n_qt = (int)((p.L + BT - 1) / BT);
+    place(n_qt, p.B * p.H, tile, unit);
+    if (p.causal) tile = n_qt - 1 - tile;
+    const int b = unit / p.H, h = unit - b * p.H, hk = h / p.group, row0 = tile * BT;
+    const int nL = latent_tokens(p.lens, b, p.L), nS = latent_tokens(p.lens, b, p.S);
+    const int all = (nS + SUB - 1) / SUB;
+    const int nit = row0 >= nL ? 0 : p.causal ? min(all, (min(row0 + BT, nL) - 1) / SUB + 1) : all;
+
+    if (threadIdx.x == 0) {
+        mbar_init(&bar.q_full, 1);
+        mbar_init(&bar.final_, 1);
+        mbar_init(&bar.fix, 1);
+        mbar_init(&bar.fixed, 1);
+        for (int i = 0; i < Q_STAGES; ++i) {
+            mbar_init(&bar.st_full[i], 1);
+            mbar_init(&bar.st_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.ds_full[i], 4);
+            mbar_init(&bar.ds_free[i], 1);
+            mbar_init(&bar.drain[i], 1);
+        }
+        bar.abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc(&bar.tmem, TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar.tmem;
+    volatile int* abort_flag = &bar.abort;
+    auto padded = [&](int it) { return p.lens && (it + 1) * SUB > nS; };  // (the last sub-tile only)
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        if (lane == 0 && nit > 0) {
+            prefetch_tmap(&tmK);
+            prefetch_tmap(&tmR);
+            prefetch_tmap(&tmV);
+            mbar_expect_tx(&bar.q_full, Z::KTILE + Z::VTILE);
+            for (int a = 0; a < Z::PANELS; ++a) tma_load_4d(smem + a * Z::SLAB, &tmQ, a * 64, row0, h, b, &bar.q_full);
+            for (int a = 0; a < DN / 64; ++a) tma_load_4d(smem + M::OFF_G + a * Z::SLAB, &tmG, a * 64, row0, h, b, &bar.q_full);
+            bool ok = true;
+            int it = 0;
+            for (; it < nit; ++it) {
+                const int st = it % Q_STAGES;
+                if (it >= Q_STAGES) ok = mbar_wait(&bar.st_empty[st], (it / Q_STAGES - 1) & 1, p.status, 121);
+                if (!ok || *abort_flag) { ok = false; break; }
+                unsigned char* d = smem + M::OFF_ST + st * Z::STAGE;
+                mbar_expect_tx(&bar.st_full[st], Z::STAGE);
+                for (int a = 0; a < DN / 64; ++a) tma_load_4d(d + a * Z::SLAB64, &tmK, a * 64, it * SUB, hk, b, &bar.st_full[st]);
+                tma_load_4d(d + (DN / 64) * Z::SLAB64, &tmR, 0, it * SUB, 0, b, &bar.st_full[st]);
+                for (int a = 0; a < DN / 64; ++a)
+                    tma_load_4d(d + (Z::PANELS + a) * Z::SLAB64, &tmV, a * 64, it * SUB, hk, b, &bar.st_full[st]);
+            }
+            if (!ok) *abort_flag = 1;
+            if (*abort_flag) {
+                mbar_wait(&bar.q_full, 0, nullptr, 0);
+                for (int n = max(0, it - Q_STAGES); n < it; ++n) mbar_wait(&bar.st_full[n % Q_STAGES], (n / Q_STAGES) & 1, nullptr, 0);
+            }
+        }
+    } else if (warp < 3) {
+        // ------------------------------------------------------------ MMA issuers: 1 the scores, 2 dQ
+        const bool lead = elect_lane();
+        const uint32_t tm = (uint32_t)uniform((int)tmem);
+        const int n_it = uniform(nit);
+        bool ok = true;
+        int st = 0, phase = 0;
+        if (warp == 1) {
+            constexpr uint32_t IDESC = idesc_f16(BT, SUB, BF16, false);
+            const uint32_t qd = desc_lo(smem_u32(smem), 16), gd = desc_lo(smem_u32(smem + M::OFF_G), 16);
+            const uint32_t sd = desc_lo(smem_u32(smem + M::OFF_ST), 16);
+            if (n_it > 0) ok = warp_wait(&bar.q_full, 0, p.status, 122);
+            for (int it = 0; it < n_it && ok; ++it) {
+                ok = warp_wait(&bar.st_full[st], phase, p.status, 123);
+                if (ok && padded(it)) {
+                    if (lead) mbar_arrive(&bar.fix);
+                    ok = warp_wait(&bar.fixed, 0, p.status, 124);
+                }
+                // S's columns hold the dS that the product two sub-tiles ago read
+                if (ok && it >= 2) ok = warp_wait(&bar.ds_free[it & 1], ((it >> 1) - 1) & 1, p.status, 125);
+                if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t k = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), v = k + (Z::PANELS * Z::SLAB64 >> 4);
+                const uint32_t s_dst = tm + S_COL + (it & 1) * SUB, p_dst = tm + DP_COL + (it & 1) * SUB;
+                if (lead) {
+#pragma unroll
+                    for (int kk = 0; kk < DN / 16; ++kk)
+                        mma_ss_lo(s_dst, qd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, k + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC, kk > 0);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        if (kk < p.rope_steps)
+                            mma_ss_lo(s_dst, qd + (DN / 64) * (Z::SLAB >> 4) + kk * 2, k + (DN / 64) * (Z::SLAB64 >> 4) + kk * 2, IDESC, 1);
+#pragma unroll
+                    for (int kk = 0; kk < DN / 16; ++kk)
+                        mma_ss_lo(p_dst, gd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, v + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC, kk > 0);
+                    mma_commit(&bar.s_full[it & 1]);
+                }
+                if (++st == Q_STAGES) st = 0, phase ^= 1;
+            }
+        } else {
+            const uint32_t idesc = idesc_f16(BT, 0, BF16, true) | (uint32_t)(DN + 16 * p.rope_steps) >> 3 << 17;
+            const uint32_t sd = desc_lo(smem_u32(smem + M::OFF_ST), Z::SLAB64);
+            for (int it = 0; it < n_it && ok; ++it) {
+                ok = warp_wait(&bar.ds_full[it & 1], (it >> 1) & 1, p.status, 126);
+                if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t k = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), ds = tm + S_COL + (it & 1) * SUB;
+                if (lead) {
+#pragma unroll
+                    for (int kk = 0; kk < SUB / 16; ++kk) mma_ts_lo(tm, ds + kk * 8, k + kk * 128, idesc, it > 0 || kk > 0);
+                    mma_commit(&bar.ds_free[it & 1]);
+                    mma_commit(&bar.st_empty[st]);
+                    if (it + 1 == n_it) mma_commit(&bar.final_);
+                }
+                if (++st == Q_STAGES) st = 0;
+            }
+        }
+        if (!ok) *abort_flag = 1;
+        __syncwarp();
+        if (__any_sync(~0u, *abort_flag)) {
+            if (lead) mma_commit(&bar.drain[warp - 1]);
+            warp_wait(&bar.drain[warp - 1], 0, nullptr, 0);
+        }
+    } else if (warp == 3) {
+        // ------------------------------------------------------------ rows of padded tokens become zeros
+        if (nit > 0 && padded(nit - 1)) {
+            const bool ok = warp_wait(&bar.fix, 0, p.status, 127);
+            if (ok) {
+                zero_rows(smem + M::OFF_ST + ((nit - 1) % Q_STAGES) * Z::STAGE, 2 * Z::PANELS - 1, max(0, nS - (nit - 1) * SUB), lane);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.fixed);
+            } else {
+                *abort_flag = 1;
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ dS: warpgroup wg takes the sub-tiles it % 2 == wg
+        const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, row = row0 + r;
+        const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+        const uint32_t s_tmem = tmem + lane_addr + S_COL + wg * SUB, p_tmem = tmem + lane_addr + DP_COL + wg * SUB;
+        const int64_t rr = ((int64_t)b * p.H + h) * p.Lpad + row;
+        const float nl = row < p.Lpad ? p.nlse2[rr] : -INFINITY, nd = row < p.Lpad ? p.ndelta[rr] : 0.0f;
+        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nl2 = f2_pack(nl, nl), nd2 = f2_pack(nd, nd);
+        const int lim = p.causal ? min(nS - 1, row) : nS - 1;  // last key this row sees
+        bool ok = true;
+        for (int it = wg; it < nit; it += 2) {
+            ok = warp_wait(&bar.s_full[wg], (it >> 1) & 1, p.status, 128);
+            if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            const int kv0 = it * SUB;
+            const bool mask = kv0 + SUB > nS || (p.causal && kv0 + SUB - 1 > row0);
+            uint32_t ra[64], rb[64];
+            tmem_ld32(s_tmem, ra);
+            tmem_ld32(s_tmem + 32, ra + 32);
+            tmem_ld32(p_tmem, rb);
+            tmem_ld32(p_tmem + 32, rb + 32);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t dk[16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const int k = 32 * c + i;
+                    float a0, a1, d0, d1;
+                    f2_unpack(f2_fma(f2_pack(__uint_as_float(ra[k]), __uint_as_float(ra[k + 1])), sc2, nl2), a0, a1);
+                    a0 = ex2(a0);
+                    a1 = ex2(a1);
+                    if (mask) {
+                        if (kv0 + k > lim) a0 = 0.0f;
+                        if (kv0 + k + 1 > lim) a1 = 0.0f;
+                    }
+                    f2_unpack(f2_mul(f2_pack(a0, a1), f2_add(f2_pack(__uint_as_float(rb[k]), __uint_as_float(rb[k + 1])), nd2)), d0, d1);
+                    dk[i / 2] = pack2<BF16>(d0, d1);
+                }
+                tmem_st16(s_tmem + 16 * c, dk);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.ds_full[wg]);
+        }
+        if (nit > 0 && ok) ok = warp_wait(&bar.final_, 0, p.status, 129);
+        if (!ok) *abort_flag = 1;
+        if (ok && !__any_sync(~0u, *abort_flag)) {
+            tc_fence_after();
+            const bool live = nit > 0 && row < nL;
+            const int parts = (DN + p.Dr) / 16;
+            for (int c = wg; c < parts; c += 2) {
+                uint32_t v[16];
+                tmem_ldx<16>(tmem + lane_addr + c * 16, v);
+                tmem_ld_wait();
+                if (!live) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] = 0u;
+                }
+                if (row < p.L) store_row16<BF16>(p.dq.at(b, h, row) + c * 16, v, p.scale);
+                __syncwarp();
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+Rows rows(const gtb_tensor4& t) { return Rows{(char*)t.data, t.stride[0], t.stride[1], t.stride[2]}; }
+
+template <int DN, bool BF16>
+int launch(const LatentSdpaArgs& a, cudaStream_t st) {
+    const char* ctx = "latent_sdpa_bwd";
+    auto kv = latent_bwd_kv_kernel<DN, BF16>;
+    auto kq = latent_bwd_q_kernel<DN, BF16>;
+    int dev = 0;
+    if (cuda_failed(cudaGetDevice(&dev), ctx)) return -1;
+    static std::atomic<uint64_t> ready{0};  // devices (of the first 64) whose kernels are set up
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(ready.load() & bit)) {
+        if (cuda_failed(cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, KvSmem<DN>::ALLOC), ctx) ||
+            cuda_failed(cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, QSmem<DN>::ALLOC), ctx))
+            return -1;
+        ready.fetch_or(bit);
+    }
+    const int64_t ctas_kv = (a.S + BT - 1) / BT * a.B * a.Hkv, ctas_q = (a.L + BT - 1) / BT * a.B * a.H;
+    if (ctas_kv > INT32_MAX || ctas_q > INT32_MAX) {
+        set_errorf("%s: too many tiles", ctx);
+        return -1;
+    }
+    // 128-row maps of what stays, 64-row maps of what streams
+    CUtensorMap q128, q64, g128, g64, k128, k64, r128, r64, v128, v64;
+    if (!make_tma_map_4d(&q128, a.q, DN + a.Dr, BF16, BT) || !make_tma_map_4d(&q64, a.q, DN + a.Dr, BF16, SUB) ||
+        !make_tma_map_4d(&g128, a.g, DN, BF16, BT) || !make_tma_map_4d(&g64, a.g, DN, BF16, SUB) ||
+        !make_tma_map_4d(&k128, a.k, DN, BF16, BT) || !make_tma_map_4d(&k64, a.k, DN, BF16, SUB) ||
+        !make_tma_map_4d(&r128, a.k_rope, a.Dr, BF16, BT) || !make_tma_map_4d(&r64, a.k_rope, a.Dr, BF16, SUB) ||
+        !make_tma_map_4d(&v128, a.v, DN, BF16, BT) || !make_tma_map_4d(&v64, a.v, DN, BF16, SUB))
+        return -1;
+    Params p{};
+    p.L = a.L;
+    p.S = a.S;
+    p.Lpad = (a.L + SUB - 1) / SUB * SUB;
+    p.B = (int)a.B;
+    p.H = (int)a.H;
+    p.Hkv = (int)a.Hkv;
+    p.group = (int)(a.H / a.Hkv);
+    p.Dr = a.Dr;
+    p.rope_steps = a.Dr / 16;
+    p.scale = a.scale;
+    p.scale_log2 = a.scale * LOG2E;
+    p.causal = a.causal;
+    p.lens = a.lens;
+    p.lse = a.lse;
+    p.o = rows(a.o);
+    p.g = rows(a.g);
+    p.dq = rows(a.dq);
+    p.dk = rows(a.dk);
+    p.dv = rows(a.dv);
+    p.dkr = rows(a.dk_rope);
+    p.status = a.status;
+    const int64_t n_row = a.B * a.H * p.Lpad, n_part = a.B * a.Hkv * a.S * a.Dr;
+    float* ws = nullptr;
+    if (cuda_failed(cudaMallocAsync((void**)&ws, (2 * n_row + n_part) * sizeof(float), st), "latent_sdpa_bwd: scratch")) return -1;
+    p.nlse2 = ws;
+    p.ndelta = ws + n_row;
+    p.dkr_part = ws + 2 * n_row;
+    constexpr int ROWS = 8 * (32 / (DN / 8)) * 2;  // rows a block of the first kernel
+    latent_bwd_pre_kernel<DN, BF16><<<(unsigned)((n_row + ROWS - 1) / ROWS), 256, 0, st>>>(p);
+    kv<<<(unsigned)ctas_kv, NTHREADS, KvSmem<DN>::ALLOC, st>>>(q64, g64, k128, r128, v128, p);
+    kq<<<(unsigned)ctas_q, NTHREADS, QSmem<DN>::ALLOC, st>>>(q128, g128, k64, r64, v64, p);
+    latent_bwd_rope_kernel<BF16><<<(unsigned)std::min<int64_t>(4096, (a.B * a.S * (a.Dr / 4) + 255) / 256), 256, 0, st>>>(p);
+    const int rc = cuda_failed(cudaGetLastError(), "latent_sdpa_bwd launch") ? -1 : 0;
+    cudaFreeAsync(ws, st);
+    return rc;
+}
+
+}  // namespace
+
+int launch_latent_sdpa_bwd(const LatentSdpaArgs& a, cudaStream_t st) {
+    const bool bf16 = a.q.dtype == BF16;
+    if (a.Dn == 128) return bf16 ? launch<128, true>(a, st) : launch<128, false>(a, st);
+    return bf16 ? launch<64, true>(a, st) : launch<64, false>(a, st);
+}
+
+}  // namespace gtb

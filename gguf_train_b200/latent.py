@@ -23,6 +23,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _C
 from .functional import _autocast_lower, _require_cuda, scaled_dot_product_attention
@@ -193,6 +194,59 @@ def _sdpa_general(q, k, k_rope, v, is_causal, scale, seq_lens):
     return torch.where(held[:, None, :, None], out, torch.zeros((), dtype=out.dtype, device=out.device))
 
 
+def _on_tensor_cores(q, k, k_rope, v) -> bool:
+    """The sizes that the native expanded kernels take; others go by scaled_dot_product_attention."""
+    Dn, Dr = k.shape[3], k_rope.shape[2]
+    return q.dtype in _STORED and Dn in (64, 128) and v.shape[3] == Dn and Dr % 16 == 0 and 16 <= Dr <= 64 and \
+        q.shape[0] <= 65535 and q.shape[1] <= 65535 and min(q.shape) > 0 and min(k.shape) > 0
+
+
+def _t4(t: torch.Tensor) -> bytes:
+    return _C.tensor4(t, _CODE[t.dtype])
+
+
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An empty tensor of t's shape, in t's layout where that is dense (q as a view of its projection)."""
+    out = torch.empty_like(t)
+    return out if _tiled(out) is out else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+class LatentSDPAFn(torch.autograd.Function):
+    """latent_sdpa on the native kernels: apply(q, k, k_rope, v, is_causal, scale, seq_lens). The backward recomputes the weights
+    from the saved log-sum-exp."""
+
+    @staticmethod
+    def _forward(q, k, k_rope, v, is_causal, scale, seq_lens, need_lse):
+        q, k, kr, v = _tiled(q), _tiled(k), _tiled(k_rope), _tiled(v)
+        out = q.new_empty(q.shape[:3] + (v.shape[3],))
+        lse = q.new_empty(q.shape[:3], dtype=torch.float32) if need_lse else None
+        rc = _C.lib.gtb_latent_sdpa_fwd(_t4(q), _t4(k), _t4(kr[:, None]), _t4(v), None if seq_lens is None else seq_lens.data_ptr(),
+                                        scale, 1 if is_causal else 0, _t4(out), None if lse is None else lse.data_ptr(),
+                                        _stream(q.device))
+        _C.check_rc(rc, "latent_sdpa")
+        return q, k, kr, v, out, lse
+
+    @staticmethod
+    def forward(ctx, q, k, k_rope, v, is_causal, scale, seq_lens):
+        q, k, kr, v, out, lse = LatentSDPAFn._forward(q, k, k_rope, v, is_causal, scale, seq_lens, True)
+        ctx.args = is_causal, scale
+        ctx.save_for_backward(q, k, kr, v, out, lse, seq_lens)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, kr, v, out, lse, seq_lens = ctx.saved_tensors
+        is_causal, scale = ctx.args
+        g = _tiled(grad_out)
+        dq, dk, dkr, dv = _like(q), _like(k), torch.empty_like(kr, memory_format=torch.contiguous_format), _like(v)
+        rc = _C.lib.gtb_latent_sdpa_bwd(_t4(g), _t4(q), _t4(k), _t4(kr[:, None]), _t4(v), _t4(out), lse.data_ptr(),
+                                        None if seq_lens is None else seq_lens.data_ptr(), scale, 1 if is_causal else 0, _t4(dq),
+                                        _t4(dk), _t4(dkr[:, None]), _t4(dv), _stream(q.device))
+        _C.check_rc(rc, "latent_sdpa_bwd")
+        return dq, dk, dkr, dv, None, None, None
+
+
 def latent_sdpa(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor, v: torch.Tensor, is_causal: bool = False,
                 scale: float | None = None, seq_lens: torch.Tensor | None = None) -> torch.Tensor:
     """Attention whose keys have a part of their own for each head and a rotary part that the heads share: q (B, H, L, Dn + Dr),
@@ -229,4 +283,10 @@ def latent_sdpa(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor, v: torch
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (math.isfinite(scale) and scale > 0.0):
         raise RuntimeError(f"latent_sdpa: scale must be positive and finite, got {scale}")
-    return _sdpa_general(q, k, k_rope, v, bool(is_causal), scale, seq_lens)
+    if not _on_tensor_cores(q, k, k_rope, v):
+        return _sdpa_general(q, k, k_rope, v, bool(is_causal), scale, seq_lens)
+    xs = (q, k, k_rope, v)
+    # (tensors of forward mode take the Function too, which refuses them)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in xs) or any(unpack_dual(t).tangent is not None for t in xs):
+        return LatentSDPAFn.apply(*xs, bool(is_causal), scale, seq_lens)
+    return LatentSDPAFn._forward(*xs, bool(is_causal), scale, seq_lens, False)[4]

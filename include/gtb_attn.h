@@ -361,6 +361,23 @@ GTB_API int gtb_latent_append(const gtb_latent *cache, const gtb_tensor4 *latent
 GTB_API int gtb_latent_attention(const gtb_tensor4 *q, const gtb_latent *cache, const gtb_latent *prefix, float scale,
                                  const int32_t *counts, gtb_tensor4 *out, float *lse, void *stream);
 
+/* Attention in the expanded form, for prompts and training: q (B,H,L,Dn+Dr), k (B,Hkv,S,Dn), k_rope (B,1,S,Dr) shared by the
+ * heads, v (B,Hkv,S,Dn); f16 or bf16 (one dtype), Dn 64 or 128, Dr a multiple of 16 from 16 to 64, H % Hkv == 0;
+ *   score = scale * (q[..Dn] . k + q[Dn..] . k_rope), out (B,H,L,Dn); is_causal masks s > l (top-left aligned).
+ *   seq_lens: NULL, or device int32 (B) with L = S: tokens from seq_lens[b] (clamped to [0, S]) on are not attended, whatever
+ *   they hold; their out is 0, and all their gradients.
+ *   lse: NULL or (B,H,L) f32, -inf where nothing is attended (out is 0 there).
+ * All tensors start on 16 bytes, with a unit innermost stride and others that are positive multiples of 8.
+ * The backward takes the forward's out and lse and writes dq, dk, dk_rope (summed over all heads) and dv, in fixed order:
+ * the same bits on every run. Its scratch (4 (2 B H L + B Hkv S Dr) bytes) comes from the stream-ordered allocator. */
+GTB_API int gtb_latent_sdpa_fwd(const gtb_tensor4 *q, const gtb_tensor4 *k, const gtb_tensor4 *k_rope, const gtb_tensor4 *v,
+                                const int32_t *seq_lens, float scale, int is_causal, gtb_tensor4 *out, float *lse,
+                                void *stream);
+GTB_API int gtb_latent_sdpa_bwd(const gtb_tensor4 *grad_out, const gtb_tensor4 *q, const gtb_tensor4 *k,
+                                const gtb_tensor4 *k_rope, const gtb_tensor4 *v, const gtb_tensor4 *out, const float *lse,
+                                const int32_t *seq_lens, float scale, int is_causal, gtb_tensor4 *dq, gtb_tensor4 *dk,
+                                gtb_tensor4 *dk_rope, gtb_tensor4 *dv, void *stream);
+
 /* Kernel family of the calling thread's last gtb_sdpa_fwd / gtb_sdpa_fwd_rope / gtb_sdpa_bwd call:
  * "tcgen05" (tensor cores, TMA), "tcgen05+rope" (the same with q rotated inside the kernel),
  * "f32_tiled" (fp32 with head size 64, register-blocked on the CUDA cores) or "simt" (one warp per
