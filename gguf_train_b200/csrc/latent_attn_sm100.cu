@@ -854,8 +854,7 @@ __global__ void latent_nothing_kernel(uint16_t* o, int64_t n, float* lse, int64_
 // 4-D map of 16-bit values with a 64-column box and 128-byte swizzle; sizes and strides (elements) from the second dimension on
 bool make_map(CUtensorMap* tm, const void* base, bool bf16, int64_t cols, const int64_t (&size)[3], const int64_t (&stride)[3],
               const int (&box)[3]) {
-    auto enc = encode_fn();
-    if (!enc) {
+    if (!encode_fn()) {
         set_error("latent_attention: cuTensorMapEncodeTiled is unavailable");
         return false;
     }
@@ -868,10 +867,8 @@ bool make_map(CUtensorMap* tm, const void* base, bool bf16, int64_t cols, const 
         }
         st[i] = (cuuint64_t)bytes;
     }
-    const cuuint32_t bx[4] = {64, (cuuint32_t)box[0], (cuuint32_t)box[1], (cuuint32_t)box[2]}, es[4] = {1, 1, 1, 1};
-    const CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, (void*)base, dims, st,
-                           bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint32_t bx[4] = {64, (cuuint32_t)box[0], (cuuint32_t)box[1], (cuuint32_t)box[2]};
+    const CUresult r = encode_tiled_4d(tm, bf16, (void*)base, dims, st, bx);
     if (r != CUDA_SUCCESS) {
         set_errorf("latent_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
         return false;

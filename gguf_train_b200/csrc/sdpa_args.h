@@ -75,6 +75,8 @@ size_t bwd_simt_scratch_bytes(const BwdArgs& a);
 // TMA: the driver's tensor-map encoder (nullptr if unavailable) and a 4-D (d, row, head, batch) map of
 // a 16-bit tensor with a 64 x box_rows box and 128-byte swizzle.
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
+// the encoder for 16-bit values in four dimensions, in this thread whether or not it has a current context (encode_fn() not null)
+CUresult encode_tiled_4d(CUtensorMap* tm, bool bf16, void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box);
 bool make_tma_map_4d(CUtensorMap* tm, const gtb_tensor4& t, int64_t d_extent, bool bf16, int box_rows);
 
 // tcgen05/TMA forward: bf16/f16, D == Dv in {64,128}, unit inner stride, no mask.
