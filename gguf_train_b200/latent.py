@@ -148,6 +148,18 @@ def _tiled(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _rows(t: torch.Tensor, code: int):
+    """_tiled(t), and the tensor4 of it (of k_rope with a dimension for its one head)."""
+    s, p = t.stride(), t.data_ptr()
+    if s[-1] != 1 or (p | s[0] << 1 | s[1] << 1 | s[-2] << 1) & 15 or min(s) <= 0:
+        t = _tiled(t)
+        s, p = t.stride(), t.data_ptr()
+    n = t.shape
+    if len(n) == 4:
+        return t, _C._pack4(p, *n, *s, code)
+    return t, _C._pack4(p, n[0], 1, n[1], n[2], s[0], s[0], s[1], s[2], code)
+
+
 def latent_attention(q: torch.Tensor, cache: LatentCache, scale: float, counts: torch.Tensor | None = None,
                      prefix: LatentCache | None = None, need_lse: bool = False):
     """Causal attention of q (B, H, Lq, latent_dim + rope_dim), in the cache's type, over the cache, which already holds the
@@ -170,11 +182,12 @@ def latent_attention(q: torch.Tensor, cache: LatentCache, scale: float, counts: 
     scale = float(scale)
     if not (math.isfinite(scale) and scale > 0.0):
         raise RuntimeError(f"latent_attention: scale must be positive and finite, got {scale}")
-    q = _tiled(q)
-    out = q.new_empty(q.shape[:3] + (cache._latent_dim,))
-    lse = q.new_empty(q.shape[:3], dtype=torch.float32) if need_lse else None
     code = _CODE[q.dtype]
-    rc = _C.lib.gtb_latent_attention(_C.tensor4(q, code), ctypes.byref(cache._native),
+    q, qt = _rows(q, code)
+    H, Lq = q.shape[1:3]
+    out = torch.empty((B, H, Lq, cache._latent_dim), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device) if need_lse else None
+    rc = _C.lib.gtb_latent_attention(qt, ctypes.byref(cache._native),
                                      None if prefix is None else ctypes.byref(prefix._native), scale,
                                      _counts("latent_attention", counts, B), _C.tensor4(out, code),
                                      None if lse is None else lse.data_ptr(), _stream(q.device))
@@ -201,10 +214,6 @@ def _on_tensor_cores(q, k, k_rope, v) -> bool:
         q.shape[0] <= 65535 and q.shape[1] <= 65535 and min(q.shape) > 0 and min(k.shape) > 0
 
 
-def _t4(t: torch.Tensor) -> bytes:
-    return _C.tensor4(t, _CODE[t.dtype])
-
-
 def _like(t: torch.Tensor) -> torch.Tensor:
     """An empty tensor of t's shape, in t's layout where that is dense (q as a view of its projection)."""
     out = torch.empty_like(t)
@@ -217,11 +226,13 @@ class LatentSDPAFn(torch.autograd.Function):
 
     @staticmethod
     def _forward(q, k, k_rope, v, is_causal, scale, seq_lens, need_lse):
-        q, k, kr, v = _tiled(q), _tiled(k), _tiled(k_rope), _tiled(v)
-        out = q.new_empty(q.shape[:3] + (v.shape[3],))
-        lse = q.new_empty(q.shape[:3], dtype=torch.float32) if need_lse else None
-        rc = _C.lib.gtb_latent_sdpa_fwd(_t4(q), _t4(k), _t4(kr[:, None]), _t4(v), None if seq_lens is None else seq_lens.data_ptr(),
-                                        scale, 1 if is_causal else 0, _t4(out), None if lse is None else lse.data_ptr(),
+        code = _CODE[q.dtype]
+        (q, qt), (k, kt), (kr, rt), (v, vt) = _rows(q, code), _rows(k, code), _rows(k_rope, code), _rows(v, code)
+        B, H, L, _ = q.shape
+        out = torch.empty((B, H, L, v.shape[3]), dtype=q.dtype, device=q.device)
+        lse = torch.empty((B, H, L), dtype=torch.float32, device=q.device) if need_lse else None
+        rc = _C.lib.gtb_latent_sdpa_fwd(qt, kt, rt, vt, None if seq_lens is None else seq_lens.data_ptr(), scale,
+                                        1 if is_causal else 0, _C.tensor4(out, code), None if lse is None else lse.data_ptr(),
                                         _stream(q.device))
         _C.check_rc(rc, "latent_sdpa")
         return q, k, kr, v, out, lse
@@ -238,11 +249,14 @@ class LatentSDPAFn(torch.autograd.Function):
     def backward(ctx, grad_out):
         q, k, kr, v, out, lse, seq_lens = ctx.saved_tensors
         is_causal, scale = ctx.args
-        g = _tiled(grad_out)
+        code = _CODE[q.dtype]
+        g, gt = _rows(grad_out, code)
+        qt, kt, rt, vt = (_rows(t, code)[1] for t in (q, k, kr, v))
         dq, dk, dkr, dv = _like(q), _like(k), torch.empty_like(kr, memory_format=torch.contiguous_format), _like(v)
-        rc = _C.lib.gtb_latent_sdpa_bwd(_t4(g), _t4(q), _t4(k), _t4(kr[:, None]), _t4(v), _t4(out), lse.data_ptr(),
-                                        None if seq_lens is None else seq_lens.data_ptr(), scale, 1 if is_causal else 0, _t4(dq),
-                                        _t4(dk), _t4(dkr[:, None]), _t4(dv), _stream(q.device))
+        rc = _C.lib.gtb_latent_sdpa_bwd(gt, qt, kt, rt, vt, _C.tensor4(out, code), lse.data_ptr(),
+                                        None if seq_lens is None else seq_lens.data_ptr(), scale, 1 if is_causal else 0,
+                                        _C.tensor4(dq, code), _C.tensor4(dk, code), _rows(dkr, code)[1], _C.tensor4(dv, code),
+                                        _stream(q.device))
         _C.check_rc(rc, "latent_sdpa_bwd")
         return dq, dk, dkr, dv, None, None, None
 
@@ -261,24 +275,25 @@ def latent_sdpa(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor, v: torch
         with torch.autocast("cuda", enabled=False):
             return latent_sdpa(*lowered, is_causal=is_causal, scale=scale, seq_lens=seq_lens)
     _require_cuda("latent_sdpa", q, k, k_rope, v, seq_lens)
-    if q.ndim != 4 or k.ndim != 4 or k_rope.ndim != 3 or v.ndim != 4:
+    qs, ks, rs, vs, dt, dev = q.shape, k.shape, k_rope.shape, v.shape, q.dtype, q.device
+    if len(qs) != 4 or len(ks) != 4 or len(rs) != 3 or len(vs) != 4:
         raise RuntimeError("latent_sdpa: q, k and v must have four dimensions and k_rope three")
-    B, H, L, D = q.shape
-    Hkv, S, Dn = k.shape[1:]
+    B, H, L, D = qs
+    _, Hkv, S, Dn = ks
     Dr = D - Dn
-    if k.shape[0] != B or tuple(v.shape[:3]) != (B, Hkv, S) or tuple(k_rope.shape) != (B, S, Dr) or Dr < 1 or Dn < 1:
+    if ks[0] != B or vs[:3] != ks[:3] or rs != (B, S, Dr) or Dr < 1 or Dn < 1:
         raise RuntimeError(f"latent_sdpa: q (B, H, L, Dn + Dr), k (B, Hkv, S, Dn), k_rope (B, S, Dr) and v (B, Hkv, S, Dv) do not "
-                           f"fit together: {list(q.shape)}, {list(k.shape)}, {list(k_rope.shape)}, {list(v.shape)}")
+                           f"fit together: {list(qs)}, {list(ks)}, {list(rs)}, {list(vs)}")
     if Hkv == 0 or H % Hkv:
         raise RuntimeError(f"latent_sdpa: num_heads ({H}) must be divisible by num_kv_heads ({Hkv})")
-    if any(t.dtype != q.dtype for t in (k, k_rope, v)) or q.dtype not in _CODE:
+    if k.dtype != dt or k_rope.dtype != dt or v.dtype != dt or dt not in _CODE:
         raise RuntimeError("latent_sdpa: q, k, k_rope and v must be f32, f16 or bf16, of one type")
-    if any(t.device != q.device for t in (k, k_rope, v)) or (seq_lens is not None and seq_lens.device != q.device):
+    if k.device != dev or k_rope.device != dev or v.device != dev or (seq_lens is not None and seq_lens.device != dev):
         raise RuntimeError("latent_sdpa: all tensors must be on one device")
     if seq_lens is not None:
         if L != S:
             raise RuntimeError(f"latent_sdpa: seq_lens needs as many queries as keys, got {L} and {S}")
-        if seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (B,) or not seq_lens.is_contiguous():
+        if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,) or not seq_lens.is_contiguous():
             raise RuntimeError(f"latent_sdpa: seq_lens must be a contiguous int32 tensor of shape ({B},)")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (math.isfinite(scale) and scale > 0.0):
@@ -287,6 +302,7 @@ def latent_sdpa(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor, v: torch
         return _sdpa_general(q, k, k_rope, v, bool(is_causal), scale, seq_lens)
     xs = (q, k, k_rope, v)
     # (tensors of forward mode take the Function too, which refuses them)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in xs) or any(unpack_dual(t).tangent is not None for t in xs):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or k_rope.requires_grad or v.requires_grad) or \
+            any([unpack_dual(t).tangent is not None for t in xs]):
         return LatentSDPAFn.apply(*xs, bool(is_causal), scale, seq_lens)
     return LatentSDPAFn._forward(*xs, bool(is_causal), scale, seq_lens, False)[4]
