@@ -29,6 +29,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "gtb_common.cuh"
 #include "latent.h"
@@ -86,10 +87,12 @@ struct Params {
     float* lse;
     float* part_o;             // [slot][row / 4][dim][row % 4]
     float2* part_ml;           // [slot][row]: offset, sum
-    int4* joins;               // items that more than one CTA worked on, by the CTA that begins them; with a split prefix, by item:
-                               // item (-1: none), first CTA, last CTA
-    int64_t* line;             // [0] tiles in all, [1] CTAs in use
-    int own_pitch;             // rows a slot of an own item, a multiple of 16
+    int4* joins;               // of each item, or where there are more of them than CTAs, of the item a CTA begins last: item (-1: one
+                               // CTA did it all), first CTA, last CTA, tokens of its sequence that attend
+    int by_item;
+    int64_t* line;             // [0] places in all, [1] CTAs in use, [2] prefix items
+    int own_rows, own_pitch;   // rows of an own item; the same to a multiple of 16: those of a slot of it
+    int join_dims;             // warps of a join block along the dims
     int64_t own_base;          // first float of own slots in part_o (split prefix)
     int* status;
 };
@@ -117,28 +120,37 @@ __device__ __forceinline__ int prefix_rows(const Params& p) {
 // items over the prefix alone: only where there are rows in it
 __device__ __forceinline__ int prefix_items(const Params& p, int P) { return p.bb && P > 0 ? p.n_pre : 0; }
 
-__device__ __forceinline__ Item item_of(const Params& p, int k, int P, int np) {
+// where item k lies among the query rows
+__device__ __forceinline__ Item item_at(const Params& p, int k, int np) {
     Item it;
     it.nh = p.hh;
     it.ni = p.ii;
-    const int pt = (P + KT - 1) / KT;
-    if (k < np) {
-        it.pre = true;
-        it.empty = false;
+    it.pre = k < np;
+    if (it.pre) {
         it.b = k * p.bb;
         it.i0 = it.h0 = 0;
         it.nb = p.bb;
+    } else {
+        k -= np;
+        it.nb = 1;
+        it.b = k / p.n_rt;
+        const int rt = k - it.b * p.n_rt, ti = rt / p.n_h;
+        it.i0 = ti * p.ii;
+        it.h0 = (rt - ti * p.n_h) * p.hh;
+    }
+    return it;
+}
+
+// and what it attends
+__device__ __forceinline__ Item item_of(const Params& p, int k, int P, int np) {
+    Item it = item_at(p, k, np);
+    const int pt = (P + KT - 1) / KT;
+    if (it.pre) {
+        it.empty = false;
         it.len = it.cnt = 0;
         it.nt_pre = it.nt = pt;
         return it;
     }
-    k -= np;
-    it.pre = false;
-    it.nb = 1;
-    it.b = k / p.n_rt;
-    const int rt = k - it.b * p.n_rt, ti = rt / p.n_h;
-    it.i0 = ti * p.ii;
-    it.h0 = (rt - ti * p.n_h) * p.hh;
     it.len = (int)min((int64_t)max(p.lens[it.b], 0), p.Smax);
     it.cnt = p.counts ? min(max(p.counts[it.b], 0), p.Lq) : p.Lq;
     const bool live = it.i0 < it.cnt;
@@ -288,6 +300,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     if (cta == 0 && threadIdx.x == 0) {
                         p.line[0] = line;
                         p.line[1] = n_cta;
+                        p.line[2] = np;
                     }
                     begin = share(line, n_cta, min(cta, n_cta - 1));
                     end = share(line, n_cta, min(cta, n_cta - 1) + 1);
@@ -471,14 +484,16 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             int64_t place = first_place + LEAD;  // of the item's first tile
             for_segments(plain, [&](const Item& it, int k, int off, int) {
                 if (off == 0) {
-                    const int4 j = make_int4(it.empty ? -1 : k, cta, cta_of(line, n_cta, place + it.nt - 1), 0);
-                    if (p.bb) p.joins[k] = j;
-                    else if (j.z > cta) mine = j;
+                    const int to = cta_of(line, n_cta, place + it.nt - 1);
+                    const bool parts = p.bb ? !it.empty : to > cta;  // (behind a split prefix all rows are joined)
+                    const int4 j = make_int4(parts ? k : -1, cta, to, it.cnt);
+                    if (p.by_item) p.joins[k] = j;
+                    else if (parts) mine = j;
                 }
                 place += it.nt + LEAD;
                 return true;
             });
-            if (!p.bb && !idle) p.joins[cta] = mine;
+            if (!p.by_item && !idle) p.joins[cta] = mine;
         }
     } else {
         // ------------------------------------------------------------ softmax, rescaling, epilogue
@@ -500,71 +515,75 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             soft_sync();
             const int lim_min = it.len - it.cnt + it.i0;   // smallest limit of a live row
-            float m[4][2], l[4][2];
+            // a row's state: minus its offset (0 before it has one), what its scores less the offset may reach without a new one, its sum
+            float nm[4][2], thr[4][2], l[4][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) m[j][0] = m[j][1] = -INFINITY, l[j][0] = l[j][1] = 0.0f;
-            for (int t = off; t < off + n && !it.empty; ++t, ++u) {
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) nm[j][c] = l[j][c] = 0.0f, thr[j][c] = -INFINITY;
+            // one tile, of GL groups of 8 columns a warp
+            auto tile = [&](auto groups, int t) {
+                constexpr int GL = decltype(groups)::value;
                 const bool pre = t < it.nt_pre;
                 const int row0 = (pre ? t : t - it.nt_pre) * KT;
                 const int valid = (pre ? P : it.len) - row0;  // cached rows of the tile
                 if (ok) ok = warp_wait(&bar.s_full[u & 1], (u >> 1) & 1, p.status, 77);
                 tc_fence_after();
                 uint32_t raw[16];
-                float (*x)[4] = (float(*)[4])raw;
-                tmem_ld_16(gl, tmem + lane_addr + (u & 1) * NR + 8 * half * gl, raw);
-                tmem_ld_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.s_free[u & 1]);
-                if (pre ? valid < KT : row0 + KT - 1 > lim_min) {
+                float (*e)[4] = (float(*)[4])raw;
+                auto scores = [&]() {  // the thread's scores, -inf where the row does not attend the key
+                    tmem_ld_16(GL, tmem + lane_addr + (u & 1) * NR + 8 * half * GL, raw);
+                    tmem_ld_wait();
+                    if (pre ? valid < KT : row0 + KT - 1 > lim_min) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j >= gl) continue;
-                        const int c = 8 * (half * gl + j) + cpair;
-                        // (rows that attend nothing take the others' way and are dropped at the end)
-                        const int l0 = pre ? P - 1 : max(ex.lim[c], -1), l1 = pre ? P - 1 : max(ex.lim[c + 1], -1);
-                        if (row0 + key0 > l0) x[j][0] = -INFINITY;
-                        if (row0 + key0 > l1) x[j][1] = -INFINITY;
-                        if (row0 + key0 + 8 > l0) x[j][2] = -INFINITY;
-                        if (row0 + key0 + 8 > l1) x[j][3] = -INFINITY;
+                        for (int j = 0; j < GL; ++j) {
+                            const int c = 8 * (half * GL + j) + cpair;
+                            // (rows that attend nothing take the others' way and are dropped at the end)
+                            const int l0 = pre ? P - 1 : max(ex.lim[c], -1), l1 = pre ? P - 1 : max(ex.lim[c + 1], -1);
+                            if (row0 + key0 > l0) e[j][0] = -INFINITY;
+                            if (row0 + key0 > l1) e[j][1] = -INFINITY;
+                            if (row0 + key0 + 8 > l0) e[j][2] = -INFINITY;
+                            if (row0 + key0 + 8 > l1) e[j][3] = -INFINITY;
+                        }
                     }
-                }
+                };
+                auto exponents = [&]() {
+#pragma unroll
+                    for (int j = 0; j < GL; ++j)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) e[j][c] = fmaf(e[j][c], p.scale_log2, nm[j][c & 1]);
+                };
+                scores();
+                exponents();
                 bool grow = false;
-                float top[4][2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j >= gl) continue;
+                for (int j = 0; j < GL; ++j)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        top[j][c] = fmaxf(x[j][c], x[j][c + 2]) * p.scale_log2;
-                        grow = grow || top[j][c] > m[j][c] + 8.0f;
-                    }
-                }
+                    for (int c = 0; c < 2; ++c) grow = grow || fmaxf(e[j][c], e[j][c + 2]) > thr[j][c];
                 if (soft_any(grow)) {
                     // the rows' maxima over the tile: over the thread's two keys, the warp's 16, the four quadrants
+                    scores();
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j >= gl) continue;
+                    for (int j = 0; j < GL; ++j) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float v = top[j][c];
+                            float v = fmaxf(e[j][c], e[j][c + 2]) * p.scale_log2;
                             v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
                             v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
                             v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
-                            if (lane < 4) ex.exch[quad][8 * (half * gl + j) + cpair + c] = v;
+                            if (lane < 4) ex.exch[quad][8 * (half * GL + j) + cpair + c] = v;
                         }
                     }
                     soft_sync();
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (j >= gl) continue;
+                    for (int j = 0; j < GL; ++j) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const int col = 8 * (half * gl + j) + cpair + c;
+                            const int col = 8 * (half * GL + j) + cpair + c;
                             const float v = fmaxf(fmaxf(ex.exch[0][col], ex.exch[1][col]), fmaxf(ex.exch[2][col], ex.exch[3][col]));
-                            const float mn = fmaxf(m[j][c], v);
-                            const float al = mn == m[j][c] ? 1.0f : ex2(m[j][c] - mn);
-                            m[j][c] = mn;
+                            const float m = thr[j][c] == -INFINITY ? -INFINITY : -nm[j][c], mn = fmaxf(m, v);
+                            const float al = mn == m ? 1.0f : ex2(m - mn);
+                            if (mn > -INFINITY) nm[j][c] = -mn, thr[j][c] = 8.0f;
                             l[j][c] *= al;
                             if (quad == 0 && lane < 4) ex.alpha[col] = al;
                         }
@@ -575,8 +594,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         tc_fence_after();
                         for (int mt = half; mt < m_tiles; mt += 2) {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                if (j >= gl) continue;
+                            for (int j = 0; j < GL; ++j) {
                                 uint32_t v[16];
                                 tmem_ldx<16>(tmem + lane_addr + O_COL + mt * NR + 16 * j, v);
                                 tmem_ld_wait();
@@ -587,31 +605,32 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         }
                         tmem_st_wait();
                     }
+                    exponents();
                 }
-                uint32_t w[4][2];
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.s_free[u & 1]);
+                uint32_t w[GL][2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j >= gl) continue;
-                    const float n0 = m[j][0] == -INFINITY ? 0.0f : -m[j][0], n1 = m[j][1] == -INFINITY ? 0.0f : -m[j][1];
-                    const float e0 = ex2(fmaf(x[j][0], p.scale_log2, n0)), e1 = ex2(fmaf(x[j][1], p.scale_log2, n1));
-                    const float e2 = ex2(fmaf(x[j][2], p.scale_log2, n0)), e3 = ex2(fmaf(x[j][3], p.scale_log2, n1));
-                    l[j][0] += e0 + e2;
-                    l[j][1] += e1 + e3;
-                    w[j][0] = pack2<BF16>(e0, e1);
-                    w[j][1] = pack2<BF16>(e2, e3);
+                for (int j = 0; j < GL; ++j) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) e[j][c] = ex2(e[j][c]);
+                    l[j][0] += e[j][0] + e[j][2];
+                    l[j][1] += e[j][1] + e[j][3];
+                    w[j][0] = pack2<BF16>(e[j][0], e[j][1]);
+                    w[j][1] = pack2<BF16>(e[j][2], e[j][3]);
                 }
                 if (u > 0 && ok) ok = warp_wait(&bar.pv_done, (u - 1) & 1, p.status, 79);  // P's buffer is free
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j >= gl) continue;
-                    unsigned char* d = sP + key0 * 128 + (((half * gl + j) ^ (key0 & 7)) << 4) + cpair * 2;
+                for (int j = 0; j < GL; ++j) {
+                    unsigned char* d = sP + key0 * 128 + (((half * GL + j) ^ (key0 & 7)) << 4) + cpair * 2;
                     *(uint32_t*)d = w[j][0];
                     *(uint32_t*)(d + 8 * 128) = w[j][1];
                 }
                 if (valid < KT) {  // rows past the end: 0 in the second product, whatever they hold
                     const int first = max(valid, 0), per = (KT - first) * 8;
-                    for (int e = st; e < per * (p.R / 64); e += NSOFT) {
-                        const int a = e / per, r = e - a * per, g = a >= GROUP && p.n_groups > 1;
+                    for (int i = st; i < per * (p.R / 64); i += NSOFT) {
+                        const int a = i / per, r = i - a * per, g = a >= GROUP && p.n_groups > 1;
                         unsigned char* base = (g ? sC1 : sC) + stage[g] * p.group_bytes[g];
                         *(uint4*)(base + (a - GROUP * g) * PANEL + first * 128 + r * 16) = make_uint4(0, 0, 0, 0);
                     }
@@ -623,6 +642,19 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar.p_full);
+            };
+            auto tiles = [&](auto groups) {
+                for (int t = off; t < off + n; ++t, ++u) tile(groups, t);
+            };
+            if (it.empty) {
+            } else if (gl == 1) {
+                tiles(std::integral_constant<int, 1>{});
+            } else if (gl == 2) {
+                tiles(std::integral_constant<int, 2>{});
+            } else if (gl == 3) {
+                tiles(std::integral_constant<int, 3>{});
+            } else {
+                tiles(std::integral_constant<int, 4>{});
             }
             // ---- the segment's rows: sums over the quadrants, then O^T a latent dim a lane
 #pragma unroll
@@ -635,7 +667,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     v += __shfl_xor_sync(~0u, v, 8);
                     v += __shfl_xor_sync(~0u, v, 16);
                     if (lane < 4) ex.exch[quad][8 * (half * gl + j) + cpair + c] = v;
-                    if (quad == 0 && lane < 4) ex.alpha[8 * (half * gl + j) + cpair + c] = m[j][c];
+                    if (quad == 0 && lane < 4) ex.alpha[8 * (half * gl + j) + cpair + c] = thr[j][c] == -INFINITY ? -INFINITY : -nm[j][c];
                 }
             }
             soft_sync();
@@ -724,124 +756,133 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
 }
 
-// Rows whose item more than one CTA worked on: a block has 8 of them (and 128 dims, 4 a lane), its warps take the parts in turn and
-// add theirs up in shared memory. Few bytes against the tiles'; what counts is that the parts' loads go out together.
-constexpr int JOIN_WARPS = 8, JOIN_ROWS = 8;
+// Rows whose item more than one CTA worked on. A block has 4 rows (a vector of the parts' layout): a warp 32 dims, one a lane, with four
+// parts' loads in flight. Its 8 warps share `join_dims` pieces of 32 dims and take the parts in turn: all along the dims
+// where items have few parts, all along the parts where a few sequences were cut into many. What it costs is latency: two
+// dependent loads (which parts, then the parts), and no more registers than let all of a step's blocks run at once.
+constexpr int JOIN_WARPS = 8, JOIN_ROWS = 4, JOIN_FLIGHT = 4;
+constexpr int MAX_CTAS = 511;  // parts of a row: one a CTA, and one more behind a split prefix
 
 template <typename T>
-__global__ void __launch_bounds__(JOIN_WARPS * 32) latent_join_kernel(const __grid_constant__ Params p) {
-    __shared__ float sum[JOIN_WARPS][JOIN_ROWS][128 + 4];
+__global__ void __launch_bounds__(JOIN_WARPS * 32, 4) latent_join_kernel(const __grid_constant__ Params p) {
+    __shared__ float4 sum[JOIN_WARPS][32];
+    __shared__ float2 sh_ml[(MAX_CTAS + 1) * JOIN_ROWS];
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the first kernel ends
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int P = prefix_rows(p), np = prefix_items(p, P);
-    // parts: CTAs c0 .. c1 of item k, its rows from `row` on; with a split prefix those of the prefix's item come first
-    int k[2], c0[2], n[2], row[2], n_src = 0;
-    const int col0 = (int)blockIdx.y * JOIN_ROWS;
-    Item it;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col0 = (int)blockIdx.y * JOIN_ROWS;
+    // parts: CTAs c0 .. c0 + n - 1 of item k, its rows from `row` on; with a split prefix those of the prefix's item come first
+    const int n_cta = (int)p.line[1], np = (int)p.line[2];
+    int k[2], c0[2], n[2] = {0, 0}, row[2], cnt;
     if (!p.bb) {
-        if ((int64_t)blockIdx.x >= p.line[1]) return;
         const int4 j = p.joins[blockIdx.x];
-        if (j.x < 0) return;
-        it = item_of(p, j.x, P, np);
-        k[0] = j.x, c0[0] = j.y, n[0] = j.z - j.y + 1, row[0] = col0;
-        n_src = 1;
+        if ((!p.by_item && (int)blockIdx.x >= n_cta) || j.x < 0) return;
+        k[0] = j.x, c0[0] = j.y, n[0] = j.z - j.y + 1, row[0] = col0, cnt = j.w;
+        k[1] = c0[1] = row[1] = 0;
     } else {
         const int b = (int)blockIdx.x;
-        it = item_of(p, np + b, P, np);
-        for (int e = np > 0 ? 0 : 1; e < 2; ++e) {
-            const int4 j = p.joins[e == 0 ? b / p.bb : np + b];
-            if (j.x < 0) continue;
-            k[n_src] = j.x, c0[n_src] = j.y, n[n_src] = j.z - j.y + 1;
-            row[n_src] = (e == 0 ? (b % p.bb) * it.rows() : 0) + col0;
-            ++n_src;
-        }
+        const int4 own = p.joins[np + b], pre = np > 0 ? p.joins[b / p.bb] : make_int4(-1, 0, 0, 0);
+        k[0] = pre.x, c0[0] = pre.y, n[0] = pre.x < 0 ? 0 : pre.z - pre.y + 1, row[0] = (b % p.bb) * p.own_rows + col0;
+        k[1] = own.x, c0[1] = own.y, n[1] = own.x < 0 ? 0 : own.z - own.y + 1, row[1] = col0;
+        cnt = own.w;
     }
-    const int rows = min(JOIN_ROWS, it.rows() - col0);
-    const int parts = (n_src > 0 ? n[0] : 0) + (n_src > 1 ? n[1] : 0);
-    auto part_of = [&](int q, const float*& o, const float2*& ml) -> int {  // part q, its first row
-        const int s = q >= n[0], c = c0[s] + q - (s ? n[0] : 0);
+    const int parts = n[0] + n[1], rows = min(JOIN_ROWS, p.own_rows - col0);
+    const int groups = JOIN_WARPS / p.join_dims, group = warp / p.join_dims;
+    const int d = ((int)blockIdx.z * p.join_dims + warp % p.join_dims) * 32 + lane;
+    // where a source's first part is, and the step from CTA to CTA (one address a part: with all of it formed each time, instructions
+    // were what this kernel waited for)
+    const float* o0[2];
+    const float2* ml0[2];
+    int64_t o_step[2];
+    const int ml_step = (p.bb ? 1 : 2) * NR;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
         int64_t so, sml;
-        slot_of(p, k[s], np, c, c == c0[s], so, sml);
-        o = p.part_o + so;
-        ml = p.part_ml + sml + row[s];
-        return row[s];
-    };
-    // each warp: the rows' largest offset and the sum in its terms, a row a lane & 7, 4 parts at a time
-    const int mine = lane & 7;
-    float m = -INFINITY, l = 0.0f;
-    for (int q = lane >> 3; q < parts; q += 4) {
-        const float* o;
-        const float2* ml;
-        part_of(q, o, ml);
-        if (mine < rows) {
-            const float2 v = ml[mine];
-            if (v.y != 0.0f) {  // (a part without a weight holds nothing)
-                const float mn = fmaxf(m, v.x);
-                l = l * ex2(m - mn) + v.y * ex2(v.x - mn);
-                m = mn;
-            }
-        }
+        slot_of(p, k[s], np, c0[s], false, so, sml);
+        const int pitch = k[s] < np ? NR : p.own_pitch;
+        o0[s] = p.part_o + so + ((int64_t)(row[s] >> 2) * p.R + d) * 4;
+        ml0[s] = p.part_ml + sml + row[s];
+        o_step[s] = (int64_t)(p.bb ? 1 : 2) * pitch * p.R;
     }
-    for (int x = 8; x < 32; x <<= 1) {
-        const float om = __shfl_xor_sync(~0u, m, x), ol = __shfl_xor_sync(~0u, l, x), mn = fmaxf(m, om);
-        l = l == 0.0f ? ol : ol == 0.0f ? l : l * ex2(m - mn) + ol * ex2(om - mn);
-        m = mn;
-    }
-    const int d = (int)blockIdx.z * 128 + lane * 4;
-    float acc[JOIN_ROWS][4] = {};
-    for (int q = warp; q < parts; q += JOIN_WARPS) {
-        const float* o;
-        const float2* ml;
-        const int r0 = part_of(q, o, ml);
-        float f = 0.0f;
-        if (mine < rows) {
-            const float2 v = ml[mine];
-            f = v.y == 0.0f ? 0.0f : ex2(v.x - m);
-        }
-        float y[4][JOIN_ROWS];
+    auto load = [&](int q0, float4* y) {  // this lane's dim of parts q0, q0 + groups, ..
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (d >= p.R) continue;
-            if ((r0 & 3) == 0 && rows == JOIN_ROWS) {
-                *(float4*)&y[e][0] = *(const float4*)(o + ((int64_t)(r0 >> 2) * p.R + d + e) * 4);
-                *(float4*)&y[e][4] = *(const float4*)(o + ((int64_t)((r0 >> 2) + 1) * p.R + d + e) * 4);
+        for (int e = 0; e < JOIN_FLIGHT; ++e) {
+            const int q = q0 + groups * e, s = q >= n[0], i = q - (s ? n[0] : 0);
+            y[e] = make_float4(0, 0, 0, 0);
+            if (q >= parts || d >= p.R) continue;
+            // (without a split prefix, the CTA that begins the item has it in its second slot)
+            const int64_t step = s ? o_step[1] : o_step[0];
+            const float* o = (s ? o0[1] : o0[0]) + i * step + (i == 0 && !p.bb ? step / 2 : 0);
+            const int r0 = (s ? row[1] : row[0]) & 3;
+            if (r0 == 0) {
+                y[e] = *(const float4*)o;
             } else {
-#pragma unroll
-                for (int r = 0; r < JOIN_ROWS; ++r)
-                    y[e][r] = r < rows ? o[((int64_t)((r0 + r) >> 2) * p.R + d + e) * 4 + ((r0 + r) & 3)] : 0.0f;
+                auto at = [&](int r) { return r < rows ? o[(int64_t)((r0 + r) >> 2) * p.R * 4 + ((r0 + r) & 3)] : 0.0f; };
+                y[e] = make_float4(at(0), at(1), at(2), at(3));
             }
         }
-#pragma unroll
-        for (int r = 0; r < JOIN_ROWS; ++r) {
-            const float fr = __shfl_sync(~0u, f, r);
-            if (fr != 0.0f && d < p.R) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[r][e] = fmaf(y[e][r], fr, acc[r][e]);
-            }
-        }
+    };
+    float4 y[JOIN_FLIGHT], next[JOIN_FLIGHT];
+    load(group, y);  // (out before the offsets and sums are asked for)
+    for (int e = threadIdx.x; e < parts * JOIN_ROWS; e += JOIN_WARPS * 32) {
+        const int q = e / JOIN_ROWS, r = e % JOIN_ROWS, s = q >= n[0], i = q - (s ? n[0] : 0);
+        sh_ml[e] = r < rows ? (s ? ml0[1] : ml0[0])[(int64_t)i * ml_step + (i == 0 && !p.bb ? NR : 0) + r] : make_float2(-INFINITY, 0.0f);
     }
-#pragma unroll
-    for (int r = 0; r < JOIN_ROWS; ++r) *(float4*)&sum[warp][r][lane * 4] = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
     __syncthreads();
-    // a row a warp
-    const float mr = __shfl_sync(~0u, m, warp), lr = __shfl_sync(~0u, l, warp);
-    int b, i, h;
-    if (warp >= rows || !row_of(p, it, col0 + warp, b, i, h)) return;
-    const int64_t orow = ((int64_t)b * p.H + h) * p.Lq + i;
-    const bool none = i >= it.cnt || lr == 0.0f;
-    if (d < p.R) {
-        const float inv = none ? 0.0f : 1.0f / lr;
-        __align__(8) T w[4];
+    // the rows' largest offset and the sum in its terms: a row a lane & 3, 8 parts at a time
+    float m = -INFINITY, l = 0.0f;
+    for (int e = lane; e < parts * JOIN_ROWS; e += 32) m = fmaxf(m, sh_ml[e].x);
+    for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
+    auto factor = [&](float2 v) { return v.y == 0.0f ? 0.0f : ex2(v.x - m); };  // (a part without a weight holds nothing)
+    for (int e = lane; e < parts * JOIN_ROWS; e += 32) l += sh_ml[e].y * factor(sh_ml[e]);
+    for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(~0u, l, x);
+    float acc[JOIN_ROWS] = {};
+    for (int q0 = group; q0 < parts; q0 += groups * JOIN_FLIGHT) {
+        const bool more = q0 + groups * JOIN_FLIGHT < parts;
+        if (more) load(q0 + groups * JOIN_FLIGHT, next);
+        // factor of part q0 + groups * e and row r in lane 4 e + r
+        const int q = q0 + groups * (lane >> 2);
+        const float f = lane < 4 * JOIN_FLIGHT && q < parts ? factor(sh_ml[q * JOIN_ROWS + (lane & 3)]) : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float a = 0.0f;
+        for (int e = 0; e < JOIN_FLIGHT; ++e) {
+            const float x[JOIN_ROWS] = {y[e].x, y[e].y, y[e].z, y[e].w};
 #pragma unroll
-            for (int g = 0; g < JOIN_WARPS; ++g) a += sum[g][warp][lane * 4 + e];
-            Elem<T>::store(w + e, none ? 0.0f : a * inv);
+            for (int r = 0; r < JOIN_ROWS; ++r) {
+                const float fr = __shfl_sync(~0u, f, 4 * e + r);
+                if (fr != 0.0f) acc[r] = fmaf(x[r], fr, acc[r]);
+            }
+            if (more) y[e] = next[e];
         }
-        *(uint2*)((T*)p.o + orow * p.R + d) = *(const uint2*)w;
     }
-    if (p.lse && lane == 0 && blockIdx.z == 0) p.lse[orow] = none ? -INFINITY : (mr + log2f(lr)) * 0.69314718055994531f;
+    if (groups > 1) {
+        sum[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        __syncthreads();
+        if (group > 0) return;
+        for (int g = 1; g < groups; ++g) {
+            const float4 z = sum[g * p.join_dims + warp][lane];
+            acc[0] += z.x;
+            acc[1] += z.y;
+            acc[2] += z.z;
+            acc[3] += z.w;
+        }
+    }
+    // lanes 0 .. 3: the rows' places in the output, and what their sums are multiplied by (0: nothing attended)
+    int orow = -1;
+    float inv = 0.0f;
+    if (lane < rows) {
+        const Item it = item_at(p, p.bb ? np + (int)blockIdx.x : k[0], np);
+        int b, i, h;
+        if (row_of(p, it, col0 + lane, b, i, h)) {
+            orow = (b * p.H + h) * p.Lq + i;
+            const bool none = i >= cnt || l == 0.0f;
+            if (!none) inv = 1.0f / l;
+            if (p.lse && blockIdx.z == 0 && warp == 0) p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < JOIN_ROWS; ++r) {
+        const int to = __shfl_sync(~0u, orow, r);
+        const float f = __shfl_sync(~0u, inv, r);
+        if (to >= 0 && d < p.R) Elem<T>::store((T*)p.o + (int64_t)to * p.R + d, f == 0.0f ? 0.0f : acc[r] * f);
+    }
 }
 
 // nothing cached and nothing before it: zeros and -inf
@@ -907,6 +948,7 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     p.ii = (p.Lq + n_i - 1) / n_i;
     p.n_rt = n_i * p.n_h;
     const int own_rows = p.hh * p.ii;
+    p.own_rows = own_rows;
     p.own_pitch = (own_rows + 15) & ~15;
     // a prefix gets items of its own where those can take the rows of several sequences
     if (a.prefix.rows && n_i == 1 && p.n_h == 1 && 2 * own_rows <= NR && p.B > 1) {
@@ -934,7 +976,7 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     p.slack = smem - used;
 
     const int64_t tiles_seq = (a.c.Smax + KT - 1) / KT + (p.prefix_lens ? (p.prefix_max + KT - 1) / KT : 0);
-    const int grid = (int)std::min<int64_t>(n_sm, items * (std::max<int64_t>(tiles_seq, 1) + LEAD));
+    const int grid = (int)std::min<int64_t>(std::min(n_sm, MAX_CTAS), items * (std::max<int64_t>(tiles_seq, 1) + LEAD));
 
     CUtensorMap mq, mqp, mc, mcp;
     const int64_t D = p.R + p.Dr, qs[3] = {p.H, p.Lq, p.B}, qt[3] = {a.q.sh, a.q.ss, a.q.sb};
@@ -947,11 +989,12 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     if (!a.prefix.rows) mcp = mc;
 
     // workspace: the line's data, then the parts
+    p.by_item = p.bb || items <= grid;
     const int64_t slots_pre = p.bb ? p.n_pre + grid : 0, slots_own = p.bb ? (int64_t)p.B * p.n_rt + grid : 2 * (int64_t)grid;
     p.own_base = slots_pre * NR * p.R;
     const int64_t n_o = p.own_base + slots_own * p.own_pitch * p.R, n_ml = (p.bb ? items + grid : 2 * (int64_t)grid) * NR;
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-    const int64_t at_joins = 256, at_ml = at_joins + up((p.bb ? items : grid) * 16), at_o = at_ml + up(n_ml * 8);
+    const int64_t at_joins = 256, at_ml = at_joins + up((p.by_item ? items : grid) * 16), at_o = at_ml + up(n_ml * 8);
     char* ws = nullptr;
     if (cuda_failed(cudaMallocAsync((void**)&ws, at_o + up(n_o * 4), st), "latent_attention: workspace")) return -1;
     p.line = (int64_t*)ws;
@@ -973,7 +1016,8 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     }
     if (!rc && (p.bb || grid > 1)) {
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(p.bb ? p.B : grid, (own_rows + JOIN_ROWS - 1) / JOIN_ROWS, (p.R + 127) / 128);
+        p.join_dims = p.bb ? 4 : items * 4 >= grid ? 8 : 1;
+        cfg.gridDim = dim3(p.bb ? p.B : (unsigned)std::min<int64_t>(items, grid), (own_rows + JOIN_ROWS - 1) / JOIN_ROWS, (p.R / 32 + p.join_dims - 1) / p.join_dims);
         cfg.blockDim = dim3(JOIN_WARPS * 32);
         cfg.stream = st;
         cudaLaunchAttribute at[1];
