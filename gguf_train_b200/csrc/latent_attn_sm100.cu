@@ -502,6 +502,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         const int key0 = quad * 16 + (lane >> 2);          // this thread's keys of a tile: key0, key0 + 8
         const int cpair = 2 * (lane & 3);                  // its columns of a group: cpair, cpair + 1
         const int m_tiles = (p.R + 127) / 128;
+        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
         bool ok = true;
         int u = 0, stage[2] = {0, 0};
         for_segments(plain, [&](const Item& it, int k, int off, int n) {
@@ -547,11 +548,13 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         }
                     }
                 };
+                // (score - offset) * scale: the difference first, so that scores of any size keep what they differ by
                 auto exponents = [&]() {
 #pragma unroll
                     for (int j = 0; j < GL; ++j)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) e[j][c] = fmaf(e[j][c], p.scale_log2, nm[j][c & 1]);
+                        for (int c = 0; c < 4; c += 2)
+                            f2_unpack(f2_mul(f2_add(f2_pack(e[j][c], e[j][c + 1]), f2_pack(nm[j][0], nm[j][1])), sc2), e[j][c], e[j][c + 1]);
                 };
                 scores();
                 exponents();
@@ -567,7 +570,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     for (int j = 0; j < GL; ++j) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            float v = fmaxf(e[j][c], e[j][c + 2]) * p.scale_log2;
+                            float v = fmaxf(e[j][c], e[j][c + 2]);
                             v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
                             v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
                             v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
@@ -582,7 +585,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                             const int col = 8 * (half * GL + j) + cpair + c;
                             const float v = fmaxf(fmaxf(ex.exch[0][col], ex.exch[1][col]), fmaxf(ex.exch[2][col], ex.exch[3][col]));
                             const float m = thr[j][c] == -INFINITY ? -INFINITY : -nm[j][c], mn = fmaxf(m, v);
-                            const float al = mn == m ? 1.0f : ex2(m - mn);
+                            const float al = mn == m ? 1.0f : ex2((m - mn) * p.scale_log2);
                             if (mn > -INFINITY) nm[j][c] = -mn, thr[j][c] = 8.0f;
                             l[j][c] *= al;
                             if (quad == 0 && lane < 4) ex.alpha[col] = al;
@@ -667,7 +670,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     v += __shfl_xor_sync(~0u, v, 8);
                     v += __shfl_xor_sync(~0u, v, 16);
                     if (lane < 4) ex.exch[quad][8 * (half * gl + j) + cpair + c] = v;
-                    if (quad == 0 && lane < 4) ex.alpha[8 * (half * gl + j) + cpair + c] = thr[j][c] == -INFINITY ? -INFINITY : -nm[j][c];
+                    if (quad == 0 && lane < 4) ex.alpha[8 * (half * gl + j) + cpair + c] = thr[j][c] == -INFINITY ? -INFINITY : -nm[j][c] * p.scale_log2;
                 }
             }
             soft_sync();

@@ -387,9 +387,9 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 for (int k = 16; k < BN; k += 16)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) pm[e] = fmax3(pm[e], x[k + e], x[k + 8 + e]);
-                const float cm = fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7])) * p.scale_log2;
+                const float cm = fmax3(fmax3(pm[0], pm[1], pm[2]), fmax3(pm[3], pm[4], pm[5]), fmaxf(pm[6], pm[7]));
                 const float m_start = m_used;
-                if (cm > m_used + 8.0f) m_used = cm;  // false while the row has no finite score
+                if ((cm - m_used) * p.scale_log2 > 8.0f) m_used = cm;  // false while the row has no finite score
                 const bool grew = m_used != m_start;
                 const float neg_m = m_used == -INFINITY ? 0.0f : -m_used;
                 const uint64_t nm2 = f2_pack(neg_m, neg_m);
@@ -400,7 +400,8 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
                         float a0, a1;
-                        f2_unpack(f2_fma(f2_pack(x[32 * c + k], x[32 * c + k + 1]), sc2, nm2), a0, a1);
+                        // (the difference first, so that scores of any size keep what they differ by)
+                        f2_unpack(f2_mul(f2_add(f2_pack(x[32 * c + k], x[32 * c + k + 1]), nm2), sc2), a0, a1);
                         a0 = ex2(a0);
                         a1 = ex2(a1);
                         ps2[(k >> 1) & 1] = f2_add(ps2[(k >> 1) & 1], f2_pack(a0, a1));
@@ -410,7 +411,7 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 }
                 if (__any_sync(~0u, grew && j > 0)) {
                     // PV_t(j-1) is complete: it was issued before S_t(j), whose completion has been seen
-                    const float alpha = grew ? ex2(m_start - m_used) : 1.0f;
+                    const float alpha = grew ? ex2((m_start - m_used) * p.scale_log2) : 1.0f;
 #pragma unroll
                     for (int c = 0; c < DN / 32; ++c) {
                         uint32_t ov[32];
@@ -424,7 +425,7 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 float s0, s1, s2, s3;
                 f2_unpack(ps2[0], s0, s1);
                 f2_unpack(ps2[1], s2, s3);
-                lsum = (grew ? lsum * ex2(m_start - m_used) : lsum) + ((s0 + s1) + (s2 + s3));
+                lsum = (grew ? lsum * ex2((m_start - m_used) * p.scale_log2) : lsum) + ((s0 + s1) + (s2 + s3));
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -451,7 +452,7 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                         *(uint4*)(orow + c * 32 + 8 * k) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
                 }
             }
-            if (lse && row < p.L) *lse = none ? -INFINITY : (m_used + log2f(lsum)) * 0.69314718055994531f;
+            if (lse && row < p.L) *lse = none ? -INFINITY : (m_used * p.scale_log2 + log2f(lsum)) * 0.69314718055994531f;
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.o_empty[t]);
