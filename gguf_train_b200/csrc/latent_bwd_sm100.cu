@@ -4,20 +4,22 @@
 //   pre     a query row: -g . out and -lse log2 e (-inf for padded rows and rows that attend nothing: weights 0).
 //   dK/dV   one CTA a 128-key tile of one (batch, kv head), over its query heads' rows, 64 at a time:
 //             S^T = [K | K_r] Q^T, dP^T = V G^T        (M = 128 keys, N = 64 queries)
-//             dV += W^T G, dK += dS^T Q                (M = 128 keys, N = dims, K = 64; W^T, dS^T through shared memory)
+//             dV += W^T G, dK += dS^T Q                (M = 128 keys, N = dims, K = 64; W^T from TMEM, dS^T from shared memory)
 //           The rotary part of dK is the sum over all heads: each CTA writes its share in f32 and a last kernel adds the
 //           heads in order, so the bits are the same on every run.
 //   dQ      one CTA a 128-query tile, over 64 keys at a time:
 //             S = Q [K | K_r]^T, dP = G V^T            (M = 128 queries, N = 64 keys)
-//             dQ += dS [K | K_r]                       (N = dims, K = 64; dS from TMEM, over S)
+//             dQ += dS [K | K_r]                       (N = dims, K = 64; dS from TMEM)
 // A fused dQ (five products instead of seven) needs f32 sums in global memory by unordered additions, and TMEM that dK's 192 columns
 // do not leave. Products of N = 64 with both operands in shared memory are bound by its bandwidth (49.5 cycles instead of 32):
 // 64 is what TMEM holds of scores next to dV and dK (320 of 512 columns with Dn = 128).
 //
 // Warps: 0 TMA producer, 1 issues the score products (and owns TMEM), 2 the gradient products, 3 zeroes rows of padded tokens in a
 // loaded stage (their product with a weight of 0 would be NaN), 4-7 and 8-11 the weights of even and odd sub-tiles, a key (dK/dV)
-// or query (dQ) a thread. In the dK/dV kernel S^T and dP^T take turns in three 64-column buffers, freed as soon as they
-// are read. Every mbarrier wait is bounded.
+// or query (dQ) a thread. TMEM of the dK/dV kernel with Dn = 128: dV 128 columns, dK 192, two S^T of 64 (over which W^T is written), one
+// dP^T; of the dQ kernel: dQ 192, two dS of 32, two S and two dP of 64. Three stages of 64 rows stream: what a stage waits for (its
+// load, the scores, the weights, the gradients) is about three times what the tensor core does on it. Every mbarrier
+// wait is bounded.
 
 #include <algorithm>
 #include <atomic>
@@ -160,20 +162,23 @@ struct Sizes {
 
 // ------------------------------------------------------------------ dK, dV
 
+constexpr int STAGES = 3;
+
 template <int DN>
 struct KvSmem {
     using Z = Sizes<DN>;
     static constexpr int OFF_V = Z::KTILE, OFF_ST = OFF_V + Z::VTILE;
-    static constexpr int OFF_W = OFF_ST + 2 * Z::STAGE, OFF_DS = OFF_W + 2 * BT * SUB * 2;
-    static constexpr int OFF_ROW = OFF_DS + 2 * BT * SUB * 2;      // [stage][-lse2, -delta][64]
-    static constexpr int OFF_BAR = OFF_ROW + 2 * 2 * SUB * 4;
+    static constexpr int OFF_DS = OFF_ST + STAGES * Z::STAGE;
+    static constexpr int OFF_ROW = OFF_DS + BT * SUB * 2;          // [stage][-lse2, -delta][64]
+    static constexpr int OFF_BAR = OFF_ROW + STAGES * 2 * SUB * 4;
     static constexpr int USED = OFF_BAR + 256;
-    static constexpr int ALLOC = USED + 1023 < SMEM_MAX ? USED + 1023 : SMEM_MAX;
-    static_assert(USED <= SMEM_MAX, "shared memory");
+    static constexpr int ALLOC = USED + 1023;
+    static_assert(ALLOC <= SMEM_MAX, "shared memory");
 };
 
 struct KvBars {
-    uint64_t kv_full, st_full[2], st_empty[2], r_full[3], r_free[3], w_full[2], w_free[2], fix[2], fixed[2], final_, drain[2];
+    uint64_t kv_full, st_full[STAGES], st_empty[STAGES], fix[STAGES], fixed[STAGES], s_full[2], dp_full, dp_free, w_full[2], w_free[2], ds_free;
+    uint64_t final_, drain[2];
     uint32_t tmem;
     int abort;
 };
@@ -186,13 +191,9 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
     using Z = Sizes<DN>;
     using M = KvSmem<DN>;
-    constexpr uint32_t DK_COL = DN, RING = 320;
+    constexpr uint32_t DK_COL = DN, S_COL = 320, S_STEP = 128, DP_COL = 384;  // S^T of sub-tile h at S_COL + 128 h, then W^T
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    if (smem - smem_raw > M::ALLOC - M::USED) {
-        if (threadIdx.x == 0) atomicCAS(p.status, 0, 100);
-        return;
-    }
     KvBars& bar = *(KvBars*)(smem + M::OFF_BAR);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int jt, unit;
@@ -205,18 +206,20 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     if (threadIdx.x == 0) {
         mbar_init(&bar.kv_full, 1);
         mbar_init(&bar.final_, 1);
-        for (int i = 0; i < 2; ++i) {
+        mbar_init(&bar.dp_full, 1);
+        mbar_init(&bar.dp_free, 4);
+        mbar_init(&bar.ds_free, 1);
+        for (int i = 0; i < STAGES; ++i) {
             mbar_init(&bar.st_full[i], 1);
             mbar_init(&bar.st_empty[i], 1);
-            mbar_init(&bar.w_full[i], 4);
-            mbar_init(&bar.w_free[i], 1);
             mbar_init(&bar.fix[i], 1);
             mbar_init(&bar.fixed[i], 1);
-            mbar_init(&bar.drain[i], 1);
         }
-        for (int i = 0; i < 3; ++i) {
-            mbar_init(&bar.r_full[i], 1);
-            mbar_init(&bar.r_free[i], 4);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.w_full[i], 4);
+            mbar_init(&bar.w_free[i], 1);
+            mbar_init(&bar.drain[i], 1);
         }
         bar.abort = 0;
         fence_mbar_init();
@@ -246,8 +249,8 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             bool ok = true;
             int it = 0;
             for (; it < nit; ++it) {
-                const int st = it & 1, h = head_of(it), q = first_of(it);
-                if (it >= 2) ok = mbar_wait(&bar.st_empty[st], ((it >> 1) - 1) & 1, p.status, 101);
+                const int st = it % STAGES, h = head_of(it), q = first_of(it);
+                if (it >= STAGES) ok = mbar_wait(&bar.st_empty[st], (it / STAGES - 1) & 1, p.status, 101);
                 if (!ok || *abort_flag) { ok = false; break; }
                 unsigned char* d = smem + M::OFF_ST + st * Z::STAGE;
                 mbar_expect_tx(&bar.st_full[st], Z::STAGE + 2 * SUB * 4);
@@ -260,7 +263,7 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             if (!ok) *abort_flag = 1;
             if (*abort_flag) {  // our copies in flight end before the CTA does
                 mbar_wait(&bar.kv_full, 0, nullptr, 0);
-                for (int n = max(0, it - 2); n < it; ++n) mbar_wait(&bar.st_full[n & 1], (n >> 1) & 1, nullptr, 0);
+                for (int n = max(0, it - STAGES); n < it; ++n) mbar_wait(&bar.st_full[n % STAGES], (n / STAGES) & 1, nullptr, 0);
             }
         }
     } else if (warp < 3) {
@@ -274,62 +277,65 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             const uint32_t kd = desc_lo(smem_u32(smem), 16), vd = desc_lo(smem_u32(smem + M::OFF_V), 16);
             const uint32_t sd = desc_lo(smem_u32(smem + M::OFF_ST), 16);
             if (n_it > 0) ok = warp_wait(&bar.kv_full, 0, p.status, 102);
-            int slot = 0, round = 0, n_fix[2] = {0, 0};  // the ring buffer to fill next and how often it has been
+            int st = 0, phase = 0, n_fix = 0;  // stage and its phase; which stages' next mended round is odd
             for (int it = 0; it < n_it && ok; ++it) {
-                const int st = it & 1;
-                ok = warp_wait(&bar.st_full[st], (it >> 1) & 1, p.status, 103);
+                const int h = it & 1;
+                ok = warp_wait(&bar.st_full[st], phase, p.status, 103);
                 if (ok && padded(it)) {
                     if (lead) mbar_arrive(&bar.fix[st]);
-                    ok = warp_wait(&bar.fixed[st], n_fix[st]++ & 1, p.status, 104);
+                    ok = warp_wait(&bar.fixed[st], (n_fix >> st) & 1, p.status, 104);
+                    n_fix ^= 1 << st;
                 }
+                // S^T's columns hold the W^T that the product two sub-tiles ago read
+                if (ok && it >= 2) ok = warp_wait(&bar.w_free[h], ((it >> 1) - 1) & 1, p.status, 105);
+                if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
+                tc_fence_after();
                 const uint32_t q = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), g = q + (Z::PANELS * Z::SLAB64 >> 4);
+                const uint32_t s_dst = tm + S_COL + h * S_STEP, dp_dst = tm + DP_COL;
+                if (lead) {
 #pragma unroll
-                for (int which = 0; which < 2; ++which) {
-                    if (ok && round > 0) ok = warp_wait(&bar.r_free[slot], (round - 1) & 1, p.status, 105);
-                    if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; continue; }
-                    tc_fence_after();
-                    const uint32_t dst = tm + RING + slot * SUB;
-                    if (lead) {
-                        if (which == 0) {
+                    for (int kk = 0; kk < DN / 16; ++kk)
+                        mma_ss_lo(s_dst, kd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, q + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC, kk > 0);
 #pragma unroll
-                            for (int kk = 0; kk < DN / 16; ++kk)
-                                mma_ss_lo(dst, kd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, q + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC,
-                                          kk > 0);
-#pragma unroll
-                            for (int kk = 0; kk < 4; ++kk)
-                                if (kk < p.rope_steps)
-                                    mma_ss_lo(dst, kd + (DN / 64) * (Z::SLAB >> 4) + kk * 2, q + (DN / 64) * (Z::SLAB64 >> 4) + kk * 2, IDESC, 1);
-                        } else {
-#pragma unroll
-                            for (int kk = 0; kk < DN / 16; ++kk)
-                                mma_ss_lo(dst, vd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, g + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC,
-                                          kk > 0);
-                        }
-                        mma_commit(&bar.r_full[slot]);
-                    }
-                    if (++slot == 3) slot = 0, ++round;
+                    for (int kk = 0; kk < 4; ++kk)
+                        if (kk < p.rope_steps)
+                            mma_ss_lo(s_dst, kd + (DN / 64) * (Z::SLAB >> 4) + kk * 2, q + (DN / 64) * (Z::SLAB64 >> 4) + kk * 2, IDESC, 1);
+                    mma_commit(&bar.s_full[h]);
                 }
+                if (it >= 1) ok = warp_wait(&bar.dp_free, (it - 1) & 1, p.status, 113);
+                if (!ok) break;
+                tc_fence_after();
+                if (lead) {
+#pragma unroll
+                    for (int kk = 0; kk < DN / 16; ++kk)
+                        mma_ss_lo(dp_dst, vd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, g + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC, kk > 0);
+                    mma_commit(&bar.dp_full);
+                }
+                if (++st == STAGES) st = 0, phase ^= 1;
             }
         } else {
             const uint32_t idesc_k = idesc_f16(BT, 0, BF16, true) | (uint32_t)(DN + 16 * p.rope_steps) >> 3 << 17;
             constexpr uint32_t IDESC_V = idesc_f16(BT, DN, BF16, true);
-            const uint32_t wd = desc_lo(smem_u32(smem + M::OFF_W), 16), sd = desc_lo(smem_u32(smem + M::OFF_ST), Z::SLAB64);
+            const uint32_t ds = desc_lo(smem_u32(smem + M::OFF_DS), 16), sd = desc_lo(smem_u32(smem + M::OFF_ST), Z::SLAB64);
+            int st = 0;
             for (int it = 0; it < n_it && ok; ++it) {
-                const int st = it & 1;
-                ok = warp_wait(&bar.w_full[st], (it >> 1) & 1, p.status, 106);
+                const int h = it & 1;
+                ok = warp_wait(&bar.w_full[h], (it >> 1) & 1, p.status, 106);
                 if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t q = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), g = q + (Z::PANELS * Z::SLAB64 >> 4);
-                const uint32_t w = (uint32_t)uniform((int)(wd + st * (BT * SUB * 2 >> 4))), ds = w + (2 * BT * SUB * 2 >> 4);
+                const uint32_t w = tm + S_COL + h * S_STEP;
                 if (lead) {
 #pragma unroll
-                    for (int kk = 0; kk < SUB / 16; ++kk) mma_ss_lo(tm, w + kk * 2, g + kk * 128, IDESC_V, it > 0 || kk > 0);
-#pragma unroll
                     for (int kk = 0; kk < SUB / 16; ++kk) mma_ss_lo(tm + DK_COL, ds + kk * 2, q + kk * 128, idesc_k, it > 0 || kk > 0);
-                    mma_commit(&bar.w_free[st]);
+                    mma_commit(&bar.ds_free);
+#pragma unroll
+                    for (int kk = 0; kk < SUB / 16; ++kk) mma_ts_lo(tm, w + kk * 8, g + kk * 128, IDESC_V, it > 0 || kk > 0);
+                    mma_commit(&bar.w_free[h]);
                     mma_commit(&bar.st_empty[st]);
                     if (it + 1 == n_it) mma_commit(&bar.final_);
                 }
+                if (++st == STAGES) st = 0;
             }
         }
         if (!ok) *abort_flag = 1;
@@ -341,12 +347,13 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     } else if (warp == 3) {
         // ------------------------------------------------------------ rows of padded tokens become zeros
         bool ok = true;
-        int n_fix[2] = {0, 0};
+        int n_fix = 0;
         for (int it = 0; it < nit && ok; ++it) {
             if (!padded(it)) continue;
-            const int st = it & 1;
-            ok = warp_wait(&bar.fix[st], n_fix[st]++ & 1, p.status, 107);
+            const int st = it % STAGES;
+            ok = warp_wait(&bar.fix[st], (n_fix >> st) & 1, p.status, 107);
             if (!ok) break;
+            n_fix ^= 1 << st;
             zero_rows(smem + M::OFF_ST + st * Z::STAGE, 2 * Z::PANELS - 1, max(0, nL - first_of(it)), lane);
             fence_proxy_async_smem();
             __syncwarp();
@@ -357,24 +364,21 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         // ------------------------------------------------------------ weights: warpgroup wg takes the sub-tiles it % 2 == wg
         const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, key = key0 + r;
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-        unsigned char* w_row = smem + M::OFF_W + wg * (BT * SUB * 2) + r * 128;
-        unsigned char* ds_row = smem + M::OFF_DS + wg * (BT * SUB * 2) + r * 128;
-        const float* nl = (const float*)(smem + M::OFF_ROW + wg * 512);
+        unsigned char* ds_row = smem + M::OFF_DS + r * 128;
+        const uint32_t s_tmem = tmem + lane_addr + S_COL + wg * S_STEP, dp_tmem = tmem + lane_addr + DP_COL;
         const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
         bool ok = true;
         for (int it = wg; it < nit; it += 2) {
-            const int n = 2 * it, s0 = n % 3, s1 = (n + 1) % 3, q0 = first_of(it);
-            ok = warp_wait(&bar.st_full[wg], (it >> 1) & 1, p.status, 108);  // the rows' lse and delta
-            if (ok) ok = warp_wait(&bar.r_full[s0], (n / 3) & 1, p.status, 109);
+            const int st = it % STAGES, q0 = first_of(it);
+            const float* nl = (const float*)(smem + M::OFF_ROW + st * 512);  // the queries' -lse2, and 64 further on their -delta
+            ok = warp_wait(&bar.s_full[wg], (it >> 1) & 1, p.status, 109);
+            if (ok) ok = warp_wait(&bar.st_full[st], (it / STAGES) & 1, p.status, 108);  // (complete: this makes its rows visible)
             if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
             tc_fence_after();
             uint32_t ra[64], rb[64];
-            tmem_ld32(tmem + lane_addr + RING + s0 * SUB, ra);
-            tmem_ld32(tmem + lane_addr + RING + s0 * SUB + 32, ra + 32);
+            tmem_ld32(s_tmem, ra);
+            tmem_ld32(s_tmem + 32, ra + 32);
             tmem_ld_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.r_free[s0]);
 #pragma unroll
             for (int i = 0; i < SUB; i += 2) {
                 float a0, a1;
@@ -387,34 +391,40 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
                 for (int i = 0; i < SUB; ++i)
                     if (key > q0 + i) ra[i] = 0u;
             }
-            ok = warp_wait(&bar.r_full[s1], ((n + 1) / 3) & 1, p.status, 110);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {  // W^T over S^T, already read: queries 16 bits each, two a column
+                uint32_t w[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i] = pack2<BF16>(__uint_as_float(ra[32 * c + 2 * i]), __uint_as_float(ra[32 * c + 2 * i + 1]));
+                tmem_st16(s_tmem + 16 * c, w);
+            }
+            ok = warp_wait(&bar.dp_full, it & 1, p.status, 110);
             if (!ok) break;
             tc_fence_after();
-            tmem_ld32(tmem + lane_addr + RING + s1 * SUB, rb);
-            tmem_ld32(tmem + lane_addr + RING + s1 * SUB + 32, rb + 32);
+            tmem_ld32(dp_tmem, rb);
+            tmem_ld32(dp_tmem + 32, rb + 32);
             tmem_ld_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.r_free[s1]);
-            if (it >= 2) ok = warp_wait(&bar.w_free[wg], ((it >> 1) - 1) & 1, p.status, 111);
+            if (lane == 0) mbar_arrive(&bar.dp_free);
+            if (it >= 1) ok = warp_wait(&bar.ds_free, (it - 1) & 1, p.status, 111);  // dK has read the last sub-tile's dS^T
             if (!ok) break;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {  // 16 bytes of W^T and of dS^T: 8 queries
-                uint32_t wv[4], dv[4];
+            for (int j = 0; j < 8; ++j) {  // 16 bytes of dS^T: 8 queries
+                uint32_t dv[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = 8 * j + 2 * e;
-                    const float p0 = __uint_as_float(ra[i]), p1 = __uint_as_float(ra[i + 1]);
                     float d0, d1;
-                    f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack(__uint_as_float(rb[i]), __uint_as_float(rb[i + 1])),
-                                                             *(const uint64_t*)(nl + SUB + i))), d0, d1);
-                    wv[e] = pack2<BF16>(p0, p1);
+                    f2_unpack(f2_mul(f2_pack(__uint_as_float(ra[i]), __uint_as_float(ra[i + 1])),
+                                     f2_add(f2_pack(__uint_as_float(rb[i]), __uint_as_float(rb[i + 1])), *(const uint64_t*)(nl + SUB + i))), d0, d1);
                     dv[e] = pack2<BF16>(d0, d1);
                 }
-                *(uint4*)(w_row + ((j ^ (r & 7)) << 4)) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
                 *(uint4*)(ds_row + ((j ^ (r & 7)) << 4)) = make_uint4(dv[0], dv[1], dv[2], dv[3]);
             }
+            tmem_st_wait();
             fence_proxy_async_smem();
+            tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.w_full[wg]);
         }
@@ -460,20 +470,18 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
 // ------------------------------------------------------------------ dQ
 
-constexpr int Q_STAGES = 3;
-
 template <int DN>
 struct QSmem {
     using Z = Sizes<DN>;
     static constexpr int OFF_G = Z::KTILE, OFF_ST = OFF_G + Z::VTILE;
-    static constexpr int OFF_BAR = OFF_ST + Q_STAGES * Z::STAGE;
+    static constexpr int OFF_BAR = OFF_ST + STAGES * Z::STAGE;
     static constexpr int USED = OFF_BAR + 256;
     static constexpr int ALLOC = USED + 1023;
     static_assert(ALLOC <= SMEM_MAX, "shared memory");
 };
 
 struct QBars {
-    uint64_t q_full, st_full[Q_STAGES], st_empty[Q_STAGES], s_full[2], ds_full[2], ds_free[2], fix, fixed, final_, drain[2];
+    uint64_t q_full, st_full[STAGES], st_empty[STAGES], s_full[2], s_free[2], ds_full[2], ds_free[2], fix, fixed, final_, drain[2];
     uint32_t tmem;
     int abort;
 };
@@ -486,7 +494,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
     using Z = Sizes<DN>;
     using M = QSmem<DN>;
-    constexpr uint32_t S_COL = 256, DP_COL = 384;  // dQ from 0; S and dP of sub-tile h at + 64 h
+    constexpr uint32_t DS_COL = 192, S_COL = 256, DP_COL = 384;  // dQ from 0; dS of sub-tile h at + 32 h, S and dP at + 64 h
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     QBars& bar = *(QBars*)(smem + M::OFF_BAR);
@@ -505,12 +513,13 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         mbar_init(&bar.final_, 1);
         mbar_init(&bar.fix, 1);
         mbar_init(&bar.fixed, 1);
-        for (int i = 0; i < Q_STAGES; ++i) {
+        for (int i = 0; i < STAGES; ++i) {
             mbar_init(&bar.st_full[i], 1);
             mbar_init(&bar.st_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.s_full[i], 1);
+            mbar_init(&bar.s_free[i], 4);
             mbar_init(&bar.ds_full[i], 4);
             mbar_init(&bar.ds_free[i], 1);
             mbar_init(&bar.drain[i], 1);
@@ -538,8 +547,8 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             bool ok = true;
             int it = 0;
             for (; it < nit; ++it) {
-                const int st = it % Q_STAGES;
-                if (it >= Q_STAGES) ok = mbar_wait(&bar.st_empty[st], (it / Q_STAGES - 1) & 1, p.status, 121);
+                const int st = it % STAGES;
+                if (it >= STAGES) ok = mbar_wait(&bar.st_empty[st], (it / STAGES - 1) & 1, p.status, 121);
                 if (!ok || *abort_flag) { ok = false; break; }
                 unsigned char* d = smem + M::OFF_ST + st * Z::STAGE;
                 mbar_expect_tx(&bar.st_full[st], Z::STAGE);
@@ -551,7 +560,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             if (!ok) *abort_flag = 1;
             if (*abort_flag) {
                 mbar_wait(&bar.q_full, 0, nullptr, 0);
-                for (int n = max(0, it - Q_STAGES); n < it; ++n) mbar_wait(&bar.st_full[n % Q_STAGES], (n / Q_STAGES) & 1, nullptr, 0);
+                for (int n = max(0, it - STAGES); n < it; ++n) mbar_wait(&bar.st_full[n % STAGES], (n / STAGES) & 1, nullptr, 0);
             }
         }
     } else if (warp < 3) {
@@ -572,8 +581,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                     if (lead) mbar_arrive(&bar.fix);
                     ok = warp_wait(&bar.fixed, 0, p.status, 124);
                 }
-                // S's columns hold the dS that the product two sub-tiles ago read
-                if (ok && it >= 2) ok = warp_wait(&bar.ds_free[it & 1], ((it >> 1) - 1) & 1, p.status, 125);
+                if (ok && it >= 2) ok = warp_wait(&bar.s_free[it & 1], ((it >> 1) - 1) & 1, p.status, 125);
                 if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
                 tc_fence_after();
                 const uint32_t k = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), v = k + (Z::PANELS * Z::SLAB64 >> 4);
@@ -591,7 +599,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                         mma_ss_lo(p_dst, gd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, v + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC, kk > 0);
                     mma_commit(&bar.s_full[it & 1]);
                 }
-                if (++st == Q_STAGES) st = 0, phase ^= 1;
+                if (++st == STAGES) st = 0, phase ^= 1;
             }
         } else {
             const uint32_t idesc = idesc_f16(BT, 0, BF16, true) | (uint32_t)(DN + 16 * p.rope_steps) >> 3 << 17;
@@ -600,7 +608,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                 ok = warp_wait(&bar.ds_full[it & 1], (it >> 1) & 1, p.status, 126);
                 if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t k = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), ds = tm + S_COL + (it & 1) * SUB;
+                const uint32_t k = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), ds = tm + DS_COL + (it & 1) * 32;
                 if (lead) {
 #pragma unroll
                     for (int kk = 0; kk < SUB / 16; ++kk) mma_ts_lo(tm, ds + kk * 8, k + kk * 128, idesc, it > 0 || kk > 0);
@@ -608,7 +616,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                     mma_commit(&bar.st_empty[st]);
                     if (it + 1 == n_it) mma_commit(&bar.final_);
                 }
-                if (++st == Q_STAGES) st = 0;
+                if (++st == STAGES) st = 0;
             }
         }
         if (!ok) *abort_flag = 1;
@@ -622,7 +630,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (nit > 0 && padded(nit - 1)) {
             const bool ok = warp_wait(&bar.fix, 0, p.status, 127);
             if (ok) {
-                zero_rows(smem + M::OFF_ST + ((nit - 1) % Q_STAGES) * Z::STAGE, 2 * Z::PANELS - 1, max(0, nS - (nit - 1) * SUB), lane);
+                zero_rows(smem + M::OFF_ST + ((nit - 1) % STAGES) * Z::STAGE, 2 * Z::PANELS - 1, max(0, nS - (nit - 1) * SUB), lane);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar.fixed);
@@ -635,6 +643,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, row = row0 + r;
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
         const uint32_t s_tmem = tmem + lane_addr + S_COL + wg * SUB, p_tmem = tmem + lane_addr + DP_COL + wg * SUB;
+        const uint32_t ds_tmem = tmem + lane_addr + DS_COL + wg * 32;
         const int64_t rr = ((int64_t)b * p.H + h) * p.Lpad + row;
         const float nl = row < p.Lpad ? p.nlse2[rr] : -INFINITY, nd = row < p.Lpad ? p.ndelta[rr] : 0.0f;
         const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nl2 = f2_pack(nl, nl), nd2 = f2_pack(nd, nd);
@@ -652,6 +661,12 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             tmem_ld32(p_tmem, rb);
             tmem_ld32(p_tmem + 32, rb + 32);
             tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.s_free[wg]);
+            if (it >= 2) ok = warp_wait(&bar.ds_free[wg], ((it >> 1) - 1) & 1, p.status, 130);  // dQ has read the dS before
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t dk[16];
@@ -669,7 +684,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                     f2_unpack(f2_mul(f2_pack(a0, a1), f2_add(f2_pack(__uint_as_float(rb[k]), __uint_as_float(rb[k + 1])), nd2)), d0, d1);
                     dk[i / 2] = pack2<BF16>(d0, d1);
                 }
-                tmem_st16(s_tmem + 16 * c, dk);
+                tmem_st16(ds_tmem + 16 * c, dk);
             }
             tmem_st_wait();
             tc_fence_before();
