@@ -227,9 +227,9 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             // key tiles; tiles and items of each query tile; items with work; halves of values that were mended
             int J = 0, u[2] = {0, 0}, nf[2] = {0, 0}, ne = 0, fixed[2] = {0, 0};
             bool ok = true;
-            auto issue_s = [&](int t, int jg) {
+            auto issue_s = [&](int t, int jg, bool loaded) {
                 const int ks = jg & 1;
-                if (!warp_wait(&bar.k_full[ks], (jg >> 1) & 1, p.status, 88)) return false;
+                if (!loaded && !warp_wait(&bar.k_full[ks], (jg >> 1) & 1, p.status, 88)) return false;
                 tc_fence_after();
                 const uint32_t q = q0 + t * (C::TILE >> 4), k = (uint32_t)uniform((int)(k0 + ks * (C::TILE >> 4))), dst = tm + t * 128;
                 if (lead) {
@@ -254,7 +254,7 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (n == 0) continue;
                 ok = warp_wait(&bar.q_full, ne & 1, p.status, 89);
                 for (int t = 0; t < 2 && ok; ++t)
-                    if (nb[t] > 0) ok = issue_s(t, J);
+                    if (nb[t] > 0) ok = issue_s(t, J, false);
                 if (!ok) break;
                 if (lead) {
                     mma_commit(&bar.k_empty[J & 1]);
@@ -264,10 +264,10 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         if (!ok || j >= nb[t]) continue;
-                        // the first product of an item overwrites O_t: the last item's output must have been read
-                        if (j == 0 && nf[t] > 0) ok = warp_wait(&bar.o_empty[t], (nf[t] - 1) & 1, p.status, 90);
-                        if (ok) ok = warp_wait(&bar.p_full[t], (u[t] + j) & 1, p.status, 91);
-                        const bool last_t = t == 1 || j >= nb[1];  // the last query tile to read this value tile
+                        // The waits for what is mostly there already come before the one for the weights: between products each
+                        // wait leaves the tensor core idle for some 115 cycles.
+                        const bool more = j + 1 < nb[t];
+                        const bool loaded = more && __all_sync(~0u, mbar_test(&bar.k_full[(J + j + 1) & 1], ((J + j + 1) >> 1) & 1));
 #pragma unroll
                         for (int v = 0; v < 2; ++v) {
                             if (ok) ok = warp_wait(&bar.v_full[v], (J + j) & 1, p.status, 92);
@@ -275,20 +275,25 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                                 if (lead && (t == 0 || j >= nb[0])) mbar_arrive(&bar.fix[v]);
                                 ok = warp_wait(&bar.v_fixed[v], fixed[v] & 1, p.status, 93);
                             }
-                            if (!ok) continue;
-                            tc_fence_after();
-                            const uint32_t vb = v0 + v * (C::VHALF >> 4), dst = tm + 256 + t * 128, pa = tm + t * 128;
-                            if (lead) {
-#pragma unroll
-                                for (int k4 = 0; k4 < 4; ++k4) {
-                                    // P_t: 16-bit pairs, keys 32 c .. in columns 32 c .. 32 c + 15
-                                    const int kk = 4 * v + k4;
-                                    mma_ts_lo(dst, pa + 32 * (kk >> 1) + 8 * (kk & 1), vb + k4 * 128, IDESC_PV, j > 0 || kk > 0);
-                                }
-                                if (last_t) mma_commit(&bar.v_empty[v]);
-                            }
                         }
-                        if (ok && j + 1 < nb[t]) ok = issue_s(t, J + j + 1);
+                        // the first product of an item overwrites O_t: the last item's output must have been read
+                        if (ok && j == 0 && nf[t] > 0) ok = warp_wait(&bar.o_empty[t], (nf[t] - 1) & 1, p.status, 90);
+                        if (ok) ok = warp_wait(&bar.p_full[t], (u[t] + j) & 1, p.status, 91);
+                        if (!ok) continue;
+                        tc_fence_after();
+                        const bool last_t = t == 1 || j >= nb[1];  // the last query tile to read this value tile
+                        const uint32_t dst = tm + 256 + t * 128, pa = tm + t * 128;
+                        if (lead) {
+#pragma unroll
+                            for (int kk = 0; kk < BN / 16; ++kk) {
+                                // P_t: 16-bit pairs, keys 32 c .. in columns 32 c .. 32 c + 15
+                                mma_ts_lo(dst, pa + 32 * (kk >> 1) + 8 * (kk & 1), v0 + (kk >> 2) * (C::VHALF >> 4) + (kk & 3) * 128, IDESC_PV,
+                                          j > 0 || kk > 0);
+                                if (kk == 3 && last_t) mma_commit(&bar.v_empty[0]);
+                            }
+                            if (last_t) mma_commit(&bar.v_empty[1]);
+                        }
+                        if (more) ok = issue_s(t, J + j + 1, loaded);
                         if (ok && j + 1 == nb[t] && lead) mma_commit(&bar.o_final[t]);
                     }
                     if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }

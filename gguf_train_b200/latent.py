@@ -214,12 +214,6 @@ def _on_tensor_cores(q, k, k_rope, v) -> bool:
         q.shape[0] <= 65535 and q.shape[1] <= 65535 and min(q.shape) > 0 and min(k.shape) > 0
 
 
-def _like(t: torch.Tensor) -> torch.Tensor:
-    """An empty tensor of t's shape, in t's layout where that is dense (q as a view of its projection)."""
-    out = torch.empty_like(t)
-    return out if _tiled(out) is out else torch.empty_like(t, memory_format=torch.contiguous_format)
-
-
 class LatentSDPAFn(torch.autograd.Function):
     """latent_sdpa on the native kernels: apply(q, k, k_rope, v, is_causal, scale, seq_lens). The backward recomputes the weights
     from the saved log-sum-exp."""
@@ -235,12 +229,12 @@ class LatentSDPAFn(torch.autograd.Function):
                                         1 if is_causal else 0, _C.tensor4(out, code), None if lse is None else lse.data_ptr(),
                                         _stream(q.device))
         _C.check_rc(rc, "latent_sdpa")
-        return q, k, kr, v, out, lse
+        return q, k, kr, v, out, lse, (qt, kt, rt, vt)
 
     @staticmethod
     def forward(ctx, q, k, k_rope, v, is_causal, scale, seq_lens):
-        q, k, kr, v, out, lse = LatentSDPAFn._forward(q, k, k_rope, v, is_causal, scale, seq_lens, True)
-        ctx.args = is_causal, scale
+        q, k, kr, v, out, lse, packed = LatentSDPAFn._forward(q, k, k_rope, v, is_causal, scale, seq_lens, True)
+        ctx.args = is_causal, scale, packed
         ctx.save_for_backward(q, k, kr, v, out, lse, seq_lens)
         return out
 
@@ -248,11 +242,11 @@ class LatentSDPAFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         q, k, kr, v, out, lse, seq_lens = ctx.saved_tensors
-        is_causal, scale = ctx.args
+        is_causal, scale, (qt, kt, rt, vt) = ctx.args
         code = _CODE[q.dtype]
         g, gt = _rows(grad_out, code)
-        qt, kt, rt, vt = (_rows(t, code)[1] for t in (q, k, kr, v))
-        dq, dk, dkr, dv = _like(q), _like(k), torch.empty_like(kr, memory_format=torch.contiguous_format), _like(v)
+        # (in the inputs' layouts where those are dense, as q's as a view of its projection; all of them start on 16 bytes)
+        dq, dk, dkr, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(kr), torch.empty_like(v)
         rc = _C.lib.gtb_latent_sdpa_bwd(gt, qt, kt, rt, vt, _C.tensor4(out, code), lse.data_ptr(),
                                         None if seq_lens is None else seq_lens.data_ptr(), scale, 1 if is_causal else 0,
                                         _C.tensor4(dq, code), _C.tensor4(dk, code), _rows(dkr, code)[1], _C.tensor4(dv, code),
