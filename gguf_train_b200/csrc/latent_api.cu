@@ -91,7 +91,7 @@ bool check_sdpa(const char* ctx, const gtb_tensor4* q, const gtb_tensor4* k, con
     if (a.Hkv == 0 ? a.H != 0 : a.H % a.Hkv) return fail(ctx, "num_heads must be divisible by num_kv_heads");
     if (a.B > 65535 || a.H > 65535) return fail(ctx, "at most 65535 sequences and heads");
     if (lens && a.L != a.S) return fail(ctx, "lengths need as many queries as keys");
-    if (!std::isfinite(scale) || !(scale > 0.0f)) return fail(ctx, "scale must be positive and finite");
+    if (!(scale > 0.0f && scale < 1e38f)) return fail(ctx, "scale must be positive and below 1e38");
     a.q = *q;
     a.k = *k;
     a.k_rope = *k_rope;
@@ -193,7 +193,7 @@ GTB_API int gtb_latent_attention(const gtb_tensor4* q, const gtb_latent* cache, 
         }
         if (H > INT32_MAX / 64 || Lq > INT32_MAX / 64 || (H > 0 && Lq > 0 && cache->B > INT32_MAX / 64 / (H * Lq)))
             return fail(ctx, "too many query rows"), -1;
-        if (!std::isfinite(scale) || !(scale > 0.0f)) return fail(ctx, "scale must be positive and finite"), -1;
+        if (!(scale > 0.0f && scale < 1e38f)) return fail(ctx, "scale must be positive and below 1e38"), -1;
         if (cache->B * H * Lq == 0) return 0;
         int64_t s = 1;
         for (int i = 3; i >= 0; --i) {

@@ -180,8 +180,8 @@ def latent_attention(q: torch.Tensor, cache: LatentCache, scale: float, counts: 
     if q.dtype != cache._rows.dtype:
         raise RuntimeError(f"latent_attention: q must be of the cache's type {cache._rows.dtype}, got {q.dtype}")
     scale = float(scale)
-    if not (math.isfinite(scale) and scale > 0.0):
-        raise RuntimeError(f"latent_attention: scale must be positive and finite, got {scale}")
+    if not 0.0 < scale < 1e38:
+        raise RuntimeError(f"latent_attention: scale must be positive and below 1e38, got {scale}")
     code = _CODE[q.dtype]
     q, qt = _rows(q, code)
     H, Lq = q.shape[1:3]
@@ -229,12 +229,12 @@ class LatentSDPAFn(torch.autograd.Function):
                                         1 if is_causal else 0, _C.tensor4(out, code), None if lse is None else lse.data_ptr(),
                                         _stream(q.device))
         _C.check_rc(rc, "latent_sdpa")
-        return q, k, kr, v, out, lse, (qt, kt, rt, vt)
+        return q, k, kr, v, out, lse
 
     @staticmethod
     def forward(ctx, q, k, k_rope, v, is_causal, scale, seq_lens):
-        q, k, kr, v, out, lse, packed = LatentSDPAFn._forward(q, k, k_rope, v, is_causal, scale, seq_lens, True)
-        ctx.args = is_causal, scale, packed
+        q, k, kr, v, out, lse = LatentSDPAFn._forward(q, k, k_rope, v, is_causal, scale, seq_lens, True)
+        ctx.args = is_causal, scale
         ctx.save_for_backward(q, k, kr, v, out, lse, seq_lens)
         return out
 
@@ -242,12 +242,14 @@ class LatentSDPAFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
         q, k, kr, v, out, lse, seq_lens = ctx.saved_tensors
-        is_causal, scale, (qt, kt, rt, vt) = ctx.args
+        is_causal, scale = ctx.args
         code = _CODE[q.dtype]
         g, gt = _rows(grad_out, code)
+        # (hooks on saved tensors may have brought them back in other places)
+        (q, qt), (k, kt), (kr, rt), (v, vt), (out, ot) = [_rows(t, code) for t in (q, k, kr, v, out)]
         # (in the inputs' layouts where those are dense, as q's as a view of its projection; all of them start on 16 bytes)
         dq, dk, dkr, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(kr), torch.empty_like(v)
-        rc = _C.lib.gtb_latent_sdpa_bwd(gt, qt, kt, rt, vt, _C.tensor4(out, code), lse.data_ptr(),
+        rc = _C.lib.gtb_latent_sdpa_bwd(gt, qt, kt, rt, vt, ot, lse.data_ptr(),
                                         None if seq_lens is None else seq_lens.data_ptr(), scale, 1 if is_causal else 0,
                                         _C.tensor4(dq, code), _C.tensor4(dk, code), _rows(dkr, code)[1], _C.tensor4(dv, code),
                                         _stream(q.device))
@@ -290,8 +292,8 @@ def latent_sdpa(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor, v: torch
         if seq_lens.dtype != torch.int32 or seq_lens.shape != (B,) or not seq_lens.is_contiguous():
             raise RuntimeError(f"latent_sdpa: seq_lens must be a contiguous int32 tensor of shape ({B},)")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not (math.isfinite(scale) and scale > 0.0):
-        raise RuntimeError(f"latent_sdpa: scale must be positive and finite, got {scale}")
+    if not 0.0 < scale < 1e38:
+        raise RuntimeError(f"latent_sdpa: scale must be positive and below 1e38, got {scale}")
     if not _on_tensor_cores(q, k, k_rope, v):
         return _sdpa_general(q, k, k_rope, v, bool(is_causal), scale, seq_lens)
     xs = (q, k, k_rope, v)

@@ -357,7 +357,9 @@ GTB_API int gtb_latent_append(const gtb_latent *cache, const gtb_tensor4 *latent
  * gives 0 and lse -inf.
  *   prefix: NULL, or a cache of one sequence (B = 1, same R, Dr and dtype) whose rows come before every sequence's own:
  *   they are read once for the whole batch. q 16-byte aligned, any strides that are multiples of 8 with a unit
- *   innermost one; out contiguous, 16-byte aligned; lse NULL or (B,H,Lq) f32; scale positive. */
+ *   innermost one; out contiguous, 16-byte aligned; lse NULL or (B,H,Lq) f32; scale positive, below 1e38.
+ * Scratch from the stream-ordered allocator: f32 parts of rows that several thread blocks worked on, at most two of 64 rows a
+ * multiprocessor (38 MB on 148 with R = 512), or behind a prefix one a sequence and a multiprocessor. */
 GTB_API int gtb_latent_attention(const gtb_tensor4 *q, const gtb_latent *cache, const gtb_latent *prefix, float scale,
                                  const int32_t *counts, gtb_tensor4 *out, float *lse, void *stream);
 
@@ -366,10 +368,11 @@ GTB_API int gtb_latent_attention(const gtb_tensor4 *q, const gtb_latent *cache, 
  *   score = scale * (q[..Dn] . k + q[Dn..] . k_rope), out (B,H,L,Dn); is_causal masks s > l (top-left aligned).
  *   seq_lens: NULL, or device int32 (B) with L = S: tokens from seq_lens[b] (clamped to [0, S]) on are not attended, whatever
  *   they hold; their out is 0, and all their gradients.
- *   lse: NULL or (B,H,L) f32, -inf where nothing is attended (out is 0 there).
+ *   lse: NULL or (B,H,L) f32, -inf where nothing is attended (out is 0 there). scale positive, below 1e38.
  * All tensors start on 16 bytes, with a unit innermost stride and others that are positive multiples of 8.
  * The backward takes the forward's out and lse and writes dq, dk, dk_rope (summed over all heads) and dv, in fixed order:
- * the same bits on every run. Its scratch (4 (2 B H L + B Hkv S Dr) bytes) comes from the stream-ordered allocator. */
+ * the same bits on every run. Its weights are 2^(score - log-sum-exp) of f32 numbers: off by about |score| 2^-22 of themselves
+ * (scores in powers of 2). Its scratch (4 (2 B H L + B Hkv S Dr) bytes) comes from the stream-ordered allocator. */
 GTB_API int gtb_latent_sdpa_fwd(const gtb_tensor4 *q, const gtb_tensor4 *k, const gtb_tensor4 *k_rope, const gtb_tensor4 *v,
                                 const int32_t *seq_lens, float scale, int is_causal, gtb_tensor4 *out, float *lse,
                                 void *stream);

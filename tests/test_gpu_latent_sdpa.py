@@ -192,3 +192,51 @@ def test_second_derivatives_are_refused():
     (dq,) = torch.autograd.grad(latent_sdpa(*leaves), leaves[0], g, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(dq.sum(), leaves[1])
+
+
+def test_gradients_of_other_shapes_and_places():
+    """A broadcast output gradient, a rotary key shared by the batch, and saved tensors kept on the host in between."""
+    from gguf_train_b200 import latent_sdpa
+
+    leaves, g = _inputs(3, 2, 2, 90, 90, 64, 32, 64, torch.bfloat16, 21)
+    one = leaves[2].detach()[:1].clone().requires_grad_()
+    out = latent_sdpa(leaves[0], leaves[1], one.expand(3, -1, -1), leaves[3], is_causal=True)
+    grads = torch.autograd.grad(out.sum(), (leaves[0], one))
+    full = one.detach().expand(3, -1, -1).contiguous().requires_grad_()
+    xs = (leaves[0], leaves[1], full, leaves[3])
+    want = torch.autograd.grad(latent_sdpa(*xs, is_causal=True), (leaves[0], full), torch.ones_like(g))
+    assert torch.equal(grads[0], want[0])
+    assert torch.equal(grads[1], want[1].sum(0, keepdim=True))
+    want = torch.autograd.grad(latent_sdpa(*leaves, is_causal=True), leaves, g)
+    with torch.autograd.graph.save_on_cpu():
+        out = latent_sdpa(*leaves, is_causal=True)
+    junk = [torch.randn_like(x) for x in leaves for _ in range(4)]  # takes what the saved tensors gave back
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, g), want)) and junk
+    # inputs that had to be copied to start on 16 bytes
+    odd = [torch.randn((*x.shape[:-1], x.shape[-1] + 3), device="cuda").to(torch.bfloat16)[..., 3:].requires_grad_() for x in leaves]
+    even = [x.detach().contiguous().requires_grad_() for x in odd]
+    with torch.autograd.graph.save_on_cpu():
+        a = latent_sdpa(*odd)
+    for x, y in zip(torch.autograd.grad(a, odd, g), torch.autograd.grad(latent_sdpa(*even), even, g)):
+        assert torch.equal(x, y)
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fw
+
+    from gguf_train_b200 import latent_sdpa
+
+    leaves, _ = _inputs(1, 1, 1, 20, 20, 64, 32, 64, torch.bfloat16, 1)
+    xs = [x.detach() for x in leaves]
+    with fw.dual_level(), pytest.raises(Exception):
+        latent_sdpa(fw.make_dual(xs[0], torch.ones_like(xs[0])), *xs[1:])
+
+
+@pytest.mark.parametrize("shape", [(0, 2, 5, 5), (2, 2, 0, 0), (1, 2, 0, 7)])
+def test_nothing_to_compute(shape):
+    from gguf_train_b200 import latent_sdpa
+
+    B, H, L, S = shape
+    r = lambda *s: torch.randn(s, device="cuda").to(torch.bfloat16)  # noqa: E731
+    out = latent_sdpa(r(B, H, L, 96), r(B, H, S, 64), r(B, S, 32), r(B, H, S, 64))
+    assert out.shape == (B, H, L, 64)
