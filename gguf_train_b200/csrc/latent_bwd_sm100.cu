@@ -7,19 +7,22 @@
 //             dV += W^T G, dK += dS^T Q                (M = 128 keys, N = dims, K = 64; W^T from TMEM, dS^T from shared memory)
 //           The rotary part of dK is the sum over all heads: each CTA writes its share in f32 and a last kernel adds the
 //           heads in order, so the bits are the same on every run.
-//   dQ      one CTA a 128-query tile, over 64 keys at a time:
-//             S = Q [K | K_r]^T, dP = G V^T            (M = 128 queries, N = 64 keys)
-//             dQ += dS [K | K_r]                       (N = dims, K = 64; dS from TMEM)
+//   dQ      one CTA a 128-query tile, over 128 keys at a time:
+//             S = Q [K | K_r]^T, dP = G V^T            (M = 128 queries, N = 128 keys)
+//             dQ += dS [K | K_r]                       (N = dims, K = 128; dS from TMEM)
 // A fused dQ (five products instead of seven) needs f32 sums in global memory by unordered additions, and TMEM that dK's 192 columns
 // do not leave. Products of N = 64 with both operands in shared memory are bound by its bandwidth (49.5 cycles instead of 32):
-// 64 is what TMEM holds of scores next to dV and dK (320 of 512 columns with Dn = 128).
+// 64 is what TMEM holds of scores next to dV and dK (320 of 512 columns with Dn = 128). Beside dQ alone 128 fit.
 //
-// Warps: 0 TMA producer, 1 issues the score products (and owns TMEM), 2 the gradient products, 3 zeroes rows of padded tokens in a
-// loaded stage (their product with a weight of 0 would be NaN), 4-7 and 8-11 the weights of even and odd sub-tiles, a key (dK/dV)
-// or query (dQ) a thread. TMEM of the dK/dV kernel with Dn = 128: dV 128 columns, dK 192, two S^T of 64 (over which W^T is written), one
-// dP^T; of the dQ kernel: dQ 192, two dS of 32, two S and two dP of 64. Three stages of 64 rows stream: what a stage waits for (its
-// load, the scores, the weights, the gradients) is about three times what the tensor core does on it. Every mbarrier
-// wait is bounded.
+// Warps: 0 TMA producer, 1 issues the score products (and owns TMEM), 2 the gradient products, 3 (dK/dV) zeroes rows of padded tokens
+// in a loaded stage (their product with a weight of 0 would be NaN), 4-7 and 8-11 the weights: in the dK/dV kernel of even
+// and odd sub-tiles, a key a thread; in the dQ kernel of a tile's two halves, a query a thread. TMEM of the dK/dV kernel with
+// Dn = 128: dV 128 columns, dK 192, two S^T of 64 (over which W^T is written), one dP^T; of the dQ kernel: dQ 192, dS 64, S 128,
+// dP 128. The dK/dV kernel streams through three stages of 64 rows: what a stage waits for (its load, the scores, the
+// weights, the gradients) is about three times what the tensor core does on it. The dQ kernel has two key tiles and one
+// value tile, which is free again as soon as dP is formed. Every mbarrier wait is bounded.
+//
+// Measured, 2 x 4096 tokens, 16 heads of 128 + 64, causal, bf16: dK/dV 398 us, dQ FIG_Q us (292 over 64 keys at a time).
 
 #include <algorithm>
 #include <atomic>
@@ -473,15 +476,15 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 template <int DN>
 struct QSmem {
     using Z = Sizes<DN>;
-    static constexpr int OFF_G = Z::KTILE, OFF_ST = OFF_G + Z::VTILE;
-    static constexpr int OFF_BAR = OFF_ST + STAGES * Z::STAGE;
+    static constexpr int OFF_G = Z::KTILE, OFF_K = OFF_G + Z::VTILE, OFF_V = OFF_K + 2 * Z::KTILE;
+    static constexpr int OFF_BAR = OFF_V + Z::VTILE;
     static constexpr int USED = OFF_BAR + 256;
     static constexpr int ALLOC = USED + 1023;
     static_assert(ALLOC <= SMEM_MAX, "shared memory");
 };
 
 struct QBars {
-    uint64_t q_full, st_full[STAGES], st_empty[STAGES], s_full[2], s_free[2], ds_full[2], ds_free[2], fix, fixed, final_, drain[2];
+    uint64_t q_full, k_full[2], k_empty[2], v_full, v_empty, s_full, s_free, dp_full, dp_free, ds_full, ds_free, final_, drain[2];
     uint32_t tmem;
     int abort;
 };
@@ -494,7 +497,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
     using Z = Sizes<DN>;
     using M = QSmem<DN>;
-    constexpr uint32_t DS_COL = 192, S_COL = 256, DP_COL = 384;  // dQ from 0; dS of sub-tile h at + 32 h, S and dP at + 64 h
+    constexpr uint32_t DS_COL = 192, S_COL = 256, DP_COL = 384;  // dQ from 0; dS as 16-bit pairs
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     QBars& bar = *(QBars*)(smem + M::OFF_BAR);
@@ -505,23 +508,23 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     if (p.causal) tile = n_qt - 1 - tile;
     const int b = unit / p.H, h = unit - b * p.H, hk = h / p.group, row0 = tile * BT;
     const int nL = latent_tokens(p.lens, b, p.L), nS = latent_tokens(p.lens, b, p.S);
-    const int all = (nS + SUB - 1) / SUB;
-    const int nit = row0 >= nL ? 0 : p.causal ? min(all, (min(row0 + BT, nL) - 1) / SUB + 1) : all;
+    const int all = (nS + BT - 1) / BT;
+    const int nit = row0 >= nL ? 0 : p.causal ? min(all, (min(row0 + BT, nL) - 1) / BT + 1) : all;
 
     if (threadIdx.x == 0) {
         mbar_init(&bar.q_full, 1);
+        mbar_init(&bar.v_full, 1);
+        mbar_init(&bar.v_empty, 1);
+        mbar_init(&bar.s_full, 1);
+        mbar_init(&bar.s_free, 8);
+        mbar_init(&bar.dp_full, 1);
+        mbar_init(&bar.dp_free, 8);
+        mbar_init(&bar.ds_full, 8);
+        mbar_init(&bar.ds_free, 1);
         mbar_init(&bar.final_, 1);
-        mbar_init(&bar.fix, 1);
-        mbar_init(&bar.fixed, 1);
-        for (int i = 0; i < STAGES; ++i) {
-            mbar_init(&bar.st_full[i], 1);
-            mbar_init(&bar.st_empty[i], 1);
-        }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&bar.s_full[i], 1);
-            mbar_init(&bar.s_free[i], 4);
-            mbar_init(&bar.ds_full[i], 4);
-            mbar_init(&bar.ds_free[i], 1);
+            mbar_init(&bar.k_full[i], 1);
+            mbar_init(&bar.k_empty[i], 1);
             mbar_init(&bar.drain[i], 1);
         }
         bar.abort = 0;
@@ -533,7 +536,6 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     tc_fence_after();
     const uint32_t tmem = bar.tmem;
     volatile int* abort_flag = &bar.abort;
-    auto padded = [&](int it) { return p.lens && (it + 1) * SUB > nS; };  // (the last sub-tile only)
 
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
@@ -545,22 +547,27 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             for (int a = 0; a < Z::PANELS; ++a) tma_load_4d(smem + a * Z::SLAB, &tmQ, a * 64, row0, h, b, &bar.q_full);
             for (int a = 0; a < DN / 64; ++a) tma_load_4d(smem + M::OFF_G + a * Z::SLAB, &tmG, a * 64, row0, h, b, &bar.q_full);
             bool ok = true;
-            int it = 0;
-            for (; it < nit; ++it) {
-                const int st = it % STAGES;
-                if (it >= STAGES) ok = mbar_wait(&bar.st_empty[st], (it / STAGES - 1) & 1, p.status, 121);
+            int nk = 0, nv = 0;
+            for (int it = 0; it < nit; ++it) {
+                const int st = it & 1;
+                if (it >= 2) ok = mbar_wait(&bar.k_empty[st], ((it >> 1) - 1) & 1, p.status, 121);
                 if (!ok || *abort_flag) { ok = false; break; }
-                unsigned char* d = smem + M::OFF_ST + st * Z::STAGE;
-                mbar_expect_tx(&bar.st_full[st], Z::STAGE);
-                for (int a = 0; a < DN / 64; ++a) tma_load_4d(d + a * Z::SLAB64, &tmK, a * 64, it * SUB, hk, b, &bar.st_full[st]);
-                tma_load_4d(d + (DN / 64) * Z::SLAB64, &tmR, 0, it * SUB, 0, b, &bar.st_full[st]);
-                for (int a = 0; a < DN / 64; ++a)
-                    tma_load_4d(d + (Z::PANELS + a) * Z::SLAB64, &tmV, a * 64, it * SUB, hk, b, &bar.st_full[st]);
+                unsigned char* d = smem + M::OFF_K + st * Z::KTILE;
+                mbar_expect_tx(&bar.k_full[st], Z::KTILE);
+                for (int a = 0; a < DN / 64; ++a) tma_load_4d(d + a * Z::SLAB, &tmK, a * 64, it * BT, hk, b, &bar.k_full[st]);
+                tma_load_4d(d + (DN / 64) * Z::SLAB, &tmR, 0, it * BT, 0, b, &bar.k_full[st]);
+                ++nk;
+                if (it >= 1) ok = mbar_wait(&bar.v_empty, (it - 1) & 1, p.status, 131);
+                if (!ok || *abort_flag) { ok = false; break; }
+                mbar_expect_tx(&bar.v_full, Z::VTILE);
+                for (int a = 0; a < DN / 64; ++a) tma_load_4d(smem + M::OFF_V + a * Z::SLAB, &tmV, a * 64, it * BT, hk, b, &bar.v_full);
+                ++nv;
             }
             if (!ok) *abort_flag = 1;
             if (*abort_flag) {
                 mbar_wait(&bar.q_full, 0, nullptr, 0);
-                for (int n = max(0, it - STAGES); n < it; ++n) mbar_wait(&bar.st_full[n % STAGES], (n / STAGES) & 1, nullptr, 0);
+                for (int n = max(0, nk - 2); n < nk; ++n) mbar_wait(&bar.k_full[n & 1], (n >> 1) & 1, nullptr, 0);
+                if (nv > 0) mbar_wait(&bar.v_full, (nv - 1) & 1, nullptr, 0);
             }
         }
     } else if (warp < 3) {
@@ -569,54 +576,59 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const uint32_t tm = (uint32_t)uniform((int)tmem);
         const int n_it = uniform(nit);
         bool ok = true;
-        int st = 0, phase = 0;
         if (warp == 1) {
-            constexpr uint32_t IDESC = idesc_f16(BT, SUB, BF16, false);
+            constexpr uint32_t IDESC = idesc_f16(BT, BT, BF16, false);
             const uint32_t qd = desc_lo(smem_u32(smem), 16), gd = desc_lo(smem_u32(smem + M::OFF_G), 16);
-            const uint32_t sd = desc_lo(smem_u32(smem + M::OFF_ST), 16);
+            const uint32_t kd = desc_lo(smem_u32(smem + M::OFF_K), 16), vd = desc_lo(smem_u32(smem + M::OFF_V), 16);
             if (n_it > 0) ok = warp_wait(&bar.q_full, 0, p.status, 122);
             for (int it = 0; it < n_it && ok; ++it) {
-                ok = warp_wait(&bar.st_full[st], phase, p.status, 123);
-                if (ok && padded(it)) {
-                    if (lead) mbar_arrive(&bar.fix);
-                    ok = warp_wait(&bar.fixed, 0, p.status, 124);
-                }
-                if (ok && it >= 2) ok = warp_wait(&bar.s_free[it & 1], ((it >> 1) - 1) & 1, p.status, 125);
+                ok = warp_wait(&bar.k_full[it & 1], (it >> 1) & 1, p.status, 123);
+                if (ok && it >= 1) ok = warp_wait(&bar.s_free, (it - 1) & 1, p.status, 125);
                 if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t k = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), v = k + (Z::PANELS * Z::SLAB64 >> 4);
-                const uint32_t s_dst = tm + S_COL + (it & 1) * SUB, p_dst = tm + DP_COL + (it & 1) * SUB;
+                const uint32_t k = (uint32_t)uniform((int)(kd + (it & 1) * (Z::KTILE >> 4)));
                 if (lead) {
 #pragma unroll
-                    for (int kk = 0; kk < DN / 16; ++kk)
-                        mma_ss_lo(s_dst, qd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, k + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC, kk > 0);
+                    for (int kk = 0; kk < DN / 16; ++kk) {
+                        const uint32_t o = (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2;
+                        mma_ss_lo(tm + S_COL, qd + o, k + o, IDESC, kk > 0);
+                    }
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        if (kk < p.rope_steps)
-                            mma_ss_lo(s_dst, qd + (DN / 64) * (Z::SLAB >> 4) + kk * 2, k + (DN / 64) * (Z::SLAB64 >> 4) + kk * 2, IDESC, 1);
-#pragma unroll
-                    for (int kk = 0; kk < DN / 16; ++kk)
-                        mma_ss_lo(p_dst, gd + (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2, v + (kk / 4) * (Z::SLAB64 >> 4) + (kk % 4) * 2, IDESC, kk > 0);
-                    mma_commit(&bar.s_full[it & 1]);
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint32_t o = (DN / 64) * (Z::SLAB >> 4) + kk * 2;
+                        if (kk < p.rope_steps) mma_ss_lo(tm + S_COL, qd + o, k + o, IDESC, 1);
+                    }
+                    mma_commit(&bar.s_full);
                 }
-                if (++st == STAGES) st = 0, phase ^= 1;
+                ok = warp_wait(&bar.v_full, it & 1, p.status, 124);
+                if (ok && it >= 1) ok = warp_wait(&bar.dp_free, (it - 1) & 1, p.status, 132);
+                if (!ok) break;
+                tc_fence_after();
+                if (lead) {
+#pragma unroll
+                    for (int kk = 0; kk < DN / 16; ++kk) {
+                        const uint32_t o = (kk / 4) * (Z::SLAB >> 4) + (kk % 4) * 2;
+                        mma_ss_lo(tm + DP_COL, gd + o, vd + o, IDESC, kk > 0);
+                    }
+                    mma_commit(&bar.dp_full);
+                    mma_commit(&bar.v_empty);
+                }
             }
         } else {
             const uint32_t idesc = idesc_f16(BT, 0, BF16, true) | (uint32_t)(DN + 16 * p.rope_steps) >> 3 << 17;
-            const uint32_t sd = desc_lo(smem_u32(smem + M::OFF_ST), Z::SLAB64);
+            const uint32_t kd = desc_lo(smem_u32(smem + M::OFF_K), Z::SLAB);
             for (int it = 0; it < n_it && ok; ++it) {
-                ok = warp_wait(&bar.ds_full[it & 1], (it >> 1) & 1, p.status, 126);
+                ok = warp_wait(&bar.ds_full, it & 1, p.status, 126);
                 if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
                 tc_fence_after();
-                const uint32_t k = (uint32_t)uniform((int)(sd + st * (Z::STAGE >> 4))), ds = tm + DS_COL + (it & 1) * 32;
+                const uint32_t k = (uint32_t)uniform((int)(kd + (it & 1) * (Z::KTILE >> 4)));
                 if (lead) {
 #pragma unroll
-                    for (int kk = 0; kk < SUB / 16; ++kk) mma_ts_lo(tm, ds + kk * 8, k + kk * 128, idesc, it > 0 || kk > 0);
-                    mma_commit(&bar.ds_free[it & 1]);
-                    mma_commit(&bar.st_empty[st]);
+                    for (int kk = 0; kk < BT / 16; ++kk) mma_ts_lo(tm, tm + DS_COL + kk * 8, k + kk * 128, idesc, it > 0 || kk > 0);
+                    mma_commit(&bar.ds_free);
+                    mma_commit(&bar.k_empty[it & 1]);
                     if (it + 1 == n_it) mma_commit(&bar.final_);
                 }
-                if (++st == STAGES) st = 0;
             }
         }
         if (!ok) *abort_flag = 1;
@@ -625,71 +637,75 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             if (lead) mma_commit(&bar.drain[warp - 1]);
             warp_wait(&bar.drain[warp - 1], 0, nullptr, 0);
         }
-    } else if (warp == 3) {
-        // ------------------------------------------------------------ rows of padded tokens become zeros
-        if (nit > 0 && padded(nit - 1)) {
-            const bool ok = warp_wait(&bar.fix, 0, p.status, 127);
-            if (ok) {
-                zero_rows(smem + M::OFF_ST + ((nit - 1) % STAGES) * Z::STAGE, 2 * Z::PANELS - 1, max(0, nS - (nit - 1) * SUB), lane);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.fixed);
-            } else {
-                *abort_flag = 1;
-            }
-        }
-    } else {
-        // ------------------------------------------------------------ dS: warpgroup wg takes the sub-tiles it % 2 == wg
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ dS: warpgroup wg has keys 64 wg .. of every tile
         const int wg = (warp - 4) >> 2, quad = warp & 3, r = quad * 32 + lane, row = row0 + r;
         const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
         const uint32_t s_tmem = tmem + lane_addr + S_COL + wg * SUB, p_tmem = tmem + lane_addr + DP_COL + wg * SUB;
-        const uint32_t ds_tmem = tmem + lane_addr + DS_COL + wg * 32;
+        const uint32_t ds_tmem = tmem + lane_addr + DS_COL + wg * (SUB / 2);
         const int64_t rr = ((int64_t)b * p.H + h) * p.Lpad + row;
         const float nl = row < p.Lpad ? p.nlse2[rr] : -INFINITY, nd = row < p.Lpad ? p.ndelta[rr] : 0.0f;
         const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), nl2 = f2_pack(nl, nl), nd2 = f2_pack(nd, nd);
         const int lim = p.causal ? min(nS - 1, row) : nS - 1;  // last key this row sees
         bool ok = true;
-        for (int it = wg; it < nit; it += 2) {
-            ok = warp_wait(&bar.s_full[wg], (it >> 1) & 1, p.status, 128);
+        for (int it = 0; it < nit; ++it) {
+            ok = warp_wait(&bar.s_full, it & 1, p.status, 128);
             if (!ok || __any_sync(~0u, *abort_flag)) { ok = false; break; }
             tc_fence_after();
-            const int kv0 = it * SUB;
+            const int kv0 = it * BT + wg * SUB;
             const bool mask = kv0 + SUB > nS || (p.causal && kv0 + SUB - 1 > row0);
-            uint32_t ra[64], rb[64];
+            uint32_t ra[SUB], rb[SUB];
             tmem_ld32(s_tmem, ra);
             tmem_ld32(s_tmem + 32, ra + 32);
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.s_free);
+#pragma unroll
+            for (int k = 0; k < SUB; k += 2) {
+                float a0, a1;
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(ra[k]), __uint_as_float(ra[k + 1])), sc2, nl2), a0, a1);
+                ra[k] = __float_as_uint(ex2(a0));
+                ra[k + 1] = __float_as_uint(ex2(a1));
+            }
+            ok = warp_wait(&bar.dp_full, it & 1, p.status, 133);
+            if (!ok) break;
+            tc_fence_after();
             tmem_ld32(p_tmem, rb);
             tmem_ld32(p_tmem + 32, rb + 32);
             tmem_ld_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.s_free[wg]);
-            if (it >= 2) ok = warp_wait(&bar.ds_free[wg], ((it >> 1) - 1) & 1, p.status, 130);  // dQ has read the dS before
+            if (lane == 0) mbar_arrive(&bar.dp_free);
+            uint32_t ds[SUB / 2];
+#pragma unroll
+            for (int k = 0; k < SUB; k += 2) {
+                float d0, d1;
+                f2_unpack(f2_mul(f2_pack(__uint_as_float(ra[k]), __uint_as_float(ra[k + 1])),
+                                 f2_add(f2_pack(__uint_as_float(rb[k]), __uint_as_float(rb[k + 1])), nd2)), d0, d1);
+                if (mask) {  // (whatever the product with a padded key's values gave)
+                    if (kv0 + k > lim) d0 = 0.0f;
+                    if (kv0 + k + 1 > lim) d1 = 0.0f;
+                }
+                ds[k / 2] = pack2<BF16>(d0, d1);
+            }
+            if (it >= 1) ok = warp_wait(&bar.ds_free, (it - 1) & 1, p.status, 130);  // dQ has read the tile's before
             if (!ok) break;
             tc_fence_after();
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t dk[16];
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const int k = 32 * c + i;
-                    float a0, a1, d0, d1;
-                    f2_unpack(f2_fma(f2_pack(__uint_as_float(ra[k]), __uint_as_float(ra[k + 1])), sc2, nl2), a0, a1);
-                    a0 = ex2(a0);
-                    a1 = ex2(a1);
-                    if (mask) {
-                        if (kv0 + k > lim) a0 = 0.0f;
-                        if (kv0 + k + 1 > lim) a1 = 0.0f;
-                    }
-                    f2_unpack(f2_mul(f2_pack(a0, a1), f2_add(f2_pack(__uint_as_float(rb[k]), __uint_as_float(rb[k + 1])), nd2)), d0, d1);
-                    dk[i / 2] = pack2<BF16>(d0, d1);
+            tmem_st16(ds_tmem, ds);
+            tmem_st16(ds_tmem + 16, ds + 16);
+            if (p.lens && (it + 1) * BT > nS) {  // key rows of padded tokens: 0 in dQ's product, whatever they hold
+                const int first = nS - it * BT, per = (BT - first) * 8;
+                for (int e = (int)threadIdx.x - 128; e < per * Z::PANELS; e += 256) {
+                    const int a = e / per;
+                    *(uint4*)(smem + M::OFF_K + (it & 1) * Z::KTILE + a * Z::SLAB + first * 128 + (e - a * per) * 16) = make_uint4(0, 0, 0, 0);
                 }
-                tmem_st16(ds_tmem + 16 * c, dk);
+                fence_proxy_async_smem();
             }
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar.ds_full[wg]);
+            if (lane == 0) mbar_arrive(&bar.ds_full);
         }
         if (nit > 0 && ok) ok = warp_wait(&bar.final_, 0, p.status, 129);
         if (!ok) *abort_flag = 1;
@@ -741,13 +757,12 @@ int launch(const LatentSdpaArgs& a, cudaStream_t st) {
         set_errorf("%s: too many tiles", ctx);
         return -1;
     }
-    // 128-row maps of what stays, 64-row maps of what streams
-    CUtensorMap q128, q64, g128, g64, k128, k64, r128, r64, v128, v64;
+    // 128-row maps, and of what streams by the dK/dV kernel 64-row ones
+    CUtensorMap q128, q64, g128, g64, k128, r128, v128;
     if (!make_tma_map_4d(&q128, a.q, DN + a.Dr, BF16, BT) || !make_tma_map_4d(&q64, a.q, DN + a.Dr, BF16, SUB) ||
         !make_tma_map_4d(&g128, a.g, DN, BF16, BT) || !make_tma_map_4d(&g64, a.g, DN, BF16, SUB) ||
-        !make_tma_map_4d(&k128, a.k, DN, BF16, BT) || !make_tma_map_4d(&k64, a.k, DN, BF16, SUB) ||
-        !make_tma_map_4d(&r128, a.k_rope, a.Dr, BF16, BT) || !make_tma_map_4d(&r64, a.k_rope, a.Dr, BF16, SUB) ||
-        !make_tma_map_4d(&v128, a.v, DN, BF16, BT) || !make_tma_map_4d(&v64, a.v, DN, BF16, SUB))
+        !make_tma_map_4d(&k128, a.k, DN, BF16, BT) || !make_tma_map_4d(&r128, a.k_rope, a.Dr, BF16, BT) ||
+        !make_tma_map_4d(&v128, a.v, DN, BF16, BT))
         return -1;
     Params p{};
     p.L = a.L;
@@ -780,7 +795,7 @@ int launch(const LatentSdpaArgs& a, cudaStream_t st) {
     constexpr int ROWS = 8 * (32 / (DN / 8)) * 2;  // rows a block of the first kernel
     latent_bwd_pre_kernel<DN, BF16><<<(unsigned)((n_row + ROWS - 1) / ROWS), 256, 0, st>>>(p);
     kv<<<(unsigned)ctas_kv, NTHREADS, KvSmem<DN>::ALLOC, st>>>(q64, g64, k128, r128, v128, p);
-    kq<<<(unsigned)ctas_q, NTHREADS, QSmem<DN>::ALLOC, st>>>(q128, g128, k64, r64, v64, p);
+    kq<<<(unsigned)ctas_q, NTHREADS, QSmem<DN>::ALLOC, st>>>(q128, g128, k128, r128, v128, p);
     latent_bwd_rope_kernel<BF16><<<(unsigned)std::min<int64_t>(4096, (a.B * a.S * (a.Dr / 4) + 255) / 256), 256, 0, st>>>(p);
     const int rc = cuda_failed(cudaGetLastError(), "latent_sdpa_bwd launch") ? -1 : 0;
     cudaFreeAsync(ws, st);
