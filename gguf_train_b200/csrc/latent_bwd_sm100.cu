@@ -22,7 +22,7 @@
 // weights, the gradients) is about three times what the tensor core does on it. The dQ kernel has two key tiles and one
 // value tile, which is free again as soon as dP is formed. Every mbarrier wait is bounded.
 //
-// Measured, 2 x 4096 tokens, 16 heads of 128 + 64, causal, bf16: dK/dV 398 us, dQ FIG_Q us (292 over 64 keys at a time).
+// Measured, 2 x 4096 tokens, 16 heads of 128 + 64, causal, bf16: dK/dV 398 us, dQ 281 us (292 over 64 keys at a time).
 
 #include <algorithm>
 #include <atomic>
