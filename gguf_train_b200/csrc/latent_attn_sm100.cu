@@ -95,9 +95,9 @@ struct Params {
     int4* joins;               // of each item, or where there are more of them than CTAs, of the item a CTA begins last: item (-1: one
                                // CTA did it all), first CTA, last CTA, tokens of its sequence that attend
     int by_item;
-    int64_t* line;             // [0] places in all, [1] CTAs in use, [2] prefix items
+    int* n_used;               // CTAs that have a share
     int own_rows, own_pitch;   // rows of an own item; the same to a multiple of 16: those of a slot of it
-    int join_dims;             // warps of a join block along the dims
+    int join_dims, join_groups;  // warps of a join block along the dims and along the parts
     int64_t own_base;          // first float of own slots in part_o (split prefix)
     int* status;
 };
@@ -302,11 +302,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 if (n_items <= NTHREADS) line = before;
                 if (k0 == 0) {
                     n_cta = (int)min((int64_t)gridDim.x, line);
-                    if (cta == 0 && threadIdx.x == 0) {
-                        p.line[0] = line;
-                        p.line[1] = n_cta;
-                        p.line[2] = np;
-                    }
+                    if (cta == 0 && threadIdx.x == 0) *p.n_used = n_cta;
                     begin = share(line, n_cta, min(cta, n_cta - 1));
                     end = share(line, n_cta, min(cta, n_cta - 1) + 1);
                 }
@@ -764,132 +760,165 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     }
 }
 
-// Rows whose item more than one CTA worked on. A block has 4 rows (a vector of the parts' layout): a warp 32 dims, one a lane, with four
-// parts' loads in flight. Its 8 warps share `join_dims` pieces of 32 dims and take the parts in turn: all along the dims
-// where items have few parts, all along the parts where a few sequences were cut into many. What it costs is latency: two
-// dependent loads (which parts, then the parts), and no more registers than let all of a step's blocks run at once.
+// Rows whose item more than one CTA worked on. A block has 4 rows (a vector of the parts' layout). A warp has 32 E dims, E a lane;
+// join_dims warps lie along the dims, join_groups of them take the parts in turn. E = 4 where that gives enough blocks, E = 1 and all
+// warps along the parts where a few sequences were cut into many.
+// What it costs is latency: of two dependent loads (which parts, then the parts), and of fetching its instructions, which
+// each SM runs about once. So what does not depend on the first kernel comes before the wait for it, loops that mostly run once are not
+// unrolled, and rows that begin within a vector have a loop of their own (32 sequences of 100 to 8192 rows, drafts of 5 tokens of 20
+// heads: issuing the first loads 0.4 instead of 2.7 us, the call 39.8 instead of 44.6).
 constexpr int JOIN_WARPS = 8, JOIN_ROWS = 4, JOIN_FLIGHT = 4;
 constexpr int MAX_CTAS = 511;  // parts of a row: one a CTA, and one more behind a split prefix
 
-template <typename T>
-__global__ void __launch_bounds__(JOIN_WARPS * 32, 4) latent_join_kernel(const __grid_constant__ Params p) {
-    __shared__ float4 sum[JOIN_WARPS][32];
+template <typename T, int E>
+__global__ void __launch_bounds__(JOIN_WARPS * 32, E == 1 ? 4 : 2) latent_join_kernel(const __grid_constant__ Params p) {
+    __shared__ float4 sum[JOIN_WARPS][E][32];
     __shared__ float2 sh_ml[(MAX_CTAS + 1) * JOIN_ROWS];
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the first kernel ends
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col0 = (int)blockIdx.y * JOIN_ROWS;
+    const int np = p.bb ? prefix_items(p, prefix_rows(p)) : 0, rows = min(JOIN_ROWS, p.own_rows - col0);
+    const int groups = p.join_groups, group = warp / p.join_dims;
+    const int d = ((int)blockIdx.z * p.join_dims + warp % p.join_dims) * 32 * E + lane;  // and every 32nd behind it, E of them
+    int orow = -1, token = 0;  // lanes 0 .. 3: the rows' places in the output
+    auto place = [&](int k) {
+        if (lane >= rows) return;
+        int b, h;
+        if (row_of(p, item_at(p, k, np), col0 + lane, b, token, h)) orow = (b * p.H + h) * p.Lq + token;
+    };
+    if (p.by_item) place(np + (int)blockIdx.x);
+    const int pre_item = p.bb ? (int)blockIdx.x / p.bb : 0, pre_row = ((int)blockIdx.x - pre_item * p.bb) * p.own_rows + col0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the first kernel ends
     // parts: CTAs c0 .. c0 + n - 1 of item k, its rows from `row` on; with a split prefix those of the prefix's item come first
-    const int n_cta = (int)p.line[1], np = (int)p.line[2];
     int k[2], c0[2], n[2] = {0, 0}, row[2], cnt;
     if (!p.bb) {
         const int4 j = p.joins[blockIdx.x];
-        if ((!p.by_item && (int)blockIdx.x >= n_cta) || j.x < 0) return;
+        if (!p.by_item && (int)blockIdx.x >= *p.n_used) return;
+        if (j.x < 0) return;
+        if (!p.by_item) place(j.x);
         k[0] = j.x, c0[0] = j.y, n[0] = j.z - j.y + 1, row[0] = col0, cnt = j.w;
         k[1] = c0[1] = row[1] = 0;
     } else {
-        const int b = (int)blockIdx.x;
-        const int4 own = p.joins[np + b], pre = np > 0 ? p.joins[b / p.bb] : make_int4(-1, 0, 0, 0);
-        k[0] = pre.x, c0[0] = pre.y, n[0] = pre.x < 0 ? 0 : pre.z - pre.y + 1, row[0] = (b % p.bb) * p.own_rows + col0;
+        const int4 own = p.joins[np + (int)blockIdx.x], pre = np > 0 ? p.joins[pre_item] : make_int4(-1, 0, 0, 0);
+        k[0] = pre.x, c0[0] = pre.y, n[0] = pre.x < 0 ? 0 : pre.z - pre.y + 1, row[0] = pre_row;
         k[1] = own.x, c0[1] = own.y, n[1] = own.x < 0 ? 0 : own.z - own.y + 1, row[1] = col0;
         cnt = own.w;
     }
-    const int parts = n[0] + n[1], rows = min(JOIN_ROWS, p.own_rows - col0);
-    const int groups = JOIN_WARPS / p.join_dims, group = warp / p.join_dims;
-    const int d = ((int)blockIdx.z * p.join_dims + warp % p.join_dims) * 32 + lane;
+    const int parts = n[0] + n[1];
     // where a source's first part is, and the step from CTA to CTA (one address a part: with all of it formed each time, instructions
     // were what this kernel waited for)
     const float* o0[2];
     const float2* ml0[2];
-    int64_t o_step[2];
+    int o_step[2];
     const int ml_step = (p.bb ? 1 : 2) * NR;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         int64_t so, sml;
         slot_of(p, k[s], np, c0[s], false, so, sml);
         const int pitch = k[s] < np ? NR : p.own_pitch;
-        o0[s] = p.part_o + so + ((int64_t)(row[s] >> 2) * p.R + d) * 4;
+        o0[s] = p.part_o + so + ((row[s] >> 2) * p.R + d) * 4;
         ml0[s] = p.part_ml + sml + row[s];
-        o_step[s] = (int64_t)(p.bb ? 1 : 2) * pitch * p.R;
+        o_step[s] = (p.bb ? 1 : 2) * pitch * p.R;
     }
-    auto load = [&](int q0, float4* y) {  // this lane's dim of parts q0, q0 + groups, ..
+    auto load = [&](int q0, float4 (*y)[E]) {  // this lane's dims of parts q0, q0 + groups, ..
 #pragma unroll
         for (int e = 0; e < JOIN_FLIGHT; ++e) {
-            const int q = q0 + groups * e, s = q >= n[0], i = q - (s ? n[0] : 0);
-            y[e] = make_float4(0, 0, 0, 0);
-            if (q >= parts || d >= p.R) continue;
+            const int q = q0 + groups * e, s = q >= n[0], i = q - (s ? n[0] : 0), step = s ? o_step[1] : o_step[0];
             // (without a split prefix, the CTA that begins the item has it in its second slot)
-            const int64_t step = s ? o_step[1] : o_step[0];
             const float* o = (s ? o0[1] : o0[0]) + i * step + (i == 0 && !p.bb ? step / 2 : 0);
-            const int r0 = (s ? row[1] : row[0]) & 3;
-            if (r0 == 0) {
-                y[e] = *(const float4*)o;
-            } else {
-                auto at = [&](int r) { return r < rows ? o[(int64_t)((r0 + r) >> 2) * p.R * 4 + ((r0 + r) & 3)] : 0.0f; };
-                y[e] = make_float4(at(0), at(1), at(2), at(3));
+            if (q < parts) {
+#pragma unroll
+                for (int c = 0; c < E; ++c)
+                    if (d + 32 * c < p.R) y[e][c] = *(const float4*)(o + 128 * c);
             }
         }
     };
-    float4 y[JOIN_FLIGHT], next[JOIN_FLIGHT];
-    load(group, y);  // (out before the offsets and sums are asked for)
-    for (int e = threadIdx.x; e < parts * JOIN_ROWS; e += JOIN_WARPS * 32) {
+    // a prefix item's rows of a sequence may begin within a vector: `skew` rows into it
+    const int skew = row[0] & 3, first = (skew ? n[0] : 0) + group;
+    float4 y[JOIN_FLIGHT][E];
+    load(first, y);  // (out before the offsets and sums are asked for)
+#pragma unroll 1
+    for (int e = threadIdx.x; e < parts * JOIN_ROWS; e += blockDim.x) {
         const int q = e / JOIN_ROWS, r = e % JOIN_ROWS, s = q >= n[0], i = q - (s ? n[0] : 0);
-        sh_ml[e] = r < rows ? (s ? ml0[1] : ml0[0])[(int64_t)i * ml_step + (i == 0 && !p.bb ? NR : 0) + r] : make_float2(-INFINITY, 0.0f);
+        sh_ml[e] = r < rows ? (s ? ml0[1] : ml0[0])[i * ml_step + (i == 0 && !p.bb ? NR : 0) + r] : make_float2(-INFINITY, 0.0f);
     }
     __syncthreads();
     // the rows' largest offset and the sum in its terms: a row a lane & 3, 8 parts at a time
     float m = -INFINITY, l = 0.0f;
+#pragma unroll 1
     for (int e = lane; e < parts * JOIN_ROWS; e += 32) m = fmaxf(m, sh_ml[e].x);
     for (int x = 4; x < 32; x <<= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
     auto factor = [&](float2 v) { return v.y == 0.0f ? 0.0f : ex2(v.x - m); };  // (a part without a weight holds nothing)
+#pragma unroll 1
     for (int e = lane; e < parts * JOIN_ROWS; e += 32) l += sh_ml[e].y * factor(sh_ml[e]);
     for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(~0u, l, x);
-    float acc[JOIN_ROWS] = {};
-    for (int q0 = group; q0 < parts; q0 += groups * JOIN_FLIGHT) {
-        const bool more = q0 + groups * JOIN_FLIGHT < parts;
-        if (more) load(q0 + groups * JOIN_FLIGHT, next);
+    float acc[E][JOIN_ROWS] = {};
+    if (skew) {
+#pragma unroll 1
+        for (int q = group; q < n[0]; q += groups) {
+            const float f = factor(sh_ml[q * JOIN_ROWS + (lane & 3)]);
+            const float* o = o0[0] + q * o_step[0];
+#pragma unroll 1
+            for (int r = 0; r < rows; ++r) {
+                const float fr = __shfl_sync(~0u, f, r);
+                const float* x = o + ((skew + r) >> 2) * p.R * 4 + ((skew + r) & 3);
+                if (fr == 0.0f) continue;
+#pragma unroll
+                for (int c = 0; c < E; ++c) {
+                    const float v = d + 32 * c < p.R ? x[128 * c] * fr : 0.0f;
+                    acc[c][0] += r == 0 ? v : 0.0f, acc[c][1] += r == 1 ? v : 0.0f, acc[c][2] += r == 2 ? v : 0.0f, acc[c][3] += r == 3 ? v : 0.0f;
+                }
+            }
+        }
+    }
+#pragma unroll 1
+    for (int q0 = first; q0 < parts; q0 += groups * JOIN_FLIGHT) {
         // factor of part q0 + groups * e and row r in lane 4 e + r
         const int q = q0 + groups * (lane >> 2);
         const float f = lane < 4 * JOIN_FLIGHT && q < parts ? factor(sh_ml[q * JOIN_ROWS + (lane & 3)]) : 0.0f;
 #pragma unroll
         for (int e = 0; e < JOIN_FLIGHT; ++e) {
-            const float x[JOIN_ROWS] = {y[e].x, y[e].y, y[e].z, y[e].w};
 #pragma unroll
             for (int r = 0; r < JOIN_ROWS; ++r) {
                 const float fr = __shfl_sync(~0u, f, 4 * e + r);
-                if (fr != 0.0f) acc[r] = fmaf(x[r], fr, acc[r]);
+                if (fr != 0.0f) {
+#pragma unroll
+                    for (int c = 0; c < E; ++c) acc[c][r] = fmaf(r == 0 ? y[e][c].x : r == 1 ? y[e][c].y : r == 2 ? y[e][c].z : y[e][c].w, fr, acc[c][r]);
+                }
             }
-            if (more) y[e] = next[e];
         }
+        load(q0 + groups * JOIN_FLIGHT, y);
     }
     if (groups > 1) {
-        sum[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+#pragma unroll
+        for (int c = 0; c < E; ++c) sum[warp][c][lane] = make_float4(acc[c][0], acc[c][1], acc[c][2], acc[c][3]);
         __syncthreads();
         if (group > 0) return;
+#pragma unroll 1
         for (int g = 1; g < groups; ++g) {
-            const float4 z = sum[g * p.join_dims + warp][lane];
-            acc[0] += z.x;
-            acc[1] += z.y;
-            acc[2] += z.z;
-            acc[3] += z.w;
+#pragma unroll
+            for (int c = 0; c < E; ++c) {
+                const float4 z = sum[g * p.join_dims + warp][c][lane];
+                acc[c][0] += z.x;
+                acc[c][1] += z.y;
+                acc[c][2] += z.z;
+                acc[c][3] += z.w;
+            }
         }
     }
-    // lanes 0 .. 3: the rows' places in the output, and what their sums are multiplied by (0: nothing attended)
-    int orow = -1;
+    // what the rows' sums are multiplied by (0: nothing attended)
     float inv = 0.0f;
-    if (lane < rows) {
-        const Item it = item_at(p, p.bb ? np + (int)blockIdx.x : k[0], np);
-        int b, i, h;
-        if (row_of(p, it, col0 + lane, b, i, h)) {
-            orow = (b * p.H + h) * p.Lq + i;
-            const bool none = i >= cnt || l == 0.0f;
-            if (!none) inv = 1.0f / l;
-            if (p.lse && blockIdx.z == 0 && warp == 0) p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-        }
+    if (orow >= 0) {
+        const bool none = token >= cnt || l == 0.0f;
+        if (!none) inv = 1.0f / l;
+        if (p.lse && blockIdx.z == 0 && warp == 0) p.lse[orow] = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
     }
 #pragma unroll
     for (int r = 0; r < JOIN_ROWS; ++r) {
         const int to = __shfl_sync(~0u, orow, r);
         const float f = __shfl_sync(~0u, inv, r);
-        if (to >= 0 && d < p.R) Elem<T>::store((T*)p.o + (int64_t)to * p.R + d, f == 0.0f ? 0.0f : acc[r] * f);
+        T* o = (T*)p.o + (int64_t)to * p.R + d;
+#pragma unroll
+        for (int c = 0; c < E; ++c)
+            if (to >= 0 && d + 32 * c < p.R) Elem<T>::store(o + 32 * c, f == 0.0f ? 0.0f : acc[c][r] * f);
     }
 }
 
@@ -1005,7 +1034,7 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     const int64_t at_joins = 256, at_ml = at_joins + up((p.by_item ? items : grid) * 16), at_o = at_ml + up(n_ml * 8);
     char* ws = nullptr;
     if (cuda_failed(cudaMallocAsync((void**)&ws, at_o + up(n_o * 4), st), "latent_attention: workspace")) return -1;
-    p.line = (int64_t*)ws;
+    p.n_used = (int*)ws;
     p.joins = (int4*)(ws + at_joins);
     p.part_ml = (float2*)(ws + at_ml);
     p.part_o = (float*)(ws + at_o);
@@ -1024,16 +1053,25 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     }
     if (!rc && (p.bb || grid > 1)) {
         cudaLaunchConfig_t cfg{};
-        p.join_dims = p.bb ? 4 : items * 4 >= grid ? 8 : 1;
-        cfg.gridDim = dim3(p.bb ? p.B : (unsigned)std::min<int64_t>(items, grid), (own_rows + JOIN_ROWS - 1) / JOIN_ROWS, (p.R / 32 + p.join_dims - 1) / p.join_dims);
-        cfg.blockDim = dim3(JOIN_WARPS * 32);
+        // 128 dims a warp (fewer instructions) where half the SMs get a block with that, else 32 (64 sequences behind a prefix: 83 us the
+        // call with 128, 106 with 32; one sequence of 32768 in 16 rows gets 4 blocks with 128, and takes 24 us with 64 blocks of 32).
+        // Along the parts as many warps as leave each JOIN_FLIGHT of them, one step's loads (2 a warp: 41.2 us instead of 39.8 for
+        // 32 sequences of 100 to 8192 rows, drafts of 5 tokens of 20 heads).
+        const int64_t join_items = p.bb ? p.B : std::min<int64_t>(items, grid), row_blocks = (own_rows + JOIN_ROWS - 1) / JOIN_ROWS;
+        const bool wide = join_items * row_blocks * 2 >= n_sm;
+        const int dims = wide ? 128 : 32, expected = (int)(grid / (p.bb ? p.n_pre : join_items)) + 2;
+        p.join_dims = wide ? (p.R + dims - 1) / dims : 1;
+        p.join_groups = 1;
+        while (2 * p.join_dims * p.join_groups <= JOIN_WARPS && (!wide || p.join_groups * JOIN_FLIGHT < expected)) p.join_groups *= 2;
+        cfg.gridDim = dim3((unsigned)join_items, (unsigned)row_blocks, (p.R + dims * p.join_dims - 1) / (dims * p.join_dims));
+        cfg.blockDim = dim3(p.join_dims * p.join_groups * 32);
         cfg.stream = st;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         at[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = at;
         cfg.numAttrs = 1;
-        if (cuda_failed(cudaLaunchKernelEx(&cfg, latent_join_kernel<T>, p), "latent_attention join launch")) rc = -1;
+        if (cuda_failed(cudaLaunchKernelEx(&cfg, wide ? latent_join_kernel<T, 4> : latent_join_kernel<T, 1>, p), "latent_attention join launch")) rc = -1;
     }
     cudaFreeAsync(ws, st);
     return rc;

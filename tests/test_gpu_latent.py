@@ -113,6 +113,26 @@ def test_attention(case, dtype, ragged):
     assert torch.equal(again, out)  # the same bits on every run
 
 
+@pytest.mark.parametrize("B,H,Lq,R,cap,P", [
+    (3, 5, 1, 192, 40, 300), (5, 3, 2, 512, 70, 5000), (60, 6, 1, 256, 70, 700), (90, 1, 3, 128, 130, 129), (41, 9, 3, 448, 65, 64),
+    (200, 2, 1, 64, 200, 0), (300, 7, 1, 320, 90, 65)])
+def test_rows_that_are_no_multiple_of_four(B, H, Lq, R, cap, P):
+    """Several sequences' rows in an item over the prefix, where a sequence's do not begin at a multiple of four rows; more items than
+    multiprocessors."""
+    from gguf_train_b200 import _C, latent_attention
+
+    gen = torch.Generator(device="cuda").manual_seed(B + H)
+    lens = [(37 * b) % (cap + 1) for b in range(B)]
+    cache = _cache(B, cap, R, 32, lens, torch.bfloat16, gen)
+    prefix = _cache(1, P + 5, R, 32, [P], torch.bfloat16, gen) if P else None
+    q = torch.randn((B, H, Lq, R + 32), device="cuda", generator=gen).to(torch.bfloat16)
+    counts = torch.randint(0, Lq + 1, (B,), device="cuda", generator=gen).to(torch.int32)
+    for c in (None, counts):
+        out, lse = latent_attention(q, cache, 0.1, counts=c, prefix=prefix, need_lse=True)
+        assert _C.device_status() == 0
+        _check(q, cache, 0.1, c, prefix, out, lse)
+
+
 @pytest.mark.parametrize("mode", [None, 0, 2])
 @pytest.mark.parametrize("dtype,source", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f16", "bf16")])
 @pytest.mark.parametrize("B,n,R,Dr,cap,lens,far", [
