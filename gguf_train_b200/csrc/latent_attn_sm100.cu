@@ -14,6 +14,9 @@
 // 16x256b shape (a thread has two keys of up to four column pairs), warps 4-7 the first half of the columns, 8-11 the second.
 // The offset of a query row is raised only when a score exceeds it by more than 2^8, so most tiles need no maximum:
 // one vote over the block (a barrier with a reduction) finds that no row grew. Sums stay with each thread until a segment's end.
+// What a tile seldom does (raising offsets) and what a segment does once (the output) are loops that are not unrolled: in the way of the
+// others, unrolled, their instructions cost fetches and registers (64 sequences of 1k to 32k 207 us with them unrolled, 202 without;
+// drafts 40.5 / 35.0; chunks 1105 / 1079).
 // Two warps issue so that neither kind of product waits behind one of the other kind that cannot start yet. A tile's panels are loaded
 // and freed in two groups, as the second product goes through them.
 //
@@ -597,7 +600,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         soft_sync();
                         tc_fence_after();
                         for (int mt = half; mt < m_tiles; mt += 2) {
-#pragma unroll
+#pragma unroll 1
                             for (int j = 0; j < GL; ++j) {
                                 uint32_t v[16];
                                 tmem_ldx<16>(tmem + lane_addr + O_COL + mt * NR + 16 * j, v);
@@ -698,9 +701,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             tc_fence_after();
             for (int mt = half; mt < m_tiles; mt += 2) {
                 const int d = mt * 128 + quad * 32 + lane;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (j >= gl) continue;
+#pragma unroll 1
+                for (int j = 0; j < gl; ++j) {
                     uint32_t v[16];
                     tmem_ldx<16>(tmem + lane_addr + O_COL + mt * NR + 16 * j, v);
                     tmem_ld_wait();
