@@ -362,7 +362,7 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             float* lse = p.lse ? p.lse + ((int64_t)it.b * p.H + it.h) * p.L + row : nullptr;
             if (nb == 0) {  // nothing to attend
                 if (row < p.L) {
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < DN / 8; ++c) *(uint4*)(orow + c * 8) = make_uint4(0, 0, 0, 0);
                     if (lse) *lse = -INFINITY;
                 }
@@ -417,7 +417,7 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
                 if (__any_sync(~0u, grew && j > 0)) {
                     // PV_t(j-1) is complete: it was issued before S_t(j), whose completion has been seen
                     const float alpha = grew ? ex2((m_start - m_used) * p.scale_log2) : 1.0f;
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < DN / 32; ++c) {
                         uint32_t ov[32];
                         tmem_ld32(o_tmem + c * 32, ov);
@@ -443,7 +443,7 @@ latent_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             tc_fence_after();
             const bool none = row >= it.nL || lsum == 0.0f;
             const float inv = none ? 0.0f : 1.0f / lsum;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < DN / 32; ++c) {
                 uint32_t ov[32], w[16];
                 tmem_ld32(o_tmem + c * 32, ov);
