@@ -22,7 +22,9 @@
 // weights, the gradients) is about three times what the tensor core does on it. The dQ kernel has two key tiles and one
 // value tile, which is free again as soon as dP is formed. Every mbarrier wait is bounded.
 //
-// Measured, 2 x 4096 tokens, 16 heads of 128 + 64, causal, bf16: dK/dV 398 us, dQ 281 us (292 over 64 keys at a time).
+// Both kinds of CTA are one launch.
+//
+// Measured apart, 2 x 4096 tokens, 16 heads of 128 + 64, causal, bf16: dK/dV 398 us, dQ 281 us (292 over 64 keys at a time).
 
 #include <algorithm>
 #include <atomic>
@@ -53,6 +55,7 @@ struct Rows {
 struct Params {
     int64_t L, S, Lpad;      // Lpad: L to a multiple of 64
     int B, H, Hkv, group, Dr, rope_steps;
+    int ctas_kv;             // CTAs of dK/dV, before those of dQ
     float scale, scale_log2;
     int causal;
     const int32_t* lens;
@@ -129,8 +132,8 @@ __global__ void __launch_bounds__(256) latent_bwd_rope_kernel(const __grid_const
 // ------------------------------------------------------------------ shared by both kernels
 
 // tile and (batch, head) unit of this CTA: superblocks of SB_UNITS units, their tiles outer, the units inner
-__device__ __forceinline__ void place(int tiles, int units, int& tile, int& unit) {
-    const int lin = (int)blockIdx.x, per = SB_UNITS * tiles, sb = lin / per, r = lin - sb * per;
+__device__ __forceinline__ void place(int lin, int tiles, int units, int& tile, int& unit) {
+    const int per = SB_UNITS * tiles, sb = lin / per, r = lin - sb * per;
     const int size = min(SB_UNITS, units - sb * SB_UNITS);
     tile = r / size;
     unit = sb * SB_UNITS + r - tile * size;
@@ -188,10 +191,8 @@ struct KvBars {
 static_assert(sizeof(KvBars) <= 256, "barrier block");
 
 template <int DN, bool BF16>
-__global__ void __launch_bounds__(NTHREADS, 1)
-latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
-                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmR,
-                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
+__device__ __forceinline__ void kv_cta(const CUtensorMap& tmQ, const CUtensorMap& tmG, const CUtensorMap& tmK, const CUtensorMap& tmR,
+                                       const CUtensorMap& tmV, const Params& p, int lin) {
     using Z = Sizes<DN>;
     using M = KvSmem<DN>;
     constexpr uint32_t DK_COL = DN, S_COL = 320, S_STEP = 128, DP_COL = 384;  // S^T of sub-tile h at S_COL + 128 h, then W^T
@@ -200,7 +201,7 @@ latent_bwd_kv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     KvBars& bar = *(KvBars*)(smem + M::OFF_BAR);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int jt, unit;
-    place((int)((p.S + BT - 1) / BT), p.B * p.Hkv, jt, unit);
+    place(lin, (int)((p.S + BT - 1) / BT), p.B * p.Hkv, jt, unit);
     const int b = unit / p.Hkv, hk = unit - b * p.Hkv, key0 = jt * BT;
     const int nL = latent_tokens(p.lens, b, p.L), nS = latent_tokens(p.lens, b, p.S);
     const int i0 = p.causal ? key0 / SUB : 0;  // first sub-tile with a query that sees this key tile
@@ -491,10 +492,8 @@ struct QBars {
 static_assert(sizeof(QBars) <= 256, "barrier block");
 
 template <int DN, bool BF16>
-__global__ void __launch_bounds__(NTHREADS, 1)
-latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG,
-                    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmR,
-                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Params p) {
+__device__ __forceinline__ void q_cta(const CUtensorMap& tmQ, const CUtensorMap& tmG, const CUtensorMap& tmK, const CUtensorMap& tmR,
+                                      const CUtensorMap& tmV, const Params& p, int lin) {
     using Z = Sizes<DN>;
     using M = QSmem<DN>;
     constexpr uint32_t DS_COL = 192, S_COL = 256, DP_COL = 384;  // dQ from 0; dS as 16-bit pairs
@@ -504,7 +503,7 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int tile, unit;
     const int n_qt = (int)((p.L + BT - 1) / BT);
-    place(n_qt, p.B * p.H, tile, unit);
+    place(lin, n_qt, p.B * p.H, tile, unit);
     if (p.causal) tile = n_qt - 1 - tile;
     const int b = unit / p.H, h = unit - b * p.H, hk = h / p.group, row0 = tile * BT;
     const int nL = latent_tokens(p.lens, b, p.L), nS = latent_tokens(p.lens, b, p.S);
@@ -735,25 +734,34 @@ latent_bwd_q_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     }
 }
 
+// The CTAs of dK/dV first, those of dQ behind them: neither waits for the other, and the second kind fills the multiprocessors as the
+// first one's last CTAs end (2 x 4096, 16 heads: 831 -> 822 us with the forward; 3 x 511 to 1023, 12 heads of 64 + 32: 114 -> 104).
+template <int DN, bool BF16>
+__global__ void __launch_bounds__(NTHREADS, 1)
+latent_bwd_kernel(const __grid_constant__ CUtensorMap q64, const __grid_constant__ CUtensorMap g64, const __grid_constant__ CUtensorMap q128,
+                  const __grid_constant__ CUtensorMap g128, const __grid_constant__ CUtensorMap k128,
+                  const __grid_constant__ CUtensorMap r128, const __grid_constant__ CUtensorMap v128, const __grid_constant__ Params p) {
+    if ((int)blockIdx.x < p.ctas_kv) kv_cta<DN, BF16>(q64, g64, k128, r128, v128, p, (int)blockIdx.x);
+    else q_cta<DN, BF16>(q128, g128, k128, r128, v128, p, (int)blockIdx.x - p.ctas_kv);
+}
+
 Rows rows(const gtb_tensor4& t) { return Rows{(char*)t.data, t.stride[0], t.stride[1], t.stride[2]}; }
 
 template <int DN, bool BF16>
 int launch(const LatentSdpaArgs& a, cudaStream_t st) {
     const char* ctx = "latent_sdpa_bwd";
-    auto kv = latent_bwd_kv_kernel<DN, BF16>;
-    auto kq = latent_bwd_q_kernel<DN, BF16>;
+    auto kern = latent_bwd_kernel<DN, BF16>;
+    constexpr int SMEM = std::max(KvSmem<DN>::ALLOC, QSmem<DN>::ALLOC);
     int dev = 0;
     if (cuda_failed(cudaGetDevice(&dev), ctx)) return -1;
     static std::atomic<uint64_t> ready{0};  // devices (of the first 64) whose kernels are set up
     const uint64_t bit = dev < 64 ? 1ull << dev : 0;
     if (!(ready.load() & bit)) {
-        if (cuda_failed(cudaFuncSetAttribute(kv, cudaFuncAttributeMaxDynamicSharedMemorySize, KvSmem<DN>::ALLOC), ctx) ||
-            cuda_failed(cudaFuncSetAttribute(kq, cudaFuncAttributeMaxDynamicSharedMemorySize, QSmem<DN>::ALLOC), ctx))
-            return -1;
+        if (cuda_failed(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM), ctx)) return -1;
         ready.fetch_or(bit);
     }
     const int64_t ctas_kv = (a.S + BT - 1) / BT * a.B * a.Hkv, ctas_q = (a.L + BT - 1) / BT * a.B * a.H;
-    if (ctas_kv > INT32_MAX || ctas_q > INT32_MAX) {
+    if (ctas_kv + ctas_q > INT32_MAX) {
         set_errorf("%s: too many tiles", ctx);
         return -1;
     }
@@ -777,6 +785,7 @@ int launch(const LatentSdpaArgs& a, cudaStream_t st) {
     p.scale = a.scale;
     p.scale_log2 = a.scale * LOG2E;
     p.causal = a.causal;
+    p.ctas_kv = (int)ctas_kv;
     p.lens = a.lens;
     p.lse = a.lse;
     p.o = rows(a.o);
@@ -794,8 +803,7 @@ int launch(const LatentSdpaArgs& a, cudaStream_t st) {
     p.dkr_part = ws + 2 * n_row;
     constexpr int ROWS = 8 * (32 / (DN / 8)) * 2;  // rows a block of the first kernel
     latent_bwd_pre_kernel<DN, BF16><<<(unsigned)((n_row + ROWS - 1) / ROWS), 256, 0, st>>>(p);
-    kv<<<(unsigned)ctas_kv, NTHREADS, KvSmem<DN>::ALLOC, st>>>(q64, g64, k128, r128, v128, p);
-    kq<<<(unsigned)ctas_q, NTHREADS, QSmem<DN>::ALLOC, st>>>(q128, g128, k128, r128, v128, p);
+    kern<<<(unsigned)(ctas_kv + ctas_q), NTHREADS, SMEM, st>>>(q64, g64, q128, g128, k128, r128, v128, p);
     latent_bwd_rope_kernel<BF16><<<(unsigned)std::min<int64_t>(4096, (a.B * a.S * (a.Dr / 4) + 255) / 256), 256, 0, st>>>(p);
     const int rc = cuda_failed(cudaGetLastError(), "latent_sdpa_bwd launch") ? -1 : 0;
     cudaFreeAsync(ws, st);
