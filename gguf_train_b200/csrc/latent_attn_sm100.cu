@@ -567,7 +567,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 for (int j = 0; j < GL; ++j)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) grow = grow || fmaxf(e[j][c], e[j][c + 2]) > thr[j][c];
-                if (soft_any(grow)) {
+                if (__builtin_expect(soft_any(grow), 0)) {
                     // the rows' maxima over the tile: over the thread's two keys, the warp's 16, the four quadrants
                     scores();
 #pragma unroll
@@ -636,6 +636,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 }
                 if (valid < KT) {  // rows past the end: 0 in the second product, whatever they hold
                     const int first = max(valid, 0), per = (KT - first) * 8;
+#pragma unroll 1
                     for (int i = st; i < per * (p.R / 64); i += NSOFT) {
                         const int a = i / per, r = i - a * per, g = a >= GROUP && p.n_groups > 1;
                         unsigned char* base = (g ? sC1 : sC) + stage[g] * p.group_bytes[g];
@@ -651,6 +652,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 if (lane == 0) mbar_arrive(&bar.p_full);
             };
             auto tiles = [&](auto groups) {
+#pragma unroll 1
                 for (int t = off; t < off + n; ++t, ++u) tile(groups, t);
             };
             if (it.empty) {
