@@ -26,10 +26,10 @@
 // prefix, rows of several sequences make up an item of their own over the prefix (where a sequence alone fills
 // an item, the prefix's tiles simply come first in its own), and every row is joined.
 //
-// What bounds it: with one token a sequence HBM (64 sequences of 1k to 32k rows of 512 + 64, 16 heads: 207 us, 6.0 TB/s); with 64
+// What bounds it: with one token a sequence HBM (64 sequences of 1k to 32k rows of 512 + 64, 16 heads: 202 us, 6.2 TB/s); with 64
 // query rows an item the shared memory that feeds the products (a tile of 512 + 64: scores 36 x 33 cycles, outputs 16 x 50,
-// its load's writes 576; 509 tokens of 32 heads over 4k to 8k, 4 sequences: 1.13 ms, 740 TFLOP/s, 3200 cycles a tile); with
-// smaller rows the chain from scores to weights, about 2000 cycles a tile.
+// its load's writes 576; 509 tokens of 32 heads over 4k to 8k, 4 sequences: 1.08 ms, 770 TFLOP/s, 3050 cycles a tile); with
+// smaller rows the chain from scores to weights.
 //
 // Rows past a sequence's end are zeroed in shared memory before the second product (a weight of 0 would make NaN of
 // them). Every mbarrier wait is bounded; the softmax warps, which also meet at block barriers, go on without
@@ -99,6 +99,7 @@ struct Params {
                                // CTA did it all), first CTA, last CTA, tokens of its sequence that attend
     int by_item;
     int* n_used;               // CTAs that have a share
+    int lead;                  // places of an item before its tiles'
     int own_rows, own_pitch;   // rows of an own item; the same to a multiple of 16: those of a slot of it
     int join_dims, join_groups;  // warps of a join block along the dims and along the parts
     int64_t own_base;          // first float of own slots in part_o (split prefix)
@@ -107,10 +108,12 @@ struct Params {
 
 static_assert(3 * 9 * PANEL + PANEL + (int)sizeof(Extra) <= SMEM_MAX, "two stages of the largest rows");
 
-// What an item costs besides its tiles (its query rows' load, the first tile's way through the empty pipeline, its output), in tiles:
-// (32 sequences of 100 to 8192 rows, drafts of 5 tokens of 20 heads: 48 us; with 0 places 59, 1 56, 6 47; 64 sequences of 1k to 32k 213,
-// 215, 213, 217)
-constexpr int LEAD = 3;
+// What an item costs besides its tiles (its query rows' load, the first tile's way through the empty pipeline, its output), in tiles; a
+// tile of at most 256 values is about half of one of 512. (32 sequences of 100 to 8192 rows of 256, drafts of 5 tokens of 20 heads: 45.4
+// us with 0 places, 40.6 with 2, 34.9 with 3, 34.3 with 5, 34.7 with 8; 12 of 3 to 640 behind 4001, 22.5, 21.0, 20.2, 18.7, 19.1; rows
+// of 512, 64 sequences behind 16k: 78.3, 75.3, 76.8, with 4 78.0; chunks of 509 tokens 1101, 1088, 1083, 1083; one token of 64
+// sequences of 1k to 32k 203, 202, 202, 204.6.)
+constexpr int lead_of(int R) { return R <= 256 ? 5 : 3; }
 
 struct Item {
     int b, i0, h0;             // first sequence, token, head
@@ -170,7 +173,7 @@ __device__ __forceinline__ Item item_of(const Params& p, int k, int P, int np) {
     return it;
 }
 
-// The line: each item takes LEAD places and one for each of its tiles; CTA c of n works on the tiles whose places are in
+// The line: each item takes `lead` places and one for each of its tiles; CTA c of n works on the tiles whose places are in
 // [share(c), share(c + 1)).
 __device__ __forceinline__ int64_t share(int64_t line, int n, int c) { return line * c / n; }
 
@@ -286,7 +289,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     for (int pass = n_items > NTHREADS ? 0 : 1; pass < 2; ++pass) {
         for (int k0 = 0; k0 < n_items; k0 += NTHREADS) {
             const int k = k0 + (int)threadIdx.x;
-            const int64_t n = k < n_items ? item_of(p, k, P, np).nt + LEAD : 0;
+            const int64_t n = k < n_items ? item_of(p, k, P, np).nt + p.lead : 0;
             int64_t incl = n;
             for (int o = 1; o < 32; o <<= 1) {
                 const int64_t y = __shfl_up_sync(~0u, incl, o);
@@ -322,7 +325,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     // from here on places count from the first item's first tile: tiles [off_first, ..) of item k_first, and on to place `last`
     const int k_first = ex.first_item;
     const int64_t first_place = ex.first_place;
-    const int off_first = max((int)(begin - first_place) - LEAD, 0), last = (int)(end - first_place) - LEAD;
+    const int off_first = max((int)(begin - first_place) - p.lead, 0), last = (int)(end - first_place) - p.lead;
     const bool idle = cta >= n_cta;
 
     tc_fence_before();
@@ -338,7 +341,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const Item it = item_of(p, k, P, np);
             const int n = uni(min(it.nt, to) - off);
             if (n <= 0) break;
-            to -= uni(it.nt) + LEAD;
+            to -= uni(it.nt) + p.lead;
             if (!f(it, k, off, n)) break;
         }
     };
@@ -485,7 +488,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         // ------------------------------------------------------------ what the join kernel has to know
         if (lane == 0) {
             int4 mine = make_int4(-1, 0, 0, 0);
-            int64_t place = first_place + LEAD;  // of the item's first tile
+            int64_t place = first_place + p.lead;  // of the item's first tile
             for_segments(plain, [&](const Item& it, int k, int off, int) {
                 if (off == 0) {
                     const int to = cta_of(line, n_cta, place + it.nt - 1);
@@ -494,7 +497,7 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     if (p.by_item) p.joins[k] = j;
                     else if (parts) mine = j;
                 }
-                place += it.nt + LEAD;
+                place += it.nt + p.lead;
                 return true;
             });
             if (!p.by_item && !idle) p.joins[cta] = mine;
@@ -1002,6 +1005,7 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
         set_error("latent_attention: too many query rows");
         return -1;
     }
+    p.lead = lead_of(p.R);
     p.panels = p.R / 64 + 1;
     p.n_groups = p.panels > GROUP + 1 ? 2 : 1;
     p.group_bytes[0] = (p.n_groups > 1 ? GROUP : p.panels) * PANEL;
@@ -1017,7 +1021,7 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     p.slack = smem - used;
 
     const int64_t tiles_seq = (a.c.Smax + KT - 1) / KT + (p.prefix_lens ? (p.prefix_max + KT - 1) / KT : 0);
-    const int grid = (int)std::min<int64_t>(std::min(n_sm, MAX_CTAS), items * (std::max<int64_t>(tiles_seq, 1) + LEAD));
+    const int grid = (int)std::min<int64_t>(std::min(n_sm, MAX_CTAS), items * (std::max<int64_t>(tiles_seq, 1) + p.lead));
 
     CUtensorMap mq, mqp, mc, mcp;
     const int64_t D = p.R + p.Dr, qs[3] = {p.H, p.Lq, p.B}, qt[3] = {a.q.sh, a.q.ss, a.q.sb};
