@@ -1061,12 +1061,12 @@ int launch(const LatentAttnArgs& a, cudaStream_t st) {
     }
     if (!rc && (p.bb || grid > 1)) {
         cudaLaunchConfig_t cfg{};
-        // 128 dims a warp (fewer instructions) where half the SMs get a block with that, else 32 (64 sequences behind a prefix: 83 us the
-        // call with 128, 106 with 32; one sequence of 32768 in 16 rows gets 4 blocks with 128, and takes 24 us with 64 blocks of 32).
-        // Along the parts as many warps as leave each JOIN_FLIGHT of them, one step's loads (2 a warp: 41.2 us instead of 39.8 for
-        // 32 sequences of 100 to 8192 rows, drafts of 5 tokens of 20 heads).
+        // 128 dims a warp (fewer instructions) where a quarter of the SMs get a block with that, else 32 (calls of 1 token, 16 heads and
+        // 512 dims with 128 / 32 a warp, us: 64 sequences behind a prefix 83 / 106; without, 16 sequences, 64 blocks, 65.0 / 66.5;
+        // 8, 42.7 / 39.3; one 42.0 / 23.0). Along the parts as many warps as leave each JOIN_FLIGHT of them, one step's loads (2 a
+        // warp: 41.2 us instead of 39.8 for 32 sequences of 100 to 8192 rows, drafts of 5 tokens of 20 heads).
         const int64_t join_items = p.bb ? p.B : std::min<int64_t>(items, grid), row_blocks = (own_rows + JOIN_ROWS - 1) / JOIN_ROWS;
-        const bool wide = join_items * row_blocks * 2 >= n_sm;
+        const bool wide = join_items * row_blocks * 4 >= n_sm;
         const int dims = wide ? 128 : 32, expected = (int)(grid / (p.bb ? p.n_pre : join_items)) + 2;
         p.join_dims = wide ? (p.R + dims - 1) / dims : 1;
         p.join_groups = 1;
