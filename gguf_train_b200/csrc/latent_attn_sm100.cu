@@ -669,6 +669,8 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 tiles(std::integral_constant<int, 4>{});
             }
             // ---- the segment's rows: sums over the quadrants, then O^T a latent dim a lane
+            // (written over the last tile's maxima and factors: no vote of a next tile lies between, and a warp may still read them)
+            soft_sync();
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 if (j >= gl) continue;
