@@ -247,6 +247,10 @@ latent_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     unsigned char* smem = (unsigned char*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     if (smem - smem_raw > p.slack) {  // (the largest rows leave less than the alignment may take; it takes nothing)
         if (threadIdx.x == 0) atomicCAS(p.status, 0, 70);
+        // the second kernel goes by this table: nothing to join
+        const int n = p.by_item ? prefix_items(p, prefix_rows(p)) + p.B * p.n_rt : (int)gridDim.x;
+        for (int k = (int)(blockIdx.x * NTHREADS + threadIdx.x); k < n; k += (int)gridDim.x * NTHREADS) p.joins[k] = make_int4(-1, 0, 0, 0);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *p.n_used = 0;
         return;
     }
     unsigned char* sQ = smem;
