@@ -241,6 +241,7 @@ GTB_API int gtb_latent_sdpa_bwd(const gtb_tensor4* grad_out, const gtb_tensor4* 
         LatentSdpaArgs a{};
         bool empty = false;
         if (!check_sdpa(ctx, q, k, k_rope, v, seq_lens, scale, a, empty)) return -1;
+        if (empty && a.B * a.S > 0) return fail(ctx, "there must be heads, queries and keys"), -1;  // (dk, dk_rope and dv have values)
         if (empty) return 0;
         gtb_tensor4 like = *q;
         like.shape[3] = a.Dn;

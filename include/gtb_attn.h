@@ -370,6 +370,8 @@ GTB_API int gtb_latent_attention(const gtb_tensor4 *q, const gtb_latent *cache, 
  *   they hold; their out is 0, and all their gradients.
  *   lse: NULL or (B,H,L) f32, -inf where nothing is attended (out is 0 there). scale positive, below 1e38.
  * All tensors start on 16 bytes, with a unit innermost stride and others that are positive multiples of 8.
+ * Without sequences, without heads, or with neither queries nor keys nothing is done, but the backward refuses keys that there is no
+ * head for (their gradients have values); queries without keys, and keys without queries, are refused.
  * The backward takes the forward's out and lse and writes dq, dk, dk_rope (summed over all heads) and dv, in fixed order:
  * the same bits on every run. Its weights are 2^(score - log-sum-exp) of f32 numbers: off by about |score| 2^-22 of themselves
  * (scores in powers of 2). Its scratch (4 (2 B H L + B Hkv S Dr) bytes) comes from the stream-ordered allocator. */
