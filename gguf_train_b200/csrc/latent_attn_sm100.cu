@@ -112,7 +112,8 @@ static_assert(3 * 9 * PANEL + PANEL + (int)sizeof(Extra) <= SMEM_MAX, "two stage
 // tile of at most 256 values is about half of one of 512. (32 sequences of 100 to 8192 rows of 256, drafts of 5 tokens of 20 heads: 45.4
 // us with 0 places, 40.6 with 2, 34.9 with 3, 34.3 with 5, 34.7 with 8; 12 of 3 to 640 behind 4001, 22.5, 21.0, 20.2, 18.7, 19.1; rows
 // of 512, 64 sequences behind 16k: 78.3, 75.3, 76.8, with 4 78.0; chunks of 509 tokens 1101, 1088, 1083, 1083; one token of 64
-// sequences of 1k to 32k 203, 202, 202, 204.6.)
+// sequences of 1k to 32k 203, 202, 202, 204.6.) Between 3 and 5 little changes, and no size between 256 and 512 was measured: the
+// border could lie anywhere there.
 constexpr int lead_of(int R) { return R <= 256 ? 5 : 3; }
 
 struct Item {

@@ -10,8 +10,8 @@
 //   dQ      one CTA a 128-query tile, over 128 keys at a time:
 //             S = Q [K | K_r]^T, dP = G V^T            (M = 128 queries, N = 128 keys)
 //             dQ += dS [K | K_r]                       (N = dims, K = 128; dS from TMEM)
-// A fused dQ (five products instead of seven) needs f32 sums in global memory by unordered additions, and TMEM that dK's 192 columns
-// do not leave. Products of N = 64 with both operands in shared memory are bound by its bandwidth (49.5 cycles instead of 32):
+// A fused dQ (five products instead of seven) needs f32 sums over the key tiles in global memory, added without an order or waiting for
+// one another, and with Dn = 128 TMEM that dK's 192 columns do not leave (with Dn = 64 there would be room: not built). Products of N = 64 with both operands in shared memory are bound by its bandwidth (49.5 cycles instead of 32):
 // 64 is what TMEM holds of scores next to dV and dK (320 of 512 columns with Dn = 128). Beside dQ alone 128 fit.
 //
 // Warps: 0 TMA producer, 1 issues the score products (and owns TMEM), 2 the gradient products, 3 (dK/dV) zeroes rows of padded tokens

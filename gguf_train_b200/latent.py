@@ -11,6 +11,9 @@ With W_k (heads, Dn, R) and W_v (heads, Dv, R) the up-projections of a latent c,
 cached rows [c | k_rope] themselves, whose latents are the values too, and leaves W_v to the caller's next product: a
 decode step reads R + Dr values a cached token for all of its heads. Both give the same attention.
 
+Scores, their maxima and sums, and outputs accumulate in f32. With 16-bit inputs the softmax weights, and in latent_sdpa's backward the
+scores' gradients too, are rounded once to the inputs' type before the tensor cores multiply them.
+
 Tensors are torch CUDA tensors; every call runs in the native library on the caller's current stream
 (include/gtb_attn.h has the exact definitions). A cache is mutable state: calls that change it, and calls that
 read it, are ordered by the streams they are issued on. latent_append and latent_attention serve and have no gradient: they
@@ -120,8 +123,9 @@ def latent_append(cache: LatentCache, latent: torch.Tensor, k_rope: torch.Tensor
     sequence b (prompts padded to one length).
 
     With `rope` (a dict of mode, 0 or 2, freq_base and freq_scale) k_rope is first rotated for its position, lens[b] + i;
-    behind a `prefix` that the batch shares, prefix.lens[0] + lens[b] + i. The rotation is rope_axes' over all of
-    rope_dim. Rows past the capacity are dropped and leave status 62 (_C.device_status()). Returns cache."""
+    behind a `prefix` that the batch shares, prefix.lens[0] + lens[b] + i (that length as it is, even where the prefix's tensor
+    holds fewer rows). The rotation is rope_axes' over all of rope_dim. Tensors that require a gradient while gradients are
+    recorded are refused. Rows past the capacity are dropped and leave status 62 (_C.device_status()). Returns cache."""
     _require_cuda("latent_append", latent, k_rope, counts)
     _same_device("latent_append", cache, latent, k_rope, counts)
     _no_gradient("latent_append", latent, k_rope, cache._rows)
@@ -182,8 +186,11 @@ def latent_attention(q: torch.Tensor, cache: LatentCache, scale: float, counts: 
     chunk of a prompt. Returns (B, H, Lq, latent_dim), the weights' sums of latents, or (out, lse) with need_lse, lse
     (B, H, Lq) float32; a query with nothing to attend gives 0 and -inf.
 
-    prefix: a LatentCache of one sequence whose rows come before every sequence's own, as those of a system prompt. The
-    batch reads them once, and each sequence's cache holds only what follows."""
+    prefix: a LatentCache of one sequence whose rows come before every sequence's own, as those of a system prompt; each
+    sequence's cache holds only what follows. Sequences of at most 32 query rows (H * Lq) read the prefix together, as many
+    as fill 64 rows; longer ones each for every 64 of their rows.
+
+    No gradient is formed: tensors that require one while gradients are recorded are refused."""
     _require_cuda("latent_attention", q, counts)
     _same_device("latent_attention", cache, q, counts)
     _no_gradient("latent_attention", q, cache._rows, *(() if prefix is None else (prefix._rows,)))
@@ -277,6 +284,9 @@ def latent_sdpa(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor, v: torch
     k (B, Hkv, S, Dn), k_rope (B, S, Dr), v (B, Hkv, S, Dv), H a multiple of Hkv; scores scale * (q[..., :Dn] . k +
     q[..., Dn:] . k_rope), scale 1 / sqrt(Dn + Dr) if not given, top-left causal masking as in
     scaled_dot_product_attention. Returns (B, H, L, Dv), differentiable in all four.
+
+    16-bit inputs with Dn = Dv of 64 or 128 and Dr a multiple of 16 up to 64 have kernels of their own, whose gradients have the same
+    bits on every run; other sizes, and f32, go by scaled_dot_product_attention with k_rope repeated for each head.
 
     seq_lens (int32, B; L = S) is for prompts padded to one length: tokens from seq_lens[b] on (which may hold anything) are not
     attended, give 0 and get zero gradients."""

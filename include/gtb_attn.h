@@ -341,8 +341,8 @@ typedef struct gtb_latent {
 /* Append rows: latent (B,1,n,R) and k_rope (B,1,n,Dr), f32/f16/bf16 (one dtype, any strides with a unit innermost one);
  * the first counts[b] of them (device int32, clamped to [0, n]; NULL: n) go to rows lens[b] .. of sequence b, rounded
  * once to the cache's type. With rope_mode 0 (pairs 2i, 2i+1) or 2 (pairs i, i + Dr/2) the rotary key is first rotated,
- * in f32, for position offset[0] + lens[b] + i (offset: device int32, the lens of a prefix, or NULL: 0), its pairs'
- * frequencies freq_scale * freq_base^(-2i / Dr) and angles those of gtb_rope_axes; with -1 it is taken as given.
+ * in f32, for position offset[0] + lens[b] + i (offset: device int32, or NULL: 0; mostly the lens of a prefix, but any number
+ * of positions, whether or not a cache holds as many rows: read as it is, below 0 as 0), its pairs' frequencies freq_scale * freq_base^(-2i / Dr) and angles those of gtb_rope_axes; with -1 it is taken as given.
  * With advance != 0 a second kernel sets lens[b] = min(lens[b] + counts[b], Smax). Rows that would land past Smax are
  * dropped and leave status 62 (gtb_device_status). */
 GTB_API int gtb_latent_append(const gtb_latent *cache, const gtb_tensor4 *latent, const gtb_tensor4 *k_rope,
@@ -355,11 +355,15 @@ GTB_API int gtb_latent_append(const gtb_latent *cache, const gtb_tensor4 *latent
  * s <= lens[b] - counts[b] + i of its sequence: score = scale * q . row, out (B,H,Lq,R) = sum of weight * latent
  * (the values' up-projection is the caller's next product). A query at or past counts[b], or with no row to attend,
  * gives 0 and lse -inf.
- *   prefix: NULL, or a cache of one sequence (B = 1, same R, Dr and dtype) whose rows come before every sequence's own:
- *   they are read once for the whole batch. q 16-byte aligned, any strides that are multiples of 8 with a unit
- *   innermost one; out contiguous, 16-byte aligned; lse NULL or (B,H,Lq) f32; scale positive, below 1e38.
- * Scratch from the stream-ordered allocator: f32 parts of rows that several thread blocks worked on, at most two of 64 rows a
- * multiprocessor (38 MB on 148 with R = 512), or behind a prefix one a sequence and a multiprocessor. */
+ *   prefix: NULL, or a cache of one sequence (B = 1, same R, Dr and dtype) whose rows come before every sequence's own.
+ *   Where H * Lq is at most 32, as many sequences as fill 64 query rows read them together; beyond that each block of up to 64 query
+ *   rows of a sequence does. q 16-byte aligned, any strides that are positive multiples of 8 with a unit innermost one; out
+ *   contiguous, 16-byte aligned; lse NULL or (B,H,Lq) f32; scale positive, below 1e38.
+ * Scores, maxima, sums and outputs are f32; a weight is rounded to the cache's type (in f16 to 11 bits, or to steps of 2^-24 of
+ * its row's largest where those are coarser) before it meets the latents, and out is rounded once.
+ * Scratch from the stream-ordered allocator, for f32 parts of rows that several thread blocks worked on, some 4 R + 8 bytes a row: two slots a
+ * multiprocessor of an item's rows (up to 64; 38 MB on 148 with R = 512). Where sequences read a prefix together, 64 rows for each
+ * multiprocessor and each such group of sequences, and H * Lq rows (to a multiple of 16) for each multiprocessor and sequence. */
 GTB_API int gtb_latent_attention(const gtb_tensor4 *q, const gtb_latent *cache, const gtb_latent *prefix, float scale,
                                  const int32_t *counts, gtb_tensor4 *out, float *lse, void *stream);
 
@@ -374,7 +378,12 @@ GTB_API int gtb_latent_attention(const gtb_tensor4 *q, const gtb_latent *cache, 
  * head for (their gradients have values); queries without keys, and keys without queries, are refused.
  * The backward takes the forward's out and lse and writes dq, dk, dk_rope (summed over all heads) and dv, in fixed order:
  * the same bits on every run. Its weights are 2^(score - log-sum-exp) of f32 numbers: off by about |score| 2^-22 of themselves
- * (scores in powers of 2). Its scratch (4 (2 B H L + B Hkv S Dr) bytes) comes from the stream-ordered allocator. */
+ * (scores in powers of 2). Its scratch, 4 (2 B H L' + B Hkv S Dr) bytes with L' = L to a multiple of 64, comes from the
+ * stream-ordered allocator.
+ * Scores, maxima, sums and what the products add up to are f32. Rounded to the inputs' type are, once each: a weight before it meets v or
+ * grad_out; ds = weight * (grad_out . v - grad_out . out) before it meets q or k (in f16 it becomes infinite past 65504, and keeps
+ * steps of 2^-24); the results. grad_out . out is formed of the rounded out. Gradients of bf16 inputs are off by some 0.0024
+ * of their norm (over a handful of keys 0.0036), where rounding the exact ones leaves 0.0017. */
 GTB_API int gtb_latent_sdpa_fwd(const gtb_tensor4 *q, const gtb_tensor4 *k, const gtb_tensor4 *k_rope, const gtb_tensor4 *v,
                                 const int32_t *seq_lens, float scale, int is_causal, gtb_tensor4 *out, float *lse,
                                 void *stream);
