@@ -381,8 +381,8 @@ GTB_API int gtb_latent_attention(const gtb_tensor4 *q, const gtb_latent *cache, 
  * (scores in powers of 2). Its scratch, 4 (2 B H L' + B Hkv S Dr) bytes with L' = L to a multiple of 64, comes from the
  * stream-ordered allocator.
  * Scores, maxima, sums and what the products add up to are f32. Rounded to the inputs' type are, once each: a weight before it meets v or
- * grad_out; ds = weight * (grad_out . v - grad_out . out) before it meets q or k (in f16 it becomes infinite past 65504, and keeps
- * steps of 2^-24); the results. grad_out . out is formed of the rounded out. Gradients of bf16 inputs are off by some 0.0024
+ * grad_out; ds = weight * (grad_out . v - grad_out . out) before it meets q or k (f16 has steps of 2^-24 for both, and ds becomes
+ * infinite past 65504); the results. grad_out . out is formed of the rounded out. Gradients of bf16 inputs are off by some 0.0024
  * of their norm (over a handful of keys 0.0036), where rounding the exact ones leaves 0.0017. */
 GTB_API int gtb_latent_sdpa_fwd(const gtb_tensor4 *q, const gtb_tensor4 *k, const gtb_tensor4 *k_rope, const gtb_tensor4 *v,
                                 const int32_t *seq_lens, float scale, int is_causal, gtb_tensor4 *out, float *lse,
